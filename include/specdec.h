@@ -346,6 +346,120 @@ int specdec_time_linear(specdec_handle *h, int role, int layer, int which, int r
 int specdec_time_attention(specdec_handle *h, int role, int layer, int q_per_req, int reps, void *flush,
                            size_t flush_bytes, float *avg_us, double *alg_bytes);
 
+/* ---------------------------------------------------------------------------
+ * Ragged decode steps over an 8-bit cache (no counterpart in the reference,
+ * whose calls take one request, or equal prompts here): the four operators of
+ * one step of a caller that schedules its own requests of unequal length --
+ * block tables and slot maps, the cache write, the attention, the token.
+ *
+ * Every buffer is DEVICE memory of the handle's device (specdec_sample: of the
+ * current device) and the caller's; `stream` is a cudaStream_t, NULL the
+ * device's default stream.  Calls are asynchronous, allocate nothing, read no
+ * device value on the host and may be captured in a graph.  A specdec_kv8
+ * owns the attention's workspace: its specdec_kv8_attend calls on different
+ * streams must be ordered by the caller.  Values on the device that are out
+ * of range (lengths, page numbers, rows) are clipped or left out, never
+ * followed.  dtype is SPECDEC_F32 or SPECDEC_BF16; strides count elements,
+ * and the head_dim values of a row and head are adjacent.
+ *
+ * Cache layer: codes [n_pages][n_kv_heads][page_tokens][head_dim] of 8 bits
+ * (-127 .. 127), scales [n_pages][n_kv_heads][page_tokens / block_tokens]; the
+ * value is code x scale.  Request b's position p lies in page
+ * table[b][p / page_tokens]; its slot is that page x page_tokens + p %
+ * page_tokens. */
+typedef struct specdec_kv8_config {
+  int32_t n_heads, n_kv_heads; /* query head h reads kv head h / (n_heads / n_kv_heads) */
+  int32_t head_dim;            /* 16, 32, 64 or 128 */
+  int32_t page_tokens;         /* positions of a page: 16, 32, 64 or 128 */
+  int32_t block_tokens;        /* positions that share a scale: 16 .. page_tokens, a power of two */
+  int32_t max_batch;           /* largest n_requests, at most 4096 */
+} specdec_kv8_config;
+
+typedef struct specdec_kv8_layer {
+  int8_t *k, *v;           /* 16-byte aligned */
+  float *k_scale, *v_scale;
+  int32_t n_pages;
+} specdec_kv8_layer;
+
+typedef struct specdec_kv8_batch {
+  int32_t *table;      /* [n_requests][table_cols] pages of each request */
+  int32_t n_requests, table_cols;
+  int32_t *kv_len;     /* [n_requests] positions of each request, its new rows included */
+  int32_t *cu_q;       /* [n_requests + 1] first new row of each request in the step's row arrays */
+  /* written by specdec_kv8_plan only (may be NULL elsewhere): */
+  int32_t *tok_req, *tok_pos; /* [max_tokens] request and position of each row, -1 past the last */
+  int64_t *slots;      /* [max_tokens] cache slot of each row, -1 past the last */
+  int32_t max_tokens;
+  int32_t *status;     /* [1] 0, or bits: 1 not enough free pages, 2 a bad length (or ring), 4 more rows than max_tokens */
+} specdec_kv8_batch;
+
+typedef struct specdec_kv8 specdec_kv8;
+
+int specdec_kv8_create(const specdec_kv8_config *cfg, int device, specdec_kv8 **out);
+int specdec_kv8_destroy(specdec_kv8 *h);
+/* Last error message of this handle (NULL: of the thread's last failed create). */
+const char *specdec_kv8_last_error(const specdec_kv8 *h);
+
+/* Block tables and slot maps of a step.  Request b holds the pages of `held`
+ * positions (its last kv_len), keeps the first keep[b] of them (rejected
+ * drafts go, 0 for a slot that is free) and gets q_len[b] new rows.  Pages it
+ * lacks come from the head of the ring of free pages in request order, pages
+ * it no longer needs go to the tail; ring[ring_cap] must be able to hold every
+ * page of the pool, ring_state = {head, free pages}.  Writes the batch's
+ * table entries of new pages, kv_len = keep + q_len, cu_q, tok_req, tok_pos,
+ * slots, status, the ring and ring_state_out.  On a status other than 0
+ * nothing moves: the step has no rows (cu_q is all 0) and kv_len = held.
+ * Outputs must not overlap inputs (two batches take turns). */
+int specdec_kv8_plan(specdec_kv8 *h, const specdec_kv8_batch *batch, const int32_t *held, const int32_t *keep,
+                     const int32_t *q_len, int32_t *ring, int ring_cap, const int32_t *ring_state,
+                     int32_t *ring_state_out, void *stream);
+
+/* Writes the step's K and V rows [n_tokens][n_kv_heads][head_dim] to the last
+ * q positions of their requests.  Per block of block_tokens positions and kv
+ * head: scale' = max(the block's scale if it has older rows, max |x| over its
+ * new finite values times the 32-bit 1/127), a scale below 2^-126 is 0; older codes become
+ * rint(code x (scale / scale')), new codes rint(x x (1 / scale')) within
+ * -127 .. 127; a NaN becomes 0, an infinity +-127. */
+int specdec_kv8_append(specdec_kv8 *h, const specdec_kv8_layer *layer, const specdec_kv8_batch *batch, const void *k,
+                       int64_t k_row_stride, int64_t k_head_stride, const void *v, int64_t v_row_stride,
+                       int64_t v_head_stride, int dtype, int n_tokens, void *stream);
+
+/* Reads the values of n cache slots back: out_k and out_v (either may be NULL)
+ * [n][n_kv_heads][head_dim], zeros for a slot outside the pool (-1). */
+int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int64_t *rows, int n, void *out_k,
+                       void *out_v, int dtype, void *stream);
+
+/* Attention of the step's query rows [n_tokens][n_heads][head_dim] over the
+ * cache: row i of request b stands at position p = kv_len - q + i and sees
+ * positions max(0, p - window + 1) .. p (window 0: from 0).  scores = scale x
+ * q . k, softmax in 32 bits, out in the rows' type, lse (may be NULL)
+ * [n_tokens][n_heads] = ln of the sum of exp(scores).  A row that sees
+ * nothing gives zeros and -infinity; a position whose page number is outside
+ * the pool is not seen; rows past cu_q[n_requests] are left as they are.
+ * max_q: the most rows of one request (it selects the kernel; the result does
+ * not depend on it). */
+int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer, const specdec_kv8_batch *batch, const void *q,
+                       int64_t q_row_stride, int64_t q_head_stride, int dtype, int n_tokens, void *out,
+                       int64_t out_row_stride, int64_t out_head_stride, float *lse, int max_q, float scale, int window,
+                       void *stream);
+
+/* One token per row of logits [rows][vocab] (vocab at most 2^20) from the
+ * row's uniform u in [0, 1).  Per row, each array NULL for its default:
+ * temperature (<= 0: the arg max; default 1), top_k (<= 0: off), top_p (>= 1:
+ * off), min_p (<= 0: off).  z = l / temperature (a NaN logit counts as
+ * -infinity), w = floor(2^31 exp(z - max z)); top-k keeps the first k tokens by
+ * z, ties to the lower index; top-p keeps those of them before which less
+ * than max(1, floor(top_p W)) of their mass W lies; min-p keeps those with
+ * exp(z - max z) >= min(min_p, 1).  The token is the first in index order at
+ * which the running sum of kept w exceeds floor(u x sum) (top_p and u to 24
+ * bits); probs (may be NULL) is w / sum.  Sums are whole numbers, so the token
+ * does not depend on their order.  A row without a logit above -infinity
+ * gives token -1 and probability 0; arg max rows give probability 1.  Errors:
+ * specdec_last_error(NULL). */
+int specdec_sample(const void *logits, int dtype, int rows, int vocab, int64_t row_stride, const float *temperature,
+                   const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *tokens,
+                   float *probs, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

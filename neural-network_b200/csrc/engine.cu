@@ -45,12 +45,16 @@
 #include "attn_dec.cuh"
 #include "gemm_w8.cuh"
 #include "gemm_sk.cuh"
+#include "status.cuh"
 
 using namespace specdec;
 
-namespace {
+// Message of the calling thread's last failed call without a handle (status.cuh).
+namespace specdec {
+thread_local std::string g_thread_err;
+}
 
-thread_local std::string g_create_err;
+namespace {
 
 struct SpecErr {
   int code;
@@ -1968,7 +1972,7 @@ void check_device_err(specdec_handle *h) {
 // ---------------------------------------------------------------------------
 extern "C" {
 
-const char *specdec_last_error(const specdec_handle *h) { return h ? h->err.c_str() : g_create_err.c_str(); }
+const char *specdec_last_error(const specdec_handle *h) { return h ? h->err.c_str() : g_thread_err.c_str(); }
 
 namespace {
 int create_impl(const specdec_config *cfg, int device, int rank, int world, const void *uid, specdec_handle **out);
@@ -1986,7 +1990,7 @@ int specdec_tp_unique_id(void *out128) {
     static_assert(sizeof(ncclUniqueId) == 128, "NCCL unique id is 128 bytes");
     std::memcpy(out128, &id, sizeof(id));
   } catch (const SpecErr &e) {
-    g_create_err = e.msg;
+    g_thread_err = e.msg;
     return e.code;
   }
   return SPECDEC_OK;
@@ -1995,7 +1999,7 @@ int specdec_tp_unique_id(void *out128) {
 int specdec_create_tp(const specdec_config *cfg, int device, int rank, int world, const void *unique_id,
                       specdec_handle **out) {
   if (world < 1 || rank < 0 || rank >= world || (world > 1 && !unique_id)) {
-    g_create_err = "bad tensor-parallel rank / size / id";
+    g_thread_err = "bad tensor-parallel rank / size / id";
     return SPECDEC_ERR_INVALID;
   }
   return create_impl(cfg, device, rank, world, unique_id, out);
@@ -2229,7 +2233,7 @@ int create_impl(const specdec_config *cfg, int device, int rank, int world, cons
       nccl_check(nccl().comm_init_rank(&h->comm, world, id, rank), "ncclCommInitRank");
     }
   } catch (const SpecErr &e) {
-    g_create_err = e.msg;
+    g_thread_err = e.msg;
     specdec_destroy(h.release());
     return e.code;
   }

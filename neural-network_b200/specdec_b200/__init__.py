@@ -38,7 +38,9 @@ EXPORTS = ("specdec_create", "specdec_destroy", "specdec_last_error", "specdec_l
            "specdec_time_linear", "specdec_generate_tree", "specdec_generate_tree_device", "specdec_tp_unique_id",
            "specdec_create_tp", "specdec_generate_ar", "specdec_generate_ar_device", "specdec_load_netw",
            "specdec_prefill", "specdec_prefill_device", "specdec_step", "specdec_step_device",
-           "specdec_session_tokens", "specdec_time_attention", "specdec_load_params_device")
+           "specdec_session_tokens", "specdec_time_attention", "specdec_load_params_device",
+           "specdec_kv8_create", "specdec_kv8_destroy", "specdec_kv8_last_error", "specdec_kv8_plan",
+           "specdec_kv8_append", "specdec_kv8_gather", "specdec_kv8_attend", "specdec_sample")
 
 # linear layers of specdec_time_linear
 LIN_QKV, LIN_OPROJ, LIN_FFN_IN, LIN_FFN_OUT, LIN_HEAD = 0, 1, 2, 3, 4
@@ -71,6 +73,22 @@ class _GenParams(C.Structure):
     _fields_ = [("max_new_tokens", C.c_int32), ("lookahead", C.c_int32), ("temperature", C.c_float),
                 ("top_k", C.c_int32), ("top_p", C.c_float), ("rng_mode", C.c_int32), ("seed", C.c_uint32),
                 ("uniforms", C.c_void_p), ("uniform_rounds", C.c_int32), ("draft_catchup", C.c_int32)]
+
+
+class _KV8Config(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_heads", "n_kv_heads", "head_dim", "page_tokens", "block_tokens",
+                                         "max_batch")]
+
+
+class _KV8Layer(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_pages", C.c_int32)]
+
+
+class _KV8Batch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("n_requests", C.c_int32), ("table_cols", C.c_int32), ("kv_len", C.c_void_p),
+                ("cu_q", C.c_void_p), ("tok_req", C.c_void_p), ("tok_pos", C.c_void_p), ("slots", C.c_void_p),
+                ("max_tokens", C.c_int32), ("status", C.c_void_p)]
 
 
 _lib = None
@@ -122,6 +140,16 @@ def load_library(path: str = LIB_PATH):
                                         C.c_size_t, C.POINTER(C.c_float), C.POINTER(C.c_double)]
     lib.specdec_time_attention.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_size_t,
                                            C.POINTER(C.c_float), C.POINTER(C.c_double)]
+    vp, i64, i32 = C.c_void_p, C.c_int64, C.c_int
+    lib.specdec_kv8_create.argtypes = [C.POINTER(_KV8Config), i32, C.POINTER(vp)]
+    lib.specdec_kv8_destroy.argtypes = [vp]
+    lib.specdec_kv8_last_error.restype = C.c_char_p
+    lib.specdec_kv8_last_error.argtypes = [vp]
+    lib.specdec_kv8_plan.argtypes = [vp, vp, vp, vp, vp, vp, i32, vp, vp, vp]
+    lib.specdec_kv8_append.argtypes = [vp, vp, vp, vp, i64, i64, vp, i64, i64, i32, i32, vp]
+    lib.specdec_kv8_gather.argtypes = [vp, vp, vp, i32, vp, vp, i32, vp]
+    lib.specdec_kv8_attend.argtypes = [vp, vp, vp, vp, i64, i64, i32, i32, vp, i64, i64, vp, i32, C.c_float, i32, vp]
+    lib.specdec_sample.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp]
     _lib = lib
     return lib
 
@@ -391,3 +419,6 @@ class Engine:
         self._check(self._lib.specdec_time_attention(self.h, role, layer, q_per_req, reps, C.c_void_p(flush_ptr),
                                                      C.c_size_t(flush_bytes), C.byref(us), C.byref(nb)))
         return float(us.value), float(nb.value)
+
+
+from .ragged import KV8, KV8Batch, KV8Layer, sample  # noqa: E402,F401

@@ -1,0 +1,187 @@
+"""Operators of a ragged decode step over an 8-bit paged cache: ``KV8.plan``
+(block tables and slot maps), ``KV8.append`` and ``KV8.gather`` (cache rows),
+``KV8.attend`` and ``sample``.  include/specdec.h has their definitions.
+
+Buffers are CUDA tensors: any object with ``data_ptr()``, ``shape``,
+``stride()``, ``dtype``, ``device`` and ``is_contiguous()``, as torch's are.
+``stream`` is a raw cudaStream_t (0: the device's default stream, torch's
+current one unless a caller changed it); tensors must be ready on it.
+Failures raise ``SpecDecError`` (a RuntimeError), wrong arguments before the
+call ``ValueError``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+import specdec_b200 as _sd
+
+_DTYPE = {"torch.float32": _sd.F32, "torch.bfloat16": _sd.BF16}
+_dtype_cache: dict = {}
+
+
+def _dtype_of(t) -> int:
+    d = _dtype_cache.get(t.dtype)
+    if d is None:
+        d = _DTYPE.get(str(t.dtype))
+        if d is None:
+            raise ValueError(f"rows must be float32 or bfloat16, not {t.dtype}")
+        _dtype_cache[t.dtype] = d
+    return d
+
+
+def _buffer(t, name: str, dtype: str, shape=None):
+    """The address of a contiguous buffer of the given type (and shape)."""
+    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or t.device.type != "cuda":
+        raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _optional(t, name: str, dtype: str, shape=None):
+    return None if t is None else _buffer(t, name, dtype, shape)
+
+
+class KV8Layer:
+    """One layer's cache: codes k, v [pages][kv heads][page tokens][head dim]
+    int8 and scales [pages][kv heads][blocks of a page] float32."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.dim() != 4 or k_scale.dim() != 3:
+            raise ValueError("codes have 4 dimensions, scales 3")
+        if tuple(k_scale.shape[:2]) != tuple(k.shape[:2]):
+            raise ValueError("scales and codes must agree on pages and kv heads")
+        self.shape, self.blocks = tuple(k.shape), k_scale.shape[2]
+        self.record = _sd._KV8Layer(_buffer(k, "k", "int8"), _buffer(v, "v", "int8", k.shape),
+                                    _buffer(k_scale, "k_scale", "float32"),
+                                    _buffer(v_scale, "v_scale", "float32", k_scale.shape), k.shape[0])
+        self.ptr = C.addressof(self.record)
+        self._keep = (k, v, k_scale, v_scale)
+
+
+class KV8Batch:
+    """The requests of a step: table [requests][columns], kv_len [requests],
+    cu_q [requests + 1] (int32), and for ``KV8.plan`` tok_req, tok_pos (int32),
+    slots (int64) of one length and status [1] (int32)."""
+
+    def __init__(self, table, kv_len, cu_q, tok_req=None, tok_pos=None, slots=None, status=None):
+        if table.dim() != 2:
+            raise ValueError("table has 2 dimensions")
+        n = table.shape[0]
+        rows = 0 if slots is None else slots.shape[0]
+        self.n_requests = n
+        self.planned = status is not None
+        self.record = _sd._KV8Batch(
+            _buffer(table, "table", "int32"), n, table.shape[1], _buffer(kv_len, "kv_len", "int32", (n,)),
+            _buffer(cu_q, "cu_q", "int32", (n + 1,)), _optional(tok_req, "tok_req", "int32", (rows,)),
+            _optional(tok_pos, "tok_pos", "int32", (rows,)), _optional(slots, "slots", "int64"), rows,
+            _optional(status, "status", "int32", (1,)))
+        self.ptr = C.addressof(self.record)
+        self._keep = (table, kv_len, cu_q, tok_req, tok_pos, slots, status)
+
+
+def _rows(t, heads: int, dim: int, name: str):
+    """(address, row stride, head stride) of rows [n][heads][dim] with adjacent dims."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 3 or sh[1] != heads or sh[2] != dim or (st[2] != 1 and dim > 1):
+        raise ValueError(f"{name} must be rows of {heads} heads x {dim} adjacent values, not {tuple(sh)}")
+    return t.data_ptr(), st[0], st[1]
+
+
+class KV8:
+    """Geometry and workspace of an 8-bit paged cache with a scale per
+    block_tokens positions and kv head, on one device."""
+
+    def __init__(self, n_heads: int, n_kv_heads: int, head_dim: int, page_tokens: int = 128, block_tokens: int = 16,
+                 max_batch: int = 256, device: int = 0):
+        lib = _sd.load_library()
+        cfg = _sd._KV8Config(n_heads, n_kv_heads, head_dim, page_tokens, block_tokens, max_batch)
+        h = C.c_void_p()
+        rc = lib.specdec_kv8_create(C.byref(cfg), device, C.byref(h))
+        if rc:
+            raise _sd.SpecDecError(rc, lib.specdec_kv8_last_error(None).decode())
+        self._lib, self.h = lib, h
+        self.n_heads, self.n_kv_heads, self.head_dim = n_heads, n_kv_heads, head_dim
+        self.page_tokens, self.block_tokens = page_tokens, block_tokens
+
+    def close(self):
+        if getattr(self, "h", None):
+            self._lib.specdec_kv8_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
+
+    def _check(self, rc: int):
+        if rc:
+            raise _sd.SpecDecError(rc, self._lib.specdec_kv8_last_error(self.h).decode())
+
+    def _layer(self, layer: KV8Layer) -> int:
+        if layer.shape[1:] != (self.n_kv_heads, self.page_tokens, self.head_dim) or \
+                layer.blocks * self.block_tokens != self.page_tokens:
+            raise ValueError(f"the layer's codes {layer.shape} and {layer.blocks} blocks a page do not fit this handle")
+        return layer.ptr
+
+    def plan(self, batch: KV8Batch, held, keep, q_len, ring, ring_state, ring_state_out, stream: int = 0) -> None:
+        """Pages, lengths, row and slot maps of a step (specdec_kv8_plan)."""
+        n = (batch.n_requests,)
+        self._check(self._lib.specdec_kv8_plan(
+            self.h, batch.ptr, _buffer(held, "held", "int32", n), _buffer(keep, "keep", "int32", n),
+            _buffer(q_len, "q_len", "int32", n), _buffer(ring, "ring", "int32"), ring.shape[0],
+            _buffer(ring_state, "ring_state", "int32", (2,)), _buffer(ring_state_out, "ring_state_out", "int32", (2,)),
+            stream or None))
+
+    def append(self, layer: KV8Layer, batch: KV8Batch, k, v, stream: int = 0) -> None:
+        """Writes rows k, v [rows][kv heads][head dim] to the requests' last positions."""
+        kp, kr, kh = _rows(k, self.n_kv_heads, self.head_dim, "k")
+        vp, vr, vh = _rows(v, self.n_kv_heads, self.head_dim, "v")
+        if v.shape[0] != k.shape[0] or v.dtype != k.dtype:
+            raise ValueError("k and v must have the same rows and type")
+        self._check(self._lib.specdec_kv8_append(self.h, self._layer(layer), batch.ptr, kp, kr, kh, vp, vr, vh,
+                                                 _dtype_of(k), k.shape[0], stream or None))
+
+    def gather(self, layer: KV8Layer, rows, out_k=None, out_v=None, stream: int = 0) -> None:
+        """Values of the cache slots `rows` (int64) into out_k, out_v [rows][kv heads][head dim]."""
+        n = rows.shape[0]
+        shape = (n, self.n_kv_heads, self.head_dim)
+        outs = [t for t in (out_k, out_v) if t is not None]
+        if not outs:
+            return
+        if any(tuple(t.shape) != shape or not t.is_contiguous() or t.dtype != outs[0].dtype for t in outs):
+            raise ValueError(f"outputs must be contiguous, of one type and shape {shape}")
+        self._check(self._lib.specdec_kv8_gather(
+            self.h, self._layer(layer), _buffer(rows, "rows", "int64"), n, None if out_k is None else out_k.data_ptr(),
+            None if out_v is None else out_v.data_ptr(), _dtype_of(outs[0]), stream or None))
+
+    def attend(self, layer: KV8Layer, batch: KV8Batch, q, out, lse=None, max_q: int = 1,
+               scale: Optional[float] = None, window: int = 0, stream: int = 0) -> None:
+        """Attention of q [rows][heads][head dim] over the cache into out (and lse
+        [rows][heads] float32); scale defaults to 1 / sqrt(head dim)."""
+        qp, qr, qh = _rows(q, self.n_heads, self.head_dim, "q")
+        op, orow, oh = _rows(out, self.n_heads, self.head_dim, "out")
+        if out.shape[0] != q.shape[0] or out.dtype != q.dtype:
+            raise ValueError("q and out must have the same rows and type")
+        lp = None if lse is None else _buffer(lse, "lse", "float32", q.shape[:2])
+        self._check(self._lib.specdec_kv8_attend(
+            self.h, self._layer(layer), batch.ptr, qp, qr, qh, _dtype_of(q), q.shape[0], op, orow, oh, lp, max_q,
+            1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, stream or None))
+
+
+def sample(logits, u, tokens, probs=None, temperature=None, top_k=None, top_p=None, min_p=None,
+           stream: int = 0) -> None:
+    """One token per row of logits [rows][vocab] from the uniforms u (specdec_sample):
+    tokens int32, probs float32 [rows]; the parameters are [rows] tensors or None."""
+    sh, st = logits.shape, logits.stride()
+    if len(sh) != 2 or (st[1] != 1 and sh[1] > 1):
+        raise ValueError("logits must be rows of adjacent values")
+    n = (sh[0],)
+    lib = _sd.load_library()
+    rc = lib.specdec_sample(
+        logits.data_ptr(), _dtype_of(logits), sh[0], sh[1], st[0], _optional(temperature, "temperature", "float32", n),
+        _optional(top_k, "top_k", "int32", n), _optional(top_p, "top_p", "float32", n),
+        _optional(min_p, "min_p", "float32", n), _buffer(u, "u", "float32", n), _buffer(tokens, "tokens", "int32", n),
+        _optional(probs, "probs", "float32", n), stream or None)
+    if rc:
+        raise _sd.SpecDecError(rc, lib.specdec_last_error(None).decode())
