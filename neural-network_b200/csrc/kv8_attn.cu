@@ -1,5 +1,33 @@
 // Attention over the 8-bit paged cache (specdec_kv8_attend).
+//
+// Per query row and head: s_j = scale sk(j) (q . ck_j), p_j = exp(s_j - m),
+// out = sum p_j sv(j) cv_j / sum p_j, with one scale pair per block of
+// positions.  Codes are whole numbers up to 127, exact in f16, so both
+// products run on the tensor cores over the codes themselves and the scales
+// enter the scores and the weights.
+//
+// Few rows per kv head (decode steps, verify blocks): kv8_decode_kernel.  The
+// cache is read once and every byte meets at most 16 rows, so HBM bounds it.
+// The cache is the products' A operand (16 positions or 16 dims a tile), the
+// rows are their N side (8 or 16 columns), which wastes nothing of the tensor
+// cores that a 128-row tile would need:
+//   S^T [16 positions][8 rows]  = K codes [16][D] x Q^T
+//   O^T [16 dims][8 rows]      += V^T codes [16 dims][16 positions] x P^T
+// A slice of 16 positions lies in one page and has one scale pair.  Every
+// warp owns whole slices and a ring of them in shared memory that it fills
+// itself with 16-byte asynchronous copies (no barrier between warps until the
+// end of an item), converts codes to f16 in registers, and keeps its running
+// maximum, sum and output; the block's warps take slices in turn and merge at
+// the end of a (request, kv head, row tile) item.
+//
+// Work is split evenly whatever the lengths are: all items' 64-position units
+// in a row, an equal share of consecutive units per block.  A block that holds
+// part of an item leaves (maximum, sum, unnormalised output) in the workspace
+// and the last of the item's blocks to arrive merges them in block order, so
+// equal calls give equal bits.
 #include "kv8_attn.cuh"
+
+#include <cuda_fp16.h>
 
 #include <cmath>
 
@@ -18,62 +46,595 @@ struct AttendArgs {
   float *lse;
   float scale;
   int window;
+  float *part;
+  int *ticket;
 };
 
-// One warp per (row, head): scores and values one position at a time with a
-// running maximum.  Right for every shape; nothing is reused between rows.
-template <typename XT>
-__global__ void __launch_bounds__(128) kv8_attend_simple_kernel(const AttendArgs a) {
-  const Kv8Geom &g = a.g;
-  const int lane = threadIdx.x & 31;
-  const int per = (g.D + 31) / 32;
-  for (long long w = blockIdx.x * 4ll + (threadIdx.x >> 5); w < static_cast<long long>(a.b.T) * g.H; w += gridDim.x * 4ll) {
-    const int row = static_cast<int>(w / g.H), h = static_cast<int>(w % g.H), hk = h / g.G;
-    int lo = 0, hi = a.b.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.b.cu_q[mid] <= row) lo = mid;
-      else hi = mid - 1;
-    }
-    const Kv8Req r = kv8_req(a.b, g.P, lo);
-    if (row < r.q0 || row >= r.q0 + r.q) continue;
-    const int pos = r.len - r.q + row - r.q0;
-    const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    float q[4], o[4], m = -INFINITY, l = 0.f;
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 32 * i;
-      o[i] = 0.f;
-      q[i] = (i < per && d < g.D) ? to_f32(static_cast<const XT *>(a.q)[row * a.q_row + h * a.q_head + d]) : 0.f;
-    }
-    for (int p = first; p <= pos; ++p) {
-      const int page = a.b.table[static_cast<long long>(lo) * a.b.cols + p / g.P];
-      if (page < 0 || page >= a.c.n_pages) continue;
-      const long long ph = static_cast<long long>(page) * g.Hkv + hk;
-      const long long at = (ph * g.P + p % g.P) * g.D;
-      const long long sat = ph * (g.P / g.t) + p % g.P / g.t;
-      float dot = 0.f;
-      for (int i = 0; i < per; ++i)
-        if (lane + 32 * i < g.D) dot += q[i] * static_cast<float>(a.c.k[at + lane + 32 * i]);
-      const float s = warp_sum(dot) * a.c.ks[sat] * a.scale;
-      const float nm = fmaxf(m, s);
-      const float al = expf(m - nm), e = expf(s - nm);
-      m = nm;
-      l = l * al + e;
-      const float ev = e * a.c.vs[sat];
-      for (int i = 0; i < per; ++i)
-        if (lane + 32 * i < g.D) o[i] = o[i] * al + ev * static_cast<float>(a.c.v[at + lane + 32 * i]);
-    }
-    for (int i = 0; i < per; ++i)
-      if (lane + 32 * i < g.D)
-        static_cast<XT *>(a.out)[row * a.o_row + h * a.o_head + lane + 32 * i] = from_f32<XT>(l > 0.f ? o[i] / l : 0.f);
-    if (a.lse && lane == 0) a.lse[w] = l > 0.f ? m + logf(l) : -INFINITY;
+constexpr int kDecWarps = 4;
+constexpr int kDecThreads = 32 * kDecWarps;
+constexpr int kSlice = 16;                       // positions of a slice
+constexpr int kUnit = kSlice * kDecWarps;        // positions of a unit: one slice a warp
+constexpr int kDecCtas = 2;                      // blocks per SM
+constexpr int kMinShare = 4;                     // units: a smaller share costs more in merging than it saves
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLazy = 8.f;                     // weights may grow to 2^8 before the maximum is moved
+
+template <int D, int NT>
+struct DecGeom {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kSliceBytes = kSlice * D;            // K or V codes of a slice
+  static constexpr int kSlot = 2 * kSliceBytes + 16;        // + the two scales and the page's validity
+  // 5 slots of 4 KB a warp at D = 128: 64 KB in flight per block, 128 KB per SM; smaller rows take 8 slots
+  static constexpr int kStages = D == 128 ? (NT == 1 ? 5 : 4) : 8;
+  static constexpr int kRing = kDecWarps * kStages * kSlot;
+  static constexpr int kMerge = kDecWarps * kRows * D * 4;  // per warp the unnormalised output
+  static constexpr int kPart = kRows * D + 2 * kRows;       // floats of a partial result
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t shared_addr(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Transpose of an 8 x 8 matrix of 16-bit values spread over the warp.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Bytes 0x64 u as f16 are 1024 + u; u = code + 128, so minus 1152 leaves the code, exactly.
+__device__ __forceinline__ uint32_t f16_codes(uint32_t biased) {
+  __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&biased), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<uint32_t *>(&h);
+}
+// Two f16 pairs of the four codes of a word (already ^ 0x80808080).
+__device__ __forceinline__ void codes4(uint32_t x, uint32_t &lo, uint32_t &hi) {
+  lo = f16_codes(__byte_perm(x, 0x64646464u, 0x4140));
+  hi = f16_codes(__byte_perm(x, 0x64646464u, 0x4342));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
+
+// Place of a 16-byte chunk of a slice row in shared memory.  K rows are read
+// by lanes (row g, chunk t and, for 128-byte rows, 4 + t): odd rows swap their
+// halves.  V rows are read 8 lanes along a row and 4 rows (2t) at once: the
+// rows' chunks are spread over the banks.
+template <int D>
+__device__ __forceinline__ int k_place(int row, int chunk) {
+  return row * D + 16 * (D == 128 ? chunk ^ ((row & 1) << 2) : chunk);
+}
+template <int D>
+__device__ __forceinline__ int v_place(int row, int chunk) {
+  if constexpr (D == 128) return row * D + 16 * (chunk ^ (row & 6));
+  const int r = (row & 8) | ((row & 7) >> 1) | ((row & 1) << 2);
+  if constexpr (D == 64) return r * D + 16 * (chunk ^ (r & 2));
+  return r * D + 16 * chunk;
+}
+
+// The request that a run of units belongs to.
+struct DecReq {
+  int b;
+  Kv8Req r;
+  int nr, nt, t0;  // row tiles, units of an item, first unit's index along the cache
+};
+
+template <int ROWS>
+__device__ __forceinline__ DecReq dec_req(const AttendArgs &a, int b) {
+  DecReq q;
+  q.b = b;
+  q.r = kv8_req(a.b, a.g.P, b);
+  q.nr = (q.r.q * a.g.G + ROWS - 1) / ROWS;
+  const int lo = a.window > 0 ? max(0, q.r.len - q.r.q - a.window + 1) : 0;
+  q.t0 = lo / kUnit;
+  q.nt = max(1, (q.r.len + kUnit - 1) / kUnit - q.t0);
+  return q;
+}
+
+// Walks consecutive units: request, item of the request, unit of the item.
+template <int ROWS>
+struct Cursor {
+  DecReq q;
+  int item, unit;
+  __device__ __forceinline__ void seek(const AttendArgs &a, const long long *pre, long long u) {
+    q = dec_req<ROWS>(a, request_of(pre, a.b.B, u));
+    const long long in = u - pre[q.b];
+    item = static_cast<int>(in / q.nt);
+    unit = static_cast<int>(in % q.nt);
   }
+  __device__ __forceinline__ void next(const AttendArgs &a, const long long *pre) {
+    if (++unit < q.nt) return;
+    unit = 0;
+    if (++item < q.nr * a.g.Hkv) return;
+    item = 0;
+    int b = q.b + 1;
+    while (b < a.b.B && pre[b + 1] == pre[b]) ++b;
+    if (b < a.b.B) q = dec_req<ROWS>(a, b);
+  }
+};
+
+template <typename XT, int D, int NT>
+__global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const __grid_constant__ AttendArgs a) {
+  using Geo = DecGeom<D, NT>;
+  constexpr int ROWS = Geo::kRows, S = Geo::kStages;
+  constexpr int KS = D / 16;       // products of 16 dims per score tile, and 16-dim tiles of the output
+  constexpr bool F32 = sizeof(XT) == 4;  // queries and weights as two f16 each: 22 bits
+  constexpr int NP = F32 ? 2 : 1;
+  extern __shared__ __align__(16) unsigned char dec_smem[];
+  unsigned char *ring = dec_smem;
+  float *merge = reinterpret_cast<float *>(dec_smem + Geo::kRing);
+  long long *pre = reinterpret_cast<long long *>(dec_smem + Geo::kRing + Geo::kMerge);
+  __shared__ long long red[kDecWarps];
+  __shared__ float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS];
+  __shared__ int s_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.g.G, Hkv = a.g.Hkv, P = a.g.P;
+
+  request_prefix(a.b.B, pre, red, [&](int b) {
+    const DecReq q = dec_req<ROWS>(a, b);
+    return static_cast<long long>(q.nr) * q.nt * Hkv;
+  });
+  const long long total = pre[a.b.B];
+  const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinShare));
+  const long long u0 = share * blockIdx.x, u1 = min(total, u0 + share);
+  if (u0 >= u1) return;
+
+  // ---- this warp's ring -------------------------------------------------
+  unsigned char *my_ring = ring + warp * S * Geo::kSlot;
+  Cursor<ROWS> load;
+  load.seek(a, pre, u0);
+  long long lu = u0;  // next unit to load
+  auto page_of = [&](const Cursor<ROWS> &c) {
+    const int p = (c.q.t0 + c.unit) * kUnit + warp * kSlice;
+    return p < c.q.r.len ? a.b.table[static_cast<long long>(c.q.b) * a.b.cols + p / P] : -1;
+  };
+  int page = page_of(load);
+  auto issue = [&](int slot) {
+    if (lu < u1) {
+      unsigned char *dst = my_ring + slot * Geo::kSlot;
+      const bool ok = page >= 0 && page < a.c.n_pages;
+      if (ok) {
+        const int p = (load.q.t0 + load.unit) * kUnit + warp * kSlice;
+        const long long ph = static_cast<long long>(page) * Hkv + load.item / load.q.nr;
+        const long long at = (ph * P + p % P) * D;
+        const uint32_t d0 = shared_addr(dst);
+#pragma unroll
+        for (int i = 0; i < (kSlice * D / 16 + 31) / 32; ++i) {
+          const int c = lane + 32 * i;
+          if (kSlice * D / 16 % 32 == 0 || c < kSlice * D / 16) {
+            const int row = c / (D / 16), ch = c % (D / 16);
+            cp_async16(d0 + k_place<D>(row, ch), a.c.k + at + 16 * c);
+            cp_async16(d0 + Geo::kSliceBytes + v_place<D>(row, ch), a.c.v + at + 16 * c);
+          }
+        }
+        const long long sat = ph * (P / a.g.t) + p % P / a.g.t;
+        if (lane < 2) cp_async4(d0 + 2 * Geo::kSliceBytes + 4 * lane, (lane ? a.c.vs : a.c.ks) + sat);
+      }
+      if (lane == 2) *reinterpret_cast<int *>(dst + 2 * Geo::kSliceBytes + 8) = ok;
+      load.next(a, pre);
+      if (++lu < u1) page = page_of(load);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) issue(i);
+
+  Cursor<ROWS> cur;
+  cur.seek(a, pre, u0);
+  bool fresh = true;
+  uint32_t qf[NP][NT][KS][2];
+  float o[NT][KS][4], m[NT][2], l[NT][2], cs[NT][2];
+  int lim[NT][2];   // last visible position of this lane's two columns (-1: none)
+  int min_lim = 0, max_lim = 0;
+  int slot = 0;
+  for (long long u = u0; u < u1; ++u) {
+    const DecReq &q = cur.q;
+    const int hk = cur.item / q.nr, row0 = cur.item % q.nr * ROWS;
+    const int n_rows = min(ROWS, q.r.q * G - row0);
+    if (fresh) {
+      // ---- the item's queries, scaled by a power of two to at most 1..2 ----
+      fresh = false;
+      min_lim = 0x7fffffff;
+      max_lim = -1;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int r = row0 + 8 * n + g;
+        const bool live = 8 * n + g < n_rows;
+        const long long at = live ? (q.r.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head : 0;
+        const XT *src = static_cast<const XT *>(a.q) + at;
+        float x[KS][4], big = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int d = D == 128 ? (s < 4 ? 16 * t + 4 * s : 64 + 16 * t + 4 * (s - 4)) : t * (D / 4) + 4 * s;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[s][j] = live ? to_f32(src[d + j]) : 0.f;
+            big = fmaxf(big, fabsf(x[s][j]));
+          }
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // 2^e <= big < 2^(e + 1); rows below 2^-100 count as 2^-100
+        const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
+        const float down = __uint_as_float((127 - e) << 23), up = __uint_as_float((127 + e) << 23);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float x0 = x[s][2 * j] * down, x1 = x[s][2 * j + 1] * down;
+            qf[0][n][s][j] = pack_f16(x0, x1);
+            if constexpr (F32) {
+              const float2 h = unpack_f16(qf[0][n][s][j]);
+              qf[NP - 1][n][s][j] = pack_f16(x0 - h.x, x1 - h.y);
+            }
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
+          cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e);
+          const int rr = 8 * n + 2 * t + j;
+          lim[n][j] = rr < n_rows ? q.r.len - q.r.q + (row0 + rr) / G : -1;
+          m[n][j] = -INFINITY;
+          l[n][j] = 0.f;
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][s][j] = 0.f;
+      }
+      min_lim = q.r.len - q.r.q + row0 / G;
+      max_lim = q.r.len - q.r.q + (row0 + n_rows - 1) / G;
+    }
+
+    // ---- one slice ----------------------------------------------------------
+    cp_wait<S - 2>();
+    __syncwarp();
+    const unsigned char *sk = my_ring + slot * Geo::kSlot, *sv = sk + Geo::kSliceBytes;
+    const int p0 = (q.t0 + cur.unit) * kUnit + warp * kSlice;
+    const bool ok = *reinterpret_cast<const int *>(sk + 2 * Geo::kSliceBytes + 8) != 0;
+    if (ok && p0 <= max_lim && (a.window <= 0 || p0 + kSlice - 1 > min_lim - a.window)) {
+      const float ksc = *reinterpret_cast<const float *>(sk + 2 * Geo::kSliceBytes);
+      const float vsc = *reinterpret_cast<const float *>(sk + 2 * Geo::kSliceBytes + 4);
+      float sc[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[n][j] = 0.f;
+      // scores: rows g and g + 8 of the slice, this lane's dims
+      uint32_t kw[2][KS];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = g + 8 * i;
+        if constexpr (D == 128) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(sk + k_place<D>(row, t + 4 * h));
+            kw[i][4 * h] = w.x; kw[i][4 * h + 1] = w.y; kw[i][4 * h + 2] = w.z; kw[i][4 * h + 3] = w.w;
+          }
+        } else if constexpr (D == 64) {
+          const uint4 w = *reinterpret_cast<const uint4 *>(sk + k_place<D>(row, t));
+          kw[i][0] = w.x; kw[i][1] = w.y; kw[i][2] = w.z; kw[i][3] = w.w;
+        } else if constexpr (D == 32) {
+          const uint2 w = *reinterpret_cast<const uint2 *>(sk + row * D + 8 * t);
+          kw[i][0] = w.x; kw[i][1] = w.y;
+        } else {
+          kw[i][0] = *reinterpret_cast<const uint32_t *>(sk + row * D + 4 * t);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        uint32_t f[4];
+        codes4(kw[0][s] ^ 0x80808080u, f[0], f[2]);
+        codes4(kw[1][s] ^ 0x80808080u, f[1], f[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) mma16816(sc[n], f, qf[p][n][s][0], qf[p][n][s][1]);
+      }
+      // softmax: this lane has positions p0 + g, p0 + g + 8 for columns 2t, 2t + 1
+      const bool whole = p0 + kSlice - 1 <= min_lim && (a.window <= 0 || p0 > max_lim - a.window);
+      // exponent of the value scale: weights are held relative to the largest p x sv
+      const int ev = max(static_cast<int>(__float_as_uint(vsc) >> 23) - 127, -90);
+      const float fev = static_cast<float>(ev);
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float f = cs[n][j] * ksc;
+          sc[n][j] *= f;
+          sc[n][j + 2] *= f;
+          if (!whole) {
+            const int first = a.window > 0 ? lim[n][j] - a.window : -1;
+            if (p0 + g > lim[n][j] || p0 + g <= first) sc[n][j] = -INFINITY;
+            if (p0 + g + 8 > lim[n][j] || p0 + g + 8 <= first) sc[n][j + 2] = -INFINITY;
+          }
+          grow |= fmaxf(sc[n][j], sc[n][j + 2]) + fev > m[n][j] + kLazy;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = fmaxf(sc[n][j], sc[n][j + 2]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float nm = fmaxf(m[n][j], top + fev);
+            const float al = m[n][j] == -INFINITY ? 0.f : exp2_fast(m[n][j] - nm);
+            m[n][j] = nm;
+            l[n][j] *= al;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              o[n][s][j] *= al;
+              o[n][s][j + 2] *= al;
+            }
+          }
+      }
+      uint32_t pf[NP][NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float base = m[n][j & 1] == -INFINITY ? 0.f : m[n][j & 1];
+          const float p = exp2_fast(sc[n][j] - base);
+          l[n][j & 1] += p;
+          w[j] = p * vsc;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t hi = pack_f16(w[2 * i], w[2 * i + 1]);
+          pf[0][n][i] = transpose8x8(hi);
+          if constexpr (F32) {
+            const float2 h = unpack_f16(hi);
+            pf[NP - 1][n][i] = transpose8x8(pack_f16(w[2 * i] - h.x, w[2 * i + 1] - h.y));
+          }
+        }
+      }
+      // output: this lane's dims KS g .. + KS and D / 2 + KS g .. of positions 2t, 2t + 1, 2t + 8, 2t + 9
+      constexpr int VB = KS < 4 ? KS : 4;  // dims a word carries
+      uint32_t vw[2][4][(KS + 3) / 4];     // [half of the dims][position]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+          const int byte = h * (D / 2) + KS * g;
+          const unsigned char *src = sv + v_place<D>(row, byte >> 4) + (byte & 15);
+          if constexpr (KS == 8) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(src);
+            vw[h][i][0] = v.x;
+            vw[h][i][1] = v.y;
+          } else if constexpr (KS == 4) {
+            vw[h][i][0] = *reinterpret_cast<const uint32_t *>(src);
+          } else if constexpr (KS == 2) {
+            vw[h][i][0] = *reinterpret_cast<const uint16_t *>(src);
+          } else {
+            vw[h][i][0] = *src;
+          }
+        }
+#pragma unroll
+      for (int c = 0; c < (KS + 3) / 4; ++c) {
+        uint32_t w[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[h][i] = vw[h][i][c] ^ 0x80808080u;
+#pragma unroll
+        for (int half = 0; half < (VB + 1) / 2; ++half) {
+          // pairs of positions (2t, 2t + 1) and (2t + 8, 2t + 9) of dims 2 half, 2 half + 1
+          uint32_t x[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[h][i] = __byte_perm(w[h][2 * i], w[h][2 * i + 1], half ? 0x7362 : 0x5140);
+#pragma unroll
+          for (int j = 0; j < (VB < 2 ? 1 : 2); ++j) {
+            uint32_t f[4];
+            const uint32_t sel = j ? 0x4342 : 0x4140;
+            f[0] = f16_codes(__byte_perm(x[0][0], 0x64646464u, sel));
+            f[1] = f16_codes(__byte_perm(x[1][0], 0x64646464u, sel));
+            f[2] = f16_codes(__byte_perm(x[0][1], 0x64646464u, sel));
+            f[3] = f16_codes(__byte_perm(x[1][1], 0x64646464u, sel));
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int p = 0; p < NP; ++p) mma16816(o[n][4 * c + 2 * half + j], f, pf[p][n][0], pf[p][n][1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    issue((slot + S - 1) % S);
+    slot = slot + 1 == S ? 0 : slot + 1;
+
+    // ---- end of the item, or of this block's share of it --------------------
+    if (cur.unit + 1 == q.nt || u + 1 == u1) {
+      const long long i0 = u - cur.unit, i1 = i0 + q.nt;
+      float *mine = merge + warp * ROWS * D;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float sum = l[n][j];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          const int r = 8 * n + 2 * t + j;
+          if (g == 0) {
+            s_m[warp][r] = m[n][j];
+            s_l[warp][r] = sum;
+          }
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            mine[r * D + KS * g + s] = o[n][s][j];
+            mine[r * D + D / 2 + KS * g + s] = o[n][s][j + 2];
+          }
+        }
+      __syncthreads();
+      const bool all = i0 >= u0 && i1 <= u1;
+      const long long c0 = i0 / share, c1 = (i1 - 1) / share;
+      float *part = a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart;
+      auto store = [&](int r, int d, float4 v, float lsum, float top) {
+        // row r of the tile, dims d .. d + 3
+        const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+        const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
+        XT *dst = static_cast<XT *>(a.out) + (q.r.q0 + i) * a.o_row + h * a.o_head + d;
+        dst[0] = from_f32<XT>(v.x * inv);
+        dst[1] = from_f32<XT>(v.y * inv);
+        dst[2] = from_f32<XT>(v.z * inv);
+        dst[3] = from_f32<XT>(v.w * inv);
+        if (a.lse && d == 0)
+          a.lse[static_cast<long long>(q.r.q0 + i) * a.g.H + h] = lsum > 0.f ? logf(lsum) + top * kLn2 : -INFINITY;
+      };
+      for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, s_m[w][r]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float lsum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) {
+          const float f = s_m[w][r] == -INFINITY ? 0.f : exp2_fast(s_m[w][r] - top);
+          const float4 x = *reinterpret_cast<const float4 *>(merge + (w * ROWS + r) * D + d);
+          lsum += s_l[w][r] * f;
+          v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+        }
+        if (all) {
+          store(r, d, v, lsum, top);
+        } else {
+          *reinterpret_cast<float4 *>(part + r * D + d) = v;
+          if (d == 0) {
+            part[ROWS * D + r] = top;
+            part[ROWS * D + ROWS + r] = lsum;
+          }
+        }
+      }
+      if (!all) {
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicAdd(a.ticket + c0, 1) == static_cast<int>(c1 - c0);
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float top = -INFINITY;
+            for (long long c = c0; c <= c1; ++c)
+              top = fmaxf(top, __ldcg(a.part + (2 * c + (c == c0)) * Geo::kPart + ROWS * D + r));
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float lsum = 0.f;
+            for (long long c = c0; c <= c1; ++c) {
+              const float *p = a.part + (2 * c + (c == c0)) * Geo::kPart;
+              const float pm = __ldcg(p + ROWS * D + r);
+              const float f = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
+              const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + r * D + d));
+              lsum += __ldcg(p + ROWS * D + ROWS + r) * f;
+              v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+            }
+            store(r, d, v, lsum, top);
+          }
+          if (threadIdx.x == 0) a.ticket[c0] = 0;
+        }
+      }
+      __syncthreads();
+      fresh = true;
+    }
+    cur.next(a, pre);
+  }
+  cp_wait<0>();
+}
+
+template <int D, int NT>
+constexpr int dec_smem_bytes(int B) {
+  return DecGeom<D, NT>::kRing + DecGeom<D, NT>::kMerge + (B + 1) * static_cast<int>(sizeof(long long));
+}
+
+template <typename XT, int D, int NT>
+void dec_launch(const specdec_kv8 *h, const AttendArgs &a, cudaStream_t st) {
+  // at most one item per row and kv head, at least one unit per block
+  const long long units = static_cast<long long>(a.b.T) * h->g.Hkv * ((static_cast<long long>(a.b.cols) * h->g.P + kUnit - 1) / kUnit);
+  const int grid = static_cast<int>(std::min(units, static_cast<long long>(kDecCtas) * h->num_sms));
+  op_launch("specdec_kv8_attend", kv8_decode_kernel<XT, D, NT>, dim3(grid), kDecThreads, dec_smem_bytes<D, NT>(a.b.B),
+            st, 1, a);
+}
+
+template <typename XT, int NT>
+void dec_launch_dim(const specdec_kv8 *h, const AttendArgs &a, cudaStream_t st) {
+  switch (h->g.D) {
+    case 16: return dec_launch<XT, 16, NT>(h, a, st);
+    case 32: return dec_launch<XT, 32, NT>(h, a, st);
+    case 64: return dec_launch<XT, 64, NT>(h, a, st);
+    default: return dec_launch<XT, 128, NT>(h, a, st);
+  }
+}
+
+template <typename XT, int NT>
+void dec_attrs(int max_batch) {
+  auto set = [](auto kernel, int bytes) {
+    op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  };
+  set(kv8_decode_kernel<XT, 16, NT>, dec_smem_bytes<16, NT>(max_batch));
+  set(kv8_decode_kernel<XT, 32, NT>, dec_smem_bytes<32, NT>(max_batch));
+  set(kv8_decode_kernel<XT, 64, NT>, dec_smem_bytes<64, NT>(max_batch));
+  set(kv8_decode_kernel<XT, 128, NT>, dec_smem_bytes<128, NT>(max_batch));
 }
 
 }  // namespace
 
-void kv8_attn_create(specdec_kv8 *) {}
-void kv8_attn_destroy(specdec_kv8 *) {}
+void kv8_attn_create(specdec_kv8 *h) {
+  dec_attrs<float, 1>(kKv8MaxBatch);
+  dec_attrs<float, 2>(kKv8MaxBatch);
+  dec_attrs<__nv_bfloat16, 1>(kKv8MaxBatch);
+  dec_attrs<__nv_bfloat16, 2>(kKv8MaxBatch);
+  const size_t blocks = static_cast<size_t>(kDecCtas) * h->num_sms;
+  const size_t part = blocks * 2 * (16 * h->g.D + 32) * sizeof(float);
+  op_cuda(cudaMalloc(&h->part, part), "cudaMalloc");
+  const cudaError_t e = cudaMalloc(&h->ticket, blocks * sizeof(int));
+  if (e != cudaSuccess) {
+    kv8_attn_destroy(h);
+    op_cuda(e, "cudaMalloc");
+  }
+  const cudaError_t z = cudaMemset(h->ticket, 0, blocks * sizeof(int));
+  if (z != cudaSuccess) {
+    kv8_attn_destroy(h);
+    op_cuda(z, "cudaMemset");
+  }
+}
+
+void kv8_attn_destroy(specdec_kv8 *h) {
+  if (h->part) cudaFree(h->part);
+  if (h->ticket) cudaFree(h->ticket);
+  h->part = nullptr;
+  h->ticket = nullptr;
+}
 
 }  // namespace specdec
 
@@ -93,13 +654,14 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
     if (b.B == 0 || b.T == 0) return;
     op_check(q && out, "null row buffer");
     DeviceScope scope(h->device);
-    const AttendArgs a{h->g, c, b, q, q_row_stride, q_head_stride, out, out_row_stride, out_head_stride, lse, scale, window};
-    const long long warps = static_cast<long long>(b.T) * h->g.H;
-    const int grid = static_cast<int>(std::min((warps + 3) / 4, 16ll * h->num_sms));
+    const AttendArgs a{h->g, c,   b,     q,      q_row_stride, q_head_stride, out, out_row_stride, out_head_stride,
+                       lse,  scale, window, h->part, h->ticket};
     const auto st = static_cast<cudaStream_t>(stream);
+    // rows of one kv head: one column tile of 8 where they fit, else two
+    const bool one = static_cast<long long>(max_q) * h->g.G <= 8;
     if (dtype == SPECDEC_F32)
-      op_launch("specdec_kv8_attend", kv8_attend_simple_kernel<float>, dim3(grid), 128, 0, st, 1, a);
+      one ? dec_launch_dim<float, 1>(h, a, st) : dec_launch_dim<float, 2>(h, a, st);
     else
-      op_launch("specdec_kv8_attend", kv8_attend_simple_kernel<__nv_bfloat16>, dim3(grid), 128, 0, st, 1, a);
+      one ? dec_launch_dim<__nv_bfloat16, 1>(h, a, st) : dec_launch_dim<__nv_bfloat16, 2>(h, a, st);
   });
 }
