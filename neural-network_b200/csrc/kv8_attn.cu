@@ -2,21 +2,24 @@
 //
 // Per query row and head: s_j = scale sk(j) (q . ck_j), p_j = exp(s_j - m),
 // out = sum p_j sv(j) cv_j / sum p_j, with one scale pair per block of
-// positions.  Codes are whole numbers up to 127, exact in f16, so both
-// products run on the tensor cores over the codes themselves and the scales
-// enter the scores and the weights.
+// positions.  Both products run on the tensor cores over the codes
+// themselves (whole numbers up to 127, exact in f16 too) and the scales enter
+// the scores and the weights.
 //
 // Few rows per kv head (decode steps, verify blocks): kv8_decode_kernel.  The
 // cache is read once and every byte meets at most 16 rows, so HBM bounds it.
 // The cache is the products' A operand (16 positions or 16 dims a tile), the
 // rows are their N side (8 or 16 columns), which wastes nothing of the tensor
 // cores that a 128-row tile would need:
-//   S^T [16 positions][8 rows]  = K codes [16][D] x Q^T
-//   O^T [16 dims][8 rows]      += V^T codes [16 dims][16 positions] x P^T
+//   S^T [16 positions][8 rows]  = K codes [16][D] x Q^T      8-bit products
+//   O^T [16 dims][8 rows]      += V^T codes [16 dims][16 positions] x P^T   f16
+// The queries enter as whole numbers of three bytes (22 bits of the row's
+// largest value), so the K codes need no conversion and the scores' sums are
+// exact; the weights span too many binades for that and enter as f16.
 // A slice of 16 positions lies in one page and has one scale pair.  Every
 // warp owns whole slices and a ring of them in shared memory that it fills
 // itself with 16-byte asynchronous copies (no barrier between warps until the
-// end of an item), converts codes to f16 in registers, and keeps its running
+// end of an item), converts V codes to f16 in registers, and keeps its running
 // maximum, sum and output; the block's warps take slices in turn and merge at
 // the end of a (request, kv head, row tile) item.
 //
@@ -48,13 +51,15 @@ struct AttendArgs {
   int window;
   float *part;
   int *ticket;
+  int p_shift, t_shift;  // log2 of page and block positions
+  int q_vec;             // query rows start at 4-element boundaries
 };
 
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kSlice = 16;                       // positions of a slice
 constexpr int kUnit = kSlice * kDecWarps;        // positions of a unit: one slice a warp
-constexpr int kDecCtas = 2;                      // blocks per SM
+constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: registers
 constexpr int kMinShare = 4;                     // units: a smaller share costs more in merging than it saves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -65,8 +70,9 @@ struct DecGeom {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSliceBytes = kSlice * D;            // K or V codes of a slice
   static constexpr int kSlot = 2 * kSliceBytes + 16;        // + the two scales and the page's validity
-  // 5 slots of 4 KB a warp at D = 128: 64 KB in flight per block, 128 KB per SM; smaller rows take 8 slots
-  static constexpr int kStages = D == 128 ? (NT == 1 ? 5 : 4) : 8;
+  // slots of 4 KB a warp at D = 128, one in use and the others in flight: 96 KB in flight per SM; smaller rows
+  // take more slots
+  static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : 4) : (D == 64 ? 6 : 8);
   static constexpr int kRing = kDecWarps * kStages * kSlot;
   static constexpr int kMerge = kDecWarps * kRows * D * 4;  // per warp the unnormalised output
   static constexpr int kPart = kRows * D + 2 * kRows;       // floats of a partial result
@@ -100,6 +106,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // Transpose of an 8 x 8 matrix of 16-bit values spread over the warp.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -112,12 +125,6 @@ __device__ __forceinline__ uint32_t f16_codes(uint32_t biased) {
   __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&biased), __half2half2(__ushort_as_half(0x6480)));
   return *reinterpret_cast<uint32_t *>(&h);
 }
-// Two f16 pairs of the four codes of a word (already ^ 0x80808080).
-__device__ __forceinline__ void codes4(uint32_t x, uint32_t &lo, uint32_t &hi) {
-  lo = f16_codes(__byte_perm(x, 0x64646464u, 0x4140));
-  hi = f16_codes(__byte_perm(x, 0x64646464u, 0x4342));
-}
-
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
@@ -128,6 +135,29 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2
 // by lanes (row g, chunk t and, for 128-byte rows, 4 + t): odd rows swap their
 // halves.  V rows are read 8 lanes along a row and 4 rows (2t) at once: the
 // rows' chunks are spread over the banks.
+// Four adjacent values (vec: at a 4-element boundary), zeros unless live.
+__device__ __forceinline__ void load4(const float *p, bool vec, bool live, float (&x)[4]) {
+  if (vec) {
+    const float4 v = live ? *reinterpret_cast<const float4 *>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = live ? p[j] : 0.f;
+  }
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16 *p, bool vec, bool live, float (&x)[4]) {
+  if (vec) {
+    const uint2 v = live ? *reinterpret_cast<const uint2 *>(p) : make_uint2(0, 0);
+    x[0] = __uint_as_float(v.x << 16);
+    x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16);
+    x[3] = __uint_as_float(v.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = live ? to_f32(p[j]) : 0.f;
+  }
+}
+
 template <int D>
 __device__ __forceinline__ int k_place(int row, int chunk) {
   return row * D + 16 * (D == 128 ? chunk ^ ((row & 1) << 2) : chunk);
@@ -159,22 +189,26 @@ __device__ __forceinline__ DecReq dec_req(const AttendArgs &a, int b) {
   return q;
 }
 
-// Walks consecutive units: request, item of the request, unit of the item.
+// Walks consecutive units: request, kv head, row tile, unit of the item.
 template <int ROWS>
 struct Cursor {
   DecReq q;
-  int item, unit;
+  int h, tile, unit;
   __device__ __forceinline__ void seek(const AttendArgs &a, const long long *pre, long long u) {
     q = dec_req<ROWS>(a, request_of(pre, a.b.B, u));
     const long long in = u - pre[q.b];
-    item = static_cast<int>(in / q.nt);
+    const int item = static_cast<int>(in / q.nt);
     unit = static_cast<int>(in % q.nt);
+    h = item / q.nr;
+    tile = item % q.nr;
   }
-  __device__ __forceinline__ void next(const AttendArgs &a, const long long *pre) {
-    if (++unit < q.nt) return;
+  // the next item (the caller counts units)
+  __device__ __forceinline__ void next_item(const AttendArgs &a, const long long *pre) {
     unit = 0;
-    if (++item < q.nr * a.g.Hkv) return;
-    item = 0;
+    if (++tile < q.nr) return;
+    tile = 0;
+    if (++h < a.g.Hkv) return;
+    h = 0;
     int b = q.b + 1;
     while (b < a.b.B && pre[b + 1] == pre[b]) ++b;
     if (b < a.b.B) q = dec_req<ROWS>(a, b);
@@ -182,11 +216,13 @@ struct Cursor {
 };
 
 template <typename XT, int D, int NT>
-__global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(const __grid_constant__ AttendArgs a) {
   using Geo = DecGeom<D, NT>;
   constexpr int ROWS = Geo::kRows, S = Geo::kStages;
   constexpr int KS = D / 16;       // products of 16 dims per score tile, and 16-dim tiles of the output
-  constexpr bool F32 = sizeof(XT) == 4;  // queries and weights as two f16 each: 22 bits
+  constexpr int KW = D / 16;       // words of codes a lane reads of a K row
+  constexpr int KM = (KW + 1) / 2; // products of 32 dims per score tile
+  constexpr bool F32 = sizeof(XT) == 4;  // weights as two f16 each: 22 bits
   constexpr int NP = F32 ? 2 : 1;
   extern __shared__ __align__(16) unsigned char dec_smem[];
   unsigned char *ring = dec_smem;
@@ -196,7 +232,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
   __shared__ float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS];
   __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int G = a.g.G, Hkv = a.g.Hkv, P = a.g.P;
+  const int G = a.g.G, Hkv = a.g.Hkv;
 
   request_prefix(a.b.B, pre, red, [&](int b) {
     const DecReq q = dec_req<ROWS>(a, b);
@@ -204,101 +240,120 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
   });
   const long long total = pre[a.b.B];
   const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinShare));
-  const long long u0 = share * blockIdx.x, u1 = min(total, u0 + share);
-  if (u0 >= u1) return;
+  const long long u0 = share * blockIdx.x;
+  if (u0 >= total) return;
+  const int n_units = static_cast<int>(min(total - u0, share));
 
   // ---- this warp's ring -------------------------------------------------
   unsigned char *my_ring = ring + warp * S * Geo::kSlot;
   Cursor<ROWS> load;
   load.seek(a, pre, u0);
-  long long lu = u0;  // next unit to load
-  auto page_of = [&](const Cursor<ROWS> &c) {
-    const int p = (c.q.t0 + c.unit) * kUnit + warp * kSlice;
-    return p < c.q.r.len ? a.b.table[static_cast<long long>(c.q.b) * a.b.cols + p / P] : -1;
-  };
-  int page = page_of(load);
-  auto issue = [&](int slot) {
-    if (lu < u1) {
-      unsigned char *dst = my_ring + slot * Geo::kSlot;
+  int to_load = n_units;                                     // units not yet asked for
+  int l_left = load.q.nt - load.unit;                        // units of the load cursor's item from here on
+  int l_pos = (load.q.t0 + load.unit) * kUnit + warp * kSlice;  // this warp's slice of that unit
+  const int32_t *l_table = a.b.table + static_cast<long long>(load.q.b) * a.b.cols;
+  int page = l_pos < load.q.r.len ? l_table[l_pos >> a.p_shift] : -1;
+  auto issue = [&](unsigned char *dst) {
+    if (to_load > 0) {
       const bool ok = page >= 0 && page < a.c.n_pages;
       if (ok) {
-        const int p = (load.q.t0 + load.unit) * kUnit + warp * kSlice;
-        const long long ph = static_cast<long long>(page) * Hkv + load.item / load.q.nr;
-        const long long at = (ph * P + p % P) * D;
+        const int in = l_pos & ((1 << a.p_shift) - 1);
+        const long long ph = static_cast<long long>(page) * Hkv + load.h;
+        const long long at = ((ph << a.p_shift) + in) * D + 16 * lane;
+        const int8_t *ksrc = a.c.k + at, *vsrc = a.c.v + at;
         const uint32_t d0 = shared_addr(dst);
 #pragma unroll
         for (int i = 0; i < (kSlice * D / 16 + 31) / 32; ++i) {
           const int c = lane + 32 * i;
           if (kSlice * D / 16 % 32 == 0 || c < kSlice * D / 16) {
             const int row = c / (D / 16), ch = c % (D / 16);
-            cp_async16(d0 + k_place<D>(row, ch), a.c.k + at + 16 * c);
-            cp_async16(d0 + Geo::kSliceBytes + v_place<D>(row, ch), a.c.v + at + 16 * c);
+            cp_async16(d0 + k_place<D>(row, ch), ksrc + 512 * i);
+            cp_async16(d0 + Geo::kSliceBytes + v_place<D>(row, ch), vsrc + 512 * i);
           }
         }
-        const long long sat = ph * (P / a.g.t) + p % P / a.g.t;
+        const long long sat = (ph << (a.p_shift - a.t_shift)) + (in >> a.t_shift);
         if (lane < 2) cp_async4(d0 + 2 * Geo::kSliceBytes + 4 * lane, (lane ? a.c.vs : a.c.ks) + sat);
       }
       if (lane == 2) *reinterpret_cast<int *>(dst + 2 * Geo::kSliceBytes + 8) = ok;
-      load.next(a, pre);
-      if (++lu < u1) page = page_of(load);
+      l_pos += kUnit;
+      if (--l_left == 0) {
+        load.next_item(a, pre);
+        l_left = load.q.nt;
+        l_pos = load.q.t0 * kUnit + warp * kSlice;
+        l_table = a.b.table + static_cast<long long>(load.q.b) * a.b.cols;
+      }
+      if (--to_load > 0) page = l_pos < load.q.r.len ? l_table[l_pos >> a.p_shift] : -1;
     }
     cp_commit();
   };
 #pragma unroll
-  for (int i = 0; i < S - 1; ++i) issue(i);
+  for (int i = 0; i < S - 1; ++i) issue(my_ring + i * Geo::kSlot);
 
   Cursor<ROWS> cur;
   cur.seek(a, pre, u0);
   bool fresh = true;
-  uint32_t qf[NP][NT][KS][2];
+  int qf[3][NT][KW];  // queries as whole numbers of 24 bits, three bytes each
   float o[NT][KS][4], m[NT][2], l[NT][2], cs[NT][2];
   int lim[NT][2];   // last visible position of this lane's two columns (-1: none)
-  int min_lim = 0, max_lim = 0;
+  int min_lim = 0, max_lim = 0, row0 = 0, n_rows = 0;
   int slot = 0;
-  for (long long u = u0; u < u1; ++u) {
+  for (int n_left = n_units; n_left > 0; --n_left) {
     const DecReq &q = cur.q;
-    const int hk = cur.item / q.nr, row0 = cur.item % q.nr * ROWS;
-    const int n_rows = min(ROWS, q.r.q * G - row0);
+    const int hk = cur.h;
     if (fresh) {
       // ---- the item's queries, scaled by a power of two to at most 1..2 ----
       fresh = false;
-      min_lim = 0x7fffffff;
-      max_lim = -1;
+      row0 = cur.tile * ROWS;
+      n_rows = min(ROWS, q.r.q * G - row0);
+      min_lim = q.r.len - q.r.q + row0 / G;
+      max_lim = q.r.len - q.r.q + (row0 + n_rows - 1) / G;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int r = row0 + 8 * n + g;
         const bool live = 8 * n + g < n_rows;
         const long long at = live ? (q.r.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head : 0;
         const XT *src = static_cast<const XT *>(a.q) + at;
-        float x[KS][4], big = 0.f;
+        float x[KW][4], big = 0.f, bad = 0.f;  // bad: 0, or a NaN where the row has a value that is not finite
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
+        for (int s = 0; s < KW; ++s) {
           const int d = D == 128 ? (s < 4 ? 16 * t + 4 * s : 64 + 16 * t + 4 * (s - 4)) : t * (D / 4) + 4 * s;
+          load4(src + d, a.q_vec, live, x[s]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            x[s][j] = live ? to_f32(src[d + j]) : 0.f;
             big = fmaxf(big, fabsf(x[s][j]));
+            bad += x[s][j] * 0.f;
           }
         }
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        // 2^e <= big < 2^(e + 1); rows below 2^-100 count as 2^-100
+#pragma unroll
+        for (int i = 1; i <= 2; i <<= 1) {
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, i));
+          bad += __shfl_xor_sync(0xffffffffu, bad, i);
+        }
+        // 2^e <= big < 2^(e + 1); rows below 2^-100 count as 2^-100.  x 2^(21 - e) is rounded to a whole number
+        // of at most 2^22: 22 bits of the row's largest value
         const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
-        const float down = __uint_as_float((127 - e) << 23), up = __uint_as_float((127 + e) << 23);
+        const float down = __uint_as_float((127 - e) << 23), up = __uint_as_float((127 + e) << 23) + bad;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KW; ++s) {
+          int w[3] = {0, 0, 0};
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float x0 = x[s][2 * j] * down, x1 = x[s][2 * j + 1] * down;
-            qf[0][n][s][j] = pack_f16(x0, x1);
-            if constexpr (F32) {
-              const float2 h = unpack_f16(qf[0][n][s][j]);
-              qf[NP - 1][n][s][j] = pack_f16(x0 - h.x, x1 - h.y);
-            }
+          for (int j = 0; j < 4; ++j) {
+            int v = __float2int_rn(x[s][j] * down * 2097152.f);
+            const int c0 = static_cast<int8_t>(v & 255);
+            v = (v - c0) >> 8;
+            const int c1 = static_cast<int8_t>(v & 255);
+            v = (v - c1) >> 8;
+            w[0] |= (c0 & 255) << (8 * j);
+            w[1] |= (c1 & 255) << (8 * j);
+            w[2] |= (v & 255) << (8 * j);
           }
+          qf[0][n][s] = w[0];
+          qf[1][n][s] = w[1];
+          qf[2][n][s] = w[2];
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
-          cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e);
+          cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e * (1.f / 2097152.f));
           const int rr = 8 * n + 2 * t + j;
           lim[n][j] = rr < n_rows ? q.r.len - q.r.q + (row0 + rr) / G : -1;
           m[n][j] = -INFINITY;
@@ -309,8 +364,6 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[n][s][j] = 0.f;
       }
-      min_lim = q.r.len - q.r.q + row0 / G;
-      max_lim = q.r.len - q.r.q + (row0 + n_rows - 1) / G;
     }
 
     // ---- one slice ----------------------------------------------------------
@@ -318,17 +371,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
     __syncwarp();
     const unsigned char *sk = my_ring + slot * Geo::kSlot, *sv = sk + Geo::kSliceBytes;
     const int p0 = (q.t0 + cur.unit) * kUnit + warp * kSlice;
-    const bool ok = *reinterpret_cast<const int *>(sk + 2 * Geo::kSliceBytes + 8) != 0;
-    if (ok && p0 <= max_lim && (a.window <= 0 || p0 + kSlice - 1 > min_lim - a.window)) {
-      const float ksc = *reinterpret_cast<const float *>(sk + 2 * Geo::kSliceBytes);
-      const float vsc = *reinterpret_cast<const float *>(sk + 2 * Geo::kSliceBytes + 4);
-      float sc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sc[n][j] = 0.f;
-      // scores: rows g and g + 8 of the slice, this lane's dims
-      uint32_t kw[2][KS];
+    const float4 tail = *reinterpret_cast<const float4 *>(sk + 2 * Geo::kSliceBytes);
+    if (__float_as_int(tail.z) && p0 <= max_lim && (a.window <= 0 || p0 + kSlice - 1 > min_lim - a.window)) {
+      const float ksc = tail.x, vsc = tail.y;
+      // scores: rows g and g + 8 of the slice, this lane's dims; exact whole numbers
+      uint32_t kw[2][KW + 1];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = g + 8 * i;
@@ -347,16 +394,24 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
         } else {
           kw[i][0] = *reinterpret_cast<const uint32_t *>(sk + row * D + 4 * t);
         }
+        kw[i][KW] = 0;
       }
+      float sc[NT][4];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        uint32_t f[4];
-        codes4(kw[0][s] ^ 0x80808080u, f[0], f[2]);
-        codes4(kw[1][s] ^ 0x80808080u, f[1], f[3]);
+      for (int n = 0; n < NT; ++n) {
+        int d[3][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int p = 0; p < 3; ++p) {
 #pragma unroll
-          for (int p = 0; p < NP; ++p) mma16816(sc[n], f, qf[p][n][s][0], qf[p][n][s][1]);
+          for (int j = 0; j < 4; ++j) d[p][j] = 0;
+#pragma unroll
+          for (int s = 0; s < KM; ++s)
+            mma16832(d[p], kw[0][2 * s], kw[1][2 * s], kw[0][2 * s + 1], kw[1][2 * s + 1], qf[p][n][2 * s],
+                     2 * s + 1 < KW ? qf[p][n][2 * s + 1 < KW ? 2 * s + 1 : 0] : 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sc[n][j] = fmaf(static_cast<float>((d[2][j] << 8) + d[1][j]), 256.f, static_cast<float>(d[0][j]));
       }
       // softmax: this lane has positions p0 + g, p0 + g + 8 for columns 2t, 2t + 1
       const bool whole = p0 + kSlice - 1 <= min_lim && (a.window <= 0 || p0 > max_lim - a.window);
@@ -472,12 +527,13 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
       }
     }
     __syncwarp();
-    issue((slot + S - 1) % S);
+    issue(my_ring + (slot == 0 ? S - 1 : slot - 1) * Geo::kSlot);
     slot = slot + 1 == S ? 0 : slot + 1;
+    ++cur.unit;
 
     // ---- end of the item, or of this block's share of it --------------------
-    if (cur.unit + 1 == q.nt || u + 1 == u1) {
-      const long long i0 = u - cur.unit, i1 = i0 + q.nt;
+    if (cur.unit == q.nt || n_left == 1) {
+      const long long i0 = u0 + (n_units - n_left) + 1 - cur.unit, i1 = i0 + q.nt;
       float *mine = merge + warp * ROWS * D;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -498,12 +554,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
           }
         }
       __syncthreads();
-      const bool all = i0 >= u0 && i1 <= u1;
+      const bool all = i0 >= u0 && i1 <= u0 + n_units;
       const long long c0 = i0 / share, c1 = (i1 - 1) / share;
       float *part = a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart;
       auto store = [&](int r, int d, float4 v, float lsum, float top) {
         // row r of the tile, dims d .. d + 3
-        const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // 0: the row saw nothing
         const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
         XT *dst = static_cast<XT *>(a.out) + (q.r.q0 + i) * a.o_row + h * a.o_head + d;
         dst[0] = from_f32<XT>(v.x * inv);
@@ -511,7 +567,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
         dst[2] = from_f32<XT>(v.z * inv);
         dst[3] = from_f32<XT>(v.w * inv);
         if (a.lse && d == 0)
-          a.lse[static_cast<long long>(q.r.q0 + i) * a.g.H + h] = lsum > 0.f ? logf(lsum) + top * kLn2 : -INFINITY;
+          a.lse[static_cast<long long>(q.r.q0 + i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
       };
       for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
@@ -566,8 +622,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) kv8_decode_kernel(const
       }
       __syncthreads();
       fresh = true;
+      cur.next_item(a, pre);
     }
-    cur.next(a, pre);
   }
   cp_wait<0>();
 }
@@ -581,7 +637,7 @@ template <typename XT, int D, int NT>
 void dec_launch(const specdec_kv8 *h, const AttendArgs &a, cudaStream_t st) {
   // at most one item per row and kv head, at least one unit per block
   const long long units = static_cast<long long>(a.b.T) * h->g.Hkv * ((static_cast<long long>(a.b.cols) * h->g.P + kUnit - 1) / kUnit);
-  const int grid = static_cast<int>(std::min(units, static_cast<long long>(kDecCtas) * h->num_sms));
+  const int grid = static_cast<int>(std::min(units, static_cast<long long>(dec_ctas(NT)) * h->num_sms));
   op_launch("specdec_kv8_attend", kv8_decode_kernel<XT, D, NT>, dim3(grid), kDecThreads, dec_smem_bytes<D, NT>(a.b.B),
             st, 1, a);
 }
@@ -607,6 +663,17 @@ void dec_attrs(int max_batch) {
   set(kv8_decode_kernel<XT, 128, NT>, dec_smem_bytes<128, NT>(max_batch));
 }
 
+int log2i(int v) {
+  int n = 0;
+  while (v > 1 << n) ++n;
+  return n;
+}
+// Whether every row and head starts at a boundary of four elements.
+bool rows_aligned(const void *p, int64_t row, int64_t head, int dtype) {
+  const uintptr_t size = dtype == SPECDEC_F32 ? 16 : 8;
+  return reinterpret_cast<uintptr_t>(p) % size == 0 && row % 4 == 0 && head % 4 == 0;
+}
+
 }  // namespace
 
 void kv8_attn_create(specdec_kv8 *h) {
@@ -614,7 +681,7 @@ void kv8_attn_create(specdec_kv8 *h) {
   dec_attrs<float, 2>(kKv8MaxBatch);
   dec_attrs<__nv_bfloat16, 1>(kKv8MaxBatch);
   dec_attrs<__nv_bfloat16, 2>(kKv8MaxBatch);
-  const size_t blocks = static_cast<size_t>(kDecCtas) * h->num_sms;
+  const size_t blocks = static_cast<size_t>(dec_ctas(1)) * h->num_sms;
   const size_t part = blocks * 2 * (16 * h->g.D + 32) * sizeof(float);
   op_cuda(cudaMalloc(&h->part, part), "cudaMalloc");
   const cudaError_t e = cudaMalloc(&h->ticket, blocks * sizeof(int));
@@ -655,7 +722,8 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
     op_check(q && out, "null row buffer");
     DeviceScope scope(h->device);
     const AttendArgs a{h->g, c,   b,     q,      q_row_stride, q_head_stride, out, out_row_stride, out_head_stride,
-                       lse,  scale, window, h->part, h->ticket};
+                       lse,  scale, window, h->part, h->ticket, log2i(h->g.P), log2i(h->g.t),
+                       rows_aligned(q, q_row_stride, q_head_stride, dtype)};
     const auto st = static_cast<cudaStream_t>(stream);
     // rows of one kv head: one column tile of 8 where they fit, else two
     const bool one = static_cast<long long>(max_q) * h->g.G <= 8;
