@@ -63,17 +63,19 @@ constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: re
 constexpr int kMinShare = 4;                     // units: a smaller share costs more in merging than it saves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNone = -1e30f;                  // the running maximum before anything was seen
 constexpr float kLazy = 8.f;                     // weights may grow to 2^8 before the maximum is moved
 
 template <int D, int NT>
 struct DecGeom {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSliceBytes = kSlice * D;            // K or V codes of a slice
-  static constexpr int kSlot = 2 * kSliceBytes + 16;        // + the two scales and the page's validity
+  static constexpr int kSlot = 2 * kSliceBytes;             // a multiple of 128: places within a row are XORed into addresses
+  static constexpr int kTail = 16;                          // per slot: the two scales, whether the page is there
   // slots of 4 KB a warp at D = 128, one in use and the others in flight: 96 KB in flight per SM; smaller rows
   // take more slots
   static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : 4) : (D == 64 ? 6 : 8);
-  static constexpr int kRing = kDecWarps * kStages * kSlot;
+  static constexpr int kRing = kDecWarps * kStages * (kSlot + kTail);
   static constexpr int kMerge = kDecWarps * kRows * D * 4;  // per warp the unnormalised output
   static constexpr int kPart = kRows * D + 2 * kRows;       // floats of a partial result
 };
@@ -105,6 +107,41 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       "%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+// d = a b, and d += a b
+__device__ __forceinline__ void mma16832_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, "
+      "%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -224,7 +261,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   constexpr int KM = (KW + 1) / 2; // products of 32 dims per score tile
   constexpr bool F32 = sizeof(XT) == 4;  // weights as two f16 each: 22 bits
   constexpr int NP = F32 ? 2 : 1;
-  extern __shared__ __align__(16) unsigned char dec_smem[];
+  extern __shared__ __align__(128) unsigned char dec_smem[];
   unsigned char *ring = dec_smem;
   float *merge = reinterpret_cast<float *>(dec_smem + Geo::kRing);
   long long *pre = reinterpret_cast<long long *>(dec_smem + Geo::kRing + Geo::kMerge);
@@ -245,7 +282,17 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   const int n_units = static_cast<int>(min(total - u0, share));
 
   // ---- this warp's ring -------------------------------------------------
-  unsigned char *my_ring = ring + warp * S * Geo::kSlot;
+  const uint32_t my_ring = shared_addr(ring) + warp * S * Geo::kSlot;
+  const uint32_t my_tails = shared_addr(ring) + kDecWarps * S * Geo::kSlot + warp * S * Geo::kTail;
+  auto tail_of = [&](uint32_t slot) { return my_tails + (slot - my_ring) / (Geo::kSlot / Geo::kTail); };
+  constexpr int kCopies = (kSlice * D / 16 + 31) / 32;  // 16-byte copies of a lane for K, and for V
+  uint32_t k_to[kCopies], v_to[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int c = lane + 32 * i;
+    k_to[i] = k_place<D>(c / (D / 16), c % (D / 16));
+    v_to[i] = Geo::kSliceBytes + v_place<D>(c / (D / 16), c % (D / 16));
+  }
   Cursor<ROWS> load;
   load.seek(a, pre, u0);
   int to_load = n_units;                                     // units not yet asked for
@@ -253,28 +300,26 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   int l_pos = (load.q.t0 + load.unit) * kUnit + warp * kSlice;  // this warp's slice of that unit
   const int32_t *l_table = a.b.table + static_cast<long long>(load.q.b) * a.b.cols;
   int page = l_pos < load.q.r.len ? l_table[l_pos >> a.p_shift] : -1;
-  auto issue = [&](unsigned char *dst) {
+  auto issue = [&](uint32_t dst) {
     if (to_load > 0) {
       const bool ok = page >= 0 && page < a.c.n_pages;
       if (ok) {
-        const int in = l_pos & ((1 << a.p_shift) - 1);
-        const long long ph = static_cast<long long>(page) * Hkv + load.h;
-        const long long at = ((ph << a.p_shift) + in) * D + 16 * lane;
+        const uint32_t in = l_pos & ((1u << a.p_shift) - 1);
+        const unsigned long long ph = static_cast<unsigned long long>(static_cast<unsigned>(page)) * static_cast<unsigned>(Hkv) + load.h;
+        const unsigned long long at = (ph << a.p_shift) * D + (in * D + 16 * lane);
         const int8_t *ksrc = a.c.k + at, *vsrc = a.c.v + at;
-        const uint32_t d0 = shared_addr(dst);
+        if (kSlice * D / 16 % 32 == 0 || lane < kSlice * D / 16) {
 #pragma unroll
-        for (int i = 0; i < (kSlice * D / 16 + 31) / 32; ++i) {
-          const int c = lane + 32 * i;
-          if (kSlice * D / 16 % 32 == 0 || c < kSlice * D / 16) {
-            const int row = c / (D / 16), ch = c % (D / 16);
-            cp_async16(d0 + k_place<D>(row, ch), ksrc + 512 * i);
-            cp_async16(d0 + Geo::kSliceBytes + v_place<D>(row, ch), vsrc + 512 * i);
+          for (int i = 0; i < kCopies; ++i) {
+            cp_async16(dst + k_to[i], ksrc + 512 * i);
+            cp_async16(dst + v_to[i], vsrc + 512 * i);
           }
         }
-        const long long sat = (ph << (a.p_shift - a.t_shift)) + (in >> a.t_shift);
-        if (lane < 2) cp_async4(d0 + 2 * Geo::kSliceBytes + 4 * lane, (lane ? a.c.vs : a.c.ks) + sat);
+        const unsigned long long sat = (ph << (a.p_shift - a.t_shift)) + (in >> a.t_shift);
+        if (lane < 2) cp_async4(tail_of(dst) + 4 * lane, (lane ? a.c.vs : a.c.ks) + sat);
       }
-      if (lane == 2) *reinterpret_cast<int *>(dst + 2 * Geo::kSliceBytes + 8) = ok;
+      if (lane == 2)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(tail_of(dst) + 8), "r"(ok ? 1 : 0) : "memory");
       l_pos += kUnit;
       if (--l_left == 0) {
         load.next_item(a, pre);
@@ -288,6 +333,9 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   };
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) issue(my_ring + i * Geo::kSlot);
+  uint32_t slot = my_ring;                             // the slot of the slice at hand
+  uint32_t free_slot = my_ring + (S - 1) * Geo::kSlot;  // the one used before it
+  const uint32_t ring_end = my_ring + S * Geo::kSlot;
 
   Cursor<ROWS> cur;
   cur.seek(a, pre, u0);
@@ -296,7 +344,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   float o[NT][KS][4], m[NT][2], l[NT][2], cs[NT][2];
   int lim[NT][2];   // last visible position of this lane's two columns (-1: none)
   int min_lim = 0, max_lim = 0, row0 = 0, n_rows = 0;
-  int slot = 0;
+  const uint32_t k_at = D == 128 || D == 64 ? k_place<D>(g, t) : g * D + (D / 4) * t;
+  const uint32_t v_at = Geo::kSliceBytes + v_place<D>(2 * t, (KS * g) >> 4) + ((KS * g) & 15);
   for (int n_left = n_units; n_left > 0; --n_left) {
     const DecReq &q = cur.q;
     const int hk = cur.h;
@@ -356,7 +405,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
           cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e * (1.f / 2097152.f));
           const int rr = 8 * n + 2 * t + j;
           lim[n][j] = rr < n_rows ? q.r.len - q.r.q + (row0 + rr) / G : -1;
-          m[n][j] = -INFINITY;
+          m[n][j] = kNone;
           l[n][j] = 0.f;
         }
 #pragma unroll
@@ -369,30 +418,27 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     // ---- one slice ----------------------------------------------------------
     cp_wait<S - 2>();
     __syncwarp();
-    const unsigned char *sk = my_ring + slot * Geo::kSlot, *sv = sk + Geo::kSliceBytes;
     const int p0 = (q.t0 + cur.unit) * kUnit + warp * kSlice;
-    const float4 tail = *reinterpret_cast<const float4 *>(sk + 2 * Geo::kSliceBytes);
-    if (__float_as_int(tail.z) && p0 <= max_lim && (a.window <= 0 || p0 + kSlice - 1 > min_lim - a.window)) {
-      const float ksc = tail.x, vsc = tail.y;
+    const uint4 tail = lds128(tail_of(slot));  // scales and whether the page is there
+    if (tail.z && p0 <= max_lim && (a.window <= 0 || p0 + kSlice - 1 > min_lim - a.window)) {
+      const float ksc = __uint_as_float(tail.x), vsc = __uint_as_float(tail.y);
       // scores: rows g and g + 8 of the slice, this lane's dims; exact whole numbers
       uint32_t kw[2][KW + 1];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int row = g + 8 * i;
+        const uint32_t at = slot + k_at + 8 * D * i;
         if constexpr (D == 128) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(sk + k_place<D>(row, t + 4 * h));
-            kw[i][4 * h] = w.x; kw[i][4 * h + 1] = w.y; kw[i][4 * h + 2] = w.z; kw[i][4 * h + 3] = w.w;
-          }
+          const uint4 w = lds128(at), x = lds128(at ^ 64);  // chunks t and t + 4
+          kw[i][0] = w.x; kw[i][1] = w.y; kw[i][2] = w.z; kw[i][3] = w.w;
+          kw[i][4] = x.x; kw[i][5] = x.y; kw[i][6] = x.z; kw[i][7] = x.w;
         } else if constexpr (D == 64) {
-          const uint4 w = *reinterpret_cast<const uint4 *>(sk + k_place<D>(row, t));
+          const uint4 w = lds128(at);
           kw[i][0] = w.x; kw[i][1] = w.y; kw[i][2] = w.z; kw[i][3] = w.w;
         } else if constexpr (D == 32) {
-          const uint2 w = *reinterpret_cast<const uint2 *>(sk + row * D + 8 * t);
+          const uint2 w = lds64(at);
           kw[i][0] = w.x; kw[i][1] = w.y;
         } else {
-          kw[i][0] = *reinterpret_cast<const uint32_t *>(sk + row * D + 4 * t);
+          kw[i][0] = lds32(at);
         }
         kw[i][KW] = 0;
       }
@@ -402,47 +448,50 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         int d[3][4];
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
+          mma16832_first(d[p], kw[0][0], kw[1][0], kw[0][1], kw[1][1], qf[p][n][0], KW > 1 ? qf[p][n][KW > 1] : 0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[p][j] = 0;
-#pragma unroll
-          for (int s = 0; s < KM; ++s)
-            mma16832(d[p], kw[0][2 * s], kw[1][2 * s], kw[0][2 * s + 1], kw[1][2 * s + 1], qf[p][n][2 * s],
-                     2 * s + 1 < KW ? qf[p][n][2 * s + 1 < KW ? 2 * s + 1 : 0] : 0);
+          for (int s = 1; s < KM; ++s)
+            mma16832(d[p], kw[0][2 * s], kw[1][2 * s], kw[0][2 * s + 1], kw[1][2 * s + 1], qf[p][n][2 * s], qf[p][n][2 * s + 1]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           sc[n][j] = fmaf(static_cast<float>((d[2][j] << 8) + d[1][j]), 256.f, static_cast<float>(d[0][j]));
       }
-      // softmax: this lane has positions p0 + g, p0 + g + 8 for columns 2t, 2t + 1
+      // softmax: this lane has positions p0 + g, p0 + g + 8 for columns 2t, 2t + 1.  Weights are held relative to the
+      // largest p x sv: the value scale's exponent ev joins the maximum
       const bool whole = p0 + kSlice - 1 <= min_lim && (a.window <= 0 || p0 > max_lim - a.window);
-      // exponent of the value scale: weights are held relative to the largest p x sv
-      const int ev = max(static_cast<int>(__float_as_uint(vsc) >> 23) - 127, -90);
-      const float fev = static_cast<float>(ev);
+      const int ev = max(static_cast<int>(tail.y >> 23) - 127, -90);
+      const float fev = static_cast<float>(ev), lazy = kLazy - fev;
+      if (!whole) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int first = a.window > 0 ? lim[n][j] - a.window : -1;
+            const float hidden = cs[n][j] * ksc < 0.f ? INFINITY : -INFINITY;  // -infinity after the scale
+            if (p0 + g > lim[n][j] || p0 + g <= first) sc[n][j] = hidden;
+            if (p0 + g + 8 > lim[n][j] || p0 + g + 8 <= first) sc[n][j + 2] = hidden;
+          }
+      }
+      float x[NT][4];
       bool grow = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float f = cs[n][j] * ksc;
-          sc[n][j] *= f;
-          sc[n][j + 2] *= f;
-          if (!whole) {
-            const int first = a.window > 0 ? lim[n][j] - a.window : -1;
-            if (p0 + g > lim[n][j] || p0 + g <= first) sc[n][j] = -INFINITY;
-            if (p0 + g + 8 > lim[n][j] || p0 + g + 8 <= first) sc[n][j + 2] = -INFINITY;
-          }
-          grow |= fmaxf(sc[n][j], sc[n][j + 2]) + fev > m[n][j] + kLazy;
-        }
+        for (int j = 0; j < 4; ++j) x[n][j] = fmaf(sc[n][j], cs[n][j & 1] * ksc, -m[n][j & 1]);
+        grow |= fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) > lazy;
+      }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(sc[n][j], sc[n][j + 2]);
+            const float f = cs[n][j] * ksc;
+            float top = fmaxf(sc[n][j] * f, sc[n][j + 2] * f);
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
             const float nm = fmaxf(m[n][j], top + fev);
-            const float al = m[n][j] == -INFINITY ? 0.f : exp2_fast(m[n][j] - nm);
+            const float al = exp2_fast(m[n][j] - nm);
             m[n][j] = nm;
             l[n][j] *= al;
 #pragma unroll
@@ -450,6 +499,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
               o[n][s][j] *= al;
               o[n][s][j + 2] *= al;
             }
+            x[n][j] = fmaf(sc[n][j], f, -nm);
+            x[n][j + 2] = fmaf(sc[n][j + 2], f, -nm);
           }
       }
       uint32_t pf[NP][NT][2];
@@ -458,8 +509,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float base = m[n][j & 1] == -INFINITY ? 0.f : m[n][j & 1];
-          const float p = exp2_fast(sc[n][j] - base);
+          const float p = exp2_fast(x[n][j]);
           l[n][j & 1] += p;
           w[j] = p * vsc;
         }
@@ -480,19 +530,19 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-          const int byte = h * (D / 2) + KS * g;
-          const unsigned char *src = sv + v_place<D>(row, byte >> 4) + (byte & 15);
+          // position 2t + (i & 1) + 8 (i >> 1); D = 64 and below keep odd positions 4 rows on
+          const uint32_t step = (i & 1) * (D == 128 ? D : 4 * D) + (i >> 1) * 8 * D;
+          const uint32_t at = (slot + v_at + step) ^ (h && D >= 64 ? D / 2 : 0);
           if constexpr (KS == 8) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(src);
+            const uint2 v = lds64(at);
             vw[h][i][0] = v.x;
             vw[h][i][1] = v.y;
           } else if constexpr (KS == 4) {
-            vw[h][i][0] = *reinterpret_cast<const uint32_t *>(src);
+            vw[h][i][0] = lds32(at);
           } else if constexpr (KS == 2) {
-            vw[h][i][0] = *reinterpret_cast<const uint16_t *>(src);
+            vw[h][i][0] = lds16(at + h * (D / 2));
           } else {
-            vw[h][i][0] = *src;
+            vw[h][i][0] = lds8(at + h * (D / 2));
           }
         }
 #pragma unroll
@@ -527,8 +577,10 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       }
     }
     __syncwarp();
-    issue(my_ring + (slot == 0 ? S - 1 : slot - 1) * Geo::kSlot);
-    slot = slot + 1 == S ? 0 : slot + 1;
+    issue(free_slot);
+    free_slot = slot;
+    slot += Geo::kSlot;
+    if (slot == ring_end) slot = my_ring;
     ++cur.unit;
 
     // ---- end of the item, or of this block's share of it --------------------
@@ -571,14 +623,14 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       };
       for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float top = -INFINITY;
+        float top = kNone;
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, s_m[w][r]);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float lsum = 0.f;
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) {
-          const float f = s_m[w][r] == -INFINITY ? 0.f : exp2_fast(s_m[w][r] - top);
+          const float f = exp2_fast(s_m[w][r] - top);
           const float4 x = *reinterpret_cast<const float4 *>(merge + (w * ROWS + r) * D + d);
           lsum += s_l[w][r] * f;
           v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
@@ -602,15 +654,14 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
           __threadfence();
           for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
-            float top = -INFINITY;
+            float top = kNone;
             for (long long c = c0; c <= c1; ++c)
               top = fmaxf(top, __ldcg(a.part + (2 * c + (c == c0)) * Geo::kPart + ROWS * D + r));
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             float lsum = 0.f;
             for (long long c = c0; c <= c1; ++c) {
               const float *p = a.part + (2 * c + (c == c0)) * Geo::kPart;
-              const float pm = __ldcg(p + ROWS * D + r);
-              const float f = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
+              const float f = exp2_fast(__ldcg(p + ROWS * D + r) - top);
               const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + r * D + d));
               lsum += __ldcg(p + ROWS * D + ROWS + r) * f;
               v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
