@@ -52,15 +52,17 @@ struct AttendArgs {
   float *part;
   int *ticket;
   int p_shift, t_shift;  // log2 of page and block positions
-  int q_vec;             // query rows start at 4-element boundaries
+  int q_vec, o_vec;      // query / output rows start at 4-element boundaries
 };
 
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
-constexpr int kSlice = 16;                       // positions of a slice
-constexpr int kUnit = kSlice * kDecWarps;        // positions of a unit: one slice a warp
+constexpr int kSlice = 16;                            // positions of a slice
+constexpr int kStep = 2;                              // slices a warp takes at a time
+constexpr int kUnit = kSlice * kStep * kDecWarps;     // positions of a unit
 constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: registers
-constexpr int kMinShare = 4;                     // units: a smaller share costs more in merging than it saves
+constexpr int kWholeItems = 4;                        // items of at most this many units are not split
+constexpr int kMergeAhead = 8;                        // partial results read at once
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNone = -1e30f;                  // the running maximum before anything was seen
@@ -70,14 +72,13 @@ template <int D, int NT>
 struct DecGeom {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSliceBytes = kSlice * D;            // K or V codes of a slice
-  static constexpr int kSlot = 2 * kSliceBytes;             // a multiple of 128: places within a row are XORed into addresses
-  static constexpr int kTail = 16;                          // per slot: the two scales, whether the page is there
-  // slots of 4 KB a warp at D = 128, one in use and the others in flight: 96 KB in flight per SM; smaller rows
-  // take more slots
-  static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : 4) : (D == 64 ? 6 : 8);
+  static constexpr int kSlot = 2 * kStep * kSliceBytes;     // a multiple of 128: places within a row are XORed into addresses
+  static constexpr int kTail = 16 * kStep;                  // per slice: the two scales, whether the page is there
+  // 8 KB a slot at D = 128: one in use and at least one in flight, 96 KB in flight per SM; small rows take more slots
+  static constexpr int kStages = D == 128 ? (NT == 1 ? 2 : 3) : (D == 64 ? 4 : 6);
   static constexpr int kRing = kDecWarps * kStages * (kSlot + kTail);
-  static constexpr int kMerge = kDecWarps * kRows * D * 4;  // per warp the unnormalised output
   static constexpr int kPart = kRows * D + 2 * kRows;       // floats of a partial result
+  static_assert(kRows * D * 4 <= kSlot, "a warp's output must fit the slot that it has just read");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
@@ -102,7 +103,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
       "%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -137,7 +138,7 @@ __device__ __forceinline__ uint32_t lds8(uint32_t addr) {
 // d = a b, and d += a b
 __device__ __forceinline__ void mma16832_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, "
       "%10};"
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
@@ -145,7 +146,7 @@ __device__ __forceinline__ void mma16832_first(int (&d)[4], uint32_t a0, uint32_
 }
 __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -195,6 +196,26 @@ __device__ __forceinline__ void load4(const __nv_bfloat16 *p, bool vec, bool liv
   }
 }
 
+__device__ __forceinline__ void store4(float *p, bool vec, float4 v) {
+  if (vec) {
+    *reinterpret_cast<float4 *>(p) = v;
+  } else {
+    p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w;
+  }
+}
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, bool vec, float4 v) {
+  if (vec) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2 *>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+  } else {
+    p[0] = from_f32<__nv_bfloat16>(v.x);
+    p[1] = from_f32<__nv_bfloat16>(v.y);
+    p[2] = from_f32<__nv_bfloat16>(v.z);
+    p[3] = from_f32<__nv_bfloat16>(v.w);
+  }
+}
+
 template <int D>
 __device__ __forceinline__ int k_place(int row, int chunk) {
   return row * D + 16 * (D == 128 ? chunk ^ ((row & 1) << 2) : chunk);
@@ -207,23 +228,40 @@ __device__ __forceinline__ int v_place(int row, int chunk) {
   return r * D + 16 * chunk;
 }
 
+// a / b where both mostly fit 32 bits.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// The batch in shared memory: per request its rows, its length and the units before it.
+struct DecBatch {
+  long long *pre;  // [B + 1]
+  int *q0, *q, *len;
+};
+
 // The request that a run of units belongs to.
 struct DecReq {
-  int b;
-  Kv8Req r;
+  int b, q0, q, len;
   int nr, nt, t0;  // row tiles, units of an item, first unit's index along the cache
 };
 
 template <int ROWS>
-__device__ __forceinline__ DecReq dec_req(const AttendArgs &a, int b) {
-  DecReq q;
-  q.b = b;
-  q.r = kv8_req(a.b, a.g.P, b);
-  q.nr = (q.r.q * a.g.G + ROWS - 1) / ROWS;
-  const int lo = a.window > 0 ? max(0, q.r.len - q.r.q - a.window + 1) : 0;
-  q.t0 = lo / kUnit;
-  q.nt = max(1, (q.r.len + kUnit - 1) / kUnit - q.t0);
-  return q;
+__device__ __forceinline__ void dec_shape(const AttendArgs &a, DecReq &r) {
+  r.nr = (r.q * a.g.G + ROWS - 1) / ROWS;
+  const int lo = a.window > 0 ? max(0, r.len - r.q - a.window + 1) : 0;
+  r.t0 = lo / kUnit;
+  r.nt = max(1, (r.len + kUnit - 1) / kUnit - r.t0);
+}
+template <int ROWS>
+__device__ __forceinline__ DecReq dec_req(const AttendArgs &a, const DecBatch &s, int b) {
+  DecReq r;
+  r.b = b;
+  r.q0 = s.q0[b];
+  r.q = s.q[b];
+  r.len = s.len[b];
+  dec_shape<ROWS>(a, r);
+  return r;
 }
 
 // Walks consecutive units: request, kv head, row tile, unit of the item.
@@ -231,26 +269,35 @@ template <int ROWS>
 struct Cursor {
   DecReq q;
   int h, tile, unit;
-  __device__ __forceinline__ void seek(const AttendArgs &a, const long long *pre, long long u) {
-    q = dec_req<ROWS>(a, request_of(pre, a.b.B, u));
-    const long long in = u - pre[q.b];
-    const int item = static_cast<int>(in / q.nt);
-    unit = static_cast<int>(in % q.nt);
+  __device__ __forceinline__ void seek(const AttendArgs &a, const DecBatch &s, long long u) {
+    q = dec_req<ROWS>(a, s, request_of(s.pre, a.b.B, u));
+    const long long in = u - s.pre[q.b];
+    const int item = static_cast<int>(quotient(in, q.nt));
+    unit = static_cast<int>(in - static_cast<long long>(item) * q.nt);
     h = item / q.nr;
-    tile = item % q.nr;
+    tile = item - h * q.nr;
   }
   // the next item (the caller counts units)
-  __device__ __forceinline__ void next_item(const AttendArgs &a, const long long *pre) {
+  __device__ __forceinline__ void next_item(const AttendArgs &a, const DecBatch &s) {
     unit = 0;
     if (++tile < q.nr) return;
     tile = 0;
     if (++h < a.g.Hkv) return;
     h = 0;
     int b = q.b + 1;
-    while (b < a.b.B && pre[b + 1] == pre[b]) ++b;
-    if (b < a.b.B) q = dec_req<ROWS>(a, b);
+    while (b < a.b.B && s.pre[b + 1] == s.pre[b]) ++b;
+    if (b < a.b.B) q = dec_req<ROWS>(a, s, b);
   }
 };
+
+// Place of four adjacent outputs in a warp's merge area, spread over the banks.
+template <int D>
+__device__ __forceinline__ int merge_place(int r, int d4) {
+  const int t = (r >> 1) & 3;
+  if constexpr (D == 128) return r * (D / 4) + (d4 ^ ((t & 1) | ((t & 2) << 1)));
+  if constexpr (D == 64) return r * (D / 4) + (d4 ^ (2 * t));
+  return r * (D / 4) + d4;
+}
 
 template <typename XT, int D, int NT>
 __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(const __grid_constant__ AttendArgs a) {
@@ -263,89 +310,117 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   constexpr int NP = F32 ? 2 : 1;
   extern __shared__ __align__(128) unsigned char dec_smem[];
   unsigned char *ring = dec_smem;
-  float *merge = reinterpret_cast<float *>(dec_smem + Geo::kRing);
-  long long *pre = reinterpret_cast<long long *>(dec_smem + Geo::kRing + Geo::kMerge);
+  DecBatch bt;
+  bt.pre = reinterpret_cast<long long *>(dec_smem + Geo::kRing);
+  bt.q0 = reinterpret_cast<int *>(bt.pre + a.b.B + 1);
+  bt.q = bt.q0 + a.b.B;
+  bt.len = bt.q + a.b.B;
   __shared__ long long red[kDecWarps];
   __shared__ float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS];
   __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = a.g.G, Hkv = a.g.Hkv;
 
-  request_prefix(a.b.B, pre, red, [&](int b) {
-    const DecReq q = dec_req<ROWS>(a, b);
+  int longest = 0;
+  request_prefix(a.b.B, bt.pre, red, [&](int b) {
+    const Kv8Req r = kv8_req(a.b, a.g.P, b);
+    DecReq q{b, bt.q0[b] = r.q0, bt.q[b] = r.q, bt.len[b] = r.len, 0, 0, 0};
+    dec_shape<ROWS>(a, q);
+    if (q.nr > 0) longest = max(longest, q.nt);
     return static_cast<long long>(q.nr) * q.nt * Hkv;
   });
-  const long long total = pre[a.b.B];
-  const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinShare));
-  const long long u0 = share * blockIdx.x;
-  if (u0 >= total) return;
-  const int n_units = static_cast<int>(min(total - u0, share));
+  const long long total = bt.pre[a.b.B];
+  const long long share = quotient(total + gridDim.x - 1, gridDim.x);
+  long long u0 = min(total, share * blockIdx.x), u1 = min(total, u0 + share);
+  // short items stay whole: their few units take less time than merging parts of them would
+  if (!__syncthreads_or(longest > kWholeItems)) {
+    auto item_start = [&](long long u) {  // of the first item that starts at u or later
+      if (u >= total) return total;
+      const int b = request_of(bt.pre, a.b.B, u);
+      const int nt = dec_req<ROWS>(a, bt, b).nt;
+      return bt.pre[b] + quotient(u - bt.pre[b] + nt - 1, nt) * nt;
+    };
+    u0 = item_start(u0);
+    u1 = item_start(u1);
+  }
+  if (u0 >= u1) return;
+  const int n_units = static_cast<int>(u1 - u0);
 
   // ---- this warp's ring -------------------------------------------------
   const uint32_t my_ring = shared_addr(ring) + warp * S * Geo::kSlot;
   const uint32_t my_tails = shared_addr(ring) + kDecWarps * S * Geo::kSlot + warp * S * Geo::kTail;
   auto tail_of = [&](uint32_t slot) { return my_tails + (slot - my_ring) / (Geo::kSlot / Geo::kTail); };
-  constexpr int kCopies = (kSlice * D / 16 + 31) / 32;  // 16-byte copies of a lane for K, and for V
+  constexpr int kCopies = (kSlice * D / 16 + 31) / 32;  // 16-byte copies of a lane for a slice's K, and its V
   uint32_t k_to[kCopies], v_to[kCopies];
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) {
     const int c = lane + 32 * i;
     k_to[i] = k_place<D>(c / (D / 16), c % (D / 16));
-    v_to[i] = Geo::kSliceBytes + v_place<D>(c / (D / 16), c % (D / 16));
+    v_to[i] = kStep * Geo::kSliceBytes + v_place<D>(c / (D / 16), c % (D / 16));
   }
   Cursor<ROWS> load;
-  load.seek(a, pre, u0);
+  load.seek(a, bt, u0);
   int to_load = n_units;                                     // units not yet asked for
   int l_left = load.q.nt - load.unit;                        // units of the load cursor's item from here on
-  int l_pos = (load.q.t0 + load.unit) * kUnit + warp * kSlice;  // this warp's slice of that unit
+  int l_pos = (load.q.t0 + load.unit) * kUnit + warp * kStep * kSlice;  // this warp's part of that unit
   const int32_t *l_table = a.b.table + static_cast<long long>(load.q.b) * a.b.cols;
-  int page = l_pos < load.q.r.len ? l_table[l_pos >> a.p_shift] : -1;
+  int page[2];  // pages of the part's first and last slice (one page unless it is 16 positions long)
+  auto read_pages = [&]() {
+    page[0] = l_pos < load.q.len ? l_table[l_pos >> a.p_shift] : -1;
+    page[1] = page[0];
+    if (a.p_shift == 4) page[1] = l_pos + kSlice < load.q.len ? l_table[(l_pos >> 4) + 1] : -1;
+  };
+  read_pages();
   auto issue = [&](uint32_t dst) {
     if (to_load > 0) {
-      const bool ok = page >= 0 && page < a.c.n_pages;
-      if (ok) {
-        const uint32_t in = l_pos & ((1u << a.p_shift) - 1);
-        const unsigned long long ph = static_cast<unsigned long long>(static_cast<unsigned>(page)) * static_cast<unsigned>(Hkv) + load.h;
-        const unsigned long long at = (ph << a.p_shift) * D + (in * D + 16 * lane);
-        const int8_t *ksrc = a.c.k + at, *vsrc = a.c.v + at;
-        if (kSlice * D / 16 % 32 == 0 || lane < kSlice * D / 16) {
 #pragma unroll
-          for (int i = 0; i < kCopies; ++i) {
-            cp_async16(dst + k_to[i], ksrc + 512 * i);
-            cp_async16(dst + v_to[i], vsrc + 512 * i);
+      for (int i = 0; i < kStep; ++i) {
+        const int pos = l_pos + i * kSlice;
+        const bool ok = page[i] >= 0 && page[i] < a.c.n_pages && pos < load.q.len;
+        if (ok) {
+          const uint32_t in = pos & ((1u << a.p_shift) - 1);
+          const unsigned long long ph = static_cast<unsigned long long>(static_cast<unsigned>(page[i])) * static_cast<unsigned>(Hkv) + load.h;
+          const unsigned long long at = (ph << a.p_shift) * D + (in * D + 16 * lane);
+          const int8_t *ksrc = a.c.k + at, *vsrc = a.c.v + at;
+          if (kSlice * D / 16 % 32 == 0 || lane < kSlice * D / 16) {
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+              cp_async16(dst + k_to[c] + i * Geo::kSliceBytes, ksrc + 512 * c);
+              cp_async16(dst + v_to[c] + i * Geo::kSliceBytes, vsrc + 512 * c);
+            }
           }
+          const unsigned long long sat = (ph << (a.p_shift - a.t_shift)) + (in >> a.t_shift);
+          if (lane < 2) cp_async4(tail_of(dst) + 16 * i + 4 * lane, (lane ? a.c.vs : a.c.ks) + sat);
         }
-        const unsigned long long sat = (ph << (a.p_shift - a.t_shift)) + (in >> a.t_shift);
-        if (lane < 2) cp_async4(tail_of(dst) + 4 * lane, (lane ? a.c.vs : a.c.ks) + sat);
+        if (lane == 2)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(tail_of(dst) + 16 * i + 8), "r"(ok ? 1 : 0) : "memory");
       }
-      if (lane == 2)
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(tail_of(dst) + 8), "r"(ok ? 1 : 0) : "memory");
       l_pos += kUnit;
       if (--l_left == 0) {
-        load.next_item(a, pre);
+        load.next_item(a, bt);
         l_left = load.q.nt;
-        l_pos = load.q.t0 * kUnit + warp * kSlice;
+        l_pos = load.q.t0 * kUnit + warp * kStep * kSlice;
         l_table = a.b.table + static_cast<long long>(load.q.b) * a.b.cols;
       }
-      if (--to_load > 0) page = l_pos < load.q.r.len ? l_table[l_pos >> a.p_shift] : -1;
+      if (--to_load > 0) read_pages();
     }
     cp_commit();
   };
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) issue(my_ring + i * Geo::kSlot);
-  uint32_t slot = my_ring;                             // the slot of the slice at hand
+  uint32_t slot = my_ring;                              // the slot of the step at hand
   uint32_t free_slot = my_ring + (S - 1) * Geo::kSlot;  // the one used before it
   const uint32_t ring_end = my_ring + S * Geo::kSlot;
 
   Cursor<ROWS> cur;
-  cur.seek(a, pre, u0);
+  cur.seek(a, bt, u0);
   bool fresh = true;
   int qf[3][NT][KW];  // queries as whole numbers of 24 bits, three bytes each
   float o[NT][KS][4], m[NT][2], l[NT][2], cs[NT][2];
   int lim[NT][2];   // last visible position of this lane's two columns (-1: none)
   int min_lim = 0, max_lim = 0, row0 = 0, n_rows = 0;
   const uint32_t k_at = D == 128 || D == 64 ? k_place<D>(g, t) : g * D + (D / 4) * t;
-  const uint32_t v_at = Geo::kSliceBytes + v_place<D>(2 * t, (KS * g) >> 4) + ((KS * g) & 15);
+  const uint32_t v_at = kStep * Geo::kSliceBytes + v_place<D>(2 * t, (KS * g) >> 4) + ((KS * g) & 15);
   for (int n_left = n_units; n_left > 0; --n_left) {
     const DecReq &q = cur.q;
     const int hk = cur.h;
@@ -353,14 +428,14 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       // ---- the item's queries, scaled by a power of two to at most 1..2 ----
       fresh = false;
       row0 = cur.tile * ROWS;
-      n_rows = min(ROWS, q.r.q * G - row0);
-      min_lim = q.r.len - q.r.q + row0 / G;
-      max_lim = q.r.len - q.r.q + (row0 + n_rows - 1) / G;
+      n_rows = min(ROWS, q.q * G - row0);
+      min_lim = q.len - q.q + row0 / G;
+      max_lim = q.len - q.q + (row0 + n_rows - 1) / G;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int r = row0 + 8 * n + g;
         const bool live = 8 * n + g < n_rows;
-        const long long at = live ? (q.r.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head : 0;
+        const long long at = live ? (q.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head : 0;
         const XT *src = static_cast<const XT *>(a.q) + at;
         float x[KW][4], big = 0.f, bad = 0.f;  // bad: 0, or a NaN where the row has a value that is not finite
 #pragma unroll
@@ -404,7 +479,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
           cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e * (1.f / 2097152.f));
           const int rr = 8 * n + 2 * t + j;
-          lim[n][j] = rr < n_rows ? q.r.len - q.r.q + (row0 + rr) / G : -1;
+          lim[n][j] = rr < n_rows ? q.len - q.q + (row0 + rr) / G : -1;
           m[n][j] = kNone;
           l[n][j] = 0.f;
         }
@@ -415,82 +490,102 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       }
     }
 
-    // ---- one slice ----------------------------------------------------------
+    // ---- one step: kStep slices ------------------------------------------------
     cp_wait<S - 2>();
     __syncwarp();
-    const int p0 = (q.t0 + cur.unit) * kUnit + warp * kSlice;
-    const uint4 tail = lds128(tail_of(slot));  // scales and whether the page is there
-    if (tail.z && p0 <= max_lim && (a.window <= 0 || p0 + kSlice - 1 > min_lim - a.window)) {
-      const float ksc = __uint_as_float(tail.x), vsc = __uint_as_float(tail.y);
-      // scores: rows g and g + 8 of the slice, this lane's dims; exact whole numbers
-      uint32_t kw[2][KW + 1];
+    issue(free_slot);
+    const int p0 = (q.t0 + cur.unit) * kUnit + warp * kStep * kSlice;
+    // scales; 0 for a slice that is not there or that no row sees
+    float ksc[kStep], vsc[kStep];
+    bool any = false, gone[kStep];  // gone: the slice's page is not there
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t at = slot + k_at + 8 * D * i;
-        if constexpr (D == 128) {
-          const uint4 w = lds128(at), x = lds128(at ^ 64);  // chunks t and t + 4
-          kw[i][0] = w.x; kw[i][1] = w.y; kw[i][2] = w.z; kw[i][3] = w.w;
-          kw[i][4] = x.x; kw[i][5] = x.y; kw[i][6] = x.z; kw[i][7] = x.w;
-        } else if constexpr (D == 64) {
-          const uint4 w = lds128(at);
-          kw[i][0] = w.x; kw[i][1] = w.y; kw[i][2] = w.z; kw[i][3] = w.w;
-        } else if constexpr (D == 32) {
-          const uint2 w = lds64(at);
-          kw[i][0] = w.x; kw[i][1] = w.y;
-        } else {
-          kw[i][0] = lds32(at);
-        }
-        kw[i][KW] = 0;
-      }
-      float sc[NT][4];
+    for (int i = 0; i < kStep; ++i) {
+      const uint4 tail = lds128(tail_of(slot) + 16 * i);
+      const int p = p0 + i * kSlice;
+      const bool seen = tail.z && p <= max_lim && (a.window <= 0 || p + kSlice - 1 > min_lim - a.window);
+      ksc[i] = seen ? __uint_as_float(tail.x) : 0.f;
+      vsc[i] = seen ? __uint_as_float(tail.y) : 0.f;
+      any |= seen;
+      gone[i] = tail.z == 0;
+    }
+    if (any) {
+      // whole: every row sees every position of the step
+      const bool whole = p0 + kStep * kSlice - 1 <= min_lim && (a.window <= 0 || p0 > max_lim - a.window) &&
+                         !gone[0] && !gone[kStep - 1];
+      float sc[kStep][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        int d[3][4];
+      for (int i = 0; i < kStep; ++i) {
+        // scores: rows g and g + 8 of the slice, this lane's dims; exact whole numbers
+        uint32_t kw[2][KW + 1];
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          mma16832_first(d[p], kw[0][0], kw[1][0], kw[0][1], kw[1][1], qf[p][n][0], KW > 1 ? qf[p][n][KW > 1] : 0);
-#pragma unroll
-          for (int s = 1; s < KM; ++s)
-            mma16832(d[p], kw[0][2 * s], kw[1][2 * s], kw[0][2 * s + 1], kw[1][2 * s + 1], qf[p][n][2 * s], qf[p][n][2 * s + 1]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          sc[n][j] = fmaf(static_cast<float>((d[2][j] << 8) + d[1][j]), 256.f, static_cast<float>(d[0][j]));
-      }
-      // softmax: this lane has positions p0 + g, p0 + g + 8 for columns 2t, 2t + 1.  Weights are held relative to the
-      // largest p x sv: the value scale's exponent ev joins the maximum
-      const bool whole = p0 + kSlice - 1 <= min_lim && (a.window <= 0 || p0 > max_lim - a.window);
-      const int ev = max(static_cast<int>(tail.y >> 23) - 127, -90);
-      const float fev = static_cast<float>(ev), lazy = kLazy - fev;
-      if (!whole) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int first = a.window > 0 ? lim[n][j] - a.window : -1;
-            const float hidden = cs[n][j] * ksc < 0.f ? INFINITY : -INFINITY;  // -infinity after the scale
-            if (p0 + g > lim[n][j] || p0 + g <= first) sc[n][j] = hidden;
-            if (p0 + g + 8 > lim[n][j] || p0 + g + 8 <= first) sc[n][j + 2] = hidden;
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t at = slot + k_at + i * Geo::kSliceBytes + 8 * D * r;
+          if constexpr (D == 128) {
+            const uint4 w = lds128(at), x = lds128(at ^ 64);  // chunks t and t + 4
+            kw[r][0] = w.x; kw[r][1] = w.y; kw[r][2] = w.z; kw[r][3] = w.w;
+            kw[r][4] = x.x; kw[r][5] = x.y; kw[r][6] = x.z; kw[r][7] = x.w;
+          } else if constexpr (D == 64) {
+            const uint4 w = lds128(at);
+            kw[r][0] = w.x; kw[r][1] = w.y; kw[r][2] = w.z; kw[r][3] = w.w;
+          } else if constexpr (D == 32) {
+            const uint2 w = lds64(at);
+            kw[r][0] = w.x; kw[r][1] = w.y;
+          } else {
+            kw[r][0] = lds32(at);
           }
+          kw[r][KW] = 0;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          int d[3][4];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            mma16832_first(d[p], kw[0][0], kw[1][0], kw[0][1], kw[1][1], qf[p][n][0], KW > 1 ? qf[p][n][KW > 1] : 0);
+#pragma unroll
+            for (int s = 1; s < KM; ++s)
+              mma16832(d[p], kw[0][2 * s], kw[1][2 * s], kw[0][2 * s + 1], kw[1][2 * s + 1], qf[p][n][2 * s], qf[p][n][2 * s + 1]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sc[i][n][j] = fmaf(static_cast<float>((d[2][j] << 8) + d[1][j]), 256.f, static_cast<float>(d[0][j]));
+        }
       }
-      float x[NT][4];
+      // softmax: this lane has positions g, g + 8 of each slice for columns 2t, 2t + 1.  Weights are held relative to
+      // the largest p x sv: the value scale's exponent joins the maximum
+      float x[kStep][NT][4], fev[kStep];
       bool grow = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+      for (int i = 0; i < kStep; ++i) {
+        fev[i] = static_cast<float>(max(static_cast<int>(__float_as_uint(vsc[i]) >> 23) - 127, -90));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[n][j] = fmaf(sc[n][j], cs[n][j & 1] * ksc, -m[n][j & 1]);
-        grow |= fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) > lazy;
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[i][n][j] = fmaf(sc[i][n][j], cs[n][j & 1] * ksc[i], -m[n][j & 1]);
+            if (!whole) {
+              const int p = p0 + i * kSlice + g + 8 * (j >> 1), last = lim[n][j & 1];
+              if (p > last || (a.window > 0 && p <= last - a.window) || gone[i]) x[i][n][j] = -INFINITY;
+            }
+          }
+          grow |= fmaxf(fmaxf(x[i][n][0], x[i][n][1]), fmaxf(x[i][n][2], x[i][n][3])) > kLazy - fev[i];
+        }
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float f = cs[n][j] * ksc;
-            float top = fmaxf(sc[n][j] * f, sc[n][j + 2] * f);
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+              const float f = cs[n][j] * ksc[i];
+#pragma unroll
+              for (int r = 0; r < 4; r += 2)
+                if (x[i][n][j + r] != -INFINITY) top = fmaxf(top, sc[i][n][j + r] * f + fev[i]);
+            }
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-            const float nm = fmaxf(m[n][j], top + fev);
+            const float nm = fmaxf(m[n][j], top);
             const float al = exp2_fast(m[n][j] - nm);
             m[n][j] = nm;
             l[n][j] *= al;
@@ -499,85 +594,91 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
               o[n][s][j] *= al;
               o[n][s][j + 2] *= al;
             }
-            x[n][j] = fmaf(sc[n][j], f, -nm);
-            x[n][j + 2] = fmaf(sc[n][j + 2], f, -nm);
+#pragma unroll
+            for (int i = 0; i < kStep; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; r += 2)
+                if (x[i][n][j + r] != -INFINITY) x[i][n][j + r] = fmaf(sc[i][n][j + r], cs[n][j] * ksc[i], -nm);
           }
       }
-      uint32_t pf[NP][NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
+      for (int i = 0; i < kStep; ++i) {
+        uint32_t pf[NP][NT][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = exp2_fast(x[n][j]);
-          l[n][j & 1] += p;
-          w[j] = p * vsc;
-        }
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t hi = pack_f16(w[2 * i], w[2 * i + 1]);
-          pf[0][n][i] = transpose8x8(hi);
-          if constexpr (F32) {
-            const float2 h = unpack_f16(hi);
-            pf[NP - 1][n][i] = transpose8x8(pack_f16(w[2 * i] - h.x, w[2 * i + 1] - h.y));
+          for (int j = 0; j < 4; ++j) {
+            const float p = exp2_fast(x[i][n][j]);
+            l[n][j & 1] += p;
+            w[j] = p * vsc[i];
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t hi = pack_f16(w[2 * r], w[2 * r + 1]);
+            pf[0][n][r] = transpose8x8(hi);
+            if constexpr (F32) {
+              const float2 h = unpack_f16(hi);
+              pf[NP - 1][n][r] = transpose8x8(pack_f16(w[2 * r] - h.x, w[2 * r + 1] - h.y));
+            }
           }
         }
-      }
-      // output: this lane's dims KS g .. + KS and D / 2 + KS g .. of positions 2t, 2t + 1, 2t + 8, 2t + 9
-      constexpr int VB = KS < 4 ? KS : 4;  // dims a word carries
-      uint32_t vw[2][4][(KS + 3) / 4];     // [half of the dims][position]
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // position 2t + (i & 1) + 8 (i >> 1); D = 64 and below keep odd positions 4 rows on
-          const uint32_t step = (i & 1) * (D == 128 ? D : 4 * D) + (i >> 1) * 8 * D;
-          const uint32_t at = (slot + v_at + step) ^ (h && D >= 64 ? D / 2 : 0);
-          if constexpr (KS == 8) {
-            const uint2 v = lds64(at);
-            vw[h][i][0] = v.x;
-            vw[h][i][1] = v.y;
-          } else if constexpr (KS == 4) {
-            vw[h][i][0] = lds32(at);
-          } else if constexpr (KS == 2) {
-            vw[h][i][0] = lds16(at + h * (D / 2));
-          } else {
-            vw[h][i][0] = lds8(at + h * (D / 2));
-          }
-        }
-#pragma unroll
-      for (int c = 0; c < (KS + 3) / 4; ++c) {
-        uint32_t w[2][4];
+        // output: this lane's dims KS g .. + KS and D / 2 + KS g .. of positions 2t, 2t + 1, 2t + 8, 2t + 9
+        constexpr int VB = KS < 4 ? KS : 4;  // dims a word carries
+        uint32_t vw[2][4][(KS + 3) / 4];     // [half of the dims][position]
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[h][i] = vw[h][i][c] ^ 0x80808080u;
+          for (int r = 0; r < 4; ++r) {
+            // position 2t + (r & 1) + 8 (r >> 1); D = 64 and below keep odd positions 4 rows on
+            const uint32_t step = (r & 1) * (D == 128 ? D : 4 * D) + (r >> 1) * 8 * D;
+            const uint32_t at = (slot + v_at + i * Geo::kSliceBytes + step) ^ (h && D >= 64 ? D / 2 : 0);
+            if constexpr (KS == 8) {
+              const uint2 v = lds64(at);
+              vw[h][r][0] = v.x;
+              vw[h][r][1] = v.y;
+            } else if constexpr (KS == 4) {
+              vw[h][r][0] = lds32(at);
+            } else if constexpr (KS == 2) {
+              vw[h][r][0] = lds16(at + h * (D / 2));
+            } else {
+              vw[h][r][0] = lds8(at + h * (D / 2));
+            }
+          }
 #pragma unroll
-        for (int half = 0; half < (VB + 1) / 2; ++half) {
-          // pairs of positions (2t, 2t + 1) and (2t + 8, 2t + 9) of dims 2 half, 2 half + 1
-          uint32_t x[2][2];
+        for (int c = 0; c < (KS + 3) / 4; ++c) {
+          uint32_t w[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) x[h][i] = __byte_perm(w[h][2 * i], w[h][2 * i + 1], half ? 0x7362 : 0x5140);
+            for (int r = 0; r < 4; ++r) w[h][r] = vw[h][r][c] ^ 0x80808080u;
 #pragma unroll
-          for (int j = 0; j < (VB < 2 ? 1 : 2); ++j) {
-            uint32_t f[4];
-            const uint32_t sel = j ? 0x4342 : 0x4140;
-            f[0] = f16_codes(__byte_perm(x[0][0], 0x64646464u, sel));
-            f[1] = f16_codes(__byte_perm(x[1][0], 0x64646464u, sel));
-            f[2] = f16_codes(__byte_perm(x[0][1], 0x64646464u, sel));
-            f[3] = f16_codes(__byte_perm(x[1][1], 0x64646464u, sel));
+          for (int half = 0; half < (VB + 1) / 2; ++half) {
+            // pairs of positions (2t, 2t + 1) and (2t + 8, 2t + 9) of dims 2 half, 2 half + 1
+            uint32_t y[2][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int p = 0; p < NP; ++p) mma16816(o[n][4 * c + 2 * half + j], f, pf[p][n][0], pf[p][n][1]);
+              for (int r = 0; r < 2; ++r) y[h][r] = __byte_perm(w[h][2 * r], w[h][2 * r + 1], half ? 0x7362 : 0x5140);
+#pragma unroll
+            for (int j = 0; j < (VB < 2 ? 1 : 2); ++j) {
+              uint32_t f[4];
+              const uint32_t sel = j ? 0x4342 : 0x4140;
+              f[0] = f16_codes(__byte_perm(y[0][0], 0x64646464u, sel));
+              f[1] = f16_codes(__byte_perm(y[1][0], 0x64646464u, sel));
+              f[2] = f16_codes(__byte_perm(y[0][1], 0x64646464u, sel));
+              f[3] = f16_codes(__byte_perm(y[1][1], 0x64646464u, sel));
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int p = 0; p < NP; ++p) mma16816(o[n][4 * c + 2 * half + j], f, pf[p][n][0], pf[p][n][1]);
+            }
           }
         }
       }
     }
     __syncwarp();
-    issue(free_slot);
+    const uint32_t done = slot - my_ring;  // the slot just read: free until the next step
     free_slot = slot;
     slot += Geo::kSlot;
     if (slot == ring_end) slot = my_ring;
@@ -586,43 +687,47 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     // ---- end of the item, or of this block's share of it --------------------
     if (cur.unit == q.nt || n_left == 1) {
       const long long i0 = u0 + (n_units - n_left) + 1 - cur.unit, i1 = i0 + q.nt;
-      float *mine = merge + warp * ROWS * D;
+      float *mine = reinterpret_cast<float *>(ring + warp * S * Geo::kSlot + done);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float sum = l[n][j];
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
           const int r = 8 * n + 2 * t + j;
           if (g == 0) {
             s_m[warp][r] = m[n][j];
             s_l[warp][r] = sum;
           }
 #pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            mine[r * D + KS * g + s] = o[n][s][j];
-            mine[r * D + D / 2 + KS * g + s] = o[n][s][j + 2];
+          for (int h = 0; h < 2; ++h) {
+            const int d = h * (D / 2) + KS * g;
+            if constexpr (KS >= 4) {
+#pragma unroll
+              for (int s = 0; s < KS; s += 4)
+                *reinterpret_cast<float4 *>(mine + 4 * merge_place<D>(r, (d + s) / 4)) =
+                    make_float4(o[n][s][j + 2 * h], o[n][s + 1][j + 2 * h], o[n][s + 2][j + 2 * h], o[n][s + 3][j + 2 * h]);
+            } else {
+#pragma unroll
+              for (int s = 0; s < KS; ++s) mine[r * D + d + s] = o[n][s][j + 2 * h];
+            }
           }
         }
       __syncthreads();
-      const bool all = i0 >= u0 && i1 <= u0 + n_units;
-      const long long c0 = i0 / share, c1 = (i1 - 1) / share;
+      const bool all = i0 >= u0 && i1 <= u1;
       float *part = a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart;
       auto store = [&](int r, int d, float4 v, float lsum, float top) {
         // row r of the tile, dims d .. d + 3
         const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // 0: the row saw nothing
         const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
-        XT *dst = static_cast<XT *>(a.out) + (q.r.q0 + i) * a.o_row + h * a.o_head + d;
-        dst[0] = from_f32<XT>(v.x * inv);
-        dst[1] = from_f32<XT>(v.y * inv);
-        dst[2] = from_f32<XT>(v.z * inv);
-        dst[3] = from_f32<XT>(v.w * inv);
+        XT *dst = static_cast<XT *>(a.out) + (q.q0 + i) * a.o_row + h * a.o_head + d;
+        store4(dst, a.o_vec, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         if (a.lse && d == 0)
-          a.lse[static_cast<long long>(q.r.q0 + i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
+          a.lse[static_cast<long long>(q.q0 + i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
       };
       for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        const int r = i / (D / 4), d4 = i % (D / 4);
         float top = kNone;
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, s_m[w][r]);
@@ -631,57 +736,72 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) {
           const float f = exp2_fast(s_m[w][r] - top);
-          const float4 x = *reinterpret_cast<const float4 *>(merge + (w * ROWS + r) * D + d);
+          const float4 y = reinterpret_cast<const float4 *>(ring + w * S * Geo::kSlot + done)[merge_place<D>(r, d4)];
           lsum += s_l[w][r] * f;
-          v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+          v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
         }
         if (all) {
-          store(r, d, v, lsum, top);
+          store(r, 4 * d4, v, lsum, top);
         } else {
-          *reinterpret_cast<float4 *>(part + r * D + d) = v;
-          if (d == 0) {
+          *reinterpret_cast<float4 *>(part + r * D + 4 * d4) = v;
+          if (d4 == 0) {
             part[ROWS * D + r] = top;
             part[ROWS * D + ROWS + r] = lsum;
           }
         }
       }
       if (!all) {
+        const int c0 = static_cast<int>(quotient(i0, share)), c1 = static_cast<int>(quotient(i1 - 1, share));
         __threadfence();
         __syncthreads();
-        if (threadIdx.x == 0) s_last = atomicAdd(a.ticket + c0, 1) == static_cast<int>(c1 - c0);
+        if (threadIdx.x == 0) s_last = atomicAdd(a.ticket + c0, 1) == c1 - c0;
         __syncthreads();
         if (s_last) {
           __threadfence();
           for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4;
-            float top = kNone;
-            for (long long c = c0; c <= c1; ++c)
-              top = fmaxf(top, __ldcg(a.part + (2 * c + (c == c0)) * Geo::kPart + ROWS * D + r));
+            const int r = i / (D / 4), d4 = i % (D / 4);
+            float top = kNone, lsum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            float lsum = 0.f;
-            for (long long c = c0; c <= c1; ++c) {
-              const float *p = a.part + (2 * c + (c == c0)) * Geo::kPart;
-              const float f = exp2_fast(__ldcg(p + ROWS * D + r) - top);
-              const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + r * D + d));
-              lsum += __ldcg(p + ROWS * D + ROWS + r) * f;
-              v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+            for (int c = c0; c <= c1; c += kMergeAhead) {
+              float pm[kMergeAhead], pl[kMergeAhead];
+              float4 pv[kMergeAhead];
+              const float was = top;
+#pragma unroll
+              for (int k = 0; k < kMergeAhead; ++k) {
+                const bool in = c + k <= c1;
+                const float *p = a.part + (2ll * (in ? c + k : c0) + (!in || c + k == c0)) * Geo::kPart;
+                pm[k] = __ldcg(p + ROWS * D + r);
+                pl[k] = __ldcg(p + ROWS * D + ROWS + r);
+                pv[k] = __ldcg(reinterpret_cast<const float4 *>(p) + r * (D / 4) + d4);
+                if (!in) pm[k] = kNone * 2;  // weight 0
+              }
+#pragma unroll
+              for (int k = 0; k < kMergeAhead; ++k) top = fmaxf(top, pm[k]);
+              const float al = exp2_fast(was - top);
+              lsum *= al;
+              v.x *= al; v.y *= al; v.z *= al; v.w *= al;
+#pragma unroll
+              for (int k = 0; k < kMergeAhead; ++k) {
+                const float f = exp2_fast(pm[k] - top);
+                lsum += pl[k] * f;
+                v.x += pv[k].x * f; v.y += pv[k].y * f; v.z += pv[k].z * f; v.w += pv[k].w * f;
+              }
             }
-            store(r, d, v, lsum, top);
+            store(r, 4 * d4, v, lsum, top);
           }
           if (threadIdx.x == 0) a.ticket[c0] = 0;
         }
       }
       __syncthreads();
       fresh = true;
-      cur.next_item(a, pre);
+      cur.next_item(a, bt);
     }
   }
-  cp_wait<0>();
 }
 
 template <int D, int NT>
 constexpr int dec_smem_bytes(int B) {
-  return DecGeom<D, NT>::kRing + DecGeom<D, NT>::kMerge + (B + 1) * static_cast<int>(sizeof(long long));
+  return DecGeom<D, NT>::kRing + (B + 1) * static_cast<int>(sizeof(long long)) + 3 * B * static_cast<int>(sizeof(int));
 }
 
 template <typename XT, int D, int NT>
@@ -774,7 +894,8 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
     DeviceScope scope(h->device);
     const AttendArgs a{h->g, c,   b,     q,      q_row_stride, q_head_stride, out, out_row_stride, out_head_stride,
                        lse,  scale, window, h->part, h->ticket, log2i(h->g.P), log2i(h->g.t),
-                       rows_aligned(q, q_row_stride, q_head_stride, dtype)};
+                       rows_aligned(q, q_row_stride, q_head_stride, dtype),
+                       rows_aligned(out, out_row_stride, out_head_stride, dtype)};
     const auto st = static_cast<cudaStream_t>(stream);
     // rows of one kv head: one column tile of 8 where they fit, else two
     const bool one = static_cast<long long>(max_q) * h->g.G <= 8;
