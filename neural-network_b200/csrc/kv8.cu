@@ -247,9 +247,11 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
 
 }  // namespace
 
-Kv8Layer kv8_layer(const specdec_kv8_layer *l) {
+Kv8Layer kv8_layer(const specdec_kv8 *h, const specdec_kv8_layer *l) {
   op_check(l && l->k && l->v && l->k_scale && l->v_scale && l->n_pages > 0, "null cache layer buffer, or no pages");
   op_check(aligned16(l->k) && aligned16(l->v), "cache code buffers must be 16-byte aligned");
+  op_check(static_cast<long long>(l->n_pages) * h->g.Hkv * (h->g.P / h->g.t) <= 0x7fffffffll,
+           "n_pages x n_kv_heads x blocks of a page must be below 2^31");
   return {l->k, l->v, l->k_scale, l->v_scale, l->n_pages};
 }
 
@@ -337,7 +339,7 @@ int specdec_kv8_append(specdec_kv8 *h, const specdec_kv8_layer *layer, const spe
                        int64_t v_head_stride, int dtype, int n_tokens, void *stream) {
   if (!h) return SPECDEC_ERR_INVALID;
   return op_guard(h->err, [&] {
-    const Kv8Layer c = kv8_layer(layer);
+    const Kv8Layer c = kv8_layer(h, layer);
     const Kv8Batch b = kv8_batch(h, batch, n_tokens);
     op_check(dtype == SPECDEC_F32 || dtype == SPECDEC_BF16, "rows must be SPECDEC_F32 or SPECDEC_BF16");
     if (b.B == 0 || b.T == 0) return;
@@ -359,7 +361,7 @@ int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int
                        void *out_v, int dtype, void *stream) {
   if (!h) return SPECDEC_ERR_INVALID;
   return op_guard(h->err, [&] {
-    const Kv8Layer c = kv8_layer(layer);
+    const Kv8Layer c = kv8_layer(h, layer);
     op_check(dtype == SPECDEC_F32 || dtype == SPECDEC_BF16, "outputs must be SPECDEC_F32 or SPECDEC_BF16");
     op_check(n >= 0, "negative row count");
     if (n == 0 || (!out_k && !out_v)) return;

@@ -58,7 +58,7 @@ struct AttendArgs {
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kSlice = 16;                            // positions of a slice
-constexpr int kStep = 2;                              // slices a warp takes at a time
+constexpr int kStep = 2;                              // slices a warp takes at a time: one page, or two of 16 positions
 constexpr int kUnit = kSlice * kStep * kDecWarps;     // positions of a unit
 constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: registers
 constexpr int kWholeItems = 4;                        // items of at most this many units are not split
@@ -73,7 +73,7 @@ struct DecGeom {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSliceBytes = kSlice * D;            // K or V codes of a slice
   static constexpr int kSlot = 2 * kStep * kSliceBytes;     // a multiple of 128: places within a row are XORed into addresses
-  static constexpr int kTail = 16 * kStep;                  // per slice: the two scales, whether the page is there
+  static constexpr int kTail = 8 * kStep;                   // per slice: the key and the value scale
   // 8 KB a slot at D = 128: one in use and at least one in flight, 96 KB in flight per SM; small rows take more slots
   static constexpr int kStages = D == 128 ? (NT == 1 ? 2 : 3) : (D == 64 ? 4 : 6);
   static constexpr int kRing = kDecWarps * kStages * (kSlot + kTail);
@@ -109,6 +109,16 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Four 8 x 16-byte matrices, one row address per lane: lane l gets bytes 4 (l % 4) .. of row l / 4 of each.
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix2(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+  r[2] = r[3] = 0;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -136,20 +146,18 @@ __device__ __forceinline__ uint32_t lds8(uint32_t addr) {
 }
 
 // d = a b, and d += a b
-__device__ __forceinline__ void mma16832_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16832_first(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, "
       "%10};"
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
-__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void mma16832(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Transpose of an 8 x 8 matrix of 16-bit values spread over the warp.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -169,32 +177,39 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
 
-// Place of a 16-byte chunk of a slice row in shared memory.  K rows are read
-// by lanes (row g, chunk t and, for 128-byte rows, 4 + t): odd rows swap their
-// halves.  V rows are read 8 lanes along a row and 4 rows (2t) at once: the
-// rows' chunks are spread over the banks.
-// Four adjacent values (vec: at a 4-element boundary), zeros unless live.
-__device__ __forceinline__ void load4(const float *p, bool vec, bool live, float (&x)[4]) {
-  if (vec) {
-    const float4 v = live ? *reinterpret_cast<const float4 *>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-  } else {
+// Four adjacent values of a row as loaded (vec: at a 4-element boundary), zeros unless live.
+template <typename XT>
+struct Quad;
+template <>
+struct Quad<float> {
+  float x[4];
+  __device__ __forceinline__ void load(const float *p, bool vec, bool live) {
+    if (vec) {
+      const float4 v = live ? *reinterpret_cast<const float4 *>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = live ? p[j] : 0.f;
+      for (int j = 0; j < 4; ++j) x[j] = live ? p[j] : 0.f;
+    }
   }
-}
-__device__ __forceinline__ void load4(const __nv_bfloat16 *p, bool vec, bool live, float (&x)[4]) {
-  if (vec) {
-    const uint2 v = live ? *reinterpret_cast<const uint2 *>(p) : make_uint2(0, 0);
-    x[0] = __uint_as_float(v.x << 16);
-    x[1] = __uint_as_float(v.x & 0xffff0000u);
-    x[2] = __uint_as_float(v.y << 16);
-    x[3] = __uint_as_float(v.y & 0xffff0000u);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = live ? to_f32(p[j]) : 0.f;
+  __device__ __forceinline__ float get(int j) const { return x[j]; }
+};
+template <>
+struct Quad<__nv_bfloat16> {
+  uint2 x;
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p, bool vec, bool live) {
+    if (vec) {
+      x = live ? *reinterpret_cast<const uint2 *>(p) : make_uint2(0, 0);
+    } else {
+      const unsigned short *u = reinterpret_cast<const unsigned short *>(p);
+      x = live ? make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16) : make_uint2(0, 0);
+    }
   }
-}
+  __device__ __forceinline__ float get(int j) const {
+    const uint32_t w = j < 2 ? x.x : x.y;
+    return __uint_as_float((j & 1) ? w & 0xffff0000u : w << 16);
+  }
+};
 
 __device__ __forceinline__ void store4(float *p, bool vec, float4 v) {
   if (vec) {
@@ -216,9 +231,15 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, bool vec, float4 v) {
   }
 }
 
+// Place of a 16-byte chunk of a slice row in shared memory.  K rows are read
+// eight at a time at one chunk: the chunks of rows that start in the same bank
+// are spread.  V rows are read 8 lanes along a row and 4 rows (2t) at once.
 template <int D>
 __device__ __forceinline__ int k_place(int row, int chunk) {
-  return row * D + 16 * (D == 128 ? chunk ^ ((row & 1) << 2) : chunk);
+  if constexpr (D == 128) return row * D + 16 * (chunk ^ (row & 7));
+  if constexpr (D == 64) return row * D + 16 * (chunk ^ ((row >> 1) & 3));
+  if constexpr (D == 32) return row * D + 16 * (chunk ^ ((row >> 2) & 1));
+  return row * D + 16 * chunk;
 }
 template <int D>
 __device__ __forceinline__ int v_place(int row, int chunk) {
@@ -227,6 +248,9 @@ __device__ __forceinline__ int v_place(int row, int chunk) {
   if constexpr (D == 64) return r * D + 16 * (chunk ^ (r & 2));
   return r * D + 16 * chunk;
 }
+
+// A value that is the same in the whole warp, as the compiler can see it.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // a / b where both mostly fit 32 bits.
 __device__ __forceinline__ long long quotient(long long a, long long b) {
@@ -256,10 +280,10 @@ __device__ __forceinline__ void dec_shape(const AttendArgs &a, DecReq &r) {
 template <int ROWS>
 __device__ __forceinline__ DecReq dec_req(const AttendArgs &a, const DecBatch &s, int b) {
   DecReq r;
-  r.b = b;
-  r.q0 = s.q0[b];
-  r.q = s.q[b];
-  r.len = s.len[b];
+  r.b = uniform(b);
+  r.q0 = uniform(s.q0[b]);
+  r.q = uniform(s.q[b]);
+  r.len = uniform(s.len[b]);
   dec_shape<ROWS>(a, r);
   return r;
 }
@@ -273,9 +297,9 @@ struct Cursor {
     q = dec_req<ROWS>(a, s, request_of(s.pre, a.b.B, u));
     const long long in = u - s.pre[q.b];
     const int item = static_cast<int>(quotient(in, q.nt));
-    unit = static_cast<int>(in - static_cast<long long>(item) * q.nt);
-    h = item / q.nr;
-    tile = item - h * q.nr;
+    unit = uniform(static_cast<int>(in - static_cast<long long>(item) * q.nt));
+    h = uniform(item / q.nr);
+    tile = uniform(item - h * q.nr);
   }
   // the next item (the caller counts units)
   __device__ __forceinline__ void next_item(const AttendArgs &a, const DecBatch &s) {
@@ -286,6 +310,7 @@ struct Cursor {
     h = 0;
     int b = q.b + 1;
     while (b < a.b.B && s.pre[b + 1] == s.pre[b]) ++b;
+    b = uniform(b);
     if (b < a.b.B) q = dec_req<ROWS>(a, s, b);
   }
 };
@@ -318,7 +343,9 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   __shared__ long long red[kDecWarps];
   __shared__ float s_m[kDecWarps][ROWS], s_l[kDecWarps][ROWS];
   __shared__ int s_last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // what decides on branches is made uniform over the warp by a shuffle or a vote, so that the products inside
+  // them need no re-convergence
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = a.g.G, Hkv = a.g.Hkv;
 
   int longest = 0;
@@ -344,57 +371,58 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     u1 = item_start(u1);
   }
   if (u0 >= u1) return;
-  const int n_units = static_cast<int>(u1 - u0);
+  const int n_units = uniform(static_cast<int>(u1 - u0));
 
   // ---- this warp's ring -------------------------------------------------
   const uint32_t my_ring = shared_addr(ring) + warp * S * Geo::kSlot;
   const uint32_t my_tails = shared_addr(ring) + kDecWarps * S * Geo::kSlot + warp * S * Geo::kTail;
   auto tail_of = [&](uint32_t slot) { return my_tails + (slot - my_ring) / (Geo::kSlot / Geo::kTail); };
   constexpr int kCopies = (kSlice * D / 16 + 31) / 32;  // 16-byte copies of a lane for a slice's K, and its V
-  uint32_t k_to[kCopies], v_to[kCopies];
-#pragma unroll
-  for (int i = 0; i < kCopies; ++i) {
-    const int c = lane + 32 * i;
-    k_to[i] = k_place<D>(c / (D / 16), c % (D / 16));
-    v_to[i] = kStep * Geo::kSliceBytes + v_place<D>(c / (D / 16), c % (D / 16));
-  }
+  // copy c of a lane goes 512 c bytes on: 4 rows at D = 128, where the chunk order of every other copy is turned, and
+  // 8 rows at D = 64, where it stays
+  const uint32_t k_to = k_place<D>(lane / (D / 16), lane % (D / 16));
+  const uint32_t v_to = kStep * Geo::kSliceBytes + v_place<D>(lane / (D / 16), lane % (D / 16));
+  constexpr uint32_t kTurn = D == 128 ? 64 : 0;
   Cursor<ROWS> load;
   load.seek(a, bt, u0);
   int to_load = n_units;                                     // units not yet asked for
   int l_left = load.q.nt - load.unit;                        // units of the load cursor's item from here on
   int l_pos = (load.q.t0 + load.unit) * kUnit + warp * kStep * kSlice;  // this warp's part of that unit
   const int32_t *l_table = a.b.table + static_cast<long long>(load.q.b) * a.b.cols;
+  const uint32_t page_bytes = static_cast<uint32_t>(D) << a.p_shift, page_blocks = 1u << (a.p_shift - a.t_shift);
   int page[2];  // pages of the part's first and last slice (one page unless it is 16 positions long)
   auto read_pages = [&]() {
     page[0] = l_pos < load.q.len ? l_table[l_pos >> a.p_shift] : -1;
-    page[1] = page[0];
-    if (a.p_shift == 4) page[1] = l_pos + kSlice < load.q.len ? l_table[(l_pos >> 4) + 1] : -1;
+    page[1] = l_pos + kSlice < load.q.len ? (a.p_shift == 4 ? l_table[(l_pos >> 4) + 1] : page[0]) : -1;
   };
   read_pages();
+  uint32_t there = 0;  // two bits a step: whether its slices' pages are there, the newest step lowest
   auto issue = [&](uint32_t dst) {
+    there <<= kStep;
     if (to_load > 0) {
+      // (page, kv head) rows and blocks fit 32 bits: the pool is checked against it
+      const uint32_t in = l_pos & ((1u << a.p_shift) - 1);
+      const uint32_t row0 = static_cast<uint32_t>(page[0]) * Hkv + load.h, row1 = static_cast<uint32_t>(page[1]) * Hkv + load.h;
+      const bool ok0 = __any_sync(0xffffffffu, static_cast<uint32_t>(page[0]) < static_cast<uint32_t>(a.c.n_pages));
+      const bool ok1 = __any_sync(0xffffffffu, static_cast<uint32_t>(page[1]) < static_cast<uint32_t>(a.c.n_pages));
+      const uint32_t in1 = a.p_shift == 4 ? 0 : in + kSlice;  // the second slice's place in its page
+      there |= (ok0 ? 1 : 0) | (ok1 ? 2 : 0);
+      auto copy = [&](int i, uint32_t row, uint32_t at) {
+        const unsigned long long off = static_cast<unsigned long long>(row) * page_bytes + (at * D + 16 * lane);
+        const int8_t *ksrc = a.c.k + off, *vsrc = a.c.v + off;
+        if (kSlice * D / 16 % 32 == 0 || lane < kSlice * D / 16) {
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        const int pos = l_pos + i * kSlice;
-        const bool ok = page[i] >= 0 && page[i] < a.c.n_pages && pos < load.q.len;
-        if (ok) {
-          const uint32_t in = pos & ((1u << a.p_shift) - 1);
-          const unsigned long long ph = static_cast<unsigned long long>(static_cast<unsigned>(page[i])) * static_cast<unsigned>(Hkv) + load.h;
-          const unsigned long long at = (ph << a.p_shift) * D + (in * D + 16 * lane);
-          const int8_t *ksrc = a.c.k + at, *vsrc = a.c.v + at;
-          if (kSlice * D / 16 % 32 == 0 || lane < kSlice * D / 16) {
-#pragma unroll
-            for (int c = 0; c < kCopies; ++c) {
-              cp_async16(dst + k_to[c] + i * Geo::kSliceBytes, ksrc + 512 * c);
-              cp_async16(dst + v_to[c] + i * Geo::kSliceBytes, vsrc + 512 * c);
-            }
+          for (int c = 0; c < kCopies; ++c) {
+            cp_async16(((dst + k_to) ^ (c & 1 ? kTurn : 0)) + i * Geo::kSliceBytes + 512 * c, ksrc + 512 * c);
+            cp_async16(((dst + v_to) ^ (c & 1 ? kTurn : 0)) + i * Geo::kSliceBytes + 512 * c, vsrc + 512 * c);
           }
-          const unsigned long long sat = (ph << (a.p_shift - a.t_shift)) + (in >> a.t_shift);
-          if (lane < 2) cp_async4(tail_of(dst) + 16 * i + 4 * lane, (lane ? a.c.vs : a.c.ks) + sat);
         }
-        if (lane == 2)
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(tail_of(dst) + 16 * i + 8), "r"(ok ? 1 : 0) : "memory");
-      }
+      };
+      if (ok0) copy(0, row0, in);
+      if (ok1) copy(1, row1, in1);
+      // lanes 0 .. 3: the slices' key and value scales
+      const uint32_t block = (lane < 2 ? row0 : row1) * page_blocks + ((lane < 2 ? in : in1) >> a.t_shift);
+      if (lane < 4 && (lane < 2 ? ok0 : ok1)) cp_async4(tail_of(dst) + 4 * lane, ((lane & 1) ? a.c.vs : a.c.ks) + block);
       l_pos += kUnit;
       if (--l_left == 0) {
         load.next_item(a, bt);
@@ -414,66 +442,71 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
 
   Cursor<ROWS> cur;
   cur.seek(a, bt, u0);
-  bool fresh = true;
   int qf[3][NT][KW];  // queries as whole numbers of 24 bits, three bytes each
   float o[NT][KS][4], m[NT][2], l[NT][2], cs[NT][2];
   int lim[NT][2];   // last visible position of this lane's two columns (-1: none)
-  int min_lim = 0, max_lim = 0, row0 = 0, n_rows = 0;
-  const uint32_t k_at = D == 128 || D == 64 ? k_place<D>(g, t) : g * D + (D / 4) * t;
+  // the item's row tile: its first row and rows; first and last position at which some row is cut off; this warp's
+  // next position; positions at which every row sees a whole step
+  int row0 = 0, n_rows = 0, min_lim = 0, max_lim = 0, p0 = 0, whole_lo = 0, whole_hi = 0;
+  Quad<XT> raw[NT][KW];
+  auto begin_item = [&]() {  // asks for the item's query rows
+    const DecReq &q = cur.q;
+    row0 = cur.tile * ROWS;
+    n_rows = min(ROWS, q.q * G - row0);
+    min_lim = q.len - q.q + row0 / G;
+    max_lim = q.len - q.q + (row0 + n_rows - 1) / G;
+    p0 = (q.t0 + cur.unit) * kUnit + warp * kStep * kSlice;
+    whole_lo = a.window > 0 ? max_lim - a.window + 1 : 0;
+    whole_hi = min_lim - kStep * kSlice + 1;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + 8 * n + g;
+      const bool live = 8 * n + g < n_rows;
+      const long long at = live ? (q.q0 + r / G) * a.q_row + (cur.h * G + r % G) * a.q_head : 0;
+      const XT *src = static_cast<const XT *>(a.q) + at + 4 * t;
+#pragma unroll
+      for (int s = 0; s < KW; ++s) raw[n][s].load(src + 16 * s, a.q_vec, live);
+    }
+  };
+  begin_item();
+  bool fresh = true;
+  const uint32_t k_row = lane & 15, k_half = lane >> 4;  // ldmatrix row and 16-byte chunk of this lane
   const uint32_t v_at = kStep * Geo::kSliceBytes + v_place<D>(2 * t, (KS * g) >> 4) + ((KS * g) & 15);
   for (int n_left = n_units; n_left > 0; --n_left) {
     const DecReq &q = cur.q;
-    const int hk = cur.h;
     if (fresh) {
       // ---- the item's queries, scaled by a power of two to at most 1..2 ----
       fresh = false;
-      row0 = cur.tile * ROWS;
-      n_rows = min(ROWS, q.q * G - row0);
-      min_lim = q.len - q.q + row0 / G;
-      max_lim = q.len - q.q + (row0 + n_rows - 1) / G;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int r = row0 + 8 * n + g;
-        const bool live = 8 * n + g < n_rows;
-        const long long at = live ? (q.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head : 0;
-        const XT *src = static_cast<const XT *>(a.q) + at;
-        float x[KW][4], big = 0.f, bad = 0.f;  // bad: 0, or a NaN where the row has a value that is not finite
+        float big = 0.f, bad = 0.f;  // bad: 0, or a NaN where the row has a value that is not finite
 #pragma unroll
-        for (int s = 0; s < KW; ++s) {
-          const int d = D == 128 ? (s < 4 ? 16 * t + 4 * s : 64 + 16 * t + 4 * (s - 4)) : t * (D / 4) + 4 * s;
-          load4(src + d, a.q_vec, live, x[s]);
+        for (int s = 0; s < KW; ++s)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            big = fmaxf(big, fabsf(x[s][j]));
-            bad += x[s][j] * 0.f;
+            big = fmaxf(big, fabsf(raw[n][s].get(j)));
+            bad = fmaf(raw[n][s].get(j), 0.f, bad);
           }
-        }
 #pragma unroll
         for (int i = 1; i <= 2; i <<= 1) {
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, i));
           bad += __shfl_xor_sync(0xffffffffu, bad, i);
         }
-        // 2^e <= big < 2^(e + 1); rows below 2^-100 count as 2^-100.  x 2^(21 - e) is rounded to a whole number
-        // of at most 2^22: 22 bits of the row's largest value
+        // 2^e <= big < 2^(e + 1); rows below 2^-100 count as 2^-100.  v = x 2^(21 - e) rounded, |v| <= 2^22: 22 bits
+        // of the row's largest value.  Its digits in base 256, -128 .. 127 each, are the bytes of v + 0x808080 less
+        // 128: three products of bytes give q . k exactly
         const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
         const float down = __uint_as_float((127 - e) << 23), up = __uint_as_float((127 + e) << 23) + bad;
 #pragma unroll
         for (int s = 0; s < KW; ++s) {
-          int w[3] = {0, 0, 0};
+          uint32_t v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            int v = __float2int_rn(x[s][j] * down * 2097152.f);
-            const int c0 = static_cast<int8_t>(v & 255);
-            v = (v - c0) >> 8;
-            const int c1 = static_cast<int8_t>(v & 255);
-            v = (v - c1) >> 8;
-            w[0] |= (c0 & 255) << (8 * j);
-            w[1] |= (c1 & 255) << (8 * j);
-            w[2] |= (v & 255) << (8 * j);
-          }
-          qf[0][n][s] = w[0];
-          qf[1][n][s] = w[1];
-          qf[2][n][s] = w[2];
+          for (int j = 0; j < 4; ++j)
+            v[j] = static_cast<uint32_t>(__float2int_rn(raw[n][s].get(j) * down * 2097152.f)) + 0x808080u;
+          const uint32_t a01 = __byte_perm(v[0], v[1], 0x5140), a23 = __byte_perm(v[2], v[3], 0x5140);  // bytes 0, 1
+          qf[0][n][s] = __byte_perm(a01, a23, 0x5410) ^ 0x80808080u;
+          qf[1][n][s] = __byte_perm(a01, a23, 0x7632) ^ 0x80808080u;
+          qf[2][n][s] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410) ^ 0x80808080u;
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
@@ -494,60 +527,53 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     cp_wait<S - 2>();
     __syncwarp();
     issue(free_slot);
-    const int p0 = (q.t0 + cur.unit) * kUnit + warp * kStep * kSlice;
-    // scales; 0 for a slice that is not there or that no row sees
-    float ksc[kStep], vsc[kStep];
-    bool any = false, gone[kStep];  // gone: the slice's page is not there
+    const uint32_t here = there >> (kStep * (S - 1));  // this step's slices
+    const uint4 tail = lds128(tail_of(slot));
+    float ksc[kStep] = {__uint_as_float(tail.x), __uint_as_float(tail.z)};
+    float vsc[kStep] = {__uint_as_float(tail.y), __uint_as_float(tail.w)};
+    const bool whole = __all_sync(0xffffffffu, p0 >= whole_lo && p0 <= whole_hi && (here & 3) == 3);
+    bool any = true;
+    if (!whole) {  // scales of 0 for a slice that is not there or that no row sees
+      any = false;
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) {
-      const uint4 tail = lds128(tail_of(slot) + 16 * i);
-      const int p = p0 + i * kSlice;
-      const bool seen = tail.z && p <= max_lim && (a.window <= 0 || p + kSlice - 1 > min_lim - a.window);
-      ksc[i] = seen ? __uint_as_float(tail.x) : 0.f;
-      vsc[i] = seen ? __uint_as_float(tail.y) : 0.f;
-      any |= seen;
-      gone[i] = tail.z == 0;
+      for (int i = 0; i < kStep; ++i) {
+        const int p = p0 + i * kSlice;
+        const bool seen = (here >> i & 1) && p <= max_lim && (a.window <= 0 || p + kSlice - 1 > min_lim - a.window);
+        ksc[i] = seen ? ksc[i] : 0.f;
+        vsc[i] = seen ? vsc[i] : 0.f;
+        any |= seen;
+      }
     }
-    if (any) {
-      // whole: every row sees every position of the step
-      const bool whole = p0 + kStep * kSlice - 1 <= min_lim && (a.window <= 0 || p0 > max_lim - a.window) &&
-                         !gone[0] && !gone[kStep - 1];
+    if (__any_sync(0xffffffffu, any)) {
       float sc[kStep][NT][4];
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
-        // scores: rows g and g + 8 of the slice, this lane's dims; exact whole numbers
-        uint32_t kw[2][KW + 1];
+        // scores: the slice's 16 positions x the rows, exact whole numbers
+        uint32_t kw[KM][4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint32_t at = slot + k_at + i * Geo::kSliceBytes + 8 * D * r;
-          if constexpr (D == 128) {
-            const uint4 w = lds128(at), x = lds128(at ^ 64);  // chunks t and t + 4
-            kw[r][0] = w.x; kw[r][1] = w.y; kw[r][2] = w.z; kw[r][3] = w.w;
-            kw[r][4] = x.x; kw[r][5] = x.y; kw[r][6] = x.z; kw[r][7] = x.w;
-          } else if constexpr (D == 64) {
-            const uint4 w = lds128(at);
-            kw[r][0] = w.x; kw[r][1] = w.y; kw[r][2] = w.z; kw[r][3] = w.w;
-          } else if constexpr (D == 32) {
-            const uint2 w = lds64(at);
-            kw[r][0] = w.x; kw[r][1] = w.y;
-          } else {
-            kw[r][0] = lds32(at);
-          }
-          kw[r][KW] = 0;
+        for (int s = 0; s < KM; ++s) {
+          const uint32_t at = slot + i * Geo::kSliceBytes + k_place<D>(k_row, D == 16 ? 0 : 2 * s + k_half);
+          if constexpr (D == 16) ldmatrix2(kw[s], at);
+          else ldmatrix4(kw[s], at);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          int d[3][4];
+          int hi[4], lo[4];
+          auto product = [&](int (&d)[4], int p, bool first) {
 #pragma unroll
-          for (int p = 0; p < 3; ++p) {
-            mma16832_first(d[p], kw[0][0], kw[1][0], kw[0][1], kw[1][1], qf[p][n][0], KW > 1 ? qf[p][n][KW > 1] : 0);
+            for (int s = 0; s < KM; ++s) {
+              const uint32_t b1 = 2 * s + 1 < KW ? qf[p][n][2 * s + 1 < KW ? 2 * s + 1 : 0] : 0;
+              if (first && s == 0) mma16832_first(d, kw[s], qf[p][n][2 * s], b1);
+              else mma16832(d, kw[s], qf[p][n][2 * s], b1);
+            }
+          };
+          product(hi, 2, true);
+          product(lo, 0, true);
 #pragma unroll
-            for (int s = 1; s < KM; ++s)
-              mma16832(d[p], kw[0][2 * s], kw[1][2 * s], kw[0][2 * s + 1], kw[1][2 * s + 1], qf[p][n][2 * s], qf[p][n][2 * s + 1]);
-          }
+          for (int j = 0; j < 4; ++j) hi[j] <<= 8;
+          product(hi, 1, false);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            sc[i][n][j] = fmaf(static_cast<float>((d[2][j] << 8) + d[1][j]), 256.f, static_cast<float>(d[0][j]));
+          for (int j = 0; j < 4; ++j) sc[i][n][j] = fmaf(static_cast<float>(hi[j]), 256.f, static_cast<float>(lo[j]));
         }
       }
       // softmax: this lane has positions g, g + 8 of each slice for columns 2t, 2t + 1.  Weights are held relative to
@@ -564,7 +590,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
             x[i][n][j] = fmaf(sc[i][n][j], cs[n][j & 1] * ksc[i], -m[n][j & 1]);
             if (!whole) {
               const int p = p0 + i * kSlice + g + 8 * (j >> 1), last = lim[n][j & 1];
-              if (p > last || (a.window > 0 && p <= last - a.window) || gone[i]) x[i][n][j] = -INFINITY;
+              if (p > last || (a.window > 0 && p <= last - a.window) || !(here >> i & 1)) x[i][n][j] = -INFINITY;
             }
           }
           grow |= fmaxf(fmaxf(x[i][n][0], x[i][n][1]), fmaxf(x[i][n][2], x[i][n][3])) > kLazy - fev[i];
@@ -683,6 +709,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     slot += Geo::kSlot;
     if (slot == ring_end) slot = my_ring;
     ++cur.unit;
+    p0 += kUnit;
 
     // ---- end of the item, or of this block's share of it --------------------
     if (cur.unit == q.nt || n_left == 1) {
@@ -714,19 +741,24 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
             }
           }
         }
+      const DecReq q = cur.q;
+      const int hk = cur.h, row0_now = row0, n_rows_now = n_rows;
+      cur.next_item(a, bt);
+      if (n_left > 1) begin_item();
+      fresh = true;
       __syncthreads();
       const bool all = i0 >= u0 && i1 <= u1;
       float *part = a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart;
       auto store = [&](int r, int d, float4 v, float lsum, float top) {
         // row r of the tile, dims d .. d + 3
         const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // 0: the row saw nothing
-        const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
+        const int i = (row0_now + r) / G, h = hk * G + (row0_now + r) % G;
         XT *dst = static_cast<XT *>(a.out) + (q.q0 + i) * a.o_row + h * a.o_head + d;
         store4(dst, a.o_vec, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         if (a.lse && d == 0)
           a.lse[static_cast<long long>(q.q0 + i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
       };
-      for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
+      for (int i = threadIdx.x; i < n_rows_now * D / 4; i += kDecThreads) {
         const int r = i / (D / 4), d4 = i % (D / 4);
         float top = kNone;
 #pragma unroll
@@ -758,7 +790,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         __syncthreads();
         if (s_last) {
           __threadfence();
-          for (int i = threadIdx.x; i < n_rows * D / 4; i += kDecThreads) {
+          for (int i = threadIdx.x; i < n_rows_now * D / 4; i += kDecThreads) {
             const int r = i / (D / 4), d4 = i % (D / 4);
             float top = kNone, lsum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -793,8 +825,6 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         }
       }
       __syncthreads();
-      fresh = true;
-      cur.next_item(a, bt);
     }
   }
 }
@@ -884,7 +914,7 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
                                   float scale, int window, void *stream) {
   if (!h) return SPECDEC_ERR_INVALID;
   return op_guard(h->err, [&] {
-    const Kv8Layer c = kv8_layer(layer);
+    const Kv8Layer c = kv8_layer(h, layer);
     const Kv8Batch b = kv8_batch(h, batch, n_tokens);
     op_check(dtype == SPECDEC_F32 || dtype == SPECDEC_BF16, "rows must be SPECDEC_F32 or SPECDEC_BF16");
     op_check(max_q >= 0 && window >= 0, "max_q and window must not be negative");
