@@ -52,6 +52,7 @@ struct AttendArgs {
   float *part;
   int *ticket;
   int p_shift, t_shift;  // log2 of page and block positions
+  int g_shift;           // log2 of the query heads of a kv head, -1 where that is no power of two
   int q_vec, o_vec;      // query / output rows start at 4-element boundaries
 };
 
@@ -258,6 +259,16 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
   return a / b;
 }
 
+// Row r of a kv head's rows of a request: new token r / G, query head r % G.
+struct RowAt {
+  int i, h;
+};
+__device__ __forceinline__ RowAt row_at(const AttendArgs &a, int r) {
+  if (a.g_shift >= 0) return {r >> a.g_shift, r & (a.g.G - 1)};
+  const int i = r / a.g.G;
+  return {i, r - i * a.g.G};
+}
+
 // The batch in shared memory: per request its rows, its length and the units before it.
 struct DecBatch {
   long long *pre;  // [B + 1]
@@ -453,8 +464,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     const DecReq &q = cur.q;
     row0 = cur.tile * ROWS;
     n_rows = min(ROWS, q.q * G - row0);
-    min_lim = q.len - q.q + row0 / G;
-    max_lim = q.len - q.q + (row0 + n_rows - 1) / G;
+    min_lim = q.len - q.q + row_at(a, row0).i;
+    max_lim = q.len - q.q + row_at(a, row0 + n_rows - 1).i;
     p0 = (q.t0 + cur.unit) * kUnit + warp * kStep * kSlice;
     whole_lo = a.window > 0 ? max_lim - a.window + 1 : 0;
     whole_hi = min_lim - kStep * kSlice + 1;
@@ -462,7 +473,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     for (int n = 0; n < NT; ++n) {
       const int r = row0 + 8 * n + g;
       const bool live = 8 * n + g < n_rows;
-      const long long at = live ? (q.q0 + r / G) * a.q_row + (cur.h * G + r % G) * a.q_head : 0;
+      const RowAt at_row = row_at(a, r);
+      const long long at = live ? (q.q0 + at_row.i) * a.q_row + (cur.h * G + at_row.h) * a.q_head : 0;
       const XT *src = static_cast<const XT *>(a.q) + at + 4 * t;
 #pragma unroll
       for (int s = 0; s < KW; ++s) raw[n][s].load(src + 16 * s, a.q_vec, live);
@@ -496,13 +508,13 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         // of the row's largest value.  Its digits in base 256, -128 .. 127 each, are the bytes of v + 0x808080 less
         // 128: three products of bytes give q . k exactly
         const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
-        const float down = __uint_as_float((127 - e) << 23), up = __uint_as_float((127 + e) << 23) + bad;
+        const float down = __uint_as_float((127 + 21 - e) << 23), up = __uint_as_float((127 + e) << 23) + bad;
 #pragma unroll
         for (int s = 0; s < KW; ++s) {
           uint32_t v[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            v[j] = static_cast<uint32_t>(__float2int_rn(raw[n][s].get(j) * down * 2097152.f)) + 0x808080u;
+            v[j] = static_cast<uint32_t>(__float2int_rn(raw[n][s].get(j) * down)) + 0x808080u;
           const uint32_t a01 = __byte_perm(v[0], v[1], 0x5140), a23 = __byte_perm(v[2], v[3], 0x5140);  // bytes 0, 1
           qf[0][n][s] = __byte_perm(a01, a23, 0x5410) ^ 0x80808080u;
           qf[1][n][s] = __byte_perm(a01, a23, 0x7632) ^ 0x80808080u;
@@ -512,7 +524,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
           cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e * (1.f / 2097152.f));
           const int rr = 8 * n + 2 * t + j;
-          lim[n][j] = rr < n_rows ? q.len - q.q + (row0 + rr) / G : -1;
+          lim[n][j] = rr < n_rows ? q.len - q.q + row_at(a, row0 + rr).i : -1;
           m[n][j] = kNone;
           l[n][j] = 0.f;
         }
@@ -749,31 +761,35 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       __syncthreads();
       const bool all = i0 >= u0 && i1 <= u1;
       float *part = a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart;
-      auto store = [&](int r, int d, float4 v, float lsum, float top) {
-        // row r of the tile, dims d .. d + 3
-        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // 0: the row saw nothing
-        const int i = (row0_now + r) / G, h = hk * G + (row0_now + r) % G;
-        XT *dst = static_cast<XT *>(a.out) + (q.q0 + i) * a.o_row + h * a.o_head + d;
+      // a warp takes rows warp, warp + 4, ...; its lanes four dims each
+      constexpr int kLanes = D / 4 < 32 ? D / 4 : 32, kRowsAtOnce = kDecThreads / kLanes;
+      const int r_first = threadIdx.x / kLanes, d4 = threadIdx.x % kLanes;
+      auto store = [&](int r, float4 v, float lsum, float top) {
+        const float inv = lsum == 0.f ? 0.f : __fdividef(1.f, lsum);  // 0: the row saw nothing
+        const RowAt at_row = row_at(a, row0_now + r);
+        const int i = q.q0 + at_row.i, h = hk * G + at_row.h;
+        XT *dst = static_cast<XT *>(a.out) + i * a.o_row + h * a.o_head + 4 * d4;
         store4(dst, a.o_vec, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-        if (a.lse && d == 0)
-          a.lse[static_cast<long long>(q.q0 + i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
+        if (a.lse && d4 == 0) a.lse[static_cast<long long>(i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
       };
-      for (int i = threadIdx.x; i < n_rows_now * D / 4; i += kDecThreads) {
-        const int r = i / (D / 4), d4 = i % (D / 4);
-        float top = kNone;
+      for (int r = r_first; r < n_rows_now; r += kRowsAtOnce) {
+        float sm[kDecWarps], top = kNone;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, s_m[w][r]);
+        for (int w = 0; w < kDecWarps; ++w) {
+          sm[w] = s_m[w][r];
+          top = fmaxf(top, sm[w]);
+        }
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float lsum = 0.f;
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) {
-          const float f = exp2_fast(s_m[w][r] - top);
+          const float f = exp2_fast(sm[w] - top);
           const float4 y = reinterpret_cast<const float4 *>(ring + w * S * Geo::kSlot + done)[merge_place<D>(r, d4)];
           lsum += s_l[w][r] * f;
           v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
         }
         if (all) {
-          store(r, 4 * d4, v, lsum, top);
+          store(r, v, lsum, top);
         } else {
           *reinterpret_cast<float4 *>(part + r * D + 4 * d4) = v;
           if (d4 == 0) {
@@ -790,8 +806,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         __syncthreads();
         if (s_last) {
           __threadfence();
-          for (int i = threadIdx.x; i < n_rows_now * D / 4; i += kDecThreads) {
-            const int r = i / (D / 4), d4 = i % (D / 4);
+          for (int r = r_first; r < n_rows_now; r += kRowsAtOnce) {
             float top = kNone, lsum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int c = c0; c <= c1; c += kMergeAhead) {
@@ -819,7 +834,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
                 v.x += pv[k].x * f; v.y += pv[k].y * f; v.z += pv[k].z * f; v.w += pv[k].w * f;
               }
             }
-            store(r, 4 * d4, v, lsum, top);
+            store(r, v, lsum, top);
           }
           if (threadIdx.x == 0) a.ticket[c0] = 0;
         }
@@ -924,6 +939,7 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
     DeviceScope scope(h->device);
     const AttendArgs a{h->g, c,   b,     q,      q_row_stride, q_head_stride, out, out_row_stride, out_head_stride,
                        lse,  scale, window, h->part, h->ticket, log2i(h->g.P), log2i(h->g.t),
+                       (h->g.G & (h->g.G - 1)) == 0 ? log2i(h->g.G) : -1,
                        rows_aligned(q, q_row_stride, q_head_stride, dtype),
                        rows_aligned(out, out_row_stride, out_head_stride, dtype)};
     const auto st = static_cast<cudaStream_t>(stream);
