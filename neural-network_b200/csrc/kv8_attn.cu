@@ -73,13 +73,15 @@ template <int D, int NT>
 struct DecGeom {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSliceBytes = kSlice * D;            // K or V codes of a slice
-  static constexpr int kSlot = 2 * kStep * kSliceBytes;     // a multiple of 128: places within a row are XORed into addresses
+  static constexpr int kHalf = kStep * kSliceBytes;         // K or V codes of a step; a multiple of 128: places within a
+                                                            // row are XORed into addresses
   static constexpr int kTail = 8 * kStep;                   // per slice: the key and the value scale
-  // 8 KB a slot at D = 128: one in use and at least one in flight, 96 KB in flight per SM; small rows take more slots
-  static constexpr int kStages = D == 128 ? (NT == 1 ? 2 : 3) : (D == 64 ? 4 : 6);
-  static constexpr int kRing = kDecWarps * kStages * (kSlot + kTail);
+  static constexpr int kRing = kDecWarps * 3 * kHalf;       // per warp two K buffers and one V buffer
+  static constexpr int kTails = kDecWarps * 2 * kTail;
+  static constexpr int kQuery = 3 * NT * 32 * (D / 4);      // the rows' three bytes as the products take them
+  static constexpr int kFixed = kRing + kTails + kQuery;
   static constexpr int kPart = kRows * D + 2 * kRows;       // floats of a partial result
-  static_assert(kRows * D * 4 <= kSlot, "a warp's output must fit the slot that it has just read");
+  static_assert(8 * D * 4 == kHalf, "a warp's output of eight rows fits the V buffer that it has just read");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
@@ -326,6 +328,29 @@ struct Cursor {
   }
 };
 
+// Byte offset of word s of plane p, column tile n of this lane's queries, and a lane's words of a plane.
+template <int KW>
+__device__ __forceinline__ uint32_t query_place(int p, int n, int lane, int s, int nt) {
+  constexpr int V = KW < 4 ? KW : 4;  // words a lane reads at once
+  return ((p * nt + n) * 32 * KW + (s / V) * 32 * V + lane * V + s % V) * 4;
+}
+template <int KW>
+__device__ __forceinline__ void query_words(uint32_t (&w)[(KW + 1) / 2 * 2], uint32_t addr) {
+  if constexpr (KW >= 4) {
+#pragma unroll
+    for (int s = 0; s < KW; s += 4) {
+      const uint4 v = lds128(addr + 128 * s);
+      w[s] = v.x; w[s + 1] = v.y; w[s + 2] = v.z; w[s + 3] = v.w;
+    }
+  } else if constexpr (KW == 2) {
+    const uint2 v = lds64(addr);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = lds32(addr);
+    w[1] = 0;
+  }
+}
+
 // Place of four adjacent outputs in a warp's merge area, spread over the banks.
 template <int D>
 __device__ __forceinline__ int merge_place(int r, int d4) {
@@ -338,7 +363,7 @@ __device__ __forceinline__ int merge_place(int r, int d4) {
 template <typename XT, int D, int NT>
 __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(const __grid_constant__ AttendArgs a) {
   using Geo = DecGeom<D, NT>;
-  constexpr int ROWS = Geo::kRows, S = Geo::kStages;
+  constexpr int ROWS = Geo::kRows;
   constexpr int KS = D / 16;       // products of 16 dims per score tile, and 16-dim tiles of the output
   constexpr int KW = D / 16;       // words of codes a lane reads of a K row
   constexpr int KM = (KW + 1) / 2; // products of 32 dims per score tile
@@ -347,7 +372,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   extern __shared__ __align__(128) unsigned char dec_smem[];
   unsigned char *ring = dec_smem;
   DecBatch bt;
-  bt.pre = reinterpret_cast<long long *>(dec_smem + Geo::kRing);
+  bt.pre = reinterpret_cast<long long *>(dec_smem + Geo::kFixed);
   bt.q0 = reinterpret_cast<int *>(bt.pre + a.b.B + 1);
   bt.q = bt.q0 + a.b.B;
   bt.len = bt.q + a.b.B;
@@ -384,15 +409,15 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   if (u0 >= u1) return;
   const int n_units = uniform(static_cast<int>(u1 - u0));
 
-  // ---- this warp's ring -------------------------------------------------
-  const uint32_t my_ring = shared_addr(ring) + warp * S * Geo::kSlot;
-  const uint32_t my_tails = shared_addr(ring) + kDecWarps * S * Geo::kSlot + warp * S * Geo::kTail;
-  auto tail_of = [&](uint32_t slot) { return my_tails + (slot - my_ring) / (Geo::kSlot / Geo::kTail); };
+  // ---- this warp's buffers: K of a step and of the next, V of a step ------
+  const uint32_t my_k = shared_addr(ring) + warp * 3 * Geo::kHalf, my_v = my_k + 2 * Geo::kHalf;
+  const uint32_t my_tails = shared_addr(ring) + Geo::kRing + warp * 2 * Geo::kTail;
+  const uint32_t queries = shared_addr(ring) + Geo::kRing + Geo::kTails;
   constexpr int kCopies = (kSlice * D / 16 + 31) / 32;  // 16-byte copies of a lane for a slice's K, and its V
   // copy c of a lane goes 512 c bytes on: 4 rows at D = 128, where the chunk order of every other copy is turned, and
   // 8 rows at D = 64, where it stays
   const uint32_t k_to = k_place<D>(lane / (D / 16), lane % (D / 16));
-  const uint32_t v_to = kStep * Geo::kSliceBytes + v_place<D>(lane / (D / 16), lane % (D / 16));
+  const uint32_t v_to = v_place<D>(lane / (D / 16), lane % (D / 16));
   constexpr uint32_t kTurn = D == 128 ? 64 : 0;
   Cursor<ROWS> load;
   load.seek(a, bt, u0);
@@ -407,33 +432,33 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     page[1] = l_pos + kSlice < load.q.len ? (a.p_shift == 4 ? l_table[(l_pos >> 4) + 1] : page[0]) : -1;
   };
   read_pages();
-  uint32_t there = 0;  // two bits a step: whether its slices' pages are there, the newest step lowest
-  auto issue = [&](uint32_t dst) {
+  uint32_t there = 0;                    // two bits a step: whether its slices' pages are there, the newest step lowest
+  uint32_t v_row0 = 0, v_row1 = 0, v_in = 0, v_in1 = 0;  // where the V of the newest step lies
+  auto copy = [&](const int8_t *base, uint32_t to, uint32_t row, uint32_t at) {
+    const int8_t *src = base + (static_cast<unsigned long long>(row) * page_bytes + (at * D + 16 * lane));
+    if (kSlice * D / 16 % 32 == 0 || lane < kSlice * D / 16) {
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) cp_async16((to ^ (c & 1 ? kTurn : 0)) + 512 * c, src + 512 * c);
+    }
+  };
+  auto issue_k = [&](uint32_t par) {  // K and the scales of the next step, into buffer par
     there <<= kStep;
     if (to_load > 0) {
       // (page, kv head) rows and blocks fit 32 bits: the pool is checked against it
-      const uint32_t in = l_pos & ((1u << a.p_shift) - 1);
-      const uint32_t row0 = static_cast<uint32_t>(page[0]) * Hkv + load.h, row1 = static_cast<uint32_t>(page[1]) * Hkv + load.h;
+      v_in = l_pos & ((1u << a.p_shift) - 1);
+      v_row0 = static_cast<uint32_t>(page[0]) * Hkv + load.h;
+      v_row1 = static_cast<uint32_t>(page[1]) * Hkv + load.h;
       const bool ok0 = __any_sync(0xffffffffu, static_cast<uint32_t>(page[0]) < static_cast<uint32_t>(a.c.n_pages));
       const bool ok1 = __any_sync(0xffffffffu, static_cast<uint32_t>(page[1]) < static_cast<uint32_t>(a.c.n_pages));
-      const uint32_t in1 = a.p_shift == 4 ? 0 : in + kSlice;  // the second slice's place in its page
+      v_in1 = a.p_shift == 4 ? 0 : v_in + kSlice;  // the second slice's place in its page
       there |= (ok0 ? 1 : 0) | (ok1 ? 2 : 0);
-      auto copy = [&](int i, uint32_t row, uint32_t at) {
-        const unsigned long long off = static_cast<unsigned long long>(row) * page_bytes + (at * D + 16 * lane);
-        const int8_t *ksrc = a.c.k + off, *vsrc = a.c.v + off;
-        if (kSlice * D / 16 % 32 == 0 || lane < kSlice * D / 16) {
-#pragma unroll
-          for (int c = 0; c < kCopies; ++c) {
-            cp_async16(((dst + k_to) ^ (c & 1 ? kTurn : 0)) + i * Geo::kSliceBytes + 512 * c, ksrc + 512 * c);
-            cp_async16(((dst + v_to) ^ (c & 1 ? kTurn : 0)) + i * Geo::kSliceBytes + 512 * c, vsrc + 512 * c);
-          }
-        }
-      };
-      if (ok0) copy(0, row0, in);
-      if (ok1) copy(1, row1, in1);
+      const uint32_t to = my_k + par * Geo::kHalf + k_to;
+      if (ok0) copy(a.c.k, to, v_row0, v_in);
+      if (ok1) copy(a.c.k, to + Geo::kSliceBytes, v_row1, v_in1);
       // lanes 0 .. 3: the slices' key and value scales
-      const uint32_t block = (lane < 2 ? row0 : row1) * page_blocks + ((lane < 2 ? in : in1) >> a.t_shift);
-      if (lane < 4 && (lane < 2 ? ok0 : ok1)) cp_async4(tail_of(dst) + 4 * lane, ((lane & 1) ? a.c.vs : a.c.ks) + block);
+      const uint32_t block = (lane < 2 ? v_row0 : v_row1) * page_blocks + ((lane < 2 ? v_in : v_in1) >> a.t_shift);
+      if (lane < 4 && (lane < 2 ? ok0 : ok1))
+        cp_async4(my_tails + par * Geo::kTail + 4 * lane, ((lane & 1) ? a.c.vs : a.c.ks) + block);
       l_pos += kUnit;
       if (--l_left == 0) {
         load.next_item(a, bt);
@@ -445,15 +470,17 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     }
     cp_commit();
   };
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i) issue(my_ring + i * Geo::kSlot);
-  uint32_t slot = my_ring;                              // the slot of the step at hand
-  uint32_t free_slot = my_ring + (S - 1) * Geo::kSlot;  // the one used before it
-  const uint32_t ring_end = my_ring + S * Geo::kSlot;
+  auto issue_v = [&]() {  // V of the step whose K was asked for last
+    if (there & 1) copy(a.c.v, my_v + v_to, v_row0, v_in);
+    if (there & 2) copy(a.c.v, my_v + v_to + Geo::kSliceBytes, v_row1, v_in1);
+    cp_commit();
+  };
+  issue_k(0);
+  issue_v();
+  uint32_t par = 0;  // K buffer of the step at hand
 
   Cursor<ROWS> cur;
   cur.seek(a, bt, u0);
-  int qf[3][NT][KW];  // queries as whole numbers of 24 bits, three bytes each
   float o[NT][KS][4], m[NT][2], l[NT][2], cs[NT][2];
   int lim[NT][2];   // last visible position of this lane's two columns (-1: none)
   // the item's row tile: its first row and rows; first and last position at which some row is cut off; this warp's
@@ -480,67 +507,71 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       for (int s = 0; s < KW; ++s) raw[n][s].load(src + 16 * s, a.q_vec, live);
     }
   };
+  // The item's queries, scaled by a power of two to at most 1..2, as whole numbers v = x 2^(21 - e) rounded, where
+  // 2^e <= the row's largest value < 2^(e + 1) (rows below 2^-100 count as 2^-100): 22 bits of that value.  The digits of
+  // v in base 256, -128 .. 127 each, are the bytes of v + 0x808080 less 128: three products of bytes give q . k exactly.
+  // Every warp finds the rows' largest values; the four convert a quarter of the words each, for all.
+  auto put_queries = [&]() {
+    const DecReq &q = cur.q;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float big = 0.f, bad = 0.f;  // bad: 0, or a NaN where the row has a value that is not finite
+#pragma unroll
+      for (int s = 0; s < KW; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          big = fmaxf(big, fabsf(raw[n][s].get(j)));
+          bad = fmaf(raw[n][s].get(j), 0.f, bad);
+        }
+#pragma unroll
+      for (int i = 1; i <= 2; i <<= 1) {
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, i));
+        bad += __shfl_xor_sync(0xffffffffu, bad, i);
+      }
+      const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
+      const float down = __uint_as_float((127 + 21 - e) << 23), up = __uint_as_float((127 + e) << 23) + bad;
+#pragma unroll
+      for (int s = 0; s < KW; ++s) {
+        if (s % kDecWarps != warp) continue;
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = static_cast<uint32_t>(__float2int_rn(raw[n][s].get(j) * down)) + 0x808080u;
+        const uint32_t a01 = __byte_perm(v[0], v[1], 0x5140), a23 = __byte_perm(v[2], v[3], 0x5140);  // bytes 0, 1
+        const uint32_t b01 = __byte_perm(v[0], v[1], 0x0062), b23 = __byte_perm(v[2], v[3], 0x0062);  // byte 2
+        const uint32_t w[3] = {__byte_perm(a01, a23, 0x5410), __byte_perm(a01, a23, 0x7632), __byte_perm(b01, b23, 0x5410)};
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(queries + query_place<KW>(p, n, lane, s, NT)), "r"(w[p] ^ 0x80808080u)
+                       : "memory");
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
+        cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e * (1.f / 2097152.f));
+        const int rr = 8 * n + 2 * t + j;
+        lim[n][j] = rr < n_rows ? q.len - q.q + row_at(a, row0 + rr).i : -1;
+        m[n][j] = kNone;
+        l[n][j] = 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][s][j] = 0.f;
+    }
+  };
   begin_item();
-  bool fresh = true;
+  put_queries();
+  __syncthreads();
   const uint32_t k_row = lane & 15, k_half = lane >> 4;  // ldmatrix row and 16-byte chunk of this lane
-  const uint32_t v_at = kStep * Geo::kSliceBytes + v_place<D>(2 * t, (KS * g) >> 4) + ((KS * g) & 15);
+  const uint32_t v_at = v_place<D>(2 * t, (KS * g) >> 4) + ((KS * g) & 15);
   for (int n_left = n_units; n_left > 0; --n_left) {
     const DecReq &q = cur.q;
-    if (fresh) {
-      // ---- the item's queries, scaled by a power of two to at most 1..2 ----
-      fresh = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float big = 0.f, bad = 0.f;  // bad: 0, or a NaN where the row has a value that is not finite
-#pragma unroll
-        for (int s = 0; s < KW; ++s)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            big = fmaxf(big, fabsf(raw[n][s].get(j)));
-            bad = fmaf(raw[n][s].get(j), 0.f, bad);
-          }
-#pragma unroll
-        for (int i = 1; i <= 2; i <<= 1) {
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, i));
-          bad += __shfl_xor_sync(0xffffffffu, bad, i);
-        }
-        // 2^e <= big < 2^(e + 1); rows below 2^-100 count as 2^-100.  v = x 2^(21 - e) rounded, |v| <= 2^22: 22 bits
-        // of the row's largest value.  Its digits in base 256, -128 .. 127 each, are the bytes of v + 0x808080 less
-        // 128: three products of bytes give q . k exactly
-        const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
-        const float down = __uint_as_float((127 + 21 - e) << 23), up = __uint_as_float((127 + e) << 23) + bad;
-#pragma unroll
-        for (int s = 0; s < KW; ++s) {
-          uint32_t v[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            v[j] = static_cast<uint32_t>(__float2int_rn(raw[n][s].get(j) * down)) + 0x808080u;
-          const uint32_t a01 = __byte_perm(v[0], v[1], 0x5140), a23 = __byte_perm(v[2], v[3], 0x5140);  // bytes 0, 1
-          qf[0][n][s] = __byte_perm(a01, a23, 0x5410) ^ 0x80808080u;
-          qf[1][n][s] = __byte_perm(a01, a23, 0x7632) ^ 0x80808080u;
-          qf[2][n][s] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410) ^ 0x80808080u;
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
-          cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e * (1.f / 2097152.f));
-          const int rr = 8 * n + 2 * t + j;
-          lim[n][j] = rr < n_rows ? q.len - q.q + row_at(a, row0 + rr).i : -1;
-          m[n][j] = kNone;
-          l[n][j] = 0.f;
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[n][s][j] = 0.f;
-      }
-    }
-
     // ---- one step: kStep slices ------------------------------------------------
-    cp_wait<S - 2>();
+    const uint32_t here = there;  // this step's slices
+    issue_k(par ^ 1);
+    cp_wait<2>();  // this step's K and scales
     __syncwarp();
-    issue(free_slot);
-    const uint32_t here = there >> (kStep * (S - 1));  // this step's slices
-    const uint4 tail = lds128(tail_of(slot));
+    const uint32_t slot = my_k + par * Geo::kHalf;
+    const uint4 tail = lds128(my_tails + par * Geo::kTail);
     float ksc[kStep] = {__uint_as_float(tail.x), __uint_as_float(tail.z)};
     float vsc[kStep] = {__uint_as_float(tail.y), __uint_as_float(tail.w)};
     const bool whole = __all_sync(0xffffffffu, p0 >= whole_lo && p0 <= whole_hi && (here & 3) == 3);
@@ -557,36 +588,43 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       }
     }
     if (__any_sync(0xffffffffu, any)) {
+      // scores: the slices' 16 positions x the rows, exact whole numbers
       float sc[kStep][NT][4];
+      uint32_t kw[kStep][KM][4];
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        // scores: the slice's 16 positions x the rows, exact whole numbers
-        uint32_t kw[KM][4];
+      for (int i = 0; i < kStep; ++i)
 #pragma unroll
         for (int s = 0; s < KM; ++s) {
           const uint32_t at = slot + i * Geo::kSliceBytes + k_place<D>(k_row, D == 16 ? 0 : 2 * s + k_half);
-          if constexpr (D == 16) ldmatrix2(kw[s], at);
-          else ldmatrix4(kw[s], at);
+          if constexpr (D == 16) ldmatrix2(kw[i][s], at);
+          else ldmatrix4(kw[i][s], at);
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          int hi[4], lo[4];
-          auto product = [&](int (&d)[4], int p, bool first) {
+      for (int n = 0; n < NT; ++n) {
+        int hi[kStep][4], lo[kStep][4];
+        auto product = [&](int (&d)[kStep][4], int p, bool first) {
+          uint32_t w[KM * 2];
+          query_words<KW>(w, queries + query_place<KW>(p, n, lane, 0, NT));
 #pragma unroll
-            for (int s = 0; s < KM; ++s) {
-              const uint32_t b1 = 2 * s + 1 < KW ? qf[p][n][2 * s + 1 < KW ? 2 * s + 1 : 0] : 0;
-              if (first && s == 0) mma16832_first(d, kw[s], qf[p][n][2 * s], b1);
-              else mma16832(d, kw[s], qf[p][n][2 * s], b1);
+          for (int s = 0; s < KM; ++s)
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+              if (first && s == 0) mma16832_first(d[i], kw[i][s], w[2 * s], w[2 * s + 1]);
+              else mma16832(d[i], kw[i][s], w[2 * s], w[2 * s + 1]);
             }
-          };
-          product(hi, 2, true);
-          product(lo, 0, true);
+        };
+        product(hi, 2, true);
+        product(lo, 0, true);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) hi[j] <<= 8;
-          product(hi, 1, false);
+        for (int i = 0; i < kStep; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sc[i][n][j] = fmaf(static_cast<float>(hi[j]), 256.f, static_cast<float>(lo[j]));
-        }
+          for (int j = 0; j < 4; ++j) hi[i][j] <<= 8;
+        product(hi, 1, false);
+#pragma unroll
+        for (int i = 0; i < kStep; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sc[i][n][j] = fmaf(static_cast<float>(hi[i][j]), 256.f, static_cast<float>(lo[i][j]));
       }
       // softmax: this lane has positions g, g + 8 of each slice for columns 2t, 2t + 1.  Weights are held relative to
       // the largest p x sv: the value scale's exponent joins the maximum
@@ -639,6 +677,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
                 if (x[i][n][j + r] != -INFINITY) x[i][n][j + r] = fmaf(sc[i][n][j + r], cs[n][j] * ksc[i], -nm);
           }
       }
+      cp_wait<1>();  // this step's V
+      __syncwarp();
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
         uint32_t pf[NP][NT][2];
@@ -670,7 +710,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
           for (int r = 0; r < 4; ++r) {
             // position 2t + (r & 1) + 8 (r >> 1); D = 64 and below keep odd positions 4 rows on
             const uint32_t step = (r & 1) * (D == 128 ? D : 4 * D) + (r >> 1) * 8 * D;
-            const uint32_t at = (slot + v_at + i * Geo::kSliceBytes + step) ^ (h && D >= 64 ? D / 2 : 0);
+            const uint32_t at = (my_v + v_at + i * Geo::kSliceBytes + step) ^ (h && D >= 64 ? D / 2 : 0);
             if constexpr (KS == 8) {
               const uint2 v = lds64(at);
               vw[h][r][0] = v.x;
@@ -716,28 +756,50 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       }
     }
     __syncwarp();
-    const uint32_t done = slot - my_ring;  // the slot just read: free until the next step
-    free_slot = slot;
-    slot += Geo::kSlot;
-    if (slot == ring_end) slot = my_ring;
     ++cur.unit;
     p0 += kUnit;
+    par ^= 1;
+    const bool last_of_item = cur.unit == q.nt || n_left == 1;
+    if (!last_of_item) {
+      cp_wait<1>();  // a step that no row saw has not waited for its V
+      issue_v();
+    }
 
     // ---- end of the item, or of this block's share of it --------------------
-    if (cur.unit == q.nt || n_left == 1) {
+    if (last_of_item) {
       const long long i0 = u0 + (n_units - n_left) + 1 - cur.unit, i1 = i0 + q.nt;
-      float *mine = reinterpret_cast<float *>(ring + warp * S * Geo::kSlot + done);
+      const DecReq q = cur.q;
+      const int hk = cur.h, row0_now = row0, n_rows_now = n_rows;
+      cur.next_item(a, bt);
+      if (n_left > 1) begin_item();
+      const bool all = i0 >= u0 && i1 <= u1;
+      const int c0 = all ? 0 : static_cast<int>(quotient(i0, share)), c1 = all ? 0 : static_cast<int>(quotient(i1 - 1, share));
+      float *part = a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart;
+      // a warp takes rows warp, warp + 4, ...; its lanes four dims each
+      constexpr int kLanes = D / 4 < 32 ? D / 4 : 32, kRowsAtOnce = kDecThreads / kLanes;
+      const int r_first = threadIdx.x / kLanes, d4 = threadIdx.x % kLanes;
+      auto store = [&](int r, float4 v, float lsum, float top) {
+        const float inv = lsum == 0.f ? 0.f : __fdividef(1.f, lsum);  // 0: the row saw nothing
+        const RowAt at_row = row_at(a, row0_now + r);
+        const int i = q.q0 + at_row.i, h = hk * G + at_row.h;
+        XT *dst = static_cast<XT *>(a.out) + i * a.o_row + h * a.o_head + 4 * d4;
+        store4(dst, a.o_vec, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        if (a.lse && d4 == 0) a.lse[static_cast<long long>(i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
+      };
+      cp_wait<1>();  // the outputs take the place of the step's V
+      __syncwarp();
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {  // eight rows at a time
+        float *mine = reinterpret_cast<float *>(ring + (warp * 3 + 2) * Geo::kHalf);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float sum = l[n][j];
 #pragma unroll
           for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-          const int r = 8 * n + 2 * t + j;
+          const int r = 2 * t + j;
           if (g == 0) {
-            s_m[warp][r] = m[n][j];
-            s_l[warp][r] = sum;
+            s_m[warp][8 * n + r] = m[n][j];
+            s_l[warp][8 * n + r] = sum;
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -753,53 +815,37 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
             }
           }
         }
-      const DecReq q = cur.q;
-      const int hk = cur.h, row0_now = row0, n_rows_now = n_rows;
-      cur.next_item(a, bt);
-      if (n_left > 1) begin_item();
-      fresh = true;
-      __syncthreads();
-      const bool all = i0 >= u0 && i1 <= u1;
-      float *part = a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart;
-      // a warp takes rows warp, warp + 4, ...; its lanes four dims each
-      constexpr int kLanes = D / 4 < 32 ? D / 4 : 32, kRowsAtOnce = kDecThreads / kLanes;
-      const int r_first = threadIdx.x / kLanes, d4 = threadIdx.x % kLanes;
-      auto store = [&](int r, float4 v, float lsum, float top) {
-        const float inv = lsum == 0.f ? 0.f : __fdividef(1.f, lsum);  // 0: the row saw nothing
-        const RowAt at_row = row_at(a, row0_now + r);
-        const int i = q.q0 + at_row.i, h = hk * G + at_row.h;
-        XT *dst = static_cast<XT *>(a.out) + i * a.o_row + h * a.o_head + 4 * d4;
-        store4(dst, a.o_vec, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-        if (a.lse && d4 == 0) a.lse[static_cast<long long>(i) * a.g.H + h] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
-      };
-      for (int r = r_first; r < n_rows_now; r += kRowsAtOnce) {
-        float sm[kDecWarps], top = kNone;
+        __syncthreads();
+        for (int r8 = r_first; r8 < min(8, n_rows_now - 8 * n); r8 += kRowsAtOnce) {
+          const int r = 8 * n + r8;
+          float sm[kDecWarps], top = kNone;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) {
-          sm[w] = s_m[w][r];
-          top = fmaxf(top, sm[w]);
-        }
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float lsum = 0.f;
+          for (int w = 0; w < kDecWarps; ++w) {
+            sm[w] = s_m[w][r];
+            top = fmaxf(top, sm[w]);
+          }
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          float lsum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) {
-          const float f = exp2_fast(sm[w] - top);
-          const float4 y = reinterpret_cast<const float4 *>(ring + w * S * Geo::kSlot + done)[merge_place<D>(r, d4)];
-          lsum += s_l[w][r] * f;
-          v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
-        }
-        if (all) {
-          store(r, v, lsum, top);
-        } else {
-          *reinterpret_cast<float4 *>(part + r * D + 4 * d4) = v;
-          if (d4 == 0) {
-            part[ROWS * D + r] = top;
-            part[ROWS * D + ROWS + r] = lsum;
+          for (int w = 0; w < kDecWarps; ++w) {
+            const float f = exp2_fast(sm[w] - top);
+            const float4 y = reinterpret_cast<const float4 *>(ring + (w * 3 + 2) * Geo::kHalf)[merge_place<D>(r8, d4)];
+            lsum += s_l[w][r] * f;
+            v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
+          }
+          if (all) {
+            store(r, v, lsum, top);
+          } else {
+            *reinterpret_cast<float4 *>(part + r * D + 4 * d4) = v;
+            if (d4 == 0) {
+              part[ROWS * D + r] = top;
+              part[ROWS * D + ROWS + r] = lsum;
+            }
           }
         }
+        if (NT > 1 && n + 1 < NT) __syncthreads();
       }
       if (!all) {
-        const int c0 = static_cast<int>(quotient(i0, share)), c1 = static_cast<int>(quotient(i1 - 1, share));
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) s_last = atomicAdd(a.ticket + c0, 1) == c1 - c0;
@@ -839,14 +885,16 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
           if (threadIdx.x == 0) a.ticket[c0] = 0;
         }
       }
+      if (n_left > 1) put_queries();
       __syncthreads();
+      issue_v();
     }
   }
 }
 
 template <int D, int NT>
 constexpr int dec_smem_bytes(int B) {
-  return DecGeom<D, NT>::kRing + (B + 1) * static_cast<int>(sizeof(long long)) + 3 * B * static_cast<int>(sizeof(int));
+  return DecGeom<D, NT>::kFixed + (B + 1) * static_cast<int>(sizeof(long long)) + 3 * B * static_cast<int>(sizeof(int));
 }
 
 template <typename XT, int D, int NT>
