@@ -7,7 +7,10 @@
 // likeliest one has weight 0; the uniforms have 24 bits, so it could hardly be
 // drawn.  A cut (top-k by count, top-p by mass) is a pair (key, ties): tokens
 // with a larger z, and the first `ties` tokens in index order with that z.
+#include <cooperative_groups.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "status.cuh"
@@ -16,7 +19,14 @@ namespace specdec {
 
 namespace {
 
-constexpr int kSampleThreads = 1024;
+constexpr int kThreads = 512;        // of a block; a cluster of blocks takes a row
+constexpr int kSlice = 16384;        // tokens of a block where the row count gives enough blocks
+constexpr int kMaxSlice = 40960;     // tokens that a block's shared memory holds
+constexpr int kMaxCluster = 8;
+constexpr int kBins = 128;
+constexpr int kCap = 2048;           // tokens of the band in which a cut is settled exactly
+constexpr float kFar = 22.2f;        // nats below the maximum from which the weight is 0: 2^31 exp(-22.2) < 1
+constexpr int kLevels = 4;
 
 struct SampleArgs {
   const void *logits;
@@ -27,6 +37,7 @@ struct SampleArgs {
   const float *top_p, *min_p, *u;
   int32_t *tokens;
   float *probs;
+  int slice;  // tokens of a block (a multiple of 8)
 };
 
 using u64 = unsigned long long;
@@ -47,45 +58,126 @@ __device__ __forceinline__ u64 part_of(u64 f, u64 total) { return f * (total >> 
 __device__ __forceinline__ float weight_e(float z, float zmax) { return z == zmax ? 1.f : expf(__fsub_rn(z, zmax)); }
 __device__ __forceinline__ uint32_t weight_w(float e) { return static_cast<uint32_t>(e * 2147483648.f); }
 
-// Exclusive prefix of v over the block; *total gets the sum.
-__device__ __forceinline__ u64 block_scan(u64 v, u64 *red, u64 *total) {
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  u64 inc = v;
+// A logit's z: NaN counts as -infinity.
+struct Scale {
+  float T, inv;  // temperature and its reciprocal (the latter for estimates only)
+  __device__ __forceinline__ float z(float l) const { return T == 1.f ? l : __fdiv_rn(l, T); }
+};
+__device__ __forceinline__ float no_nan(float l) { return isnan(l) ? -INFINITY : l; }
+
+__device__ __forceinline__ u64 warp_sum_u64(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ u64 warp_scan_u64(u64 v) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 n = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += n;
+    const u64 n = __shfl_up_sync(0xffffffffu, v, o);
+    if (static_cast<int>(threadIdx.x & 31) >= o) v += n;
   }
+  return v;
+}
+// Sum over the block, in every thread; red holds a value per warp.
+__device__ __forceinline__ u64 block_sum_u64(u64 v, u64 *red) {
+  v = warp_sum_u64(v);
   __syncthreads();
-  if (lane == 31) red[wid] = inc;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  u64 all = 0;
+  for (int w = 0; w < kThreads / 32; ++w) all += red[w];
+  return all;
+}
+// Exclusive prefix over the block; *total gets the sum.
+__device__ __forceinline__ u64 block_scan_u64(u64 v, u64 *red, u64 *total) {
+  const u64 inc = warp_scan_u64(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = inc;
   __syncthreads();
   u64 run = inc - v, all = 0;
-  for (int w = 0; w < kSampleThreads / 32; ++w) {
-    if (w < wid) run += red[w];
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < static_cast<int>(threadIdx.x >> 5)) run += red[w];
     all += red[w];
   }
   *total = all;
   return run;
 }
 
+// Radix selection, 8 bits a pass, by the whole block.  each(f) calls
+// f(value, weight) for every entry; returns the value v at which the sum of
+// weights over descending values first reaches `want` (at least 1), and in
+// *left want minus the sum over values above v, in *at the weight at v.
+template <typename Each>
+__device__ uint32_t radix_select(u64 want, Each &&each, u64 *hist, u64 *out, u64 *left, u64 *at) {
+  uint32_t value = 0;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256; i += kThreads) hist[i] = 0;
+    __syncthreads();
+    each([&](uint32_t v, u64 w) {
+      if (shift == 24 || (v >> (shift + 8)) == (value >> (shift + 8))) atomicAdd(&hist[(v >> shift) & 255], w);
+    });
+    __syncthreads();
+    if (threadIdx.x < 32) {  // lane l holds bins 255 - 8 l .. 248 - 8 l, in descending order
+      const int lane = threadIdx.x;
+      u64 mine = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += hist[255 - 8 * lane - i];
+      const u64 inc = warp_scan_u64(mine);
+      const uint32_t reach = __ballot_sync(0xffffffffu, inc >= want);
+      const int who = reach ? __ffs(reach) - 1 : 31;
+      if (lane == who) {
+        u64 run = inc - mine;
+        int bin = 255 - 8 * lane;
+        for (int i = 0; i < 7 && run + hist[bin] < want; ++i) run += hist[bin--];
+        out[0] = bin;
+        out[1] = want - run;
+        out[2] = hist[bin];
+      }
+    }
+    __syncthreads();
+    value |= static_cast<uint32_t>(out[0]) << shift;
+    want = out[1];
+  }
+  *left = want;
+  *at = out[2];
+  __syncthreads();
+  return value;
+}
+
+// The tokens kept so far: those with a larger key, and those with this key up
+// to index idx.  Logits above hi have a larger key for sure, those below lo a
+// smaller one; between them the key decides.
+struct Cut {
+  uint32_t key;
+  int idx;
+  float lo, hi;
+};
+__device__ __forceinline__ bool kept_by(const Cut &c, const Scale &sc, float l, int idx) {
+  if (l > c.hi) return true;
+  if (!(l >= c.lo)) return false;
+  const uint32_t k = float_key(sc.z(l));
+  return k > c.key || (k == c.key && idx <= c.idx);
+}
+
+// The whole row by one block, straight from global memory: for rows whose cut
+// the estimates below cannot settle (over kCap equal logits at the cut, scaled
+// logits outside the normal range) and for vocabularies that do not fit the
+// cluster's shared memory.
 template <typename XT>
-__global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const SampleArgs a) {
-  __shared__ float redf[32];
-  __shared__ int redi[32];
-  __shared__ u64 red[32];
-  __shared__ u64 hist[256];
-  __shared__ uint32_t s_key;
-  __shared__ u64 s_left;
-  const int b = blockIdx.x, V = a.V;
+__device__ void sample_whole_row(const SampleArgs &a, int b, u64 *hist, u64 *red, u64 *out) {
   const XT *x = static_cast<const XT *>(a.logits) + b * a.row_stride;
   const float T = a.temperature ? a.temperature[b] : 1.f;
   const bool greedy = !(T > 0.f);
+  const int V = a.V;
   auto zat = [&](int i) {
-    const float l = to_f32(x[i]);
-    return isnan(l) ? -INFINITY : greedy ? l : __fdiv_rn(l, T);
+    const float l = no_nan(to_f32(x[i]));
+    return greedy ? l : __fdiv_rn(l, T);
   };
+  __shared__ float redf[32];
+  __shared__ int redi[32];
   ArgMax am{-INFINITY, 0x7fffffff};
-  for (int i = threadIdx.x; i < V; i += kSampleThreads) am = argmax_merge(am, {zat(i), i});
+  for (int i = threadIdx.x; i < V; i += kThreads) am = argmax_merge(am, {zat(i), i});
   am = block_argmax(am, redf, redi);
   const float zmax = am.v;
   if (zmax == -INFINITY || greedy) {
@@ -98,97 +190,58 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
   const int k = a.top_k ? a.top_k[b] : 0;
   const float top_p = a.top_p ? a.top_p[b] : 1.f;
   const float min_e = a.min_p ? fminf(a.min_p[b], 1.f) : 0.f;
-  // the cut so far: every token
-  uint32_t cut = 0;
-  int ties = V;
-  // Finds the key at which the running sum of f over descending keys of the
-  // kept tokens reaches `want` (the sum over larger keys is below it), 8 bits
-  // a pass; `left` = want minus the sum over larger keys.
-  auto select = [&](u64 want, auto &&f) {
-    uint32_t key = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kSampleThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < V; i += kSampleThreads) {
+  uint32_t cut = 0;  // no key is 0
+  u64 ties = 0, left, at;
+  if (k > 0 && k < V) {
+    cut = radix_select(k, [&](auto &&f) { for (int i = threadIdx.x; i < V; i += kThreads) f(float_key(zat(i)), u64(1)); },
+                       hist, out, &left, &at);
+    ties = left;
+  }
+  if (top_p < 1.f) {
+    u64 mass = 0;
+    for (int i = threadIdx.x; i < V; i += kThreads) {
+      const float z = zat(i);
+      if (float_key(z) > cut) mass += weight_w(weight_e(z, zmax));
+    }
+    mass = block_sum_u64(mass, red) + ties * (cut ? weight_w(weight_e(key_float(cut), zmax)) : 0);
+    u64 most = part_of(static_cast<u64>(rintf(fmaxf(top_p, 0.f) * 16777216.f)), mass);
+    if (most < 1) most = 1;
+    const uint32_t kc = cut;
+    const u64 kt = ties;
+    cut = radix_select(most, [&](auto &&f) {
+      for (int i = threadIdx.x; i < V; i += kThreads) {
         const float z = zat(i);
         const uint32_t kk = float_key(z);
-        if (shift == 24 || (kk >> (shift + 8)) == (key >> (shift + 8))) atomicAdd(&hist[(kk >> shift) & 255], f(z, kk));
+        if (kk >= kc) f(kk, static_cast<u64>(weight_w(weight_e(z, zmax))));
       }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        u64 run = 0;
-        int bin = 255;
-        for (; bin > 0; --bin) {
-          if (run + hist[bin] >= want) break;
-          run += hist[bin];
-        }
-        s_key = key | static_cast<uint32_t>(bin) << shift;
-        s_left = want - run;
-      }
-      __syncthreads();
-      key = s_key;
-      want = s_left;
-      __syncthreads();
-    }
-    return key;
-  };
-  if (k > 0 && k < V) {
-    cut = select(k, [&](float, uint32_t) { return u64(1); });
-    ties = static_cast<int>(s_left);
-  }
-  auto sum_kept = [&]() {
-    u64 s = 0, total;
-    for (int i = threadIdx.x; i < V; i += kSampleThreads) {
-      const float z = zat(i);
-      if (float_key(z) > cut) s += weight_w(weight_e(z, zmax));
-    }
-    block_scan(s, red, &total);
-    return total;
-  };
-  if (top_p < 1.f) {
-    const u64 cw = weight_w(weight_e(key_float(cut), zmax));
-    u64 mass = sum_kept();
-    if (cut == 0) ties = 0;  // no token has key 0
-    mass += static_cast<u64>(ties) * cw;
-    const u64 p24 = static_cast<u64>(rintf(fmaxf(top_p, 0.f) * 16777216.f));
-    u64 most = part_of(p24, mass);
-    if (most < 1) most = 1;
-    // the mass over larger keys reaches `most`: inside the top-k set
-    const uint32_t kc = cut;
-    const int kt = ties;
-    const uint32_t pc = select(most, [&](float z, uint32_t kk) {
-      return kk >= kc ? static_cast<u64>(weight_w(weight_e(z, zmax))) : 0ull;
-    });
-    const u64 w = weight_w(weight_e(key_float(pc), zmax));
-    const u64 n = w ? (s_left + w - 1) / w : 0;
-    ties = static_cast<int>(min(n, static_cast<u64>(pc == kc ? kt : V)));
-    cut = pc;
+    }, hist, out, &left, &at);
+    const u64 w = weight_w(weight_e(key_float(cut), zmax));
+    ties = w ? (left + w - 1) / w : 0;
+    if (cut == kc) ties = min(ties, kt);
   }
   // running sums in index order, one run of tokens a thread
-  const int per = (V + kSampleThreads - 1) / kSampleThreads;
+  const int per = (V + kThreads - 1) / kThreads;
   const int i0 = min(V, static_cast<int>(threadIdx.x) * per), i1 = min(V, i0 + per);
   u64 nt = 0, total;
   for (int i = i0; i < i1; ++i) nt += float_key(zat(i)) == cut;
-  const u64 t0 = block_scan(nt, red, &total);
-  auto run_over = [&](u64 sum, auto &&at) {
+  const u64 t0 = block_scan_u64(nt, red, &total);
+  auto run_over = [&](u64 sum, auto &&stop) {
     u64 tie = t0;
     for (int i = i0; i < i1; ++i) {
       const float z = zat(i);
       const uint32_t kk = float_key(z);
-      bool keep = kk > cut;
-      if (kk == cut) keep = tie++ < static_cast<u64>(ties);
+      if (!(kk > cut || (kk == cut && tie++ < ties))) continue;
       const float e = weight_e(z, zmax);
-      if (!keep || !(e >= min_e)) continue;
+      if (!(e >= min_e)) continue;
       const u64 w = weight_w(e);
-      if (at(i, sum, w)) return sum;
+      if (stop(i, sum, w)) return sum;
       sum += w;
     }
     return sum;
   };
   const u64 mine = run_over(0, [](int, u64, u64) { return false; });
-  const u64 before = block_scan(mine, red, &total);
-  const float uu = a.u[b];
-  const u64 u24 = static_cast<u64>(fminf(fmaxf(uu * 16777216.f, 0.f), 16777215.f));
+  const u64 before = block_scan_u64(mine, red, &total);
+  const u64 u24 = static_cast<u64>(fminf(fmaxf(a.u[b] * 16777216.f, 0.f), 16777215.f));
   const u64 target = part_of(u24, total);
   if (target >= before && target < before + mine)
     run_over(before, [&](int i, u64 sum, u64 w) {
@@ -197,6 +250,416 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
       if (a.probs) a.probs[b] = __fdiv_rn(static_cast<float>(w), static_cast<float>(total));
       return true;
     });
+}
+
+template <typename XT>
+__global__ void __launch_bounds__(kThreads) sample_whole_kernel(const SampleArgs a) {
+  __shared__ u64 hist[256], red[32], out[3];
+  sample_whole_row<XT>(a, blockIdx.x, hist, red, out);
+}
+
+// What the blocks of a cluster tell each other: every block writes its own
+// entry in every block's copy, then the cluster meets.
+struct Shared {
+  float high[kMaxCluster];
+  int first[kMaxCluster];
+  uint32_t counts[kMaxCluster][kBins];
+  u64 mass[kMaxCluster], above[kMaxCluster];
+  int n[kMaxCluster];
+  float min_above[kMaxCluster], max_below[kMaxCluster];
+  Cut cut;
+  int slow;
+  // of this block alone
+  u64 hist[256], red[32], out[3];
+  uint32_t total[kBins];
+  float redf[32];
+  int redi[32], n_local, band[2];
+};
+
+// Eight logits from a 16- or 32-byte run.
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// One row per cluster, its logits read once and held in the blocks' shared
+// memory.  A cut (top-k by count, top-p by mass) is found from the outside in:
+// the counts of tokens in 128 bins of their distance to the maximum (each lane
+// of a warp counts in a column of its own, so no two lanes meet in a bank or a
+// word) give the bins in which the cut lies -- for a mass by bounds, since a
+// bin's weights differ by at most its width --, the tokens of those bins are
+// listed, or binned again where they are too many, and the exact cut is
+// selected from the list in whole numbers.  The list is checked to hold the
+// cut: what lies outside it is strictly above or below; a row that fails, and
+// one that never narrows, is done by sample_whole_row.
+template <typename XT>
+__global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleArgs a) {
+  namespace cg = cooperative_groups;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  extern __shared__ __align__(16) unsigned char sample_smem[];
+  Shared &sh = *reinterpret_cast<Shared *>(sample_smem);
+  uint32_t *columns = reinterpret_cast<uint32_t *>(sample_smem + sizeof(Shared));  // [kBins][32]
+  uint2 *list = reinterpret_cast<uint2 *>(columns);                               // [kCap] (logit, index), after the counts
+  uint2 *merged = list + kCap;                                                    // [kCap] of the cluster, in block 0
+  float *row = reinterpret_cast<float *>(merged + kCap);                          // [slice + 16]
+  auto meet = [&]() { cluster.sync(); };
+  auto tell = [&](auto *p, auto v) {  // writes *p in every block
+    for (int r = 0; r < C; ++r) *cluster.map_shared_rank(p, r) = v;
+  };
+
+  // ---- the slice, its maximum ------------------------------------------------
+  const int V = a.V, i_begin = min(V, rank * a.slice), i_end = min(V, i_begin + a.slice), n = i_end - i_begin;
+  const XT *x = static_cast<const XT *>(a.logits) + b * a.row_stride + i_begin;
+  // the first `head` tokens come before a 16-byte boundary; token i lies at row[i + 8 - head], so that runs of eight
+  // are aligned in shared memory too
+  constexpr int kAlign = 16 / sizeof(XT);
+  const int head = min(n, static_cast<int>((kAlign - reinterpret_cast<uintptr_t>(x) / sizeof(XT) % kAlign) % kAlign));
+  const int off = 8 - head, n4 = (n + off + 3) / 4;  // float4s of the row, its edges filled with -infinity
+  const float T = a.temperature ? a.temperature[b] : 1.f;
+  const bool greedy = !(T > 0.f);
+  float high = -INFINITY;
+  for (int i = tid; i < off; i += kThreads) row[i] = -INFINITY;
+  for (int i = n + off + tid; i < 4 * n4; i += kThreads) row[i] = -INFINITY;
+  for (int i = tid; i < head; i += kThreads) {
+    const float l = no_nan(to_f32(x[i]));
+    row[i + off] = l;
+    high = fmaxf(high, l);
+  }
+  const int runs = (n - head) / 8;
+#pragma unroll 4
+  for (int i = tid; i < runs; i += kThreads) {
+    float v[8];
+    load8(x + head + 8 * i, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = no_nan(v[j]);
+      high = fmaxf(high, v[j]);
+    }
+    *reinterpret_cast<float4 *>(row + 8 + 8 * i) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(row + 12 + 8 * i) = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  for (int i = head + 8 * runs + tid; i < n; i += kThreads) {
+    const float l = no_nan(to_f32(x[i]));
+    row[i + off] = l;
+    high = fmaxf(high, l);
+  }
+  high = block_max(high, sh.redf);
+  if (tid == 0) tell(&sh.high[rank], high);
+  meet();
+  high = -INFINITY;
+  for (int r = 0; r < C; ++r) high = fmaxf(high, sh.high[r]);
+  // every pass: f(logit, index in the row)
+  auto each = [&](auto &&f) {
+    for (int q = tid; q < n4; q += kThreads) {
+      const float4 v = reinterpret_cast<const float4 *>(row)[q];
+      const int i = i_begin + 4 * q - off;
+      f(v.x, i);
+      f(v.y, i + 1);
+      f(v.z, i + 2);
+      f(v.w, i + 3);
+    }
+  };
+  if (high == -INFINITY || greedy) {
+    int first = 0x7fffffff;
+    if (greedy && high != -INFINITY)
+      each([&](float l, int i) { if (l == high) first = min(first, i); });
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) sh.redi[warp] = first;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kThreads / 32; ++w) first = min(first, sh.redi[w]);
+      *cluster.map_shared_rank(&sh.first[rank], 0) = first;
+    }
+    meet();
+    if (rank == 0 && tid == 0) {
+      for (int r = 0; r < C; ++r) first = min(first, sh.first[r]);
+      a.tokens[b] = high == -INFINITY ? -1 : first;
+      if (a.probs) a.probs[b] = high == -INFINITY ? 0.f : 1.f;
+    }
+    return;
+  }
+  const Scale sc{T, 1.f / T};
+  const float zmax = sc.z(high);
+  const int k = a.top_k ? a.top_k[b] : 0;
+  const float top_p = a.top_p ? a.top_p[b] : 1.f;
+  const float min_e = a.min_p ? fminf(a.min_p[b], 1.f) : 0.f;
+  const bool has_k = k > 0 && k < V, has_p = top_p < 1.f;
+  // temperatures and logits for which equal z means nearly equal logits
+  bool slow = !(T >= 9.1e-13f && T <= 1.1e12f && fabsf(high) < 1.2e24f);
+  Cut cut{0, -1, -INFINITY, -INFINITY};
+  auto far_of = [&](float l) { return (high - l) * sc.inv; };  // the distance to the maximum, falling with l
+
+  // The cut at which the count (or mass) over descending z first reaches `want`, among the tokens that `in` keeps.
+  auto search = [&](bool by_mass, u64 want, const Cut in) {
+    float lo = 0.f, hi = kFar;
+    u64 base = 0;  // count or mass above lo
+    for (int level = 0; level < kLevels; ++level) {
+      const float width = (hi - lo) * (1.f / kBins), per = 1.f / width;
+      for (int i = tid; i < kBins * 32; i += kThreads) columns[i] = 0;
+      __syncthreads();
+      each([&](float l, int i) {
+        const float d = far_of(l);
+        if (d >= lo && d < hi && kept_by(in, sc, l, i))
+          atomicAdd(&columns[min(kBins - 1, static_cast<int>((d - lo) * per)) * 32 + lane], 1u);
+      });
+      __syncthreads();
+      for (int j = warp; j < kBins; j += kThreads / 32) {
+        const uint32_t c = __reduce_add_sync(0xffffffffu, columns[j * 32 + lane]);
+        if (lane == 0) tell(&sh.counts[rank][j], c);
+      }
+      meet();
+      if (warp == 0) {  // lane l: bins 4 l .. 4 l + 3
+        u64 c[4], some = 0, most = 0;
+        float w_hi[4], w_lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          c[j] = 0;
+          for (int r = 0; r < C; ++r) c[j] += sh.counts[r][4 * lane + j];
+          const float d = lo + (4 * lane + j) * width;
+          w_hi[j] = by_mass ? fminf(expf(-d) * 1.0001f, 1.f) * 2147483648.f : 1.f;
+          w_lo[j] = by_mass ? fmaxf(expf(-(d + width)) * 0.9999f * 2147483648.f - 1.f, 0.f) : 1.f;
+          most += c[j] * static_cast<u64>(by_mass ? ceilf(w_hi[j]) : 1.f);
+          some += c[j] * static_cast<u64>(w_lo[j]);
+        }
+        u64 run_hi = base + warp_scan_u64(most) - most, run_lo = base + warp_scan_u64(some) - some;
+        // the first bin that may reach `want`, and the first that must
+        int first = kBins, sure = kBins;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          run_hi += c[j] * static_cast<u64>(by_mass ? ceilf(w_hi[j]) : 1.f);
+          run_lo += c[j] * static_cast<u64>(w_lo[j]);
+          if (run_hi >= want) first = min(first, 4 * lane + j);
+          if (run_lo >= want) sure = min(sure, 4 * lane + j);
+        }
+        first = __reduce_min_sync(0xffffffffu, first);
+        sure = __reduce_min_sync(0xffffffffu, sure);
+        if (lane == 0) {
+          sh.band[0] = first;
+          sh.band[1] = sure;
+        }
+      }
+      __syncthreads();
+      const int b0 = sh.band[0], b1 = min(sh.band[1], kBins - 1);
+      if (b0 == kBins) {
+        if (!by_mass && level == 0) return in;  // the cut lies among tokens of weight 0: every other is kept
+        slow = true;
+        return in;
+      }
+      const float new_lo = b0 == 0 ? lo : lo + (b0 - 0.02f) * width, new_hi = b1 == kBins - 1 ? hi : lo + (b1 + 1.02f) * width;
+      // what lies above the band, and the band's tokens
+      if (tid == 0) sh.n_local = 0;
+      __syncthreads();
+      u64 above = 0;
+      float min_above = INFINITY, max_below = -INFINITY;
+      each([&](float l, int i) {
+        const float d = far_of(l);
+        if (!(d < kFar) || !kept_by(in, sc, l, i)) return;
+        if (d < new_lo) {
+          above += by_mass ? weight_w(weight_e(sc.z(l), zmax)) : 1u;
+          min_above = fminf(min_above, l);
+        } else if (d < new_hi) {
+          const int at = atomicAdd(&sh.n_local, 1);
+          if (at < kCap) list[at] = make_uint2(__float_as_uint(l), i);
+        } else {
+          max_below = fmaxf(max_below, l);
+        }
+      });
+      above = block_sum_u64(above, sh.red);
+      min_above = -block_max(-min_above, sh.redf);
+      max_below = block_max(max_below, sh.redf);
+      if (tid == 0) {
+        tell(&sh.above[rank], above);
+        tell(&sh.n[rank], sh.n_local);
+        tell(&sh.min_above[rank], min_above);
+        tell(&sh.max_below[rank], max_below);
+      }
+      meet();
+      base = 0;
+      int n_all = 0;
+      for (int r = 0; r < C; ++r) {
+        base += sh.above[r];
+        n_all += sh.n[r];
+        min_above = fminf(min_above, sh.min_above[r]);
+        max_below = fmaxf(max_below, sh.max_below[r]);
+      }
+      if (n_all > kCap) {  // too many: bin them again
+        lo = new_lo;
+        hi = new_hi;
+        meet();  // the entries above have been read
+        continue;
+      }
+      if (rank == 0) {
+        for (int r = 0, at = 0; r < C; at += sh.n[r++]) {
+          const uint2 *src = cluster.map_shared_rank(list, r);
+          for (int i = tid; i < sh.n[r]; i += kThreads) {
+            const uint2 e = src[i];
+            merged[at + i] = make_uint2(float_key(sc.z(__uint_as_float(e.x))), e.y);
+          }
+        }
+        __syncthreads();
+        u64 all = 0;
+        for (int i = tid; i < n_all; i += kThreads)
+          all += by_mass ? weight_w(weight_e(key_float(merged[i].x), zmax)) : 1u;
+        all = block_sum_u64(all, sh.red);
+        bool bad = !(base < want && want <= base + all);
+        Cut c = in;
+        if (!bad) {
+          u64 left, at;
+          c.key = radix_select(want - base, [&](auto &&f) {
+            for (int i = tid; i < n_all; i += kThreads)
+              f(merged[i].x, by_mass ? static_cast<u64>(weight_w(weight_e(key_float(merged[i].x), zmax))) : u64(1));
+          }, sh.hist, sh.out, &left, &at);
+          const float z = key_float(c.key);
+          const u64 w = by_mass ? weight_w(weight_e(z, zmax)) : 1u;
+          const u64 ties = (left + w - 1) / w;  // w > 0: the sum was reached here
+          c.idx = 0x7fffffff;
+          if (at > ties * w) {  // not all of them: those with the lowest indexes
+            u64 l2, a2;
+            c.idx = static_cast<int>(~radix_select(ties, [&](auto &&f) {
+              for (int i = tid; i < n_all; i += kThreads)
+                if (merged[i].x == c.key) f(~merged[i].y, u64(1));
+            }, sh.hist, sh.out, &l2, &a2));
+          }
+          if (c.key == in.key) c.idx = min(c.idx, in.idx);
+          const float l = z * T, margin = fabsf(l) * 1e-6f + 8.3e-25f;
+          c.lo = l - margin;
+          c.hi = l + margin;
+          // the tokens with this key are all listed, or cut off already
+          bad = float_key(sc.z(min_above)) <= c.key || float_key(sc.z(max_below)) >= c.key;
+        }
+        if (tid == 0) {
+          tell(&sh.cut, c);
+          tell(&sh.slow, bad ? 1 : 0);
+        }
+      }
+      meet();
+      slow = sh.slow != 0;
+      return sh.cut;
+    }
+    slow = true;
+    return in;
+  };
+
+  if (!slow && has_k) cut = search(false, k, cut);
+  if (!slow && has_p) {
+    u64 mass = 0;
+    each([&](float l, int i) {
+      if (far_of(l) < kFar && kept_by(cut, sc, l, i)) mass += weight_w(weight_e(sc.z(l), zmax));
+    });
+    mass = block_sum_u64(mass, sh.red);
+    if (tid == 0) tell(&sh.mass[rank], mass);
+    meet();
+    mass = 0;
+    for (int r = 0; r < C; ++r) mass += sh.mass[r];
+    u64 most = part_of(static_cast<u64>(rintf(fmaxf(top_p, 0.f) * 16777216.f)), mass);
+    cut = search(true, most < 1 ? 1 : most, cut);
+  }
+  if (slow) {
+    if (rank == 0) sample_whole_row<XT>(a, b, sh.hist, sh.red, sh.out);
+    return;
+  }
+
+  // ---- the draw: running sums in index order, a run of float4s a warp -----------
+  const int seg = (n4 + kThreads / 32 - 1) / (kThreads / 32);
+  const int q0 = min(n4, warp * seg), q1 = min(n4, q0 + seg);
+  // a logit below this one has e < min_p for sure
+  const float low = min_e > 0.f ? high + T * (logf(min_e) - 1e-3f) - fabsf(high) * 1e-5f : -INFINITY;
+  auto weight_at = [&](float l, int i) -> u64 {
+    if (!(far_of(l) < kFar) || l < low || !kept_by(cut, sc, l, i)) return 0;
+    const float e = weight_e(sc.z(l), zmax);
+    return e >= min_e ? weight_w(e) : 0u;
+  };
+  u64 mine = 0;
+  for (int q = q0 + lane; q < q1; q += 32) {
+    const float4 v = reinterpret_cast<const float4 *>(row)[q];
+    const int i = i_begin + 4 * q - off;
+    mine += weight_at(v.x, i) + weight_at(v.y, i + 1) + weight_at(v.z, i + 2) + weight_at(v.w, i + 3);
+  }
+  mine = warp_sum_u64(mine);
+  __syncthreads();
+  if (lane == 0) sh.red[warp] = mine;
+  __syncthreads();
+  u64 before = 0, total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += sh.red[w];
+    total += sh.red[w];
+  }
+  if (tid == 0) tell(&sh.mass[rank], total);
+  meet();
+  total = 0;
+  for (int r = 0; r < C; ++r) {
+    if (r < rank) before += sh.mass[r];
+    total += sh.mass[r];
+  }
+  const u64 u24 = static_cast<u64>(fminf(fmaxf(a.u[b] * 16777216.f, 0.f), 16777215.f));
+  const u64 target = part_of(u24, total);
+  if (target < before || target >= before + mine) return;
+  for (int q = q0; q < q1; q += 32) {
+    u64 w[4] = {0, 0, 0, 0};
+    const int i = i_begin + 4 * (q + lane) - off;
+    if (q + lane < q1) {
+      const float4 v = reinterpret_cast<const float4 *>(row)[q + lane];
+      w[0] = weight_at(v.x, i);
+      w[1] = weight_at(v.y, i + 1);
+      w[2] = weight_at(v.z, i + 2);
+      w[3] = weight_at(v.w, i + 3);
+    }
+    const u64 sum = w[0] + w[1] + w[2] + w[3], inc = warp_scan_u64(sum);
+    const u64 all = __shfl_sync(0xffffffffu, inc, 31);
+    if (target < before + all) {
+      u64 run = before + inc - sum;
+      if (target >= run && target < run + sum) {
+        int j = 0;
+        while (target >= run + w[j]) run += w[j++];
+        a.tokens[b] = i + j;
+        if (a.probs) a.probs[b] = __fdiv_rn(static_cast<float>(w[j]), static_cast<float>(total));
+      }
+      return;
+    }
+    before += all;
+  }
+}
+
+size_t cluster_smem(int slice) {
+  return sizeof(Shared) + 2 * kCap * sizeof(uint2) + (static_cast<size_t>(slice) + 16) * sizeof(float);
+}
+
+template <typename XT>
+void launch(const SampleArgs &args, cudaStream_t st) {
+  SampleArgs a = args;
+  // a block for every kSlice tokens; more where the rows alone would leave multiprocessors idle (148 of them), down to
+  // 2,048 tokens a block, below which the meetings cost more than the passes
+  int c = 1;
+  while (c < kMaxCluster && (a.V > c * kSlice || (a.rows * c < 148 && a.V > c * 2048))) c *= 2;
+  a.slice = ((a.V + c - 1) / c + 7) / 8 * 8;
+  if (a.slice > kMaxSlice) {
+    op_launch("specdec_sample", sample_whole_kernel<XT>, dim3(a.rows), kThreads, 0, st, 1, a);
+    return;
+  }
+  const size_t smem = cluster_smem(a.slice);
+  static std::atomic<unsigned long long> ready{0};  // devices whose kernel has its shared memory limit
+  int device = 0;
+  op_cuda(cudaGetDevice(&device), "cudaGetDevice");
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(ready.load() & bit)) {
+    op_cuda(cudaFuncSetAttribute(sample_cluster_kernel<XT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(cluster_smem(kMaxSlice))),
+            "cudaFuncSetAttribute");
+    ready.fetch_or(bit);
+  }
+  op_launch("specdec_sample", sample_cluster_kernel<XT>, dim3(static_cast<unsigned>(a.rows) * c), kThreads, smem, st, c, a);
 }
 
 }  // namespace
@@ -214,11 +677,9 @@ extern "C" int specdec_sample(const void *logits, int dtype, int rows, int vocab
     op_check(row_stride >= vocab || rows <= 1, "row_stride must be at least vocab");
     if (rows == 0) return;
     op_check(logits && u && tokens, "null sampling buffer");
-    const SampleArgs a{logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, probs};
+    op_check(rows <= (1 << 24), "rows must be at most 2^24");
+    const SampleArgs a{logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, probs, 0};
     const auto st = static_cast<cudaStream_t>(stream);
-    if (dtype == SPECDEC_F32)
-      op_launch("specdec_sample", sample_rows_kernel<float>, dim3(rows), kSampleThreads, 0, st, 1, a);
-    else
-      op_launch("specdec_sample", sample_rows_kernel<__nv_bfloat16>, dim3(rows), kSampleThreads, 0, st, 1, a);
+    dtype == SPECDEC_F32 ? launch<float>(a, st) : launch<__nv_bfloat16>(a, st);
   });
 }

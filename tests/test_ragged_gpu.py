@@ -435,7 +435,7 @@ def check_sample(l, u, T, k, p, m, tok, prob):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("V,B,pad", [(1, 3, 0), (2, 9, 1), (37, 64, 3), (1000, 40, 0), (2048, 33, 0), (32000, 24, 0),
-                                    (50257, 9, 1), (131073, 5, 0), (300001, 2, 7)])
+                                    (50257, 9, 1), (131073, 5, 0), (300001, 2, 7), (400003, 2, 1)])
 def test_sample(gpu_lib, dtype, V, B, pad):
     rng = np.random.default_rng(V)
     l = rng.normal(0, 3, (B, V)) + (rng.random((B, V)) < 4 / V) * rng.uniform(0, 12, (B, V))
@@ -458,7 +458,7 @@ def test_sample(gpu_lib, dtype, V, B, pad):
         check_sample(l, u, full["T"], full["k"], full["p"], full["m"], *run_sample(l, u, dtype=dtype, **kw))
 
 
-@pytest.mark.parametrize("V", [5, 4097, 40000, 200003])
+@pytest.mark.parametrize("V", [5, 4097, 40000, 200003, 500001])
 def test_sample_ties_go_to_the_lowest_index(gpu_lib, V):
     # equal logits: every weight is 2^31 exactly, so the token is floor(u n) of the first n kept
     u = np.array([0, 0.25, 0.5, 0.999, 1 - 2.0 ** -24], np.float32)
@@ -497,6 +497,33 @@ def test_sample_empty_infinite_and_odd_rows(gpu_lib):
         assert prob.tolist() == [0, 0, 0.5, 1, 1, 0.5]
     tok, prob = run_sample(l, u, T=[0.0, 0, 0, -1, 0, 0])
     assert tok.tolist() == [-1, -1, 7, 21, 5, 11] and prob.tolist() == [0, 0, 1, 1, 1, 1]
+
+
+def test_sample_extreme_temperatures(gpu_lib):
+    # z that all round to one value, or to infinities: ties by index
+    V = 5000
+    rng = np.random.default_rng(2)
+    l = np.sort(rng.normal(0, 1, (4, V)).astype(np.float32), axis=1)
+    T = np.array([1e38, 1e30, 1e-38, 1e-20], np.float32)
+    u = np.array([0.5, 0.999, 0.5, 0.5], np.float32)
+    for kw in (dict(), dict(k=[7] * 4), dict(p=[0.5] * 4), dict(k=[100] * 4, p=[0.3] * 4)):
+        full = dict(k=[0] * 4, p=[1.0] * 4) | kw
+        tok, prob = run_sample(l, u, T=T, **kw)
+        check_sample(l, u, T, full["k"], full["p"], [0] * 4, tok, prob)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sample_flat_rows(gpu_lib, dtype):
+    # nearly flat logits put thousands of tokens around every cut
+    V, B = 60000, 12
+    rng = np.random.default_rng(4)
+    l = rng.normal(0, np.array([1e-3, 0.05, 0.5] * 4)[:, None], (B, V))
+    l = np.asarray(torch.tensor(l).to(DT[dtype]).float())
+    u = rng.random(B).astype(np.float32).clip(0, 1 - 2.0 ** -24)
+    k = np.array([0, 30000, 5000, 0] * 3)
+    p = np.array([0.5, 1, 0.9, 0.999, 0.03, 0.5] * 2, np.float32)
+    one, zero = np.ones(B, np.float32), np.zeros(B, np.float32)
+    check_sample(l, u, one, k, p, zero, *run_sample(l, u, one, k, p, zero, dtype))
 
 
 def test_sample_frequencies(gpu_lib):
