@@ -24,7 +24,7 @@ constexpr int kSlice = 16384;        // tokens of a block where the row count gi
 constexpr int kMaxSlice = 40960;     // tokens that a block's shared memory holds
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 128;
-constexpr int kCap = 2048;           // tokens of the band in which a cut is settled exactly
+constexpr int kCap = 1024;           // tokens that are sorted to settle a cut exactly
 constexpr float kFar = 22.2f;        // nats below the maximum from which the weight is 0: 2^31 exp(-22.2) < 1
 constexpr int kLevels = 4;
 
@@ -145,6 +145,23 @@ __device__ uint32_t radix_select(u64 want, Each &&each, u64 *hist, u64 *out, u64
   return value;
 }
 
+// Bitonic sort of `size` values (a power of two, at most 2 kThreads) in
+// descending order, by the whole block.
+__device__ void sort_down(u64 *v, int size) {
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int p = threadIdx.x; p < size / 2; p += kThreads) {
+        const int i = 2 * p - (p & (j - 1)), o = i + j;  // the pair (i, i + j)
+        const u64 x = v[i], y = v[o];
+        if ((x < y) == ((i & k) == 0)) {
+          v[i] = y;
+          v[o] = x;
+        }
+      }
+      __syncthreads();
+    }
+}
+
 // The tokens kept so far: those with a larger key, and those with this key up
 // to index idx.  Logits above hi have a larger key for sure, those below lo a
 // smaller one; between them the key decides.
@@ -260,20 +277,18 @@ __global__ void __launch_bounds__(kThreads) sample_whole_kernel(const SampleArgs
 
 // What the blocks of a cluster tell each other: every block writes its own
 // entry in every block's copy, then the cluster meets.
-struct Shared {
+struct alignas(16) Shared {
   float high[kMaxCluster];
   int first[kMaxCluster];
-  uint32_t counts[kMaxCluster][kBins];
+  u64 counts[kMaxCluster][kBins];
   u64 mass[kMaxCluster], above[kMaxCluster];
   int n[kMaxCluster];
   float min_above[kMaxCluster], max_below[kMaxCluster];
-  Cut cut;
-  int slow;
   // of this block alone
   u64 hist[256], red[32], out[3];
-  uint32_t total[kBins];
   float redf[32];
-  int redi[32], n_local, band[2];
+  int redi[32], n_local, band[2], at;
+  unsigned char shift[kBins];
 };
 
 // Eight logits from a 16- or 32-byte run.
@@ -294,14 +309,16 @@ __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
 
 // One row per cluster, its logits read once and held in the blocks' shared
 // memory.  A cut (top-k by count, top-p by mass) is found from the outside in:
-// the counts of tokens in 128 bins of their distance to the maximum (each lane
-// of a warp counts in a column of its own, so no two lanes meet in a bank or a
-// word) give the bins in which the cut lies -- for a mass by bounds, since a
-// bin's weights differ by at most its width --, the tokens of those bins are
-// listed, or binned again where they are too many, and the exact cut is
-// selected from the list in whole numbers.  The list is checked to hold the
-// cut: what lies outside it is strictly above or below; a row that fails, and
-// one that never narrows, is done by sample_whole_row.
+// the counts (or the masses, in 32 bits with a shift per bin) of the tokens in
+// 128 bins of their distance to the maximum give the bins in which the cut
+// lies; each lane of a warp adds to a column of its own, so no two lanes meet
+// in a bank or a word.  Where the tokens down to those bins are few, they are
+// listed and sorted, and every filter and the draw are settled on that list.
+// Else the tokens of the bins alone are listed, or binned again where they are
+// too many, the exact cut is taken from their sorted list, and the draw passes
+// over the row.  A list is checked to hold its cut: what lies outside it is
+// strictly above or below; a row that fails, and one that never narrows, is
+// done by sample_whole_row.
 template <typename XT>
 __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleArgs a) {
   namespace cg = cooperative_groups;
@@ -311,9 +328,9 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   extern __shared__ __align__(16) unsigned char sample_smem[];
   Shared &sh = *reinterpret_cast<Shared *>(sample_smem);
   uint32_t *columns = reinterpret_cast<uint32_t *>(sample_smem + sizeof(Shared));  // [kBins][32]
-  uint2 *list = reinterpret_cast<uint2 *>(columns);                               // [kCap] (logit, index), after the counts
-  uint2 *merged = list + kCap;                                                    // [kCap] of the cluster, in block 0
-  float *row = reinterpret_cast<float *>(merged + kCap);                          // [slice + 16]
+  uint2 *list = reinterpret_cast<uint2 *>(columns + kBins * 32);                  // [kCap] (logit, index) of this block
+  u64 *sorted = reinterpret_cast<u64 *>(list + kCap);                             // [kCap] of the cluster
+  float *row = reinterpret_cast<float *>(sorted + kCap);                          // [slice + 16]
   auto meet = [&]() { cluster.sync(); };
   auto tell = [&](auto *p, auto v) {  // writes *p in every block
     for (int r = 0; r < C; ++r) *cluster.map_shared_rank(p, r) = v;
@@ -401,170 +418,288 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   Cut cut{0, -1, -INFINITY, -INFINITY};
   auto far_of = [&](float l) { return (high - l) * sc.inv; };  // the distance to the maximum, falling with l
 
-  // The cut at which the count (or mass) over descending z first reaches `want`, among the tokens that `in` keeps.
-  auto search = [&](bool by_mass, u64 want, const Cut in) {
-    float lo = 0.f, hi = kFar;
-    u64 base = 0;  // count or mass above lo
-    for (int level = 0; level < kLevels; ++level) {
-      const float width = (hi - lo) * (1.f / kBins), per = 1.f / width;
-      for (int i = tid; i < kBins * 32; i += kThreads) columns[i] = 0;
-      __syncthreads();
+  // The tokens of all blocks' lists in `sorted`, by descending key and ascending index (key above, ~index below), filled
+  // with zeros to a power of two.  The caller has met after the lists' end.
+  auto merge = [&](int n_all) {
+    int size = 32;
+    while (size < n_all) size *= 2;
+    for (int i = n_all + tid; i < size; i += kThreads) sorted[i] = 0;
+    for (int r = 0, at = 0; r < C; at += sh.n[r++]) {
+      const uint2 *src = cluster.map_shared_rank(list, r);
+      for (int i = tid; i < sh.n[r]; i += kThreads) {
+        const uint2 e = src[i];
+        sorted[at + i] = static_cast<u64>(float_key(sc.z(__uint_as_float(e.x)))) << 32 | static_cast<uint32_t>(~e.y);
+      }
+    }
+    __syncthreads();
+    sort_down(sorted, size);
+  };
+  auto sorted_w = [&](int i) { return weight_w(weight_e(key_float(static_cast<uint32_t>(sorted[i] >> 32)), zmax)); };
+  // The first place of `sorted` at which the running sum of f reaches want; n_all where it does not.
+  auto reach = [&](int n_all, u64 want, auto &&f) {
+    if (tid == 0) sh.at = n_all;
+    const int i = 2 * tid;
+    const u64 w0 = i < n_all ? f(i) : 0, w1 = i + 1 < n_all ? f(i + 1) : 0;
+    u64 all;
+    const u64 before = block_scan_u64(w0 + w1, sh.red, &all);
+    if (before < want && want <= before + w0 + w1) sh.at = before + w0 >= want ? i : i + 1;
+    __syncthreads();
+    const int at = sh.at;
+    __syncthreads();
+    return at;
+  };
+  auto cut_at = [&](int i) {
+    const u64 e = sorted[i];
+    Cut c;
+    c.key = static_cast<uint32_t>(e >> 32);
+    c.idx = static_cast<int>(~static_cast<uint32_t>(e));
+    const float l = key_float(c.key) * T, margin = fabsf(l) * 1e-6f + 8.3e-25f;
+    c.lo = l - margin;
+    c.hi = l + margin;
+    return c;
+  };
+
+  // Counts (or masses) of the tokens kept by `in` in bins between lo and hi, to every block; a mass's sum goes to sh.mass.
+  // Returns the first bin in which the running sum may reach want(), and in sure the first in which it must.
+  auto bins = [&](bool by_mass, float lo, float hi, u64 base, const Cut in, auto &&want, int &sure) {
+    const float width = (hi - lo) * (1.f / kBins), per = 1.f / width;
+    for (int i = tid; i < kBins * 32; i += kThreads) columns[i] = 0;
+    if (by_mass && tid < kBins)  // a column's sum of up to slice / 32 weights of the bin fits 32 bits
+      sh.shift[tid] = max(0, static_cast<int>((__float_as_uint(expf(-(lo + tid * width)) * 1.01f * 2147483648.f * (a.slice / 32 + 4)) >> 23)) - 127 - 31);
+    __syncthreads();
+    u64 mine = 0;
+    if (by_mass) {
+      each([&](float l, int i) {
+        const float d = far_of(l);
+        if (!(d >= lo && d < hi) || !kept_by(in, sc, l, i)) return;
+        const uint32_t w = weight_w(weight_e(sc.z(l), zmax));
+        const int j = min(kBins - 1, static_cast<int>((d - lo) * per));
+        mine += w;
+        atomicAdd(&columns[j * 32 + lane], w >> sh.shift[j]);
+      });
+      mine = block_sum_u64(mine, sh.red);
+    } else {
       each([&](float l, int i) {
         const float d = far_of(l);
         if (d >= lo && d < hi && kept_by(in, sc, l, i))
           atomicAdd(&columns[min(kBins - 1, static_cast<int>((d - lo) * per)) * 32 + lane], 1u);
       });
-      __syncthreads();
-      for (int j = warp; j < kBins; j += kThreads / 32) {
-        const uint32_t c = __reduce_add_sync(0xffffffffu, columns[j * 32 + lane]);
-        if (lane == 0) tell(&sh.counts[rank][j], c);
-      }
-      meet();
-      if (warp == 0) {  // lane l: bins 4 l .. 4 l + 3
-        u64 c[4], some = 0, most = 0;
-        float w_hi[4], w_lo[4];
+    }
+    __syncthreads();
+    for (int j = warp; j < kBins; j += kThreads / 32) {
+      // 32 columns of up to 31 bits: the sum in two halves
+      const uint32_t c = columns[j * 32 + lane];
+      const uint32_t low = __reduce_add_sync(0xffffffffu, c & 0xffffu), high16 = __reduce_add_sync(0xffffffffu, c >> 16);
+      const u64 sum = (static_cast<u64>(high16) << 16) + low;
+      if (lane == 0) tell(&sh.counts[rank][j], sum);
+    }
+    if (tid == 0) tell(&sh.mass[rank], mine);
+    meet();
+    if (warp == 0) {  // lane l: bins 4 l .. 4 l + 3
+      const u64 target = want();
+      u64 some[4], most[4], sum_some = 0, sum_most = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          c[j] = 0;
-          for (int r = 0; r < C; ++r) c[j] += sh.counts[r][4 * lane + j];
-          const float d = lo + (4 * lane + j) * width;
-          w_hi[j] = by_mass ? fminf(expf(-d) * 1.0001f, 1.f) * 2147483648.f : 1.f;
-          w_lo[j] = by_mass ? fmaxf(expf(-(d + width)) * 0.9999f * 2147483648.f - 1.f, 0.f) : 1.f;
-          most += c[j] * static_cast<u64>(by_mass ? ceilf(w_hi[j]) : 1.f);
-          some += c[j] * static_cast<u64>(w_lo[j]);
+      for (int j = 0; j < 4; ++j) {
+        u64 c = 0;
+        for (int r = 0; r < C; ++r) c += sh.counts[r][4 * lane + j];
+        some[j] = most[j] = c;
+        if (by_mass) {  // a shift leaves at least 2^20 of a weight, so it drops less than 2^-20 of the sum
+          some[j] = c << sh.shift[4 * lane + j];
+          most[j] = some[j] + (sh.shift[4 * lane + j] ? some[j] >> 18 : 0);
         }
-        u64 run_hi = base + warp_scan_u64(most) - most, run_lo = base + warp_scan_u64(some) - some;
-        // the first bin that may reach `want`, and the first that must
-        int first = kBins, sure = kBins;
+        sum_some += some[j];
+        sum_most += most[j];
+      }
+      u64 run_some = base + warp_scan_u64(sum_some) - sum_some, run_most = base + warp_scan_u64(sum_most) - sum_most;
+      int first = kBins, must = kBins;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          run_hi += c[j] * static_cast<u64>(by_mass ? ceilf(w_hi[j]) : 1.f);
-          run_lo += c[j] * static_cast<u64>(w_lo[j]);
-          if (run_hi >= want) first = min(first, 4 * lane + j);
-          if (run_lo >= want) sure = min(sure, 4 * lane + j);
+      for (int j = 3; j >= 0; --j) {
+        u64 s = run_some, m = run_most;
+        for (int i = 0; i <= j; ++i) {
+          s += some[i];
+          m += most[i];
         }
-        first = __reduce_min_sync(0xffffffffu, first);
-        sure = __reduce_min_sync(0xffffffffu, sure);
-        if (lane == 0) {
-          sh.band[0] = first;
-          sh.band[1] = sure;
-        }
+        if (m >= target) first = 4 * lane + j;
+        if (s >= target) must = 4 * lane + j;
       }
-      __syncthreads();
-      const int b0 = sh.band[0], b1 = min(sh.band[1], kBins - 1);
-      if (b0 == kBins) {
-        if (!by_mass && level == 0) return in;  // the cut lies among tokens of weight 0: every other is kept
-        slow = true;
-        return in;
+      first = __reduce_min_sync(0xffffffffu, first);
+      must = __reduce_min_sync(0xffffffffu, must);
+      if (lane == 0) {
+        sh.band[0] = first;
+        sh.band[1] = must;
       }
+    }
+    __syncthreads();
+    sure = sh.band[1];
+    return sh.band[0];
+  };
+  // Lists the tokens kept by `in` between lo and hi; counts (or sums) those above lo; all to every block.  Returns the
+  // number listed by all blocks; above and the nearest logits outside come back too.
+  auto collect = [&](bool by_mass, float lo, float hi, const Cut in, u64 &above, float &min_above, float &max_below) {
+    if (tid == 0) sh.n_local = 0;
+    __syncthreads();
+    above = 0;
+    min_above = INFINITY;
+    max_below = -INFINITY;
+    each([&](float l, int i) {
+      const float d = far_of(l);
+      if (!(d < hi)) {
+        max_below = fmaxf(max_below, l);
+        return;
+      }
+      if (!kept_by(in, sc, l, i)) return;
+      if (d < lo) {
+        above += by_mass ? weight_w(weight_e(sc.z(l), zmax)) : 1u;
+        min_above = fminf(min_above, l);
+      } else {
+        const int at = atomicAdd(&sh.n_local, 1);
+        if (at < kCap) list[at] = make_uint2(__float_as_uint(l), i);
+      }
+    });
+    above = block_sum_u64(above, sh.red);
+    min_above = -block_max(-min_above, sh.redf);
+    max_below = block_max(max_below, sh.redf);
+    if (tid == 0) {
+      tell(&sh.above[rank], above);
+      tell(&sh.n[rank], sh.n_local);
+      tell(&sh.min_above[rank], min_above);
+      tell(&sh.max_below[rank], max_below);
+    }
+    meet();
+    above = 0;
+    int n_all = 0;
+    for (int r = 0; r < C; ++r) {
+      above += sh.above[r];
+      n_all += sh.n[r];
+      min_above = fminf(min_above, sh.min_above[r]);
+      max_below = fmaxf(max_below, sh.max_below[r]);
+    }
+    return n_all;
+  };
+  auto below_cut = [&](float l, const Cut &c) { return l == -INFINITY || float_key(sc.z(l)) < c.key; };
+  auto above_cut = [&](float l, const Cut &c) { return l == INFINITY || float_key(sc.z(l)) > c.key; };
+  const u64 p24 = static_cast<u64>(rintf(fminf(fmaxf(top_p, 0.f), 1.f) * 16777216.f));
+  auto most_of = [&](u64 mass) { return max(part_of(p24, mass), u64(1)); };
+  const u64 u24 = static_cast<u64>(fminf(fmaxf(a.u[b] * 16777216.f, 0.f), 16777215.f));
+
+  // The cut at which the count (or mass) over descending z first reaches its target, among the tokens that `in` keeps.
+  // b0, b1: the bins of the first level, already found.
+  auto search = [&](bool by_mass, u64 want, const Cut in, int b0, int b1) {
+    float lo = 0.f, hi = kFar;
+    for (int level = 0; level < kLevels && !slow; ++level) {
+      const float width = (hi - lo) * (1.f / kBins);
+      if (b0 >= kBins) break;
+      b1 = min(b1, kBins - 1);
       const float new_lo = b0 == 0 ? lo : lo + (b0 - 0.02f) * width, new_hi = b1 == kBins - 1 ? hi : lo + (b1 + 1.02f) * width;
-      // what lies above the band, and the band's tokens
-      if (tid == 0) sh.n_local = 0;
-      __syncthreads();
-      u64 above = 0;
-      float min_above = INFINITY, max_below = -INFINITY;
-      each([&](float l, int i) {
-        const float d = far_of(l);
-        if (!(d < kFar) || !kept_by(in, sc, l, i)) return;
-        if (d < new_lo) {
-          above += by_mass ? weight_w(weight_e(sc.z(l), zmax)) : 1u;
-          min_above = fminf(min_above, l);
-        } else if (d < new_hi) {
-          const int at = atomicAdd(&sh.n_local, 1);
-          if (at < kCap) list[at] = make_uint2(__float_as_uint(l), i);
-        } else {
-          max_below = fmaxf(max_below, l);
-        }
-      });
-      above = block_sum_u64(above, sh.red);
-      min_above = -block_max(-min_above, sh.redf);
-      max_below = block_max(max_below, sh.redf);
-      if (tid == 0) {
-        tell(&sh.above[rank], above);
-        tell(&sh.n[rank], sh.n_local);
-        tell(&sh.min_above[rank], min_above);
-        tell(&sh.max_below[rank], max_below);
-      }
-      meet();
-      base = 0;
-      int n_all = 0;
-      for (int r = 0; r < C; ++r) {
-        base += sh.above[r];
-        n_all += sh.n[r];
-        min_above = fminf(min_above, sh.min_above[r]);
-        max_below = fmaxf(max_below, sh.max_below[r]);
-      }
-      if (n_all > kCap) {  // too many: bin them again
-        lo = new_lo;
-        hi = new_hi;
-        meet();  // the entries above have been read
-        continue;
-      }
-      if (rank == 0) {
-        for (int r = 0, at = 0; r < C; at += sh.n[r++]) {
-          const uint2 *src = cluster.map_shared_rank(list, r);
-          for (int i = tid; i < sh.n[r]; i += kThreads) {
-            const uint2 e = src[i];
-            merged[at + i] = make_uint2(float_key(sc.z(__uint_as_float(e.x))), e.y);
-          }
-        }
-        __syncthreads();
-        u64 all = 0;
-        for (int i = tid; i < n_all; i += kThreads)
-          all += by_mass ? weight_w(weight_e(key_float(merged[i].x), zmax)) : 1u;
-        all = block_sum_u64(all, sh.red);
-        bool bad = !(base < want && want <= base + all);
+      u64 above;
+      float min_above, max_below;
+      const int n_all = collect(by_mass, new_lo, new_hi, in, above, min_above, max_below);
+      if (n_all <= kCap) {
+        merge(n_all);
+        const int at = above < want ? reach(n_all, want - above, [&](int i) { return by_mass ? static_cast<u64>(sorted_w(i)) : u64(1); }) : n_all;
         Cut c = in;
-        if (!bad) {
-          u64 left, at;
-          c.key = radix_select(want - base, [&](auto &&f) {
-            for (int i = tid; i < n_all; i += kThreads)
-              f(merged[i].x, by_mass ? static_cast<u64>(weight_w(weight_e(key_float(merged[i].x), zmax))) : u64(1));
-          }, sh.hist, sh.out, &left, &at);
-          const float z = key_float(c.key);
-          const u64 w = by_mass ? weight_w(weight_e(z, zmax)) : 1u;
-          const u64 ties = (left + w - 1) / w;  // w > 0: the sum was reached here
-          c.idx = 0x7fffffff;
-          if (at > ties * w) {  // not all of them: those with the lowest indexes
-            u64 l2, a2;
-            c.idx = static_cast<int>(~radix_select(ties, [&](auto &&f) {
-              for (int i = tid; i < n_all; i += kThreads)
-                if (merged[i].x == c.key) f(~merged[i].y, u64(1));
-            }, sh.hist, sh.out, &l2, &a2));
-          }
-          if (c.key == in.key) c.idx = min(c.idx, in.idx);
-          const float l = z * T, margin = fabsf(l) * 1e-6f + 8.3e-25f;
-          c.lo = l - margin;
-          c.hi = l + margin;
-          // the tokens with this key are all listed, or cut off already
-          bad = float_key(sc.z(min_above)) <= c.key || float_key(sc.z(max_below)) >= c.key;
-        }
-        if (tid == 0) {
-          tell(&sh.cut, c);
-          tell(&sh.slow, bad ? 1 : 0);
-        }
+        if (at < n_all) c = cut_at(at);
+        slow = at == n_all || !above_cut(min_above, c) || !below_cut(max_below, c);
+        meet();  // the lists have been read
+        return c;
       }
-      meet();
-      slow = sh.slow != 0;
-      return sh.cut;
+      lo = new_lo;
+      hi = new_hi;
+      meet();  // what the blocks told each other has been read
+      b0 = bins(by_mass, lo, hi, above, in, [&]() { return want; }, b1);
     }
     slow = true;
     return in;
   };
 
-  if (!slow && has_k) cut = search(false, k, cut);
-  if (!slow && has_p) {
-    u64 mass = 0;
-    each([&](float l, int i) {
-      if (far_of(l) < kFar && kept_by(cut, sc, l, i)) mass += weight_w(weight_e(sc.z(l), zmax));
-    });
-    mass = block_sum_u64(mass, sh.red);
-    if (tid == 0) tell(&sh.mass[rank], mass);
-    meet();
-    mass = 0;
-    for (int r = 0; r < C; ++r) mass += sh.mass[r];
-    u64 most = part_of(static_cast<u64>(rintf(fmaxf(top_p, 0.f) * 16777216.f)), mass);
-    cut = search(true, most < 1 ? 1 : most, cut);
+  if (!slow && (has_k || has_p)) {
+    // the bins of the first cut, and the list of everything down to it
+    int b1, b0 = bins(!has_k, 0.f, kFar, 0, cut, [&]() {
+      if (has_k) return static_cast<u64>(k);
+      u64 mass = 0;
+      for (int r = 0; r < C; ++r) mass += sh.mass[r];
+      return most_of(mass);
+    }, b1);
+    u64 mass_all = 0;
+    for (int r = 0; r < C; ++r) mass_all += sh.mass[r];
+    // has_k and no bin: fewer than k tokens have a weight above 0, and all of them are kept
+    u64 above = 0;
+    float min_above = INFINITY, max_below = -INFINITY;
+    const float hi = b0 >= kBins || b1 >= kBins - 1 ? kFar : (b1 + 1.02f) * (kFar / kBins);
+    const int n_all = collect(false, 0.f, hi, cut, above, min_above, max_below);
+    if (n_all <= kCap) {
+      if (rank == 0) {
+        merge(n_all);
+        // how many of the list the filters keep
+        int n = n_all;
+        bool bad = false;
+        if (has_k && b0 < kBins) {
+          n = k;
+          bad = n > n_all || !below_cut(max_below, cut_at(max(0, min(n, n_all) - 1)));
+          n = min(n, n_all);
+        }
+        u64 mass = mass_all;
+        const int i = 2 * tid;
+        if (has_p) {
+          if (has_k) mass = block_sum_u64((i < n ? sorted_w(i) : 0u) + static_cast<u64>(i + 1 < n ? sorted_w(i + 1) : 0u), sh.red);
+          const int at = reach(n, most_of(mass), [&](int j) { return static_cast<u64>(sorted_w(j)); });
+          bad = bad || at == n;
+          if (at < n) {
+            if (!has_k) bad = bad || !below_cut(max_below, cut_at(at));
+            n = at + 1;
+          }
+        }
+        if (!bad) {
+          // the kept tokens by index: (index, weight) sorted again; min-p leaves its tokens with weight 0
+          __syncthreads();
+          u64 e[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            e[j] = 0;
+            if (i + j < n) {
+              const float w_e = weight_e(key_float(static_cast<uint32_t>(sorted[i + j] >> 32)), zmax);
+              const uint32_t w = w_e >= min_e ? weight_w(w_e) : 0u;
+              e[j] = sorted[i + j] << 32 | w;  // ~index above: descending is by ascending index
+            }
+          }
+          __syncthreads();
+          int size = 32;
+          while (size < n) size *= 2;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (i + j < size) sorted[i + j] = e[j];
+          __syncthreads();
+          sort_down(sorted, size);
+          const u64 total = block_sum_u64((i < n ? sorted[i] & 0xffffffffu : 0) + (i + 1 < n ? sorted[i + 1] & 0xffffffffu : 0), sh.red);
+          const int at = reach(n, part_of(u24, total) + 1, [&](int j) { return sorted[j] & 0xffffffffu; });
+          if (tid == 0) {
+            a.tokens[b] = static_cast<int>(~static_cast<uint32_t>(sorted[at] >> 32));
+            if (a.probs) a.probs[b] = __fdiv_rn(static_cast<float>(sorted[at] & 0xffffffffu), static_cast<float>(total));
+          }
+        }
+        if (tid == 0) tell(&sh.first[0], bad ? 1 : 0);
+      }
+      meet();  // the lists have been read
+      if (!sh.first[0]) return;
+      slow = true;
+    } else {
+      meet();  // what the blocks told each other has been read
+      if (has_k && b0 < kBins) cut = search(false, k, cut, b0, b1);
+      if (has_p && !slow) {
+        u64 most = 0;
+        if (has_k) {
+          b0 = bins(true, 0.f, kFar, 0, cut, [&]() {
+            u64 mass = 0;
+            for (int r = 0; r < C; ++r) mass += sh.mass[r];
+            return most_of(mass);
+          }, b1);
+          mass_all = 0;
+          for (int r = 0; r < C; ++r) mass_all += sh.mass[r];
+        }
+        most = most_of(mass_all);
+        cut = search(true, most, cut, b0, b1);
+      }
+    }
   }
   if (slow) {
     if (rank == 0) sample_whole_row<XT>(a, b, sh.hist, sh.red, sh.out);
@@ -603,7 +738,6 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     if (r < rank) before += sh.mass[r];
     total += sh.mass[r];
   }
-  const u64 u24 = static_cast<u64>(fminf(fmaxf(a.u[b] * 16777216.f, 0.f), 16777215.f));
   const u64 target = part_of(u24, total);
   if (target < before || target >= before + mine) return;
   for (int q = q0; q < q1; q += 32) {
@@ -633,7 +767,7 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
 }
 
 size_t cluster_smem(int slice) {
-  return sizeof(Shared) + 2 * kCap * sizeof(uint2) + (static_cast<size_t>(slice) + 16) * sizeof(float);
+  return sizeof(Shared) + kBins * 32 * sizeof(uint32_t) + 2 * kCap * sizeof(u64) + (static_cast<size_t>(slice) + 16) * sizeof(float);
 }
 
 template <typename XT>
