@@ -145,9 +145,27 @@ __device__ uint32_t radix_select(u64 want, Each &&each, u64 *hist, u64 *out, u64
   return value;
 }
 
-// Bitonic sort of `size` values (a power of two, at most 2 kThreads) in
-// descending order, by the whole block.
-__device__ void sort_down(u64 *v, int size) {
+// Sorts the n <= 2 kThreads distinct values of v in descending order, by the
+// whole block; spare holds as many.  Few values find their places by counting
+// the larger ones (two threads a value), more go through a bitonic network.
+__device__ void sort_down(u64 *v, u64 *spare, int n) {
+  if (n <= kThreads / 2) {
+    const int i = threadIdx.x >> 1;
+    const u64 mine = i < n ? v[i] : 0;
+    int larger = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x & 1; j < n; j += 2) larger += v[j] > mine;
+    larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+    if (i < n && (threadIdx.x & 1) == 0) spare[larger] = mine;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < n) v[threadIdx.x] = spare[threadIdx.x];
+    __syncthreads();
+    return;
+  }
+  int size = kThreads;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) v[i] = 0;
+  __syncthreads();
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
       for (int p = threadIdx.x; p < size / 2; p += kThreads) {
@@ -162,19 +180,18 @@ __device__ void sort_down(u64 *v, int size) {
     }
 }
 
-// The tokens kept so far: those with a larger key, and those with this key up
-// to index idx.  Logits above hi have a larger key for sure, those below lo a
-// smaller one; between them the key decides.
+// The tokens that a filter keeps: those with a larger key, and those with this
+// key up to index idx.  Values (logits, or bits of e) above hi have a larger
+// key for sure, those below lo a smaller one; between them the key decides.
+template <typename T>
 struct Cut {
   uint32_t key;
   int idx;
-  float lo, hi;
+  T lo, hi;
 };
-__device__ __forceinline__ bool kept_by(const Cut &c, const Scale &sc, float l, int idx) {
-  if (l > c.hi) return true;
-  if (!(l >= c.lo)) return false;
+__device__ __forceinline__ bool keeps(uint32_t key, int idx, const Scale &sc, float l, int i) {
   const uint32_t k = float_key(sc.z(l));
-  return k > c.key || (k == c.key && idx <= c.idx);
+  return k > key || (k == key && i <= idx);
 }
 
 // The whole row by one block, straight from global memory: for rows whose cut
@@ -279,16 +296,15 @@ __global__ void __launch_bounds__(kThreads) sample_whole_kernel(const SampleArgs
 // entry in every block's copy, then the cluster meets.
 struct alignas(16) Shared {
   float high[kMaxCluster];
-  int first[kMaxCluster];
+  int first[kMaxCluster], bad;
   u64 counts[kMaxCluster][kBins];
   u64 mass[kMaxCluster], above[kMaxCluster];
-  int n[kMaxCluster];
+  int n[kMaxCluster], n_top[kMaxCluster];
   float min_above[kMaxCluster], max_below[kMaxCluster];
   // of this block alone
   u64 hist[256], red[32], out[3];
   float redf[32];
-  int redi[32], n_local, band[2], at;
-  unsigned char shift[kBins];
+  int redi[32], n_local, n_local_top, band[2], at;
 };
 
 // Eight logits from a 16- or 32-byte run.
@@ -308,17 +324,20 @@ __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
 }
 
 // One row per cluster, its logits read once and held in the blocks' shared
-// memory.  A cut (top-k by count, top-p by mass) is found from the outside in:
-// the counts (or the masses, in 32 bits with a shift per bin) of the tokens in
-// 128 bins of their distance to the maximum give the bins in which the cut
-// lies; each lane of a warp adds to a column of its own, so no two lanes meet
-// in a bank or a word.  Where the tokens down to those bins are few, they are
-// listed and sorted, and every filter and the draw are settled on that list.
-// Else the tokens of the bins alone are listed, or binned again where they are
-// too many, the exact cut is taken from their sorted list, and the draw passes
-// over the row.  A list is checked to hold its cut: what lies outside it is
-// strictly above or below; a row that fails, and one that never narrows, is
-// done by sample_whole_row.
+// memory.  A cut is found from the outside in: the tokens (for top-k), or their
+// weights (for top-p, in 32 bits with a shift), are added up in 128 bins of
+// their distance to the maximum, or of the bits of e; each lane of a warp adds
+// to a column of its own, so no two lanes meet in a bank or a word.  Where the
+// tokens down to the bins that hold the cut are few, they are listed and
+// sorted, and every filter and the draw are settled on that list.  Else only
+// the bins' tokens are listed, or binned again by finer bins where they are too
+// many, the exact cut is taken from their sorted list, and the draw passes over
+// the row.  Top-p works on e, which takes the logits' place in shared memory
+// (the exponential is taken once a token); e orders tokens as z does but for
+// the last bits, and within 8 units of them z decides, read again.  A list of
+// logits is checked to hold its cut: what lies outside it is strictly above or
+// below.  A row that fails, and one that never narrows, is done by
+// sample_whole_row.
 template <typename XT>
 __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleArgs a) {
   namespace cg = cooperative_groups;
@@ -327,13 +346,14 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   extern __shared__ __align__(16) unsigned char sample_smem[];
   Shared &sh = *reinterpret_cast<Shared *>(sample_smem);
-  uint32_t *columns = reinterpret_cast<uint32_t *>(sample_smem + sizeof(Shared));  // [kBins][32]
-  uint2 *list = reinterpret_cast<uint2 *>(columns + kBins * 32);                  // [kCap] (logit, index) of this block
-  u64 *sorted = reinterpret_cast<u64 *>(list + kCap);                             // [kCap] of the cluster
-  float *row = reinterpret_cast<float *>(sorted + kCap);                          // [slice + 16]
+  uint32_t *columns = reinterpret_cast<uint32_t *>(sample_smem + sizeof(Shared));  // [kBins][32]; also sorting's spare room
+  uint2 *list = reinterpret_cast<uint2 *>(columns + kBins * 32);  // [kCap] (logit, index) of this block
+  int *list_top = reinterpret_cast<int *>(list), *list_band = list_top + kCap;  // or [kCap] indexes each
+  u64 *sorted = reinterpret_cast<u64 *>(list + kCap);             // [kCap] of the cluster
+  float *row = reinterpret_cast<float *>(sorted + kCap);          // [slice + 16]
   auto meet = [&]() { cluster.sync(); };
-  auto tell = [&](auto *p, auto v) {  // writes *p in every block
-    for (int r = 0; r < C; ++r) *cluster.map_shared_rank(p, r) = v;
+  auto tell = [&](auto *p, auto v) {  // writes *p in every block; called by whole warps with a uniform v
+    if (lane < C) *cluster.map_shared_rank(p, lane) = v;
   };
 
   // ---- the slice, its maximum ------------------------------------------------
@@ -373,11 +393,11 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     high = fmaxf(high, l);
   }
   high = block_max(high, sh.redf);
-  if (tid == 0) tell(&sh.high[rank], high);
+  if (warp == 0) tell(&sh.high[rank], high);
   meet();
   high = -INFINITY;
   for (int r = 0; r < C; ++r) high = fmaxf(high, sh.high[r]);
-  // every pass: f(logit, index in the row)
+  // a pass over the slice: f(value, index in the row)
   auto each = [&](auto &&f) {
     for (int q = tid; q < n4; q += kThreads) {
       const float4 v = reinterpret_cast<const float4 *>(row)[q];
@@ -413,33 +433,28 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   const float top_p = a.top_p ? a.top_p[b] : 1.f;
   const float min_e = a.min_p ? fminf(a.min_p[b], 1.f) : 0.f;
   const bool has_k = k > 0 && k < V, has_p = top_p < 1.f;
+  const u64 p24 = static_cast<u64>(rintf(fminf(fmaxf(top_p, 0.f), 1.f) * 16777216.f));
+  auto most_of = [&](u64 mass) { return max(part_of(p24, mass), u64(1)); };
+  const u64 u24 = static_cast<u64>(fminf(fmaxf(a.u[b] * 16777216.f, 0.f), 16777215.f));
   // temperatures and logits for which equal z means nearly equal logits
   bool slow = !(T >= 9.1e-13f && T <= 1.1e12f && fabsf(high) < 1.2e24f);
-  Cut cut{0, -1, -INFINITY, -INFINITY};
   auto far_of = [&](float l) { return (high - l) * sc.inv; };  // the distance to the maximum, falling with l
+  const float4 *row4 = reinterpret_cast<const float4 *>(row);
+  const XT *whole = static_cast<const XT *>(a.logits) + b * a.row_stride;
+  auto logit = [&](int i) { return no_nan(to_f32(whole[i])); };
+  auto w_of = [&](uint32_t bits) { return weight_w(__uint_as_float(bits)); };
+  auto key_w = [&](u64 e) { return weight_w(weight_e(key_float(static_cast<uint32_t>(e >> 32)), zmax)); };
+  // (key, ~index): descending order is by descending key, then by ascending index
+  auto entry = [&](float l, int i) { return static_cast<u64>(float_key(sc.z(l))) << 32 | static_cast<uint32_t>(~i); };
+  auto entry_key = [&](u64 e) { return static_cast<uint32_t>(e >> 32); };
+  auto entry_index = [&](u64 e) { return static_cast<int>(~static_cast<uint32_t>(e)); };
+  u64 *spare = reinterpret_cast<u64 *>(columns);
 
-  // The tokens of all blocks' lists in `sorted`, by descending key and ascending index (key above, ~index below), filled
-  // with zeros to a power of two.  The caller has met after the lists' end.
-  auto merge = [&](int n_all) {
-    int size = 32;
-    while (size < n_all) size *= 2;
-    for (int i = n_all + tid; i < size; i += kThreads) sorted[i] = 0;
-    for (int r = 0, at = 0; r < C; at += sh.n[r++]) {
-      const uint2 *src = cluster.map_shared_rank(list, r);
-      for (int i = tid; i < sh.n[r]; i += kThreads) {
-        const uint2 e = src[i];
-        sorted[at + i] = static_cast<u64>(float_key(sc.z(__uint_as_float(e.x)))) << 32 | static_cast<uint32_t>(~e.y);
-      }
-    }
-    __syncthreads();
-    sort_down(sorted, size);
-  };
-  auto sorted_w = [&](int i) { return weight_w(weight_e(key_float(static_cast<uint32_t>(sorted[i] >> 32)), zmax)); };
-  // The first place of `sorted` at which the running sum of f reaches want; n_all where it does not.
-  auto reach = [&](int n_all, u64 want, auto &&f) {
-    if (tid == 0) sh.at = n_all;
+  // The first place of `sorted` at which the running sum of f reaches want; n where it does not.
+  auto reach = [&](int n, u64 want, auto &&f) {
+    if (tid == 0) sh.at = n;
     const int i = 2 * tid;
-    const u64 w0 = i < n_all ? f(i) : 0, w1 = i + 1 < n_all ? f(i + 1) : 0;
+    const u64 w0 = i < n ? f(i) : 0, w1 = i + 1 < n ? f(i + 1) : 0;
     u64 all;
     const u64 before = block_scan_u64(w0 + w1, sh.red, &all);
     if (before < want && want <= before + w0 + w1) sh.at = before + w0 >= want ? i : i + 1;
@@ -448,52 +463,18 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     __syncthreads();
     return at;
   };
-  auto cut_at = [&](int i) {
-    const u64 e = sorted[i];
-    Cut c;
-    c.key = static_cast<uint32_t>(e >> 32);
-    c.idx = static_cast<int>(~static_cast<uint32_t>(e));
-    const float l = key_float(c.key) * T, margin = fabsf(l) * 1e-6f + 8.3e-25f;
-    c.lo = l - margin;
-    c.hi = l + margin;
-    return c;
-  };
-
-  // Counts (or masses) of the tokens kept by `in` in bins between lo and hi, to every block; a mass's sum goes to sh.mass.
-  // Returns the first bin in which the running sum may reach want(), and in sure the first in which it must.
-  auto bins = [&](bool by_mass, float lo, float hi, u64 base, const Cut in, auto &&want, int &sure) {
-    const float width = (hi - lo) * (1.f / kBins), per = 1.f / width;
-    for (int i = tid; i < kBins * 32; i += kThreads) columns[i] = 0;
-    if (by_mass && tid < kBins)  // a column's sum of up to slice / 32 weights of the bin fits 32 bits
-      sh.shift[tid] = max(0, static_cast<int>((__float_as_uint(expf(-(lo + tid * width)) * 1.01f * 2147483648.f * (a.slice / 32 + 4)) >> 23)) - 127 - 31);
+  // The columns' sums to every block's counts, `mine` to every block's mass; then the first bin in which the running sum
+  // of all blocks' counts may reach want(), and in `must` the first in which it does; scale(bin) is the bin's shift.
+  auto settle = [&](u64 mine, u64 base, auto &&want, auto &&scale, int &must) {
     __syncthreads();
-    u64 mine = 0;
-    if (by_mass) {
-      each([&](float l, int i) {
-        const float d = far_of(l);
-        if (!(d >= lo && d < hi) || !kept_by(in, sc, l, i)) return;
-        const uint32_t w = weight_w(weight_e(sc.z(l), zmax));
-        const int j = min(kBins - 1, static_cast<int>((d - lo) * per));
-        mine += w;
-        atomicAdd(&columns[j * 32 + lane], w >> sh.shift[j]);
-      });
-      mine = block_sum_u64(mine, sh.red);
-    } else {
-      each([&](float l, int i) {
-        const float d = far_of(l);
-        if (d >= lo && d < hi && kept_by(in, sc, l, i))
-          atomicAdd(&columns[min(kBins - 1, static_cast<int>((d - lo) * per)) * 32 + lane], 1u);
-      });
-    }
-    __syncthreads();
+#pragma unroll
     for (int j = warp; j < kBins; j += kThreads / 32) {
-      // 32 columns of up to 31 bits: the sum in two halves
-      const uint32_t c = columns[j * 32 + lane];
+      const uint32_t c = columns[j * 32 + lane];  // 32 columns of up to 32 bits: the sum in two halves
       const uint32_t low = __reduce_add_sync(0xffffffffu, c & 0xffffu), high16 = __reduce_add_sync(0xffffffffu, c >> 16);
-      const u64 sum = (static_cast<u64>(high16) << 16) + low;
-      if (lane == 0) tell(&sh.counts[rank][j], sum);
+      tell(&sh.counts[rank][j], (static_cast<u64>(high16) << 16) + low);
     }
-    if (tid == 0) tell(&sh.mass[rank], mine);
+    mine = block_sum_u64(mine, sh.red);
+    if (warp == 0) tell(&sh.mass[rank], mine);
     meet();
     if (warp == 0) {  // lane l: bins 4 l .. 4 l + 3
       const u64 target = want();
@@ -502,203 +483,319 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
       for (int j = 0; j < 4; ++j) {
         u64 c = 0;
         for (int r = 0; r < C; ++r) c += sh.counts[r][4 * lane + j];
-        some[j] = most[j] = c;
-        if (by_mass) {  // a shift leaves at least 2^20 of a weight, so it drops less than 2^-20 of the sum
-          some[j] = c << sh.shift[4 * lane + j];
-          most[j] = some[j] + (sh.shift[4 * lane + j] ? some[j] >> 18 : 0);
-        }
-        sum_some += some[j];
-        sum_most += most[j];
+        const int shift = scale(4 * lane + j);  // it leaves at least 2^20 of a weight: it drops less than 2^-20 of the sum
+        sum_some += some[j] = c << shift;
+        sum_most += most[j] = some[j] + (shift ? some[j] >> 18 : 0);
       }
       u64 run_some = base + warp_scan_u64(sum_some) - sum_some, run_most = base + warp_scan_u64(sum_most) - sum_most;
-      int first = kBins, must = kBins;
+      int first = kBins, sure = kBins;
 #pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        u64 s = run_some, m = run_most;
-        for (int i = 0; i <= j; ++i) {
-          s += some[i];
-          m += most[i];
-        }
-        if (m >= target) first = 4 * lane + j;
-        if (s >= target) must = 4 * lane + j;
+      for (int j = 0; j < 4; ++j) {
+        run_some += some[j];
+        run_most += most[j];
+        if (run_most >= target) first = min(first, 4 * lane + j);
+        if (run_some >= target) sure = min(sure, 4 * lane + j);
       }
       first = __reduce_min_sync(0xffffffffu, first);
-      must = __reduce_min_sync(0xffffffffu, must);
+      sure = __reduce_min_sync(0xffffffffu, sure);
       if (lane == 0) {
         sh.band[0] = first;
-        sh.band[1] = must;
+        sh.band[1] = sure;
       }
     }
     __syncthreads();
-    sure = sh.band[1];
+    must = sh.band[1];
     return sh.band[0];
   };
-  // Lists the tokens kept by `in` between lo and hi; counts (or sums) those above lo; all to every block.  Returns the
-  // number listed by all blocks; above and the nearest logits outside come back too.
-  auto collect = [&](bool by_mass, float lo, float hi, const Cut in, u64 &above, float &min_above, float &max_below) {
+  auto clear_columns = [&]() {
+    for (int i = tid; i < kBins * 8; i += kThreads) reinterpret_cast<uint4 *>(columns)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  };
+  auto no_shift = [](int) { return 0; };
+  auto sum_told = [&](const u64 *v) {
+    u64 sum = 0;
+    for (int r = 0; r < C; ++r) sum += v[r];
+    return sum;
+  };
+
+  // ---- top-k: bins of the distance to the maximum --------------------------------
+  auto count_bins = [&](float lo, float hi, u64 base, u64 want, int &must) {
+    const float per = kBins / (hi - lo);
+    clear_columns();
+    for (int q = tid; q < n4; q += kThreads) {
+      const float4 v = row4[q];
+      const float d[4] = {far_of(v.x), far_of(v.y), far_of(v.z), far_of(v.w)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (d[j] >= lo && d[j] < hi) atomicAdd(&columns[min(kBins - 1, static_cast<int>((d[j] - lo) * per)) * 32 + lane], 1u);
+    }
+    return settle(0, base, [&]() { return want; }, no_shift, must);
+  };
+  // Lists the tokens between lo and hi and counts those above lo, to every block; returns the number listed.
+  auto collect = [&](float lo, float hi, u64 &above, float &min_above, float &max_below) {
     if (tid == 0) sh.n_local = 0;
     __syncthreads();
-    above = 0;
+    uint32_t mine = 0;
     min_above = INFINITY;
     max_below = -INFINITY;
     each([&](float l, int i) {
       const float d = far_of(l);
-      if (!(d < hi)) {
-        max_below = fmaxf(max_below, l);
-        return;
-      }
-      if (!kept_by(in, sc, l, i)) return;
       if (d < lo) {
-        above += by_mass ? weight_w(weight_e(sc.z(l), zmax)) : 1u;
+        ++mine;
         min_above = fminf(min_above, l);
-      } else {
+      } else if (d < hi) {
         const int at = atomicAdd(&sh.n_local, 1);
         if (at < kCap) list[at] = make_uint2(__float_as_uint(l), i);
+      } else {
+        max_below = fmaxf(max_below, l);
       }
     });
-    above = block_sum_u64(above, sh.red);
+    above = block_sum_u64(mine, sh.red);
     min_above = -block_max(-min_above, sh.redf);
     max_below = block_max(max_below, sh.redf);
-    if (tid == 0) {
+    if (warp == 0) {
       tell(&sh.above[rank], above);
       tell(&sh.n[rank], sh.n_local);
       tell(&sh.min_above[rank], min_above);
       tell(&sh.max_below[rank], max_below);
     }
     meet();
-    above = 0;
+    above = sum_told(sh.above);
     int n_all = 0;
     for (int r = 0; r < C; ++r) {
-      above += sh.above[r];
       n_all += sh.n[r];
       min_above = fminf(min_above, sh.min_above[r]);
       max_below = fmaxf(max_below, sh.max_below[r]);
     }
     return n_all;
   };
-  auto below_cut = [&](float l, const Cut &c) { return l == -INFINITY || float_key(sc.z(l)) < c.key; };
-  auto above_cut = [&](float l, const Cut &c) { return l == INFINITY || float_key(sc.z(l)) > c.key; };
-  const u64 p24 = static_cast<u64>(rintf(fminf(fmaxf(top_p, 0.f), 1.f) * 16777216.f));
-  auto most_of = [&](u64 mass) { return max(part_of(p24, mass), u64(1)); };
-  const u64 u24 = static_cast<u64>(fminf(fmaxf(a.u[b] * 16777216.f, 0.f), 16777215.f));
-
-  // The cut at which the count (or mass) over descending z first reaches its target, among the tokens that `in` keeps.
-  // b0, b1: the bins of the first level, already found.
-  auto search = [&](bool by_mass, u64 want, const Cut in, int b0, int b1) {
-    float lo = 0.f, hi = kFar;
-    for (int level = 0; level < kLevels && !slow; ++level) {
-      const float width = (hi - lo) * (1.f / kBins);
-      if (b0 >= kBins) break;
-      b1 = min(b1, kBins - 1);
-      const float new_lo = b0 == 0 ? lo : lo + (b0 - 0.02f) * width, new_hi = b1 == kBins - 1 ? hi : lo + (b1 + 1.02f) * width;
-      u64 above;
-      float min_above, max_below;
-      const int n_all = collect(by_mass, new_lo, new_hi, in, above, min_above, max_below);
-      if (n_all <= kCap) {
-        merge(n_all);
-        const int at = above < want ? reach(n_all, want - above, [&](int i) { return by_mass ? static_cast<u64>(sorted_w(i)) : u64(1); }) : n_all;
-        Cut c = in;
-        if (at < n_all) c = cut_at(at);
-        slow = at == n_all || !above_cut(min_above, c) || !below_cut(max_below, c);
-        meet();  // the lists have been read
-        return c;
+  auto merge = [&](int n_all) {  // all blocks' listed tokens, sorted
+    for (int r = 0, at = 0; r < C; at += sh.n[r++]) {
+      const uint2 *src = cluster.map_shared_rank(list, r);
+      for (int i = tid; i < sh.n[r]; i += kThreads) {
+        const uint2 e = src[i];
+        sorted[at + i] = entry(__uint_as_float(e.x), static_cast<int>(e.y));
       }
-      lo = new_lo;
-      hi = new_hi;
-      meet();  // what the blocks told each other has been read
-      b0 = bins(by_mass, lo, hi, above, in, [&]() { return want; }, b1);
     }
-    slow = true;
-    return in;
+    __syncthreads();
+    sort_down(sorted, spare, n_all);
+  };
+  auto outside = [&](u64 e, float min_above, float max_below) {  // whether these lie strictly above and below the entry
+    const uint32_t key = entry_key(e);
+    return (min_above == INFINITY || float_key(sc.z(min_above)) > key) && (max_below == -INFINITY || float_key(sc.z(max_below)) < key);
   };
 
-  if (!slow && (has_k || has_p)) {
-    // the bins of the first cut, and the list of everything down to it
-    int b1, b0 = bins(!has_k, 0.f, kFar, 0, cut, [&]() {
-      if (has_k) return static_cast<u64>(k);
-      u64 mass = 0;
-      for (int r = 0; r < C; ++r) mass += sh.mass[r];
-      return most_of(mass);
-    }, b1);
-    u64 mass_all = 0;
-    for (int r = 0; r < C; ++r) mass_all += sh.mass[r];
-    // has_k and no bin: fewer than k tokens have a weight above 0, and all of them are kept
-    u64 above = 0;
-    float min_above = INFINITY, max_below = -INFINITY;
-    const float hi = b0 >= kBins || b1 >= kBins - 1 ? kFar : (b1 + 1.02f) * (kFar / kBins);
-    const int n_all = collect(false, 0.f, hi, cut, above, min_above, max_below);
+  // ---- the kept tokens of a sorted list: min-p, then the draw (by one block) --------
+  auto draw_from = [&](int n) {
+    const int i = 2 * tid;
+    u64 e[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      e[j] = 0;
+      if (i + j < n) {
+        const float w_e = weight_e(key_float(entry_key(sorted[i + j])), zmax);
+        e[j] = sorted[i + j] << 32 | (w_e >= min_e ? weight_w(w_e) : 0u);  // (~index, weight)
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (i + j < n) sorted[i + j] = e[j];
+    __syncthreads();
+    sort_down(sorted, spare, n);
+    const u64 total = block_sum_u64((i < n ? sorted[i] & 0xffffffffu : 0) + (i + 1 < n ? sorted[i + 1] & 0xffffffffu : 0), sh.red);
+    const int at = reach(n, part_of(u24, total) + 1, [&](int j) { return sorted[j] & 0xffffffffu; });
+    if (tid == 0) {
+      a.tokens[b] = static_cast<int>(~static_cast<uint32_t>(sorted[at] >> 32));
+      if (a.probs) a.probs[b] = __fdiv_rn(static_cast<float>(sorted[at] & 0xffffffffu), static_cast<float>(total));
+    }
+  };
+
+  Cut<float> top{0, -1, -INFINITY, -INFINITY};  // top-k's cut, over logits
+  if (!slow && has_k) {
+    int b1, b0 = count_bins(0.f, kFar, 0, k, b1);
+    const bool all = b0 >= kBins;  // fewer than k tokens have a weight above 0: all of them are kept
+    float lo = 0.f, hi = all ? kFar : (b0 + 1.02f) * (kFar / kBins), min_above, max_below;
+    u64 above;
+    int n_all = collect(lo, hi, above, min_above, max_below);
     if (n_all <= kCap) {
       if (rank == 0) {
         merge(n_all);
-        // how many of the list the filters keep
-        int n = n_all;
-        bool bad = false;
-        if (has_k && b0 < kBins) {
-          n = k;
-          bad = n > n_all || !below_cut(max_below, cut_at(max(0, min(n, n_all) - 1)));
-          n = min(n, n_all);
+        int n = all ? n_all : k;
+        bool bad = !all && (n > n_all || !outside(sorted[min(n, n_all) - 1], INFINITY, max_below));
+        if (!bad && has_p) {
+          const int i = 2 * tid;
+          const u64 mass = block_sum_u64((i < n ? key_w(sorted[i]) : 0u) + static_cast<u64>(i + 1 < n ? key_w(sorted[i + 1]) : 0u), sh.red);
+          n = reach(n, most_of(mass), [&](int j) { return static_cast<u64>(key_w(sorted[j])); }) + 1;
         }
-        u64 mass = mass_all;
-        const int i = 2 * tid;
-        if (has_p) {
-          if (has_k) mass = block_sum_u64((i < n ? sorted_w(i) : 0u) + static_cast<u64>(i + 1 < n ? sorted_w(i + 1) : 0u), sh.red);
-          const int at = reach(n, most_of(mass), [&](int j) { return static_cast<u64>(sorted_w(j)); });
-          bad = bad || at == n;
-          if (at < n) {
-            if (!has_k) bad = bad || !below_cut(max_below, cut_at(at));
-            n = at + 1;
-          }
-        }
-        if (!bad) {
-          // the kept tokens by index: (index, weight) sorted again; min-p leaves its tokens with weight 0
-          __syncthreads();
-          u64 e[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            e[j] = 0;
-            if (i + j < n) {
-              const float w_e = weight_e(key_float(static_cast<uint32_t>(sorted[i + j] >> 32)), zmax);
-              const uint32_t w = w_e >= min_e ? weight_w(w_e) : 0u;
-              e[j] = sorted[i + j] << 32 | w;  // ~index above: descending is by ascending index
-            }
-          }
-          __syncthreads();
-          int size = 32;
-          while (size < n) size *= 2;
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (i + j < size) sorted[i + j] = e[j];
-          __syncthreads();
-          sort_down(sorted, size);
-          const u64 total = block_sum_u64((i < n ? sorted[i] & 0xffffffffu : 0) + (i + 1 < n ? sorted[i + 1] & 0xffffffffu : 0), sh.red);
-          const int at = reach(n, part_of(u24, total) + 1, [&](int j) { return sorted[j] & 0xffffffffu; });
-          if (tid == 0) {
-            a.tokens[b] = static_cast<int>(~static_cast<uint32_t>(sorted[at] >> 32));
-            if (a.probs) a.probs[b] = __fdiv_rn(static_cast<float>(sorted[at] & 0xffffffffu), static_cast<float>(total));
-          }
-        }
-        if (tid == 0) tell(&sh.first[0], bad ? 1 : 0);
+        if (!bad) draw_from(n);
+        if (warp == 0) tell(&sh.bad, bad ? 1 : 0);
       }
       meet();  // the lists have been read
-      if (!sh.first[0]) return;
+      if (!sh.bad) return;
       slow = true;
-    } else {
-      meet();  // what the blocks told each other has been read
-      if (has_k && b0 < kBins) cut = search(false, k, cut, b0, b1);
-      if (has_p && !slow) {
-        u64 most = 0;
-        if (has_k) {
-          b0 = bins(true, 0.f, kFar, 0, cut, [&]() {
-            u64 mass = 0;
-            for (int r = 0; r < C; ++r) mass += sh.mass[r];
-            return most_of(mass);
-          }, b1);
-          mass_all = 0;
-          for (int r = 0; r < C; ++r) mass_all += sh.mass[r];
+    } else if (!all) {
+      float width = kFar / kBins;
+      for (int level = 0;; ++level) {
+        const float new_lo = b0 == 0 ? lo : lo + (b0 - 0.02f) * width;
+        hi = b0 == kBins - 1 ? hi : lo + (b0 + 1.02f) * width;
+        lo = new_lo;
+        meet();  // what the blocks told each other has been read
+        n_all = collect(lo, hi, above, min_above, max_below);
+        if (n_all <= kCap) {
+          merge(n_all);
+          const u64 want = k - above;  // the cut's place in the list
+          slow = above >= static_cast<u64>(k) || want > static_cast<u64>(n_all);
+          if (!slow) {
+            const u64 e = sorted[want - 1];
+            const float l = key_float(entry_key(e)) * T, margin = fabsf(l) * 1e-6f + 8.3e-25f;
+            top = {entry_key(e), entry_index(e), l - margin, l + margin};
+            slow = !outside(e, min_above, max_below);
+          }
+          meet();  // the lists have been read
+          break;
         }
-        most = most_of(mass_all);
-        cut = search(true, most, cut, b0, b1);
+        if (level + 1 == kLevels) {
+          slow = true;
+          break;
+        }
+        meet();
+        width = (hi - lo) / kBins;
+        b0 = count_bins(lo, hi, above, k, b1);
+        if (b0 >= kBins) {
+          slow = true;
+          break;
+        }
       }
+    } else {
+      meet();
+    }
+  }
+  auto in_top = [&](float l, int i) { return l > top.hi || (l >= top.lo && keeps(top.key, top.idx, sc, l, i)); };
+  auto e_of = [&](float l, int i) { return has_k && !in_top(l, i) ? 0.f : weight_e(sc.z(l), zmax); };
+
+  Cut<uint32_t> nucleus{0, -1, 0, 0};  // top-p's cut, over the bits of e
+  if (!slow && has_p) {
+    // e takes the logits' place; bins of its exponent and two bits more, 0 for e in 1 .. 1/2 and up
+    constexpr int kTop = 0x3f800000 >> 21;
+    auto shift_of = [](uint32_t bits) { return max(0, static_cast<int>(bits >> 23) - 117); };
+    clear_columns();
+    u64 mine = 0;
+    for (int q = tid; q < n4; q += kThreads) {
+      const float4 v = row4[q];
+      const int i = i_begin + 4 * q - off;
+      const float e[4] = {e_of(v.x, i), e_of(v.y, i + 1), e_of(v.z, i + 2), e_of(v.w, i + 3)};
+      reinterpret_cast<float4 *>(row)[q] = make_float4(e[0], e[1], e[2], e[3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = weight_w(e[j]), bits = __float_as_uint(e[j]);
+        mine += w;
+        if (w) atomicAdd(&columns[(kTop - (bits >> 21)) * 32 + lane], w >> shift_of(bits));
+      }
+    }
+    int b1, b0 = settle(mine, 0, [&]() { return most_of(sum_told(sh.mass)); },
+                        [&](int j) { return shift_of(static_cast<uint32_t>(kTop - j) << 21); }, b1);
+    const u64 most = most_of(sum_told(sh.mass));
+    slow = b0 >= kBins || b1 >= kBins;
+    uint32_t lo = 0, hi = 0;  // the bits of e between which the cut lies
+    if (!slow) {
+      lo = static_cast<uint32_t>(kTop - b1) << 21;
+      hi = static_cast<uint32_t>(kTop - b0 + 1) << 21;
+    }
+    for (int step = 14; !slow; step -= 7) {
+      const uint32_t from = lo - 8, to = hi + 8;  // beyond them z is strictly smaller or larger
+      if (tid == 0) sh.n_local = sh.n_local_top = 0;
+      __syncthreads();
+      u64 sum = 0;
+      each([&](float e, int i) {
+        const uint32_t bits = __float_as_uint(e);
+        if (bits < from) return;
+        if (bits >= to) {
+          sum += w_of(bits);
+          if (step == 14) {
+            const int at = atomicAdd(&sh.n_local_top, 1);
+            if (at < kCap) list_top[at] = i;
+          }
+        } else {
+          const int at = atomicAdd(&sh.n_local, 1);
+          if (at < kCap) list_band[at] = i;
+        }
+      });
+      sum = block_sum_u64(sum, sh.red);
+      if (warp == 0) {
+        tell(&sh.above[rank], sum);
+        tell(&sh.n[rank], sh.n_local);
+        tell(&sh.n_top[rank], sh.n_local_top);
+      }
+      meet();
+      const u64 above = sum_told(sh.above);
+      int n_band = 0, n_top = 0;
+      for (int r = 0; r < C; ++r) {
+        n_band += sh.n[r];
+        n_top += sh.n_top[r];
+      }
+      const bool short_list = step == 14 && n_band + n_top <= kCap;
+      if (short_list || n_band <= kCap) {
+        // the listed tokens with their z, read again
+        const int n_all = n_band + (short_list ? n_top : 0);
+        if (!short_list || rank == 0) {
+          int at = 0;
+          for (int r = 0; r < C; ++r) {
+            const int *band = cluster.map_shared_rank(list_band, r), *up = cluster.map_shared_rank(list_top, r);
+            const int nb = sh.n[r], nt = short_list ? sh.n_top[r] : 0;
+            for (int i = tid; i < nb + nt; i += kThreads) {
+              const int idx = i < nb ? band[i] : up[i - nb];
+              sorted[at + i] = entry(logit(idx), idx);
+            }
+            at += nb + nt;
+          }
+          __syncthreads();
+          sort_down(sorted, spare, n_all);
+          const u64 want = short_list ? most : most - above;  // above < most: the cut lies below
+          const int place = reach(n_all, want, [&](int j) { return static_cast<u64>(key_w(sorted[j])); });
+          if (short_list) {
+            if (place < n_all) draw_from(place + 1);
+            if (warp == 0) tell(&sh.bad, place == n_all ? 1 : 0);
+          } else {
+            slow = place == n_all || above >= most;
+            if (!slow) {
+              const u64 e = sorted[place];
+              const uint32_t bits = __float_as_uint(weight_e(key_float(entry_key(e)), zmax));
+              nucleus = {entry_key(e), entry_index(e), bits - 8, bits + 8};
+            }
+          }
+        }
+        meet();  // the lists have been read
+        if (short_list) {
+          if (!sh.bad) return;
+          slow = true;
+        }
+        break;
+      }
+      if (step < 0 || b0 != b1) {
+        slow = true;
+        break;
+      }
+      // too many: finer bins of the bits that follow
+      meet();  // what the blocks told each other has been read
+      clear_columns();
+      mine = 0;
+      each([&](float e, int) {
+        const uint32_t bits = __float_as_uint(e);
+        if (bits < lo) return;
+        if (bits >= hi) mine += w_of(bits);
+        else atomicAdd(&columns[(127 - ((bits >> step) & 127)) * 32 + lane], w_of(bits) >> shift_of(bits));
+      });
+      const uint32_t base_bits = lo;
+      // what lies above the bins comes with the masses
+      auto shift_here = [&](int) { return shift_of(base_bits); };
+      b0 = settle(mine, 0, [&]() {
+        const u64 base = sum_told(sh.mass);
+        return most > base ? most - base : u64(1);
+      }, shift_here, b1);
+      slow = b0 >= kBins || b1 >= kBins;
+      lo = base_bits + (static_cast<uint32_t>(127 - b1) << step);
+      hi = base_bits + (static_cast<uint32_t>(128 - b0) << step);
     }
   }
   if (slow) {
@@ -706,21 +803,28 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     return;
   }
 
-  // ---- the draw: running sums in index order, a run of float4s a warp -----------
+  // ---- the draw over the row: running sums in index order, a run of float4s a warp ---
   const int seg = (n4 + kThreads / 32 - 1) / (kThreads / 32);
   const int q0 = min(n4, warp * seg), q1 = min(n4, q0 + seg);
-  // a logit below this one has e < min_p for sure
-  const float low = min_e > 0.f ? high + T * (logf(min_e) - 1e-3f) - fabsf(high) * 1e-5f : -INFINITY;
-  auto weight_at = [&](float l, int i) -> u64 {
-    if (!(far_of(l) < kFar) || l < low || !kept_by(cut, sc, l, i)) return 0;
-    const float e = weight_e(sc.z(l), zmax);
+  // a logit below this one has e < min_p, or weight 0, for sure
+  const float low = fmaxf(min_e > 0.f ? high + T * (logf(min_e) - 1e-3f) - fabsf(high) * 1e-5f : -INFINITY, high - T * kFar - fabsf(high) * 1e-5f);
+  auto weight_at = [&](float v, int i) -> uint32_t {
+    float e;
+    if (has_p) {
+      e = v;
+      const uint32_t bits = __float_as_uint(e);
+      if (bits < nucleus.hi && (bits < nucleus.lo || !keeps(nucleus.key, nucleus.idx, sc, logit(i), i))) e = 0.f;
+    } else {
+      e = v >= low ? e_of(v, i) : 0.f;
+    }
     return e >= min_e ? weight_w(e) : 0u;
   };
   u64 mine = 0;
   for (int q = q0 + lane; q < q1; q += 32) {
-    const float4 v = reinterpret_cast<const float4 *>(row)[q];
+    const float4 v = row4[q];
     const int i = i_begin + 4 * q - off;
-    mine += weight_at(v.x, i) + weight_at(v.y, i + 1) + weight_at(v.z, i + 2) + weight_at(v.w, i + 3);
+    const uint32_t w[4] = {weight_at(v.x, i), weight_at(v.y, i + 1), weight_at(v.z, i + 2), weight_at(v.w, i + 3)};
+    mine += static_cast<u64>(w[0]) + w[1] + static_cast<u64>(w[2]) + w[3];
   }
   mine = warp_sum_u64(mine);
   __syncthreads();
@@ -731,26 +835,26 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     if (w < warp) before += sh.red[w];
     total += sh.red[w];
   }
-  if (tid == 0) tell(&sh.mass[rank], total);
+  if (warp == 0) tell(&sh.above[rank], total);
   meet();
   total = 0;
   for (int r = 0; r < C; ++r) {
-    if (r < rank) before += sh.mass[r];
-    total += sh.mass[r];
+    if (r < rank) before += sh.above[r];
+    total += sh.above[r];
   }
   const u64 target = part_of(u24, total);
   if (target < before || target >= before + mine) return;
   for (int q = q0; q < q1; q += 32) {
-    u64 w[4] = {0, 0, 0, 0};
+    uint32_t w[4] = {0, 0, 0, 0};
     const int i = i_begin + 4 * (q + lane) - off;
     if (q + lane < q1) {
-      const float4 v = reinterpret_cast<const float4 *>(row)[q + lane];
+      const float4 v = row4[q + lane];
       w[0] = weight_at(v.x, i);
       w[1] = weight_at(v.y, i + 1);
       w[2] = weight_at(v.z, i + 2);
       w[3] = weight_at(v.w, i + 3);
     }
-    const u64 sum = w[0] + w[1] + w[2] + w[3], inc = warp_scan_u64(sum);
+    const u64 sum = static_cast<u64>(w[0]) + w[1] + static_cast<u64>(w[2]) + w[3], inc = warp_scan_u64(sum);
     const u64 all = __shfl_sync(0xffffffffu, inc, 31);
     if (target < before + all) {
       u64 run = before + inc - sum;
