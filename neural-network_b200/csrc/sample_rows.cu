@@ -339,7 +339,7 @@ __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
 // below.  A row that fails, and one that never narrows, is done by
 // sample_whole_row.
 template <typename XT>
-__global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const SampleArgs a) {
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -397,21 +397,35 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   meet();
   high = -INFINITY;
   for (int r = 0; r < C; ++r) high = fmaxf(high, sh.high[r]);
-  // a pass over the slice: f(value, index in the row)
-  auto each = [&](auto &&f) {
-    for (int q = tid; q < n4; q += kThreads) {
-      const float4 v = reinterpret_cast<const float4 *>(row)[q];
-      const int i = i_begin + 4 * q - off;
-      f(v.x, i);
-      f(v.y, i + 1);
-      f(v.z, i + 2);
-      f(v.w, i + 3);
+  // a pass over the slice by whole warps: f(four values, index of the first in the row), `none` where there is no token
+  const float4 *row4 = reinterpret_cast<const float4 *>(row);
+  auto each4 = [&](float none, auto &&f) {
+    for (int q = tid; q - lane < n4; q += kThreads) {
+      const float4 x = q < n4 ? row4[q] : make_float4(none, none, none, none);
+      const float v[4] = {x.x, x.y, x.z, x.w};
+      f(v, i_begin + 4 * q - off);
+    }
+  };
+  // put(place, j) for those of a thread's four tokens j for which `is` holds, places counted up in `count`; by whole warps.
+  auto append4 = [&](const bool (&is)[4], int *count, auto &&put) {
+    if (!__any_sync(0xffffffffu, is[0] || is[1] || is[2] || is[3])) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t who = __ballot_sync(0xffffffffu, is[j]);
+      if (!who) continue;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(count, __popc(who));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+      if (is[j] && at < kCap) put(at, j);
     }
   };
   if (high == -INFINITY || greedy) {
     int first = 0x7fffffff;
     if (greedy && high != -INFINITY)
-      each([&](float l, int i) { if (l == high) first = min(first, i); });
+      each4(-INFINITY, [&](const float (&l)[4], int i) {
+        for (int j = 3; j >= 0; --j)
+          if (l[j] == high) first = min(first, i + j);
+      });
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) sh.redi[warp] = first;
     __syncthreads();
@@ -439,7 +453,6 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   // temperatures and logits for which equal z means nearly equal logits
   bool slow = !(T >= 9.1e-13f && T <= 1.1e12f && fabsf(high) < 1.2e24f);
   auto far_of = [&](float l) { return (high - l) * sc.inv; };  // the distance to the maximum, falling with l
-  const float4 *row4 = reinterpret_cast<const float4 *>(row);
   const XT *whole = static_cast<const XT *>(a.logits) + b * a.row_stride;
   auto logit = [&](int i) { return no_nan(to_f32(whole[i])); };
   auto w_of = [&](uint32_t bits) { return weight_w(__uint_as_float(bits)); };
@@ -538,18 +551,22 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     uint32_t mine = 0;
     min_above = INFINITY;
     max_below = -INFINITY;
-    each([&](float l, int i) {
-      const float d = far_of(l);
-      if (d < lo) {
-        ++mine;
-        min_above = fminf(min_above, l);
-      } else if (d < hi) {
-        const int at = atomicAdd(&sh.n_local, 1);
-        if (at < kCap) list[at] = make_uint2(__float_as_uint(l), i);
-      } else {
-        max_below = fmaxf(max_below, l);
+    each4(-INFINITY, [&](const float (&l)[4], int i) {
+      bool is[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float d = far_of(l[j]);
+        is[j] = d >= lo && d < hi;
+        if (d < lo) {
+          ++mine;
+          min_above = fminf(min_above, l[j]);
+        } else if (!is[j]) {
+          max_below = fmaxf(max_below, l[j]);
+        }
       }
+      append4(is, &sh.n_local, [&](int at, int j) { list[at] = make_uint2(__float_as_uint(l[j]), i + j); });
     });
+    __syncthreads();
     above = block_sum_u64(mine, sh.red);
     min_above = -block_max(-min_above, sh.redf);
     max_below = block_max(max_below, sh.redf);
@@ -569,16 +586,20 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     }
     return n_all;
   };
-  auto merge = [&](int n_all) {  // all blocks' listed tokens, sorted
-    for (int r = 0, at = 0; r < C; at += sh.n[r++]) {
-      const uint2 *src = cluster.map_shared_rank(list, r);
-      for (int i = tid; i < sh.n[r]; i += kThreads) {
-        const uint2 e = src[i];
-        sorted[at + i] = entry(__uint_as_float(e.x), static_cast<int>(e.y));
-      }
+  // Place p of the blocks' lists of n[r] entries one after the other: the block, p becoming the place in its list.
+  auto block_of = [&](const int *n, int &p) {
+    int r = 0;
+    while (p >= n[r]) p -= n[r++];
+    return r;
+  };
+  auto merge = [&](int n_all) {  // all blocks' listed tokens
+    for (int i = tid; i < n_all; i += kThreads) {
+      int p = i;
+      const int r = block_of(sh.n, p);
+      const uint2 e = cluster.map_shared_rank(list, r)[p];
+      sorted[i] = entry(__uint_as_float(e.x), static_cast<int>(e.y));
     }
     __syncthreads();
-    sort_down(sorted, spare, n_all);
   };
   auto outside = [&](u64 e, float min_above, float max_below) {  // whether these lie strictly above and below the entry
     const uint32_t key = entry_key(e);
@@ -597,18 +618,31 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
         e[j] = sorted[i + j] << 32 | (w_e >= min_e ? weight_w(w_e) : 0u);  // (~index, weight)
       }
     }
-    __syncthreads();
+    const u64 total = block_sum_u64((e[0] & 0xffffffffu) + (e[1] & 0xffffffffu), sh.red);
+    const u64 target = part_of(u24, total);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       if (i + j < n) sorted[i + j] = e[j];
     __syncthreads();
-    sort_down(sorted, spare, n);
-    const u64 total = block_sum_u64((i < n ? sorted[i] & 0xffffffffu : 0) + (i + 1 < n ? sorted[i + 1] & 0xffffffffu : 0), sh.red);
-    const int at = reach(n, part_of(u24, total) + 1, [&](int j) { return sorted[j] & 0xffffffffu; });
-    if (tid == 0) {
-      a.tokens[b] = static_cast<int>(~static_cast<uint32_t>(sorted[at] >> 32));
-      if (a.probs) a.probs[b] = __fdiv_rn(static_cast<float>(sorted[at] & 0xffffffffu), static_cast<float>(total));
+    auto write = [&](u64 x) {
+      a.tokens[b] = static_cast<int>(~static_cast<uint32_t>(x >> 32));
+      if (a.probs) a.probs[b] = __fdiv_rn(static_cast<float>(x & 0xffffffffu), static_cast<float>(total));
+    };
+    if (n <= kThreads / 2) {  // two threads a token add up the weights before it
+      const u64 mine = (tid >> 1) < n ? sorted[tid >> 1] : 0;
+      u64 before = 0;
+#pragma unroll 4
+      for (int j = tid & 1; j < n; j += 2) {
+        const u64 x = sorted[j];
+        before += x > mine ? x & 0xffffffffu : 0;  // a larger ~index: a smaller index
+      }
+      before += __shfl_xor_sync(0xffffffffu, before, 1);
+      if ((tid >> 1) < n && (tid & 1) == 0 && before <= target && target < before + (mine & 0xffffffffu)) write(mine);
+      return;
     }
+    sort_down(sorted, spare, n);
+    const int at = reach(n, target + 1, [&](int j) { return sorted[j] & 0xffffffffu; });
+    if (tid == 0) write(sorted[at]);
   };
 
   Cut<float> top{0, -1, -INFINITY, -INFINITY};  // top-k's cut, over logits
@@ -621,6 +655,7 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     if (n_all <= kCap) {
       if (rank == 0) {
         merge(n_all);
+        sort_down(sorted, spare, n_all);
         int n = all ? n_all : k;
         bool bad = !all && (n > n_all || !outside(sorted[min(n, n_all) - 1], INFINITY, max_below));
         if (!bad && has_p) {
@@ -644,6 +679,7 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
         n_all = collect(lo, hi, above, min_above, max_below);
         if (n_all <= kCap) {
           merge(n_all);
+          sort_down(sorted, spare, n_all);
           const u64 want = k - above;  // the cut's place in the list
           slow = above >= static_cast<u64>(k) || want > static_cast<u64>(n_all);
           if (!slow) {
@@ -704,23 +740,24 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     }
     for (int step = 14; !slow; step -= 7) {
       const uint32_t from = lo - 8, to = hi + 8;  // beyond them z is strictly smaller or larger
+      // every token above the band is listed too where they may be few: there are at most most / w(band) of them
+      const bool list_all = step == 14 && most < static_cast<u64>(4 * kCap) * w_of(lo);
       if (tid == 0) sh.n_local = sh.n_local_top = 0;
       __syncthreads();
       u64 sum = 0;
-      each([&](float e, int i) {
-        const uint32_t bits = __float_as_uint(e);
-        if (bits < from) return;
-        if (bits >= to) {
-          sum += w_of(bits);
-          if (step == 14) {
-            const int at = atomicAdd(&sh.n_local_top, 1);
-            if (at < kCap) list_top[at] = i;
-          }
-        } else {
-          const int at = atomicAdd(&sh.n_local, 1);
-          if (at < kCap) list_band[at] = i;
+      each4(0.f, [&](const float (&e)[4], int i) {
+        bool up[4], band[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t bits = __float_as_uint(e[j]);
+          up[j] = bits >= to;
+          band[j] = !up[j] && bits >= from;
+          if (up[j]) sum += w_of(bits);
         }
+        append4(band, &sh.n_local, [&](int at, int j) { list_band[at] = i + j; });
+        if (list_all) append4(up, &sh.n_local_top, [&](int at, int j) { list_top[at] = i + j; });
       });
+      __syncthreads();
       sum = block_sum_u64(sum, sh.red);
       if (warp == 0) {
         tell(&sh.above[rank], sum);
@@ -734,20 +771,16 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
         n_band += sh.n[r];
         n_top += sh.n_top[r];
       }
-      const bool short_list = step == 14 && n_band + n_top <= kCap;
+      const bool short_list = list_all && n_band + n_top <= kCap;
       if (short_list || n_band <= kCap) {
         // the listed tokens with their z, read again
         const int n_all = n_band + (short_list ? n_top : 0);
         if (!short_list || rank == 0) {
-          int at = 0;
-          for (int r = 0; r < C; ++r) {
-            const int *band = cluster.map_shared_rank(list_band, r), *up = cluster.map_shared_rank(list_top, r);
-            const int nb = sh.n[r], nt = short_list ? sh.n_top[r] : 0;
-            for (int i = tid; i < nb + nt; i += kThreads) {
-              const int idx = i < nb ? band[i] : up[i - nb];
-              sorted[at + i] = entry(logit(idx), idx);
-            }
-            at += nb + nt;
+          for (int i = tid; i < n_all; i += kThreads) {
+            int p = i < n_band ? i : i - n_band;
+            const int r = block_of(i < n_band ? sh.n : sh.n_top, p);
+            const int idx = cluster.map_shared_rank(i < n_band ? list_band : list_top, r)[p];
+            sorted[i] = entry(logit(idx), idx);
           }
           __syncthreads();
           sort_down(sorted, spare, n_all);
@@ -780,11 +813,13 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
       meet();  // what the blocks told each other has been read
       clear_columns();
       mine = 0;
-      each([&](float e, int) {
-        const uint32_t bits = __float_as_uint(e);
-        if (bits < lo) return;
-        if (bits >= hi) mine += w_of(bits);
-        else atomicAdd(&columns[(127 - ((bits >> step) & 127)) * 32 + lane], w_of(bits) >> shift_of(bits));
+      each4(0.f, [&](const float (&e)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t bits = __float_as_uint(e[j]);
+          if (bits >= hi) mine += w_of(bits);
+          else if (bits >= lo) atomicAdd(&columns[(127 - ((bits >> step) & 127)) * 32 + lane], w_of(bits) >> shift_of(bits));
+        }
       });
       const uint32_t base_bits = lo;
       // what lies above the bins comes with the masses
