@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
       for (int j = 0; j < 4; ++j) {
         u64 c = 0;
         for (int r = 0; r < C; ++r) c += sh.counts[r][4 * lane + j];
-        const int shift = scale(4 * lane + j);  // it leaves at least 2^20 of a weight: it drops less than 2^-20 of the sum
+        const int shift = scale(4 * lane + j);  // it leaves at least 2^19 of a weight: it drops less than 2^-19 of the sum
         sum_some += some[j] = c << shift;
         sum_most += most[j] = some[j] + (shift ? some[j] >> 18 : 0);
       }
@@ -738,10 +738,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
       lo = static_cast<uint32_t>(kTop - b1) << 21;
       hi = static_cast<uint32_t>(kTop - b0 + 1) << 21;
     }
-    for (int step = 14; !slow; step -= 7) {
+    for (int level = 0; !slow; ++level) {
       const uint32_t from = lo - 8, to = hi + 8;  // beyond them z is strictly smaller or larger
       // every token above the band is listed too where they may be few: there are at most most / w(band) of them
-      const bool list_all = step == 14 && most < static_cast<u64>(4 * kCap) * w_of(lo);
+      const bool list_all = level == 0 && most < static_cast<u64>(4 * kCap) * w_of(lo);
       if (tid == 0) sh.n_local = sh.n_local_top = 0;
       __syncthreads();
       u64 sum = 0;
@@ -805,11 +805,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
         }
         break;
       }
-      if (step < 0 || b0 != b1) {
+      if (hi - lo == 1) {  // that many equal weights
         slow = true;
         break;
       }
-      // too many: finer bins of the bits that follow
+      // too many: 128 finer bins from hi down
+      const int step = max(0, 25 - __clz(hi - lo - 1));  // (hi - lo - 1) >> step < 128
+      const uint32_t top_bits = hi - 1, low_bits = lo;
+      const int shift = shift_of(top_bits);  // one for all: it leaves 2^19 of the lowest weight
       meet();  // what the blocks told each other has been read
       clear_columns();
       mine = 0;
@@ -817,20 +820,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t bits = __float_as_uint(e[j]);
-          if (bits >= hi) mine += w_of(bits);
-          else if (bits >= lo) atomicAdd(&columns[(127 - ((bits >> step) & 127)) * 32 + lane], w_of(bits) >> shift_of(bits));
+          if (bits > top_bits) mine += w_of(bits);
+          else if (bits >= low_bits) atomicAdd(&columns[((top_bits - bits) >> step) * 32 + lane], w_of(bits) >> shift);
         }
       });
-      const uint32_t base_bits = lo;
       // what lies above the bins comes with the masses
-      auto shift_here = [&](int) { return shift_of(base_bits); };
       b0 = settle(mine, 0, [&]() {
         const u64 base = sum_told(sh.mass);
         return most > base ? most - base : u64(1);
-      }, shift_here, b1);
+      }, [&](int) { return shift; }, b1);
       slow = b0 >= kBins || b1 >= kBins;
-      lo = base_bits + (static_cast<uint32_t>(127 - b1) << step);
-      hi = base_bits + (static_cast<uint32_t>(128 - b0) << step);
+      hi = top_bits + 1 - (static_cast<uint32_t>(b0) << step);
+      lo = max(low_bits, top_bits + 1 - (static_cast<uint32_t>(b1 + 1) << step));
     }
   }
   if (slow) {
