@@ -136,24 +136,92 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
 // has older rows, a x (1 / 127)); older rows are brought to scale', new rows
 // become rint(x x (1 / scale')).  A scale below the smallest normal number is
 // 0 (its codes are 0), so 1 / scale' is finite.
+//
+// Bound by HBM: every value is read once and its code written once.  A unit's
+// values stay in registers between the maximum and the codes, up to eight runs
+// of eight adjacent values a lane (all of them in flight at once), so a block
+// of 16 x 128 takes one warp and no barrier, one of 128 x 128 eight warps.
 constexpr float kInv127 = 1.f / 127.f;
+constexpr int kRun = 8;  // adjacent values that a lane handles together
 
-__device__ __forceinline__ int quant_code(float x, float inv) {
+__device__ __forceinline__ uint32_t quant_code(float x, float inv) {
   const float c = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
-  return isnan(x) ? 0 : static_cast<int>(c);
+  return isnan(x) ? 0u : static_cast<uint32_t>(static_cast<int>(c)) & 255u;
 }
+
+// Eight adjacent values (vec: at a 16-byte boundary).
+template <typename XT>
+struct Run;
+template <>
+struct Run<__nv_bfloat16> {
+  uint4 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p, bool vec) {
+    if (vec) {
+      v = __ldg(reinterpret_cast<const uint4 *>(p));
+    } else {
+      const unsigned short *u = reinterpret_cast<const unsigned short *>(p);
+      v = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+    }
+  }
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ float get(int j) const {
+    const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+    return __uint_as_float((j & 1) ? w & 0xffff0000u : w << 16);
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&f)[kRun], bool vec) {
+    if (vec) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&t);
+      }
+      *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      for (int j = 0; j < kRun; ++j) p[j] = __float2bfloat16_rn(f[j]);
+    }
+  }
+};
+template <>
+struct Run<float> {
+  float v[kRun];
+  __device__ __forceinline__ void load(const float *p, bool vec) {
+    if (vec) {
+      const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      for (int j = 0; j < kRun; ++j) v[j] = p[j];
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) v[j] = 0.f;
+  }
+  __device__ __forceinline__ float get(int j) const { return v[j]; }
+  static __device__ __forceinline__ void store(float *p, const float (&f)[kRun], bool vec) {
+    if (vec) {
+      *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
+      *(reinterpret_cast<float4 *>(p) + 1) = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      for (int j = 0; j < kRun; ++j) p[j] = f[j];
+    }
+  }
+};
 
 struct AppendArgs {
   Kv8Geom g;
   Kv8Layer c;
   Kv8Batch b;
-  const void *x[2];           // K and V rows
+  const void *x[2];                         // K and V rows
   long long row_stride[2], head_stride[2];  // elements
+  int vec[2];                               // rows and heads start at 16-byte boundaries
 };
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 256;
 
-template <typename XT>
+// RUNS runs a lane, WARPS warps a unit: RUNS x WARPS x 256 values = block_tokens x head_dim.
+template <typename XT, int RUNS, int WARPS>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendArgs a) {
   extern __shared__ int append_smem[];
   int *pre = append_smem;  // [B + 1] blocks touched before a request
@@ -164,76 +232,161 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
     const Kv8Req r = kv8_req(a.b, g.P, b);
     return (r.q > 0 && r.len >= r.q) ? (r.len - 1) / g.t - (r.len - r.q) / g.t + 1 : 0;
   });
+  constexpr int kGroups = kAppendThreads / 32 / WARPS;  // units a block works on at a time
+  const int warp = threadIdx.x >> 5, group = warp / WARPS, lane = threadIdx.x % (32 * WARPS);
+  const int per_row = g.D / kRun;
   const long long units = static_cast<long long>(pre[a.b.B]) * g.Hkv * 2;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int kv = static_cast<int>(u & 1), h = static_cast<int>((u >> 1) % g.Hkv);
-    const int blk = static_cast<int>((u >> 1) / g.Hkv);
-    const int b = request_of(pre, a.b.B, blk);
+  for (long long u = static_cast<long long>(blockIdx.x) * kGroups + group; u < units; u += static_cast<long long>(gridDim.x) * kGroups) {
+    const int kv = static_cast<int>(u & 1);
+    const uint32_t blk = static_cast<uint32_t>((u >> 1) / g.Hkv), h = static_cast<uint32_t>((u >> 1) - static_cast<long long>(blk) * g.Hkv);
+    const int b = request_of(pre, a.b.B, static_cast<int>(blk));
     const Kv8Req r = kv8_req(a.b, g.P, b);
     const int start = r.len - r.q;
-    const int p0 = (start / g.t + blk - pre[b]) * g.t;  // the block's first position
-    const int lo = max(p0, start), hi = min(p0 + g.t, r.len);
+    const int p0 = (start / g.t + static_cast<int>(blk) - pre[b]) * g.t;  // the block's first position
+    const int n_old = max(0, start - p0), n = min(g.t, r.len - p0);       // older rows, rows in all
     const int page = a.b.table[static_cast<long long>(b) * a.b.cols + p0 / g.P];
     if (page < 0 || page >= a.c.n_pages) continue;
-    const long long row0 = (static_cast<long long>(page) * g.Hkv + h) * g.P + p0 % g.P;
-    int8_t *code = (kv ? a.c.v : a.c.k) + row0 * g.D;
-    float *sc = (kv ? a.c.vs : a.c.ks) + (static_cast<long long>(page) * g.Hkv + h) * (g.P / g.t) + p0 % g.P / g.t;
-    const XT *x = static_cast<const XT *>(a.x[kv]) + (r.q0 + lo - start) * a.row_stride[kv] + h * a.head_stride[kv];
-    const int n = (hi - lo) * g.D, n_old = (lo - p0) * g.D;
-    float m = 0.f;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const float v = fabsf(to_f32(x[i / g.D * a.row_stride[kv] + i % g.D]));
-      if (v < INFINITY) m = fmaxf(m, v);
+    const long long ph = static_cast<long long>(page) * g.Hkv + h;
+    int8_t *code = (kv ? a.c.v : a.c.k) + (ph * g.P + p0 % g.P) * g.D;
+    float *sc = (kv ? a.c.vs : a.c.ks) + ph * (g.P / g.t) + p0 % g.P / g.t;
+    const XT *x = static_cast<const XT *>(a.x[kv]) + (r.q0 + p0 - start) * a.row_stride[kv] + h * a.head_stride[kv];
+    Run<XT> v[RUNS];
+    int row[RUNS];
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int e = lane + 32 * WARPS * i;
+      row[i] = e / per_row;
+      if (row[i] >= n_old && row[i] < n) v[i].load(x + row[i] * a.row_stride[kv] + (e - row[i] * per_row) * kRun, a.vec[kv]);
+      else v[i].zero();
     }
-    m = warp_max(m);
-    if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = m;
-    __syncthreads();
-    for (int w = 0; w < kAppendThreads / 32; ++w) m = fmaxf(m, redf[w]);
     const float old = n_old ? *sc : 0.f;
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const float f = fabsf(v[i].get(j));
+        m = fmaxf(m, f < INFINITY ? f : 0.f);
+      }
+    m = warp_max(m);
+    if constexpr (WARPS > 1) {  // the group's own barrier: groups may have different numbers of units left
+      if ((threadIdx.x & 31) == 0) redf[warp] = m;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WARPS) : "memory");
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, redf[group * WARPS + w]);
+    }
     float s = fmaxf(old, __fmul_rn(m, kInv127));
     if (s < 1.17549435e-38f) s = 0.f;
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
     const float factor = s > old ? __fdiv_rn(old, s) : 1.f;
-    __syncthreads();  // every thread has read the scale and the partial maxima
-    if (threadIdx.x == 0) *sc = s;
-    if (factor != 1.f)
-      for (int i = threadIdx.x; i < n_old; i += blockDim.x)
-        code[i] = static_cast<int8_t>(rintf(__fmul_rn(static_cast<float>(code[i]), factor)));
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const float v = to_f32(x[i / g.D * a.row_stride[kv] + i % g.D]);
-      code[n_old + i] = s > 0.f ? static_cast<int8_t>(quant_code(v, inv)) : 0;
+    if constexpr (WARPS > 1)  // every warp of the group has read the scale and the maxima
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WARPS) : "memory");
+    else
+      __syncwarp();
+    if (lane == 0) *sc = s;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      uint2 *to = reinterpret_cast<uint2 *>(code + (lane + 32 * WARPS * i) * kRun);
+      if (row[i] < n_old) {
+        if (factor == 1.f) continue;
+        const uint2 w = *to;
+        uint32_t o[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const int c = static_cast<int8_t>(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u);
+          const int d = static_cast<int>(rintf(__fmul_rn(static_cast<float>(c), factor)));
+          o[j >> 2] |= (static_cast<uint32_t>(d) & 255u) << (8 * (j & 3));
+        }
+        *to = make_uint2(o[0], o[1]);
+      } else if (row[i] < n) {
+        uint32_t o[2] = {0, 0};
+        if (s > 0.f) {
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) o[j >> 2] |= quant_code(v[i].get(j), inv) << (8 * (j & 3));
+        }
+        *to = make_uint2(o[0], o[1]);
+      }
     }
   }
 }
 
-// Cache read: the values code * scale of given rows, [n][Hkv][D].
+template <typename XT, int RUNS, int WARPS>
+void append_launch(const specdec_kv8 *h, const AppendArgs &a, cudaStream_t st) {
+  const long long units = (static_cast<long long>(a.b.T) / h->g.t + 2ll * a.b.B) * h->g.Hkv * 2;
+  const int groups = kAppendThreads / 32 / WARPS;
+  const int grid = static_cast<int>(std::min((units + groups - 1) / groups, 8ll * h->num_sms));
+  op_launch("specdec_kv8_append", kv8_append_kernel<XT, RUNS, WARPS>, dim3(grid), kAppendThreads, (a.b.B + 1) * sizeof(int), st, 1, a);
+}
+template <typename XT>
+void append_any(const specdec_kv8 *h, const AppendArgs &a, cudaStream_t st) {
+  switch (h->g.t * h->g.D / 256) {
+    case 1: return append_launch<XT, 1, 1>(h, a, st);
+    case 2: return append_launch<XT, 2, 1>(h, a, st);
+    case 4: return append_launch<XT, 4, 1>(h, a, st);
+    case 8: return append_launch<XT, 8, 1>(h, a, st);
+    case 16: return append_launch<XT, 8, 2>(h, a, st);
+    case 32: return append_launch<XT, 8, 4>(h, a, st);
+    default: return append_launch<XT, 8, 8>(h, a, st);
+  }
+}
+
+// Cache read: the values code * scale of given rows, [n][Hkv][D].  A thread
+// takes runs of eight values of K and of V, four of each in flight.
 struct GatherArgs {
   Kv8Geom g;
   Kv8Layer c;
   const int64_t *rows;
   int n;
   void *out[2];
+  int vec;
 };
 
+constexpr int kGatherThreads = 256;
+constexpr int kGatherAhead = 4;
+
 template <typename XT>
-__global__ void __launch_bounds__(256) kv8_gather_kernel(const GatherArgs a) {
+__global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const GatherArgs a) {
   const Kv8Geom &g = a.g;
-  const long long total = static_cast<long long>(a.n) * g.Hkv * g.D;
-  const long long all = static_cast<long long>(a.c.n_pages) * g.P;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const int d = static_cast<int>(i % g.D), h = static_cast<int>(i / g.D % g.Hkv);
-    const int64_t row = a.rows[i / g.D / g.Hkv];
-    for (int kv = 0; kv < 2; ++kv) {
-      if (!a.out[kv]) continue;
-      float v = 0.f;
-      if (row >= 0 && row < all) {
-        const long long ph = row / g.P * g.Hkv + h;
-        const int off = static_cast<int>(row % g.P);
-        v = static_cast<float>((kv ? a.c.v : a.c.k)[(ph * g.P + off) * g.D + d]) *
-            (kv ? a.c.vs : a.c.ks)[ph * (g.P / g.t) + off / g.t];
+  const uint32_t per_row = static_cast<uint32_t>(g.Hkv) * (g.D / kRun);  // runs of a row
+  const long long total = static_cast<long long>(a.n) * per_row;
+  const long long slots = static_cast<long long>(a.c.n_pages) * g.P;
+  const long long stride = static_cast<long long>(gridDim.x) * kGatherThreads;
+  for (long long i0 = static_cast<long long>(blockIdx.x) * kGatherThreads + threadIdx.x; i0 < total; i0 += stride * kGatherAhead) {
+    uint2 w[kGatherAhead][2];
+    float s[kGatherAhead][2];
+#pragma unroll
+    for (int k = 0; k < kGatherAhead; ++k) {
+      const long long i = i0 + k * stride;
+      const bool in = i < total;
+      const long long n = !in ? 0 : (i >> 32) ? i / per_row : static_cast<uint32_t>(i) / per_row;
+      const uint32_t e = static_cast<uint32_t>(i - n * per_row), h = e / (g.D / kRun), d = (e - h * (g.D / kRun)) * kRun;
+      const int64_t slot = in ? a.rows[n] : -1;
+      const bool ok = slot >= 0 && slot < slots;
+      const long long page = ok ? slot / g.P : 0, ph = page * g.Hkv + h;
+      const int off = ok ? static_cast<int>(slot - page * g.P) : 0;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        w[k][kv] = make_uint2(0, 0);
+        s[k][kv] = 0.f;
+        if (ok && a.out[kv]) {
+          w[k][kv] = *reinterpret_cast<const uint2 *>((kv ? a.c.v : a.c.k) + (ph * g.P + off) * g.D + d);
+          s[k][kv] = (kv ? a.c.vs : a.c.ks)[ph * (g.P / g.t) + off / g.t];
+        }
       }
-      static_cast<XT *>(a.out[kv])[i] = from_f32<XT>(v);
+    }
+#pragma unroll
+    for (int k = 0; k < kGatherAhead; ++k) {
+      const long long i = i0 + k * stride;
+      if (i >= total) break;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        if (!a.out[kv]) continue;
+        float f[kRun];
+#pragma unroll
+        for (int j = 0; j < kRun; ++j)
+          f[j] = static_cast<float>(static_cast<int8_t>(((j < 4 ? w[k][kv].x : w[k][kv].y) >> (8 * (j & 3))) & 255u)) * s[k][kv];
+        Run<XT>::store(static_cast<XT *>(a.out[kv]) + i * kRun, f, a.vec);
+      }
     }
   }
 }
@@ -345,15 +498,12 @@ int specdec_kv8_append(specdec_kv8 *h, const specdec_kv8_layer *layer, const spe
     if (b.B == 0 || b.T == 0) return;
     op_check(k && v, "null row buffer");
     DeviceScope scope(h->device);
-    const AppendArgs a{h->g, c, b, {k, v}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride}};
-    const long long units = (static_cast<long long>(b.T) / h->g.t + 2ll * b.B) * h->g.Hkv * 2;
-    const int grid = static_cast<int>(std::min(units, 16ll * h->num_sms));
-    const size_t smem = (b.B + 1) * sizeof(int);
+    const int size = dtype == SPECDEC_F32 ? 4 : 2;
+    auto vec = [&](const void *p, int64_t row, int64_t head) { return aligned16(p) && row * size % 16 == 0 && head * size % 16 == 0; };
+    const AppendArgs a{h->g, c, b, {k, v}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride},
+                       {vec(k, k_row_stride, k_head_stride), vec(v, v_row_stride, v_head_stride)}};
     const auto st = static_cast<cudaStream_t>(stream);
-    if (dtype == SPECDEC_F32)
-      op_launch("specdec_kv8_append", kv8_append_kernel<float>, dim3(grid), kAppendThreads, smem, st, 1, a);
-    else
-      op_launch("specdec_kv8_append", kv8_append_kernel<__nv_bfloat16>, dim3(grid), kAppendThreads, smem, st, 1, a);
+    dtype == SPECDEC_F32 ? append_any<float>(h, a, st) : append_any<__nv_bfloat16>(h, a, st);
   });
 }
 
@@ -367,14 +517,15 @@ int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int
     if (n == 0 || (!out_k && !out_v)) return;
     op_check(rows, "null row list");
     DeviceScope scope(h->device);
-    const GatherArgs a{h->g, c, rows, n, {out_k, out_v}};
-    const long long total = static_cast<long long>(n) * h->g.Hkv * h->g.D;
-    const int grid = static_cast<int>(std::min((total + 255) / 256, 16ll * h->num_sms));
+    const GatherArgs a{h->g, c, rows, n, {out_k, out_v}, (!out_k || aligned16(out_k)) && (!out_v || aligned16(out_v))};
+    const long long total = static_cast<long long>(n) * h->g.Hkv * (h->g.D / kRun);
+    const long long per_block = static_cast<long long>(kGatherThreads) * kGatherAhead;
+    const int grid = static_cast<int>(std::max(1ll, std::min((total + per_block - 1) / per_block, 8ll * h->num_sms)));
     const auto st = static_cast<cudaStream_t>(stream);
     if (dtype == SPECDEC_F32)
-      op_launch("specdec_kv8_gather", kv8_gather_kernel<float>, dim3(grid), 256, 0, st, 1, a);
+      op_launch("specdec_kv8_gather", kv8_gather_kernel<float>, dim3(grid), kGatherThreads, 0, st, 1, a);
     else
-      op_launch("specdec_kv8_gather", kv8_gather_kernel<__nv_bfloat16>, dim3(grid), 256, 0, st, 1, a);
+      op_launch("specdec_kv8_gather", kv8_gather_kernel<__nv_bfloat16>, dim3(grid), kGatherThreads, 0, st, 1, a);
   });
 }
 
