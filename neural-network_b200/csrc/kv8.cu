@@ -144,9 +144,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
 constexpr float kInv127 = 1.f / 127.f;
 constexpr int kRun = 8;  // adjacent values that a lane handles together
 
-__device__ __forceinline__ uint32_t quant_code(float x, float inv) {
-  const float c = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
-  return isnan(x) ? 0u : static_cast<uint32_t>(static_cast<int>(c)) & 255u;
+// rint(x) of |x| < 2^22 in the low bits: adding 1.5 x 2^23 rounds to whole numbers, to even on a tie, as rint does.
+__device__ __forceinline__ uint32_t rint_bits(float x) { return __float_as_uint(__fadd_rn(x, 12582912.f)); }
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// The code of any value: a NaN is 0, what is beyond 127 (infinities) stays there.
+__device__ __forceinline__ uint32_t any_code(float x, float inv) {
+  return isnan(x) ? 0u : rint_bits(fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f));
 }
 
 // Eight adjacent values (vec: at a 16-byte boundary).
@@ -164,6 +169,16 @@ struct Run<__nv_bfloat16> {
     }
   }
   __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  // bits of the largest |x|, those of an infinity or a NaN where there is one
+  __device__ __forceinline__ uint32_t top() const {
+    auto mag = [](uint32_t w) {
+      w &= 0x7fff7fffu;
+      return *reinterpret_cast<const __nv_bfloat162 *>(&w);
+    };
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(mag(v.x), mag(v.y)), __hmax2_nan(mag(v.z), mag(v.w)));
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(&m);
+    return max(w << 16, w & 0xffff0000u);
+  }
   __device__ __forceinline__ float get(int j) const {
     const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
     return __uint_as_float((j & 1) ? w & 0xffff0000u : w << 16);
@@ -198,6 +213,12 @@ struct Run<float> {
 #pragma unroll
     for (int j = 0; j < kRun; ++j) v[j] = 0.f;
   }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    return m;
+  }
   __device__ __forceinline__ float get(int j) const { return v[j]; }
   static __device__ __forceinline__ void store(float *p, const float (&f)[kRun], bool vec) {
     if (vec) {
@@ -226,7 +247,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   extern __shared__ int append_smem[];
   int *pre = append_smem;  // [B + 1] blocks touched before a request
   __shared__ int red[kAppendThreads / 32];
-  __shared__ float redf[kAppendThreads / 32];
+  __shared__ uint32_t tops[kAppendThreads / 32];
   const Kv8Geom &g = a.g;
   request_prefix(a.b.B, pre, red, [&](int b) {
     const Kv8Req r = kv8_req(a.b, g.P, b);
@@ -260,20 +281,36 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
       else v[i].zero();
     }
     const float old = n_old ? *sc : 0.f;
-    float m = 0.f;
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < RUNS; ++i)
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        const float f = fabsf(v[i].get(j));
-        m = fmaxf(m, f < INFINITY ? f : 0.f);
-      }
-    m = warp_max(m);
+    for (int i = 0; i < RUNS; ++i) top = max(top, v[i].top());
+    top = __reduce_max_sync(0xffffffffu, top);
     if constexpr (WARPS > 1) {  // the group's own barrier: groups may have different numbers of units left
-      if ((threadIdx.x & 31) == 0) redf[warp] = m;
+      if ((threadIdx.x & 31) == 0) tops[warp] = top;
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WARPS) : "memory");
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, redf[group * WARPS + w]);
+      for (int w = 0; w < WARPS; ++w) top = max(top, tops[group * WARPS + w]);
+    }
+    float m = __uint_as_float(top);
+    const bool finite = top < 0x7f800000u;
+    if (!finite) {  // the largest finite value
+      uint32_t t = 0;
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const uint32_t f = __float_as_uint(v[i].get(j)) & 0x7fffffffu;
+          t = max(t, f < 0x7f800000u ? f : 0u);
+        }
+      t = __reduce_max_sync(0xffffffffu, t);
+      if constexpr (WARPS > 1) {
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WARPS) : "memory");
+        if ((threadIdx.x & 31) == 0) tops[warp] = t;
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WARPS) : "memory");
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) t = max(t, tops[group * WARPS + w]);
+      }
+      m = __uint_as_float(t);
     }
     float s = fmaxf(old, __fmul_rn(m, kInv127));
     if (s < 1.17549435e-38f) s = 0.f;
@@ -300,9 +337,13 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
         *to = make_uint2(o[0], o[1]);
       } else if (row[i] < n) {
         uint32_t o[2] = {0, 0};
-        if (s > 0.f) {
+        if (s > 0.f) {  // |x / scale'| <= 127 (1 + 2^-22) where x is finite: rint needs no bounds
+          uint32_t c[kRun];
 #pragma unroll
-          for (int j = 0; j < kRun; ++j) o[j >> 2] |= quant_code(v[i].get(j), inv) << (8 * (j & 3));
+          for (int j = 0; j < kRun; ++j)
+            c[j] = finite ? rint_bits(__fmul_rn(v[i].get(j), inv)) : any_code(v[i].get(j), inv);
+          o[0] = low_bytes(c[0], c[1], c[2], c[3]);
+          o[1] = low_bytes(c[4], c[5], c[6], c[7]);
         }
         *to = make_uint2(o[0], o[1]);
       }
@@ -330,62 +371,74 @@ void append_any(const specdec_kv8 *h, const AppendArgs &a, cudaStream_t st) {
   }
 }
 
-// Cache read: the values code * scale of given rows, [n][Hkv][D].  A thread
-// takes runs of eight values of K and of V, four of each in flight.
+// Cache read: the values code * scale of given rows, [n][Hkv][D].  `span` lanes
+// take the runs of 16 codes of a row (or of one of `split` parts of it, where
+// the rows alone are few) in turn, K and V of two runs in flight.  A code byte
+// c + 128 in the low bits of 2^23 is 2^23 + 128 + c as a float: one
+// subtraction leaves c.
 struct GatherArgs {
   Kv8Geom g;
   Kv8Layer c;
   const int64_t *rows;
   int n;
   void *out[2];
-  int vec;
+  int vec, span, split;
 };
 
 constexpr int kGatherThreads = 256;
-constexpr int kGatherAhead = 4;
+constexpr int kGatherAhead = 2;
 
 template <typename XT>
 __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const GatherArgs a) {
   const Kv8Geom &g = a.g;
-  const uint32_t per_row = static_cast<uint32_t>(g.Hkv) * (g.D / kRun);  // runs of a row
-  const long long total = static_cast<long long>(a.n) * per_row;
+  const int per_head = g.D / 16, per_row = g.Hkv * per_head;
   const long long slots = static_cast<long long>(a.c.n_pages) * g.P;
-  const long long stride = static_cast<long long>(gridDim.x) * kGatherThreads;
-  for (long long i0 = static_cast<long long>(blockIdx.x) * kGatherThreads + threadIdx.x; i0 < total; i0 += stride * kGatherAhead) {
-    uint2 w[kGatherAhead][2];
-    float s[kGatherAhead][2];
+  const long long stride = static_cast<long long>(gridDim.x) * kGatherThreads / a.span;
+  for (long long part = (static_cast<long long>(blockIdx.x) * kGatherThreads + threadIdx.x) / a.span;
+       part < static_cast<long long>(a.n) * a.split; part += stride) {
+    const long long n = part / a.split;
+    const int64_t slot = a.rows[n];
+    const bool ok = slot >= 0 && slot < slots;
+    const long long page = ok ? slot / g.P : 0;
+    const int off = ok ? static_cast<int>(slot - page * g.P) : 0;
+    const int step = a.span * a.split;
+    for (int e0 = static_cast<int>(part - n * a.split) * a.span + threadIdx.x % a.span; e0 < per_row; e0 += step * kGatherAhead) {
+      uint4 w[kGatherAhead][2];
+      float s[kGatherAhead][2];
 #pragma unroll
-    for (int k = 0; k < kGatherAhead; ++k) {
-      const long long i = i0 + k * stride;
-      const bool in = i < total;
-      const long long n = !in ? 0 : (i >> 32) ? i / per_row : static_cast<uint32_t>(i) / per_row;
-      const uint32_t e = static_cast<uint32_t>(i - n * per_row), h = e / (g.D / kRun), d = (e - h * (g.D / kRun)) * kRun;
-      const int64_t slot = in ? a.rows[n] : -1;
-      const bool ok = slot >= 0 && slot < slots;
-      const long long page = ok ? slot / g.P : 0, ph = page * g.Hkv + h;
-      const int off = ok ? static_cast<int>(slot - page * g.P) : 0;
+      for (int k = 0; k < kGatherAhead; ++k) {
+        const int e = e0 + k * step, h = e / per_head, d = (e - h * per_head) * 16;
+        const long long ph = page * g.Hkv + h;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        w[k][kv] = make_uint2(0, 0);
-        s[k][kv] = 0.f;
-        if (ok && a.out[kv]) {
-          w[k][kv] = *reinterpret_cast<const uint2 *>((kv ? a.c.v : a.c.k) + (ph * g.P + off) * g.D + d);
-          s[k][kv] = (kv ? a.c.vs : a.c.ks)[ph * (g.P / g.t) + off / g.t];
+        for (int kv = 0; kv < 2; ++kv) {
+          w[k][kv] = make_uint4(0, 0, 0, 0);
+          s[k][kv] = 0.f;
+          if (ok && e < per_row && a.out[kv]) {
+            w[k][kv] = *reinterpret_cast<const uint4 *>((kv ? a.c.v : a.c.k) + (ph * g.P + off) * g.D + d);
+            s[k][kv] = (kv ? a.c.vs : a.c.ks)[ph * (g.P / g.t) + off / g.t];
+          }
         }
       }
-    }
 #pragma unroll
-    for (int k = 0; k < kGatherAhead; ++k) {
-      const long long i = i0 + k * stride;
-      if (i >= total) break;
+      for (int k = 0; k < kGatherAhead; ++k) {
+        const int e = e0 + k * step;
+        if (e >= per_row) break;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        if (!a.out[kv]) continue;
-        float f[kRun];
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!a.out[kv]) continue;
+          const uint32_t q[4] = {w[k][kv].x, w[k][kv].y, w[k][kv].z, w[k][kv].w};
+          XT *to = static_cast<XT *>(a.out[kv]) + (n * per_row + e) * 16;
 #pragma unroll
-        for (int j = 0; j < kRun; ++j)
-          f[j] = static_cast<float>(static_cast<int8_t>(((j < 4 ? w[k][kv].x : w[k][kv].y) >> (8 * (j & 3))) & 255u)) * s[k][kv];
-        Run<XT>::store(static_cast<XT *>(a.out[kv]) + i * kRun, f, a.vec);
+          for (int half = 0; half < 2; ++half) {
+            float f[kRun];
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) {
+              const uint32_t x = q[2 * half + (j >> 2)] ^ 0x80808080u;
+              f[j] = __fmul_rn(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f, s[k][kv]);
+            }
+            Run<XT>::store(to + half * kRun, f, a.vec);
+          }
+        }
       }
     }
   }
@@ -517,10 +570,14 @@ int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int
     if (n == 0 || (!out_k && !out_v)) return;
     op_check(rows, "null row list");
     DeviceScope scope(h->device);
-    const GatherArgs a{h->g, c, rows, n, {out_k, out_v}, (!out_k || aligned16(out_k)) && (!out_v || aligned16(out_v))};
-    const long long total = static_cast<long long>(n) * h->g.Hkv * (h->g.D / kRun);
-    const long long per_block = static_cast<long long>(kGatherThreads) * kGatherAhead;
-    const int grid = static_cast<int>(std::max(1ll, std::min((total + per_block - 1) / per_block, 8ll * h->num_sms)));
+    // lanes of a row: up to a warp; parts of a row: as many as give every multiprocessor 32 warps
+    const int per_row = h->g.Hkv * (h->g.D / 16);
+    int span = 1, split = 1;
+    while (span < 32 && span < per_row) span *= 2;
+    while (static_cast<long long>(n) * split * span < 32ll * 32 * h->num_sms && split * span * 2 <= per_row) split *= 2;
+    const GatherArgs a{h->g, c, rows, n, {out_k, out_v}, (!out_k || aligned16(out_k)) && (!out_v || aligned16(out_v)), span, split};
+    const long long lanes = static_cast<long long>(n) * split * span;
+    const int grid = static_cast<int>(std::min((lanes + kGatherThreads - 1) / kGatherThreads, 16ll * h->num_sms));
     const auto st = static_cast<cudaStream_t>(stream);
     if (dtype == SPECDEC_F32)
       op_launch("specdec_kv8_gather", kv8_gather_kernel<float>, dim3(grid), kGatherThreads, 0, st, 1, a);
