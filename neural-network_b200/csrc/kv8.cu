@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
 }
 
 // ---------------------------------------------------------------------------
-// Cache write.  One unit = the new rows of one scale block, one kv head, K or
+// Cache write.  One unit = the new rows of one scale block and kv head, K then
 // V: a = max |x| over the finite new values, scale' = max(scale if the block
 // has older rows, a x (1 / 127)); older rows are brought to scale', new rows
 // become rint(x x (1 / scale')).  A scale below the smallest normal number is
@@ -255,29 +255,33 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   });
   constexpr int kGroups = kAppendThreads / 32 / WARPS;  // units a block works on at a time
   const int warp = threadIdx.x >> 5, group = warp / WARPS, lane = threadIdx.x % (32 * WARPS);
-  const int per_row = g.D / kRun;
-  const long long units = static_cast<long long>(pre[a.b.B]) * g.Hkv * 2;
+  const int per_row_shift = 31 - __clz(g.D / kRun), t_shift = 31 - __clz(g.t), p_shift = 31 - __clz(g.P);
+  const long long units = static_cast<long long>(pre[a.b.B]) * g.Hkv;
   for (long long u = static_cast<long long>(blockIdx.x) * kGroups + group; u < units; u += static_cast<long long>(gridDim.x) * kGroups) {
-    const int kv = static_cast<int>(u & 1);
-    const uint32_t blk = static_cast<uint32_t>((u >> 1) / g.Hkv), h = static_cast<uint32_t>((u >> 1) - static_cast<long long>(blk) * g.Hkv);
+    const uint32_t blk = static_cast<uint32_t>((u >> 32) ? u / g.Hkv : static_cast<uint32_t>(u) / static_cast<uint32_t>(g.Hkv));
+    const uint32_t h = static_cast<uint32_t>(u - static_cast<long long>(blk) * g.Hkv);
     const int b = request_of(pre, a.b.B, static_cast<int>(blk));
     const Kv8Req r = kv8_req(a.b, g.P, b);
     const int start = r.len - r.q;
-    const int p0 = (start / g.t + static_cast<int>(blk) - pre[b]) * g.t;  // the block's first position
-    const int n_old = max(0, start - p0), n = min(g.t, r.len - p0);       // older rows, rows in all
-    const int page = a.b.table[static_cast<long long>(b) * a.b.cols + p0 / g.P];
+    const int p0 = ((start >> t_shift) + static_cast<int>(blk) - pre[b]) << t_shift;  // the block's first position
+    const int n_old = max(0, start - p0), n = min(g.t, r.len - p0);  // older rows, rows in all
+    const int page = a.b.table[static_cast<long long>(b) * a.b.cols + (p0 >> p_shift)];
     if (page < 0 || page >= a.c.n_pages) continue;
     const long long ph = static_cast<long long>(page) * g.Hkv + h;
-    int8_t *code = (kv ? a.c.v : a.c.k) + (ph * g.P + p0 % g.P) * g.D;
-    float *sc = (kv ? a.c.vs : a.c.ks) + ph * (g.P / g.t) + p0 % g.P / g.t;
+    const int in = p0 & (g.P - 1);
+    const long long code_at = ((ph << p_shift) + in) * g.D, scale_at = (ph << (p_shift - t_shift)) + (in >> t_shift);
+#pragma unroll 1
+    for (int kv = 0; kv < 2; ++kv) {
+    int8_t *code = (kv ? a.c.v : a.c.k) + code_at;
+    float *sc = (kv ? a.c.vs : a.c.ks) + scale_at;
     const XT *x = static_cast<const XT *>(a.x[kv]) + (r.q0 + p0 - start) * a.row_stride[kv] + h * a.head_stride[kv];
     Run<XT> v[RUNS];
     int row[RUNS];
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
       const int e = lane + 32 * WARPS * i;
-      row[i] = e / per_row;
-      if (row[i] >= n_old && row[i] < n) v[i].load(x + row[i] * a.row_stride[kv] + (e - row[i] * per_row) * kRun, a.vec[kv]);
+      row[i] = e >> per_row_shift;
+      if (row[i] >= n_old && row[i] < n) v[i].load(x + row[i] * a.row_stride[kv] + (e - (row[i] << per_row_shift)) * kRun, a.vec[kv]);
       else v[i].zero();
     }
     const float old = n_old ? *sc : 0.f;
@@ -336,24 +340,24 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
         }
         *to = make_uint2(o[0], o[1]);
       } else if (row[i] < n) {
-        uint32_t o[2] = {0, 0};
-        if (s > 0.f) {  // |x / scale'| <= 127 (1 + 2^-22) where x is finite: rint needs no bounds
-          uint32_t c[kRun];
+        uint32_t c[kRun];
+        if (finite) {  // |x / scale'| <= 127 (1 + 2^-22): rint needs no bounds; 1 / scale' is 0 where scale' is
 #pragma unroll
-          for (int j = 0; j < kRun; ++j)
-            c[j] = finite ? rint_bits(__fmul_rn(v[i].get(j), inv)) : any_code(v[i].get(j), inv);
-          o[0] = low_bytes(c[0], c[1], c[2], c[3]);
-          o[1] = low_bytes(c[4], c[5], c[6], c[7]);
+          for (int j = 0; j < kRun; ++j) c[j] = rint_bits(__fmul_rn(v[i].get(j), inv));
+        } else {
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) c[j] = s > 0.f ? any_code(v[i].get(j), inv) : 0u;
         }
-        *to = make_uint2(o[0], o[1]);
+        *to = make_uint2(low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7]));
       }
+    }
     }
   }
 }
 
 template <typename XT, int RUNS, int WARPS>
 void append_launch(const specdec_kv8 *h, const AppendArgs &a, cudaStream_t st) {
-  const long long units = (static_cast<long long>(a.b.T) / h->g.t + 2ll * a.b.B) * h->g.Hkv * 2;
+  const long long units = (static_cast<long long>(a.b.T) / h->g.t + 2ll * a.b.B) * h->g.Hkv;
   const int groups = kAppendThreads / 32 / WARPS;
   const int grid = static_cast<int>(std::min((units + groups - 1) / groups, 8ll * h->num_sms));
   op_launch("specdec_kv8_append", kv8_append_kernel<XT, RUNS, WARPS>, dim3(grid), kAppendThreads, (a.b.B + 1) * sizeof(int), st, 1, a);
@@ -373,7 +377,7 @@ void append_any(const specdec_kv8 *h, const AppendArgs &a, cudaStream_t st) {
 
 // Cache read: the values code * scale of given rows, [n][Hkv][D].  `span` lanes
 // take the runs of 16 codes of a row (or of one of `split` parts of it, where
-// the rows alone are few) in turn, K and V of two runs in flight.  A code byte
+// the rows alone are few) in turn, K and V of four runs in flight.  A code byte
 // c + 128 in the low bits of 2^23 is 2^23 + 128 + c as a float: one
 // subtraction leaves c.
 struct GatherArgs {
@@ -386,7 +390,7 @@ struct GatherArgs {
 };
 
 constexpr int kGatherThreads = 256;
-constexpr int kGatherAhead = 2;
+constexpr int kGatherAhead = 4;
 
 template <typename XT>
 __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const GatherArgs a) {
