@@ -375,73 +375,81 @@ void append_any(const specdec_kv8 *h, const AppendArgs &a, cudaStream_t st) {
   }
 }
 
-// Cache read: the values code * scale of given rows, [n][Hkv][D].  `span` lanes
-// take the runs of 16 codes of a row (or of one of `split` parts of it, where
-// the rows alone are few) in turn, K and V of four runs in flight.  A code byte
-// c + 128 in the low bits of 2^23 is 2^23 + 128 + c as a float: one
-// subtraction leaves c.
+// Cache read: the values code * scale of given rows, [n][Hkv][D].  A warp takes
+// one head of a group of rows (16 at D = 128), so that rows that follow each
+// other in the cache are read in one piece; K, then V, four runs of 16 codes a
+// lane in flight each.  A code byte c + 128 in the low bits of 2^23 is
+// 2^23 + 128 + c as a float: one subtraction leaves c.
 struct GatherArgs {
   Kv8Geom g;
   Kv8Layer c;
   const int64_t *rows;
   int n;
   void *out[2];
-  int vec, span, split;
+  int vec;
 };
 
 constexpr int kGatherThreads = 256;
 constexpr int kGatherAhead = 4;
 
 template <typename XT>
-__global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const GatherArgs a) {
+__global__ void __launch_bounds__(kGatherThreads, 4) kv8_gather_kernel(const GatherArgs a) {
   const Kv8Geom &g = a.g;
-  const int per_head = g.D / 16, per_row = g.Hkv * per_head;
-  const long long slots = static_cast<long long>(a.c.n_pages) * g.P;
-  const long long stride = static_cast<long long>(gridDim.x) * kGatherThreads / a.span;
-  for (long long part = (static_cast<long long>(blockIdx.x) * kGatherThreads + threadIdx.x) / a.span;
-       part < static_cast<long long>(a.n) * a.split; part += stride) {
-    const long long n = part / a.split;
-    const int64_t slot = a.rows[n];
-    const bool ok = slot >= 0 && slot < slots;
-    const long long page = ok ? slot / g.P : 0;
-    const int off = ok ? static_cast<int>(slot - page * g.P) : 0;
-    const int step = a.span * a.split;
-    for (int e0 = static_cast<int>(part - n * a.split) * a.span + threadIdx.x % a.span; e0 < per_row; e0 += step * kGatherAhead) {
-      uint4 w[kGatherAhead][2];
-      float s[kGatherAhead][2];
+  const int lanes = g.D / 16, at_once = 32 / lanes, lane = threadIdx.x & 31;  // lanes of a row, rows a load
+  const int p_shift = 31 - __clz(g.P), t_shift = 31 - __clz(g.t);
+  const int d = lane % lanes * 16, mine = lane / lanes;
+  const long long slots = static_cast<long long>(a.c.n_pages) << p_shift;
+  const long long tasks = (static_cast<long long>(a.n) + at_once * kGatherAhead - 1) / (at_once * kGatherAhead) * g.Hkv;
+  for (long long task = (static_cast<long long>(blockIdx.x) * kGatherThreads + threadIdx.x) >> 5; task < tasks;
+       task += static_cast<long long>(gridDim.x) * (kGatherThreads / 32)) {
+    const long long group = (task >> 32) ? task / g.Hkv : static_cast<uint32_t>(task) / static_cast<uint32_t>(g.Hkv);
+    const int h = static_cast<int>(task - group * g.Hkv);
+    const long long n0 = group * (at_once * kGatherAhead) + mine;
+    long long at[kGatherAhead], block[kGatherAhead];  // code and scale places; -1: no such slot
+#pragma unroll
+    for (int k = 0; k < kGatherAhead; ++k) {
+      const long long n = n0 + k * at_once;
+      const int64_t slot = n < a.n ? a.rows[n] : -1;
+      at[k] = -1;
+      block[k] = 0;
+      if (slot >= 0 && slot < slots) {
+        const long long ph = (slot >> p_shift) * g.Hkv + h;
+        const int off = static_cast<int>(slot & (g.P - 1));
+        at[k] = ((ph << p_shift) + off) * g.D + d;
+        block[k] = (ph << (p_shift - t_shift)) + (off >> t_shift);
+      }
+    }
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      if (!a.out[kv]) continue;
+      const int8_t *codes = kv ? a.c.v : a.c.k;
+      const float *scales = kv ? a.c.vs : a.c.ks;
+      uint4 w[kGatherAhead];
+      float s[kGatherAhead];
 #pragma unroll
       for (int k = 0; k < kGatherAhead; ++k) {
-        const int e = e0 + k * step, h = e / per_head, d = (e - h * per_head) * 16;
-        const long long ph = page * g.Hkv + h;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          w[k][kv] = make_uint4(0, 0, 0, 0);
-          s[k][kv] = 0.f;
-          if (ok && e < per_row && a.out[kv]) {
-            w[k][kv] = *reinterpret_cast<const uint4 *>((kv ? a.c.v : a.c.k) + (ph * g.P + off) * g.D + d);
-            s[k][kv] = (kv ? a.c.vs : a.c.ks)[ph * (g.P / g.t) + off / g.t];
-          }
+        w[k] = make_uint4(0, 0, 0, 0);
+        s[k] = 0.f;
+        if (at[k] >= 0) {
+          w[k] = __ldg(reinterpret_cast<const uint4 *>(codes + at[k]));
+          s[k] = __ldg(scales + block[k]);
         }
       }
 #pragma unroll
       for (int k = 0; k < kGatherAhead; ++k) {
-        const int e = e0 + k * step;
-        if (e >= per_row) break;
+        const long long n = n0 + k * at_once;
+        if (n >= a.n) break;
+        const uint32_t q[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+        XT *to = static_cast<XT *>(a.out[kv]) + (n * g.Hkv + h) * g.D + d;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!a.out[kv]) continue;
-          const uint32_t q[4] = {w[k][kv].x, w[k][kv].y, w[k][kv].z, w[k][kv].w};
-          XT *to = static_cast<XT *>(a.out[kv]) + (n * per_row + e) * 16;
+        for (int half = 0; half < 2; ++half) {
+          float f[kRun];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float f[kRun];
-#pragma unroll
-            for (int j = 0; j < kRun; ++j) {
-              const uint32_t x = q[2 * half + (j >> 2)] ^ 0x80808080u;
-              f[j] = __fmul_rn(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f, s[k][kv]);
-            }
-            Run<XT>::store(to + half * kRun, f, a.vec);
+          for (int j = 0; j < kRun; ++j) {
+            const uint32_t x = q[2 * half + (j >> 2)] ^ 0x80808080u;
+            f[j] = __fmul_rn(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f, s[k]);
           }
+          Run<XT>::store(to + half * kRun, f, a.vec);
         }
       }
     }
@@ -574,14 +582,10 @@ int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int
     if (n == 0 || (!out_k && !out_v)) return;
     op_check(rows, "null row list");
     DeviceScope scope(h->device);
-    // lanes of a row: up to a warp; parts of a row: as many as give every multiprocessor 32 warps
-    const int per_row = h->g.Hkv * (h->g.D / 16);
-    int span = 1, split = 1;
-    while (span < 32 && span < per_row) span *= 2;
-    while (static_cast<long long>(n) * split * span < 32ll * 32 * h->num_sms && split * span * 2 <= per_row) split *= 2;
-    const GatherArgs a{h->g, c, rows, n, {out_k, out_v}, (!out_k || aligned16(out_k)) && (!out_v || aligned16(out_v)), span, split};
-    const long long lanes = static_cast<long long>(n) * split * span;
-    const int grid = static_cast<int>(std::min((lanes + kGatherThreads - 1) / kGatherThreads, 16ll * h->num_sms));
+    const GatherArgs a{h->g, c, rows, n, {out_k, out_v}, (!out_k || aligned16(out_k)) && (!out_v || aligned16(out_v))};
+    const long long rows_a_warp = 32 / (h->g.D / 16) * kGatherAhead;
+    const long long warps = (n + rows_a_warp - 1) / rows_a_warp * h->g.Hkv;
+    const int grid = static_cast<int>(std::min((warps + 7) / 8, 16ll * h->num_sms));
     const auto st = static_cast<cudaStream_t>(stream);
     if (dtype == SPECDEC_F32)
       op_launch("specdec_kv8_gather", kv8_gather_kernel<float>, dim3(grid), kGatherThreads, 0, st, 1, a);
