@@ -376,9 +376,9 @@ void append_any(const specdec_kv8 *h, const AppendArgs &a, cudaStream_t st) {
 }
 
 // Cache read: the values code * scale of given rows, [n][Hkv][D].  A warp takes
-// one head of a group of rows (16 at D = 128), so that rows that follow each
-// other in the cache are read in one piece; K, then V, four runs of 16 codes a
-// lane in flight each.  A code byte c + 128 in the low bits of 2^23 is
+// one head of a group of rows (8 at D = 128), so that rows that follow each
+// other in the cache are read in one piece; K and V, four runs of 8 codes a lane in
+// flight each (16 codes would leave every store with half-written sectors).  A code byte c + 128 in the low bits of 2^23 is
 // 2^23 + 128 + c as a float: one subtraction leaves c.
 struct GatherArgs {
   Kv8Geom g;
@@ -395,9 +395,9 @@ constexpr int kGatherAhead = 4;
 template <typename XT>
 __global__ void __launch_bounds__(kGatherThreads, 4) kv8_gather_kernel(const GatherArgs a) {
   const Kv8Geom &g = a.g;
-  const int lanes = g.D / 16, at_once = 32 / lanes, lane = threadIdx.x & 31;  // lanes of a row, rows a load
-  const int p_shift = 31 - __clz(g.P), t_shift = 31 - __clz(g.t);
-  const int d = lane % lanes * 16, mine = lane / lanes;
+  const int lanes = g.D / kRun, at_once = 32 / lanes, lane = threadIdx.x & 31;  // lanes of a row, rows a load
+  const int p_shift = 31 - __clz(g.P), scale_shift = 31 - __clz(g.t) + 31 - __clz(g.D);
+  const int d = lane % lanes * kRun, mine = lane / lanes;
   const long long slots = static_cast<long long>(a.c.n_pages) << p_shift;
   const long long tasks = (static_cast<long long>(a.n) + at_once * kGatherAhead - 1) / (at_once * kGatherAhead) * g.Hkv;
   for (long long task = (static_cast<long long>(blockIdx.x) * kGatherThreads + threadIdx.x) >> 5; task < tasks;
@@ -405,52 +405,45 @@ __global__ void __launch_bounds__(kGatherThreads, 4) kv8_gather_kernel(const Gat
     const long long group = (task >> 32) ? task / g.Hkv : static_cast<uint32_t>(task) / static_cast<uint32_t>(g.Hkv);
     const int h = static_cast<int>(task - group * g.Hkv);
     const long long n0 = group * (at_once * kGatherAhead) + mine;
-    long long at[kGatherAhead], block[kGatherAhead];  // code and scale places; -1: no such slot
+    long long at[kGatherAhead];  // code places; -1: no such slot
 #pragma unroll
     for (int k = 0; k < kGatherAhead; ++k) {
       const long long n = n0 + k * at_once;
       const int64_t slot = n < a.n ? a.rows[n] : -1;
       at[k] = -1;
-      block[k] = 0;
       if (slot >= 0 && slot < slots) {
         const long long ph = (slot >> p_shift) * g.Hkv + h;
         const int off = static_cast<int>(slot & (g.P - 1));
         at[k] = ((ph << p_shift) + off) * g.D + d;
-        block[k] = (ph << (p_shift - t_shift)) + (off >> t_shift);
       }
     }
+    uint2 w[2][kGatherAhead];
+    float s[2][kGatherAhead];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int k = 0; k < kGatherAhead; ++k) {
+        w[kv][k] = make_uint2(0, 0);
+        s[kv][k] = 0.f;
+        if (at[k] >= 0 && a.out[kv]) {
+          w[kv][k] = __ldg(reinterpret_cast<const uint2 *>((kv ? a.c.v : a.c.k) + at[k]));
+          s[kv][k] = __ldg((kv ? a.c.vs : a.c.ks) + (at[k] >> scale_shift));
+        }
+      }
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       if (!a.out[kv]) continue;
-      const int8_t *codes = kv ? a.c.v : a.c.k;
-      const float *scales = kv ? a.c.vs : a.c.ks;
-      uint4 w[kGatherAhead];
-      float s[kGatherAhead];
-#pragma unroll
-      for (int k = 0; k < kGatherAhead; ++k) {
-        w[k] = make_uint4(0, 0, 0, 0);
-        s[k] = 0.f;
-        if (at[k] >= 0) {
-          w[k] = __ldg(reinterpret_cast<const uint4 *>(codes + at[k]));
-          s[k] = __ldg(scales + block[k]);
-        }
-      }
 #pragma unroll
       for (int k = 0; k < kGatherAhead; ++k) {
         const long long n = n0 + k * at_once;
         if (n >= a.n) break;
-        const uint32_t q[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-        XT *to = static_cast<XT *>(a.out[kv]) + (n * g.Hkv + h) * g.D + d;
+        float f[kRun];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float f[kRun];
-#pragma unroll
-          for (int j = 0; j < kRun; ++j) {
-            const uint32_t x = q[2 * half + (j >> 2)] ^ 0x80808080u;
-            f[j] = __fmul_rn(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f, s[k]);
-          }
-          Run<XT>::store(to + half * kRun, f, a.vec);
+        for (int j = 0; j < kRun; ++j) {
+          const uint32_t x = (j < 4 ? w[kv][k].x : w[kv][k].y) ^ 0x80808080u;
+          f[j] = __fmul_rn(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f, s[kv][k]);
         }
+        Run<XT>::store(static_cast<XT *>(a.out[kv]) + (n * g.Hkv + h) * g.D + d, f, a.vec);
       }
     }
   }
@@ -583,7 +576,7 @@ int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int
     op_check(rows, "null row list");
     DeviceScope scope(h->device);
     const GatherArgs a{h->g, c, rows, n, {out_k, out_v}, (!out_k || aligned16(out_k)) && (!out_v || aligned16(out_v))};
-    const long long rows_a_warp = 32 / (h->g.D / 16) * kGatherAhead;
+    const long long rows_a_warp = 32 / (h->g.D / kRun) * kGatherAhead;
     const long long warps = (n + rows_a_warp - 1) / rows_a_warp * h->g.Hkv;
     const int grid = static_cast<int>(std::min((warps + 7) / 8, 16ll * h->num_sms));
     const auto st = static_cast<cudaStream_t>(stream);
