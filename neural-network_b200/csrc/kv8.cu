@@ -36,63 +36,95 @@ struct PlanArgs {
   int32_t *status;
 };
 
-constexpr int kPlanThreads = 256;
-
-struct PlanReq {
-  long long q;
-  int take, give;
-  bool bad;
-};
-__device__ __forceinline__ PlanReq plan_req(const PlanArgs &a, int b) {
-  const long long held = a.held[b], keep = a.keep[b], q = a.q_len[b];
-  const long long cap = static_cast<long long>(a.cols) * a.P;
-  PlanReq r{0, 0, 0, held < 0 || keep < 0 || keep > held || q < 0 || held > cap || keep + q > cap};
-  if (!r.bad) {
-    const int have = static_cast<int>((held + a.P - 1) / a.P), need = static_cast<int>((keep + q + a.P - 1) / a.P);
-    r.q = q;
-    r.take = max(0, need - have);
-    r.give = max(0, have - need);
-  }
-  return r;
-}
+constexpr int kPlanThreads = 512;
+constexpr int kPlanBytes = 2 * 8 + 2 * 4;  // shared memory of a request
 
 __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a) {
   extern __shared__ long long plan_smem[];
-  long long *cu = plan_smem;       // [B + 1] first row of a request
-  long long *mv = cu + a.B + 1;    // [B + 1] pages taken (low 32 bits) and given back (high) before it
-  __shared__ long long red[kPlanThreads / 32];
+  long long *cu = plan_smem;                            // [B + 1] first row of a request
+  long long *mv = cu + a.B + 1;                         // [B + 1] pages taken (low half) and given back (high) before it
+  int *keeps = reinterpret_cast<int *>(mv + a.B + 1);   // [B] positions kept
+  int *haves = keeps + a.B;                             // [B] pages held
+  __shared__ long long red[2][kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int p_shift = 31 - __clz(a.P);
+  const long long cap = static_cast<long long>(a.cols) << p_shift;
+  auto pages = [&](long long n) { return (n + a.P - 1) >> p_shift; };
+
+  // Both prefix sums at once; a thread owns a run of consecutive requests.
+  const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(a.B, static_cast<int>(threadIdx.x) * per), b1 = min(a.B, b0 + per);
+  long long rows = 0, moves = 0;
   int bad = 0;
-  request_prefix(a.B, cu, red, [&](int b) {
-    const PlanReq r = plan_req(a, b);
-    bad |= r.bad;
-    return r.q;
-  });
-  request_prefix(a.B, mv, red, [&](int b) {
-    const PlanReq r = plan_req(a, b);
-    return static_cast<long long>(r.take) | static_cast<long long>(r.give) << 32;
-  });
-  bad = __syncthreads_or(bad);
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) {
+    const long long held = a.held[b], keep = a.keep[b], q = a.q_len[b];
+    const bool ok = held >= 0 && keep >= 0 && keep <= held && q >= 0 && held <= cap && keep + q <= cap;
+    const long long more = ok ? pages(keep + q) - pages(held) : 0;
+    const long long m = more >= 0 ? more : -more << 32;
+    cu[b] = ok ? q : 0;
+    mv[b] = m;
+    keeps[b] = static_cast<int>(keep);
+    haves[b] = static_cast<int>(pages(held));
+    rows += cu[b];
+    moves += m;
+    bad |= !ok;
+  }
+  long long inc_r = rows, inc_m = moves;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long r = __shfl_up_sync(0xffffffffu, inc_r, o), m = __shfl_up_sync(0xffffffffu, inc_m, o);
+    if (lane >= o) {
+      inc_r += r;
+      inc_m += m;
+    }
+  }
+  if (lane == 31) {
+    red[0][wid] = inc_r;
+    red[1][wid] = inc_m;
+  }
   const long long head = a.ring_state[0], count = a.ring_state[1];
+  bad = __syncthreads_or(bad);
+  long long run_r = inc_r - rows, run_m = inc_m - moves;
+  for (int w = 0; w < wid; ++w) {
+    run_r += red[0][w];
+    run_m += red[1][w];
+  }
+  for (int b = b0; b < b1; ++b) {
+    const long long r = cu[b], m = mv[b];
+    cu[b] = run_r;
+    mv[b] = run_m;
+    run_r += r;
+    run_m += m;
+  }
+  if (threadIdx.x == kPlanThreads - 1) {
+    cu[a.B] = run_r;
+    mv[a.B] = run_m;
+  }
+  __syncthreads();
+
   const long long takes = mv[a.B] & 0xffffffffll, gives = mv[a.B] >> 32;
   const bool ring_ok = head >= 0 && head < a.ring_cap && count >= 0 && count <= a.ring_cap;
   const int status = ((!ring_ok || takes > count) ? 1 : 0) | (bad ? 2 : 0) | (cu[a.B] > a.T ? 4 : 0) |
                      ((ring_ok && count - takes + gives > a.ring_cap) ? 2 : 0);
   const bool fine = status == 0;
-  const long long tid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
+  // ring places wrap at most twice: head, count and the moves are each at most ring_cap
+  auto place = [&](long long i) {
+    if (i >= a.ring_cap) i -= a.ring_cap;
+    return i >= a.ring_cap ? i - a.ring_cap : i;
+  };
+  const long long tid = static_cast<long long>(blockIdx.x) * kPlanThreads + threadIdx.x;
+  const long long stride = static_cast<long long>(gridDim.x) * kPlanThreads;
   if (tid == 0) {
     *a.status = status;
-    a.ring_out[0] = fine ? static_cast<int>((head + takes) % a.ring_cap) : static_cast<int>(head);
-    a.ring_out[1] = fine ? static_cast<int>(count - takes + gives) : static_cast<int>(count);
+    a.ring_out[0] = static_cast<int>(fine ? place(head + takes) : head);
+    a.ring_out[1] = static_cast<int>(fine ? count - takes + gives : count);
   }
   for (long long b = tid; b <= a.B; b += stride) {
     a.cu_q[b] = fine ? static_cast<int>(cu[b]) : 0;
-    if (b < a.B) a.kv_len[b] = fine ? a.keep[b] + a.q_len[b] : a.held[b];
+    if (b < a.B) a.kv_len[b] = fine ? keeps[b] + static_cast<int>(cu[b + 1] - cu[b]) : a.held[b];
   }
-  auto pages = [&](int n) { return (static_cast<long long>(n) + a.P - 1) / a.P; };
   if (fine) {
-    auto low = [&](int b) { return mv[b] & 0xffffffffll; };
-    auto high = [&](int b) { return mv[b] >> 32; };
     auto find = [&](long long u, auto &&at) {  // the last request with at(b) <= u
       int lo = 0, hi = a.B - 1;
       while (lo < hi) {
@@ -102,14 +134,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
       }
       return lo;
     };
+    auto low = [&](int b) { return mv[b] & 0xffffffffll; };
+    auto high = [&](int b) { return mv[b] >> 32; };
     for (long long i = tid; i < takes; i += stride) {
       const int b = find(i, low);
-      a.table[static_cast<long long>(b) * a.cols + pages(a.held[b]) + (i - low(b))] = a.ring[(head + i) % a.ring_cap];
+      a.table[static_cast<long long>(b) * a.cols + haves[b] + (i - low(b))] = a.ring[place(head + i)];
     }
     for (long long i = tid; i < gives; i += stride) {
       const int b = find(i, high);
-      const long long need = pages(a.keep[b] + a.q_len[b]);
-      a.ring[(head + count + i) % a.ring_cap] = a.table[static_cast<long long>(b) * a.cols + need + (i - high(b))];
+      const long long need = pages(keeps[b] + (cu[b + 1] - cu[b]));
+      a.ring[place(head + count + i)] = a.table[static_cast<long long>(b) * a.cols + need + (i - high(b))];
     }
   }
   for (long long t = tid; t < a.T; t += stride) {
@@ -117,12 +151,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
     long long slot = -1;
     if (fine && t < cu[a.B]) {
       req = request_of(cu, a.B, t);
-      pos = a.keep[req] + static_cast<int>(t - cu[req]);
-      const long long col = pos / a.P, have = pages(a.held[req]);
+      pos = keeps[req] + static_cast<int>(t - cu[req]);
+      const int col = pos >> p_shift, have = haves[req];
       // a page taken in this call is read from the ring: its table entry is being written
       const long long page = col < have ? a.table[static_cast<long long>(req) * a.cols + col]
-                                        : a.ring[(head + (mv[req] & 0xffffffffll) + col - have) % a.ring_cap];
-      slot = page * a.P + pos % a.P;
+                                        : a.ring[place(head + (mv[req] & 0xffffffffll) + col - have)];
+      slot = (page << p_shift) + (pos & (a.P - 1));
     }
     a.tok_req[t] = req;
     a.tok_pos[t] = pos;
@@ -501,7 +535,7 @@ int specdec_kv8_create(const specdec_kv8_config *cfg, int device, specdec_kv8 **
     h->device = device;
     op_cuda(cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device), "device attributes");
     op_cuda(cudaFuncSetAttribute(kv8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 2 * (kKv8MaxBatch + 1) * static_cast<int>(sizeof(long long))),
+                                 (kKv8MaxBatch + 1) * kPlanBytes),
             "cudaFuncSetAttribute");
     kv8_attn_create(h.get());
     *out = h.release();
@@ -538,9 +572,10 @@ int specdec_kv8_plan(specdec_kv8 *h, const specdec_kv8_batch *batch, const int32
     DeviceScope scope(h->device);
     const PlanArgs a{held, keep, q_len, b.table, b.B, b.cols, h->g.P, ring, ring_cap, ring_state, ring_state_out,
                      b.kv_len, b.cu_q, batch->tok_req, batch->tok_pos, batch->slots, b.T, batch->status};
+    // a thread per row, in at most two blocks per multiprocessor: each repeats the scan
     const int work = std::max(b.T, b.B);
-    const int grid = std::max(1, std::min(h->num_sms, (work + 4 * kPlanThreads - 1) / (4 * kPlanThreads)));
-    op_launch("specdec_kv8_plan", kv8_plan_kernel, dim3(grid), kPlanThreads, 2 * (b.B + 1) * sizeof(long long),
+    const int grid = std::max(1, std::min(2 * h->num_sms, (work + kPlanThreads - 1) / kPlanThreads));
+    op_launch("specdec_kv8_plan", kv8_plan_kernel, dim3(grid), kPlanThreads, (b.B + 1) * kPlanBytes,
               static_cast<cudaStream_t>(stream), 1, a);
   });
 }

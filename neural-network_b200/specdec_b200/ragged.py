@@ -3,7 +3,7 @@
 ``KV8.attend`` and ``sample``.  include/specdec.h has their definitions.
 
 Buffers are CUDA tensors: any object with ``data_ptr()``, ``shape``,
-``stride()``, ``dtype``, ``device`` and ``is_contiguous()``, as torch's are.
+``stride()``, ``dtype``, ``is_cuda`` and ``is_contiguous()``, as torch's are.
 ``stream`` is a raw cudaStream_t (0: the device's default stream, torch's
 current one unless a caller changed it); tensors must be ready on it.
 Failures raise ``SpecDecError`` (a RuntimeError), wrong arguments before the
@@ -17,25 +17,29 @@ from typing import Optional
 
 import specdec_b200 as _sd
 
-_DTYPE = {"torch.float32": _sd.F32, "torch.bfloat16": _sd.BF16}
-_dtype_cache: dict = {}
+_ROWS = {"float32": _sd.F32, "bfloat16": _sd.BF16}
+_names: dict = {}  # dtype object -> its name
+
+
+def _name_of(dtype) -> str:
+    name = _names.get(dtype)
+    if name is None:
+        name = _names[dtype] = str(dtype).rpartition(".")[2]
+    return name
 
 
 def _dtype_of(t) -> int:
-    d = _dtype_cache.get(t.dtype)
+    d = _ROWS.get(_name_of(t.dtype))
     if d is None:
-        d = _DTYPE.get(str(t.dtype))
-        if d is None:
-            raise ValueError(f"rows must be float32 or bfloat16, not {t.dtype}")
-        _dtype_cache[t.dtype] = d
+        raise ValueError(f"rows must be float32 or bfloat16, not {t.dtype}")
     return d
 
 
 def _buffer(t, name: str, dtype: str, shape=None):
     """The address of a contiguous buffer of the given type (and shape)."""
-    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or t.device.type != "cuda":
+    if (_names.get(t.dtype) or _name_of(t.dtype)) != dtype or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -85,7 +89,7 @@ class KV8Batch:
 def _rows(t, heads: int, dim: int, name: str):
     """(address, row stride, head stride) of rows [n][heads][dim] with adjacent dims."""
     sh, st = t.shape, t.stride()
-    if len(sh) != 3 or sh[1] != heads or sh[2] != dim or (st[2] != 1 and dim > 1):
+    if len(sh) != 3 or sh[1] != heads or sh[2] != dim or st[2] != 1:
         raise ValueError(f"{name} must be rows of {heads} heads x {dim} adjacent values, not {tuple(sh)}")
     return t.data_ptr(), st[0], st[1]
 
@@ -149,7 +153,7 @@ class KV8:
         outs = [t for t in (out_k, out_v) if t is not None]
         if not outs:
             return
-        if any(tuple(t.shape) != shape or not t.is_contiguous() or t.dtype != outs[0].dtype for t in outs):
+        if any(t.shape != shape or not t.is_contiguous() or t.dtype != outs[0].dtype for t in outs):
             raise ValueError(f"outputs must be contiguous, of one type and shape {shape}")
         self._check(self._lib.specdec_kv8_gather(
             self.h, self._layer(layer), _buffer(rows, "rows", "int64"), n, None if out_k is None else out_k.data_ptr(),
