@@ -443,6 +443,11 @@ int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer, const spe
                        int64_t out_row_stride, int64_t out_head_stride, float *lse, int max_q, float scale, int window,
                        void *stream);
 
+/* Waits for `stream` and reports what its specdec_kv8_attend calls could not:
+ * SPECDEC_ERR_CUDA if a bounded wait inside one gave up (its output is not
+ * valid) since the last check. */
+int specdec_kv8_check(specdec_kv8 *h, void *stream);
+
 /* One token per row of logits [rows][vocab] (vocab at most 2^20) from the
  * row's uniform u in [0, 1).  Per row, each array NULL for its default:
  * temperature (<= 0: the arg max; default 1), top_k (<= 0: off), top_p (>= 1:

@@ -107,4 +107,5 @@ struct specdec_kv8 {
   std::string err;
   float *part = nullptr;  // attention: partial results of split items
   int *ticket = nullptr;  // attention: arrivals per split item, 0 between launches
+  int *err_word = nullptr;  // attention: set by a bounded wait that gave up (part of ticket's allocation)
 };

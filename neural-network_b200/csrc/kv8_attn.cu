@@ -38,24 +38,6 @@ namespace specdec {
 
 namespace {
 
-struct AttendArgs {
-  Kv8Geom g;
-  Kv8Layer c;
-  Kv8Batch b;
-  const void *q;
-  long long q_row, q_head;  // strides in elements
-  void *out;
-  long long o_row, o_head;
-  float *lse;
-  float scale;
-  int window;
-  float *part;
-  int *ticket;
-  int p_shift, t_shift;  // log2 of page and block positions
-  int g_shift;           // log2 of the query heads of a kv head, -1 where that is no power of two
-  int q_vec, o_vec;      // query / output rows start at 4-element boundaries
-};
-
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kSlice = 16;                            // positions of a slice
@@ -63,12 +45,8 @@ constexpr int kStep = 2;                              // slices a warp takes at 
 constexpr int kUnit = kSlice * kStep * kDecWarps;     // positions of a unit
 constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: registers
 constexpr int kWholeItems = 4;                        // items of at most this many units are not split
+constexpr int kChunkRows = 32;                        // rows of a kv head above which the tensor tiles are faster
 constexpr int kMergeAhead = 8;                        // partial results read at once
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNone = -1e30f;                  // the running maximum before anything was seen
-constexpr float kLazy = 8.f;                     // weights may grow to 2^8 before the maximum is moved
-
 template <int D, int NT>
 struct DecGeom {
   static constexpr int kRows = 8 * NT;
@@ -97,12 +75,6 @@ __device__ __forceinline__ void cp_wait() {
 }
 __device__ __forceinline__ uint32_t shared_addr(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -169,70 +141,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-// Bytes 0x64 u as f16 are 1024 + u; u = code + 128, so minus 1152 leaves the code, exactly.
-__device__ __forceinline__ uint32_t f16_codes(uint32_t biased) {
-  __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&biased), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
-
-// Four adjacent values of a row as loaded (vec: at a 4-element boundary), zeros unless live.
-template <typename XT>
-struct Quad;
-template <>
-struct Quad<float> {
-  float x[4];
-  __device__ __forceinline__ void load(const float *p, bool vec, bool live) {
-    if (vec) {
-      const float4 v = live ? *reinterpret_cast<const float4 *>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = live ? p[j] : 0.f;
-    }
-  }
-  __device__ __forceinline__ float get(int j) const { return x[j]; }
-};
-template <>
-struct Quad<__nv_bfloat16> {
-  uint2 x;
-  __device__ __forceinline__ void load(const __nv_bfloat16 *p, bool vec, bool live) {
-    if (vec) {
-      x = live ? *reinterpret_cast<const uint2 *>(p) : make_uint2(0, 0);
-    } else {
-      const unsigned short *u = reinterpret_cast<const unsigned short *>(p);
-      x = live ? make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16) : make_uint2(0, 0);
-    }
-  }
-  __device__ __forceinline__ float get(int j) const {
-    const uint32_t w = j < 2 ? x.x : x.y;
-    return __uint_as_float((j & 1) ? w & 0xffff0000u : w << 16);
-  }
-};
-
-__device__ __forceinline__ void store4(float *p, bool vec, float4 v) {
-  if (vec) {
-    *reinterpret_cast<float4 *>(p) = v;
-  } else {
-    p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w;
-  }
-}
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, bool vec, float4 v) {
-  if (vec) {
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-    *reinterpret_cast<uint2 *>(p) =
-        make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-  } else {
-    p[0] = from_f32<__nv_bfloat16>(v.x);
-    p[1] = from_f32<__nv_bfloat16>(v.y);
-    p[2] = from_f32<__nv_bfloat16>(v.z);
-    p[3] = from_f32<__nv_bfloat16>(v.w);
-  }
-}
 
 // Place of a 16-byte chunk of a slice row in shared memory.  K rows are read
 // eight at a time at one chunk: the chunks of rows that start in the same bank
@@ -251,31 +160,6 @@ __device__ __forceinline__ int v_place(int row, int chunk) {
   if constexpr (D == 64) return r * D + 16 * (chunk ^ (r & 2));
   return r * D + 16 * chunk;
 }
-
-// A value that is the same in the whole warp, as the compiler can see it.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
-
-// a / b where both mostly fit 32 bits.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
-}
-
-// Row r of a kv head's rows of a request: new token r / G, query head r % G.
-struct RowAt {
-  int i, h;
-};
-__device__ __forceinline__ RowAt row_at(const AttendArgs &a, int r) {
-  if (a.g_shift >= 0) return {r >> a.g_shift, r & (a.g.G - 1)};
-  const int i = r / a.g.G;
-  return {i, r - i * a.g.G};
-}
-
-// The batch in shared memory: per request its rows, its length and the units before it.
-struct DecBatch {
-  long long *pre;  // [B + 1]
-  int *q0, *q, *len;
-};
 
 // The request that a run of units belongs to.
 struct DecReq {
@@ -946,14 +830,16 @@ void kv8_attn_create(specdec_kv8 *h) {
   dec_attrs<__nv_bfloat16, 1>(kKv8MaxBatch);
   dec_attrs<__nv_bfloat16, 2>(kKv8MaxBatch);
   const size_t blocks = static_cast<size_t>(dec_ctas(1)) * h->num_sms;
-  const size_t part = blocks * 2 * (16 * h->g.D + 32) * sizeof(float);
+  const size_t part = std::max(blocks * 2 * (16 * h->g.D + 32) * sizeof(float), kv8_chunk_part_bytes(h));
+  kv8_chunk_create(h);
   op_cuda(cudaMalloc(&h->part, part), "cudaMalloc");
-  const cudaError_t e = cudaMalloc(&h->ticket, blocks * sizeof(int));
+  const cudaError_t e = cudaMalloc(&h->ticket, (blocks + 1) * sizeof(int));
   if (e != cudaSuccess) {
     kv8_attn_destroy(h);
     op_cuda(e, "cudaMalloc");
   }
-  const cudaError_t z = cudaMemset(h->ticket, 0, blocks * sizeof(int));
+  h->err_word = h->ticket + blocks;
+  const cudaError_t z = cudaMemset(h->ticket, 0, (blocks + 1) * sizeof(int));
   if (z != cudaSuccess) {
     kv8_attn_destroy(h);
     op_cuda(z, "cudaMemset");
@@ -989,13 +875,33 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
                        lse,  scale, window, h->part, h->ticket, log2i(h->g.P), log2i(h->g.t),
                        (h->g.G & (h->g.G - 1)) == 0 ? log2i(h->g.G) : -1,
                        rows_aligned(q, q_row_stride, q_head_stride, dtype),
-                       rows_aligned(out, out_row_stride, out_head_stride, dtype)};
+                       rows_aligned(out, out_row_stride, out_head_stride, dtype), h->err_word};
     const auto st = static_cast<cudaStream_t>(stream);
+    // Many rows per kv head: every cached value meets all of them, and the products bound the call, so they go to the
+    // 128-row tensor tiles; measured on 4 requests of 32 / 8 heads over 4,096 positions, FIGURES
+    if (dtype == SPECDEC_BF16 && h->g.D >= 64 && b.B <= kChunkMaxBatch && static_cast<long long>(max_q) * h->g.G > kChunkRows) {
+      kv8_chunk_launch(h, a, st);
+      return;
+    }
     // rows of one kv head: one column tile of 8 where they fit, else two
     const bool one = static_cast<long long>(max_q) * h->g.G <= 8;
     if (dtype == SPECDEC_F32)
       one ? dec_launch_dim<float, 1>(h, a, st) : dec_launch_dim<float, 2>(h, a, st);
     else
       one ? dec_launch_dim<__nv_bfloat16, 1>(h, a, st) : dec_launch_dim<__nv_bfloat16, 2>(h, a, st);
+  });
+}
+
+extern "C" int specdec_kv8_check(specdec_kv8 *h, void *stream) {
+  if (!h) return SPECDEC_ERR_INVALID;
+  return op_guard(h->err, [&] {
+    DeviceScope scope(h->device);
+    const auto st = static_cast<cudaStream_t>(stream);
+    int bits = 0;
+    op_cuda(cudaMemcpyAsync(&bits, h->err_word, sizeof(int), cudaMemcpyDeviceToHost, st), "specdec_kv8_check");
+    op_cuda(cudaStreamSynchronize(st), "specdec_kv8_check");
+    if (!bits) return;
+    op_cuda(cudaMemsetAsync(h->err_word, 0, sizeof(int), st), "specdec_kv8_check");
+    op_fail(SPECDEC_ERR_CUDA, "a wait inside specdec_kv8_attend did not end within its limit");
   });
 }

@@ -1,0 +1,714 @@
+// Attention over the 8-bit paged cache for many rows per kv head (chunks of a
+// prompt, wide verify blocks): the formulas of kv8_attn.cu on tcgen05.
+//
+// With 128 and more rows every cached code meets all of them and the call is
+// bound by its products and exponentials, not by HBM: a tile of 128 rows x 128
+// positions x 128 dims is 256 tensor cycles a product, 1,024 cycles of
+// exponentials (16 a cycle and SM) and about as many issue slots for the rest
+// of the softmax.  One persistent block per SM takes 256 rows of a (request, kv
+// head) at a time:
+//   4 converter warps   codes from global memory through registers (one tile
+//                       ahead) into f16 tiles of K and V in shared memory, two
+//                       buffers each, 128-byte swizzle: once for 256 rows
+//   1 issuing thread    S = Q K^T (M = 128 rows, N = 128 positions) and
+//                       O += P V (A = P from tensor memory, N = D) for each of
+//                       the two row tiles in turn
+//   2 x 4 softmax warps one per row tile, thread = row = tensor memory lane:
+//                       the maximum, then weights p = 2^(s - m) whose f16
+//                       products with the value scales go back to tensor
+//                       memory in the place of the scores
+// The products of one row tile run while the other tile's warps are in their
+// softmax.  Tensor memory: scores 2 x 128 columns, outputs 2 x D.  A row's
+// maximum is moved (and its output rescaled) only when a weight would exceed
+// 2^8.  The queries are scaled by a power of two per row, so that bf16 rows are
+// exact in f16; codes are whole numbers, exact too.
+// Units (tiles of 128 positions) of all items are shared out evenly, as in
+// kv8_attn.cu; partial results of an item meet in the workspace.  Every wait
+// is bounded; one that gives up sets the handle's error word and ends the
+// block after the products in flight.
+#include <algorithm>
+
+#include "gemm.cuh"
+#include "kv8_attn.cuh"
+
+namespace specdec {
+
+namespace {
+
+constexpr int kTileRows = 128;    // rows of a softmax warpgroup, lanes of tensor memory
+constexpr int kItemRows = 256;
+constexpr int kTilePos = 128;     // positions of a unit
+constexpr int kSlices = kTilePos / 16;
+constexpr int kSoftmaxThreads = 256;
+constexpr int kConverterWarps = 4;
+constexpr int kChunkThreads = kSoftmaxThreads + 32 * kConverterWarps + 32;
+constexpr int kScaleSlots = 4;    // the scales of a tile stay until both softmax groups are past it
+constexpr int kWholeChunks = 2;   // items of at most this many units are not split
+constexpr int kMergeParts = 4;
+
+template <int D>
+struct ChunkGeom {
+  static constexpr int kAtom = kTilePos * 128;          // 64 dims of 128 rows, two bytes each
+  static constexpr int kTile = D / 64 * kAtom;
+  static constexpr int kTiles = 6 * kTile;              // Q of both row tiles, K and V twice
+  static constexpr int kScales = kScaleSlots * (2 * kSlices + 4) * 4;
+  static constexpr int kFixed = kTiles + kScales;
+  static constexpr int kPart = kItemRows * (D + 2);     // floats of a partial result
+};
+
+// kind::f16, D fp32, A and B f16, M = 128.  S: A and B K-major, N = 128.  O: A from tensor memory, B (V) MN-major, N = D.
+constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kTilePos >> 3) << 17) | (8u << 24);
+template <int D>
+constexpr uint32_t idesc_o() {
+  return (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
+}
+
+// MN-major operand of atoms of 64 columns (kAtom bytes apart), 128-byte swizzle; along K rows are 128 bytes apart,
+// groups of 8 rows 1024 bytes.
+__device__ __forceinline__ uint64_t desc_mn128(uint32_t saddr, int atom_bytes) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(atom_bytes >> 4) << 16) | (64ull << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+// D[tmem] (+)= A[tmem] B
+__device__ __forceinline__ void tc_mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// 32 columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A phase of an mbarrier, for at most about two seconds; false: gave up, or another role did.
+__device__ __forceinline__ bool chunk_wait(uint64_t *bar, uint32_t phase, volatile int *stop) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(phase)
+        : "memory");
+    if (done) return true;
+    if ((it & 63) == 63) {
+      if (*stop) return false;
+      const uint64_t now = global_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > 2000000000ull) return false;
+    }
+  }
+}
+__device__ __forceinline__ void chunk_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// A row tile pair of a request: 256 rows from row0, n of them there; its first unit along the cache and its units.
+struct ChunkTile {
+  int row0, n, t0, nt;
+};
+__device__ __forceinline__ ChunkTile chunk_tile(const AttendArgs &a, int q, int len, int rt) {
+  ChunkTile t;
+  t.row0 = rt * kItemRows;
+  t.n = min(kItemRows, q * a.g.G - t.row0);
+  const int first = len - q + row_at(a, t.row0).i, last = len - q + row_at(a, t.row0 + t.n - 1).i;  // positions of the rows
+  t.t0 = a.window > 0 ? max(0, first - a.window + 1) / kTilePos : 0;
+  t.nt = max(1, (last < 0 ? 0 : last / kTilePos + 1) - t.t0);
+  return t;
+}
+
+// Walks consecutive units: request, kv head, row tile pair, unit.
+struct ChunkCursor {
+  int b, q0, q, len, nr, h, rt, unit;
+  ChunkTile t;
+  __device__ __forceinline__ void enter(const AttendArgs &a, const DecBatch &s, int req) {
+    b = req;
+    q0 = s.q0[b];
+    q = s.q[b];
+    len = s.len[b];
+    nr = (q * a.g.G + kItemRows - 1) / kItemRows;
+  }
+  __device__ __forceinline__ void seek(const AttendArgs &a, const DecBatch &s, long long u) {
+    enter(a, s, request_of(s.pre, a.b.B, u));
+    const long long in = u - s.pre[b], per_head = (s.pre[b + 1] - s.pre[b]) / a.g.Hkv;
+    h = static_cast<int>(in / per_head);
+    long long left = in - h * per_head;
+    for (rt = 0;; ++rt) {
+      t = chunk_tile(a, q, len, rt);
+      if (left < t.nt) break;
+      left -= t.nt;
+    }
+    unit = static_cast<int>(left);
+  }
+  __device__ __forceinline__ void next(const AttendArgs &a, const DecBatch &s) {
+    if (++unit < t.nt) return;
+    unit = 0;
+    if (++rt == nr) {
+      rt = 0;
+      if (++h == a.g.Hkv) {
+        h = 0;
+        int n = b + 1;
+        while (n < a.b.B && s.pre[n + 1] == s.pre[n]) ++n;
+        if (n == a.b.B) return;  // past the last unit
+        enter(a, s, n);
+      }
+    }
+    t = chunk_tile(a, q, len, rt);
+  }
+  __device__ __forceinline__ int pos() const { return (t.t0 + unit) * kTilePos; }
+  // rows of row tile w, the positions of its first and last row, and whether it sees anything of the tile at p
+  __device__ __forceinline__ int rows(int w) const { return max(0, min(kTileRows, t.n - w * kTileRows)); }
+  __device__ __forceinline__ int first(const AttendArgs &a, int w) const { return len - q + row_at(a, t.row0 + w * kTileRows).i; }
+  __device__ __forceinline__ int last(const AttendArgs &a, int w) const {
+    return len - q + row_at(a, t.row0 + w * kTileRows + rows(w) - 1).i;
+  }
+  __device__ __forceinline__ bool active(const AttendArgs &a, int w, int p) const {
+    return rows(w) > 0 && p <= last(a, w) && (a.window <= 0 || p + kTilePos - 1 > first(a, w) - a.window);
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __grid_constant__ AttendArgs a) {
+  using Geo = ChunkGeom<D>;
+  using XT = __nv_bfloat16;
+  constexpr int kAtoms = D / 64;
+  extern __shared__ unsigned char chunk_smem[];
+  unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(chunk_smem) + 1023) & ~uintptr_t(1023));
+  unsigned char *q_smem = base, *k_smem = base + 2 * Geo::kTile, *v_smem = base + 4 * Geo::kTile;
+  float *scales = reinterpret_cast<float *>(base + Geo::kTiles);  // per slot: key scales, value scales, slices there
+  DecBatch bt;
+  bt.pre = reinterpret_cast<long long *>(base + Geo::kFixed);
+  bt.q0 = reinterpret_cast<int *>(bt.pre + a.b.B + 1);
+  bt.q = bt.q0 + a.b.B;
+  bt.len = bt.q + a.b.B;
+  __shared__ long long red[kChunkThreads / 32];
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], q_full[2], o_full[2], mma_done;
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_stop;
+  __shared__ int s_last;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  constexpr int kIssuer = (kSoftmaxThreads >> 5) + kConverterWarps;
+
+  if (warp == kIssuer) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], kConverterWarps);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], kConverterWarps);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&q_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(&mma_done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_stop = 0;
+  }
+  int longest = 0;
+  request_prefix(a.b.B, bt.pre, red, [&](int b) {
+    const Kv8Req r = kv8_req(a.b, a.g.P, b);
+    bt.q0[b] = r.q0;
+    bt.q[b] = r.q;
+    bt.len[b] = r.len;
+    long long n = 0;
+    const int nr = (r.q * a.g.G + kItemRows - 1) / kItemRows;
+    for (int rt = 0; rt < nr; ++rt) {
+      const int nt = chunk_tile(a, r.q, r.len, rt).nt;
+      longest = max(longest, nt);
+      n += nt;
+    }
+    return n * a.g.Hkv;
+  });
+  const long long total = bt.pre[a.b.B];
+  const long long share = quotient(total + gridDim.x - 1, gridDim.x);
+  long long u0 = min(total, share * blockIdx.x), u1 = min(total, u0 + share);
+  if (!__syncthreads_or(longest > kWholeChunks)) {  // short items stay whole
+    auto item_start = [&](long long u) {
+      if (u >= total) return total;
+      ChunkCursor c;
+      c.seek(a, bt, u);
+      return c.unit == 0 ? u : u + c.t.nt - c.unit;
+    };
+    u0 = item_start(u0);
+    u1 = item_start(u1);
+  }
+  const int n_units = uniform(static_cast<int>(u1 - u0));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  auto give_up = [&]() {
+    if (!s_stop) {
+      s_stop = 1;
+      if (a.err) atomicOr(a.err, 1);
+    }
+  };
+
+  if (warp >= (kSoftmaxThreads >> 5) && warp < kIssuer) {
+    // ---- converters ----------------------------------------------------------
+    // A warp has 32 positions of a tile: of 8 positions at a time 4 lanes read 64 codes each, one 64-dim atom after the other.
+    const int w = warp - (kSoftmaxThreads >> 5), row_in = lane >> 2, c16 = lane & 3;
+    constexpr int kLoads = 4 * kAtoms;
+    uint4 rk[kLoads], rv[kLoads];
+    float sc = 0.f;
+    uint32_t there = 0;
+    ChunkCursor cur;
+    int left = n_units;
+    if (left > 0) cur.seek(a, bt, u0);
+    int pages[4];
+    auto find_pages = [&]() {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = cur.pos() + 32 * w + 8 * i;
+        const int page = p < cur.len ? a.b.table[static_cast<long long>(cur.b) * a.b.cols + (p >> a.p_shift)] : -1;
+        pages[i] = page >= 0 && page < a.c.n_pages ? page : -1;
+      }
+    };
+    auto load = [&](const int8_t *src, uint4 (&r)[kLoads]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = cur.pos() + 32 * w + 8 * i + row_in;
+        const long long ph = static_cast<long long>(pages[i]) * a.g.Hkv + cur.h;
+        const long long at = ((ph << a.p_shift) + (p & (a.g.P - 1))) * D + 16 * c16;
+#pragma unroll
+        for (int t = 0; t < kAtoms; ++t)
+          r[i * kAtoms + t] = pages[i] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + at + 64 * t)) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto put = [&](unsigned char *dst, const uint4 (&r)[kLoads]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 32 * w + 8 * i + row_in;
+#pragma unroll
+        for (int t = 0; t < kAtoms; ++t) {
+          const uint4 v = r[i * kAtoms + t];
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          uint32_t f[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t y = x[j] ^ 0x80808080u;
+            f[2 * j] = f16_codes(__byte_perm(y, 0x64646464u, 0x4140));
+            f[2 * j + 1] = f16_codes(__byte_perm(y, 0x64646464u, 0x4342));
+          }
+          unsigned char *line = dst + t * Geo::kAtom + row * 128;
+          *reinterpret_cast<uint4 *>(line + (((2 * c16) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<uint4 *>(line + (((2 * c16 + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+        }
+      }
+    };
+    // lanes 0 .. 3 of a warp: key and value scales of its two slices
+    auto load_scales = [&]() {
+      const int slice = 2 * w + (lane >> 1 & 1), p = cur.pos() + 16 * slice;
+      const int page = (lane & 2) ? pages[2] : pages[0];
+      sc = 0.f;
+      if (lane < 4 && page >= 0) {
+        const long long ph = static_cast<long long>(page) * a.g.Hkv + cur.h;
+        sc = ((lane & 1) ? a.c.vs : a.c.ks)[(ph << (a.p_shift - a.t_shift)) + ((p & (a.g.P - 1)) >> a.t_shift)];
+      }
+      there = __ballot_sync(0xffffffffu, lane < 2 && (lane ? pages[2] : pages[0]) >= 0);
+    };
+    auto publish = [&](uint64_t *bar) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) chunk_arrive(bar);
+    };
+    if (left > 0) {
+      find_pages();
+      load(a.c.k, rk);
+      load(a.c.v, rv);
+      load_scales();
+    }
+    bool ok = true;
+    for (int n = 0; left > 0 && ok; ++n, --left) {
+      const int buf = n & 1;
+      const uint32_t ph = (n >> 1) & 1;
+      ok = chunk_wait(&k_empty[buf], ph ^ 1, &s_stop);
+      if (!ok) break;
+      put(k_smem + buf * Geo::kTile, rk);
+      float *slot = scales + (n % kScaleSlots) * (2 * kSlices + 4);
+      if (lane < 4) slot[(lane & 1) * kSlices + 2 * w + (lane >> 1)] = sc;
+      if (lane == 0) reinterpret_cast<unsigned char *>(slot + 2 * kSlices)[w] = static_cast<unsigned char>(there);
+      publish(&k_full[buf]);
+      uint4 keep[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) keep[i] = rv[i];
+      if (left > 1) {
+        cur.next(a, bt);
+        find_pages();
+        load(a.c.k, rk);
+        load(a.c.v, rv);
+        load_scales();
+      }
+      ok = chunk_wait(&v_empty[buf], ph ^ 1, &s_stop);
+      if (!ok) break;
+      put(v_smem + buf * Geo::kTile, keep);
+      publish(&v_full[buf]);
+    }
+    if (!ok) give_up();
+  } else if (warp == kIssuer) {
+    // ---- products --------------------------------------------------------------
+    if (lane == 0 && n_units > 0) {
+      bool ok = true;
+      int n_act[2] = {0, 0}, n_seg[2] = {0, 0};  // active units and segments of each row tile so far
+      bool begun[2] = {false, false};            // the segment's first products of a row tile are issued
+      ChunkCursor cur, nxt;
+      cur.seek(a, bt, u0);
+      const uint32_t qa = smem_u32(q_smem), ka = smem_u32(k_smem), va = smem_u32(v_smem);
+      auto issue_s = [&](int w, int n, const ChunkCursor &c, bool first) -> bool {
+        if (!chunk_wait(&k_full[n & 1], (n >> 1) & 1, &s_stop)) return false;  // of every unit: phases are told apart by parity
+        if (!c.active(a, w, c.pos())) return true;
+        if (first && !chunk_wait(&q_full[w], n_seg[w]++ & 1, &s_stop)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t at = (kk >> 2) * Geo::kAtom + 32 * (kk & 3);
+          tc_mma(tmem + 128 * w, umma_desc_k128(qa + w * Geo::kTile + at), umma_desc_k128(ka + (n & 1) * Geo::kTile + at), kIdescS, kk ? 1u : 0u);
+        }
+        tc_commit(&s_full[w]);
+        return true;
+      };
+      for (int w = 0; w < 2; ++w) {
+        const bool act = cur.active(a, w, cur.pos());
+        ok = ok && issue_s(w, 0, cur, true);
+        begun[w] = act;
+      }
+      tc_commit(&k_empty[0]);
+      bool opened[2] = {false, false};  // the segment's output has a first product
+      for (int n = 0; n < n_units && ok; ++n) {
+        const bool more = n + 1 < n_units;
+        nxt = cur;
+        if (more) nxt.next(a, bt);
+        const bool ends = !more || nxt.unit == 0;
+        ok = chunk_wait(&v_full[n & 1], (n >> 1) & 1, &s_stop);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (ok && cur.active(a, w, cur.pos())) {
+            ok = chunk_wait(&p_full[w], n_act[w]++ & 1, &s_stop);
+            if (ok) {
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < kTilePos / 16; ++kk)
+                tc_mma_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, desc_mn128(va + (n & 1) * Geo::kTile + 2048 * kk, Geo::kAtom),
+                          idesc_o<D>(), (kk || opened[w]) ? 1u : 0u);
+              opened[w] = true;
+            }
+          }
+          if (ends) {
+            if (ok && opened[w]) tc_commit(&o_full[w]);
+            opened[w] = begun[w] = false;
+          } else if (ok) {
+            const bool act = nxt.active(a, w, nxt.pos());
+            ok = issue_s(w, n + 1, nxt, !begun[w]);
+            begun[w] = begun[w] || act;
+          }
+        }
+        // a new segment's scores wait for its queries, which come after both groups have their outputs: not before
+        // both groups' products are issued
+        if (ends && more) {
+          for (int w = 0; w < 2; ++w) {
+            ok = ok && issue_s(w, n + 1, nxt, true);
+            begun[w] = nxt.active(a, w, nxt.pos());
+          }
+        }
+        tc_commit(&v_empty[n & 1]);
+        if (more) tc_commit(&k_empty[(n + 1) & 1]);
+        cur = nxt;
+      }
+      if (!ok) give_up();
+      tc_commit(&mma_done);  // every product has ended before the block moves on
+      if (!chunk_wait(&mma_done, 0, &s_stop) && !mbar_wait(&mma_done, 0)) give_up();
+    }
+  } else if (warp < (kSoftmaxThreads >> 5)) {
+    // ---- softmax and output: thread = row -------------------------------------------
+    const int w = warp >> 2, r = threadIdx.x & 127, r_item = threadIdx.x;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t s_at = tmem + lanes + 128 * w, o_at = tmem + lanes + 256 + 128 * w;
+    ChunkCursor cur;
+    if (n_units > 0) cur.seek(a, bt, u0);
+    bool ok = true;
+    int n_act = 0, n_seg = 0;
+    for (int n = 0; n < n_units;) {
+      // the segment: units of the item within this block's share
+      const int units = min(cur.t.nt - cur.unit, n_units - n);
+      const int rows = cur.rows(w), first_pos = rows > 0 ? cur.first(a, w) : 0, last_pos = rows > 0 ? cur.last(a, w) : -1;
+      const int p_begin = cur.pos(), p_end = p_begin + units * kTilePos;  // last_pos or the window may leave nothing of it
+      bool any = false;
+      for (int i = 0; i < units && !any; ++i) any = cur.active(a, w, p_begin + i * kTilePos);
+      const RowAt at_row = row_at(a, cur.t.row0 + r_item);
+      const bool live = r < rows;
+      const int lim = live ? cur.len - cur.q + at_row.i : -1;
+      const long long token = cur.q0 + at_row.i;
+      const int head = cur.h * a.g.G + at_row.h;
+      float m = kNone, l = 0.f, cs = 0.f;
+      if (any && ok) {
+        // the queries: a power of two times f16, and a NaN in cs where the row has a value that is not finite
+        const XT *src = static_cast<const XT *>(a.q) + (live ? token * a.q_row + head * a.q_head : 0);
+        float big = 0.f, bad = 0.f;
+#pragma unroll 8
+        for (int d = 0; d < D; d += 4) {
+          Quad<XT> x;
+          x.load(src + d, a.q_vec, live);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            big = fmaxf(big, fabsf(x.get(j)));
+            bad = fmaf(x.get(j), 0.f, bad);
+          }
+        }
+        const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
+        const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+        cs = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
+        unsigned char *row = q_smem + w * Geo::kTile + r * 128;
+#pragma unroll 4
+        for (int d = 0; d < D; d += 8) {
+          Quad<XT> x, y;
+          x.load(src + d, a.q_vec, live);
+          y.load(src + d + 4, a.q_vec, live);
+          const uint4 f = make_uint4(pack_f16(x.get(0) * down, x.get(1) * down), pack_f16(x.get(2) * down, x.get(3) * down),
+                                     pack_f16(y.get(0) * down, y.get(1) * down), pack_f16(y.get(2) * down, y.get(3) * down));
+          *reinterpret_cast<uint4 *>(row + (d >> 6) * Geo::kAtom + ((((d & 63) >> 3) ^ (r & 7)) << 4)) = f;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) chunk_arrive(&q_full[w]);
+      }
+      bool opened = false;
+      for (int i = 0; i < units; ++i, ++n) {
+        const int p0 = p_begin + i * kTilePos;
+        if (!ok || !cur.active(a, w, p0)) continue;
+        ok = chunk_wait(&s_full[w], n_act++ & 1, &s_stop);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tc_fence_after();
+        const float *slot = scales + (n % kScaleSlots) * (2 * kSlices + 4);
+        const uint32_t there4 = *reinterpret_cast<const uint32_t *>(slot + 2 * kSlices);  // two bits a byte
+        const bool whole = p0 + kTilePos - 1 <= first_pos && (a.window <= 0 || p0 > last_pos - a.window) && there4 == 0x03030303u;
+        auto slice_there = [&](int s) { return (there4 >> (8 * (s >> 1) + (s & 1))) & 1; };
+        auto hidden = [&](int c) {
+          const int p = p0 + c;
+          return p > lim || (a.window > 0 && p <= lim - a.window) || !slice_there(c >> 4);
+        };
+        // the largest weight x value scale, by exponent
+        float top = kNone;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          tmem_ld32(s_at + 32 * c, s);
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (hidden(32 * c + j)) s[j] = -INFINITY;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mx = s[16 * h];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[16 * h + j]);
+            const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(slot[kSlices + 2 * c + h]) >> 23) - 127, -90));
+            if (mx != -INFINITY) top = fmaxf(top, mx * (cs * slot[2 * c + h]) + ev);
+          }
+        }
+        if (__any_sync(0xffffffffu, top > m + kLazy)) {
+          const float nm = top > m + kLazy ? top : m;
+          const float al = exp2_fast(m - nm);
+          m = nm;
+          l *= al;
+          if (opened) {  // the products so far have ended: this tile's scores were issued after them
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              uint32_t x[16];
+              tmem_ld32(o_at + 32 * c, o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(o[j] * al);
+              tmem_st16(o_at + 32 * c, x);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(o[16 + j] * al);
+              tmem_st16(o_at + 32 * c + 16, x);
+            }
+          }
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          uint32_t f[16];
+          tmem_ld32(s_at + 32 * c, s);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float k = cs * slot[2 * c + h], v = slot[kSlices + 2 * c + h];
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              float x0 = fmaf(s[16 * h + j], k, -m), x1 = fmaf(s[16 * h + j + 1], k, -m);
+              float v0 = v, v1 = v;
+              if (!whole) {  // a scale that a row does not see may be anything
+                if (hidden(32 * c + 16 * h + j)) { x0 = -INFINITY; v0 = 0.f; }
+                if (hidden(32 * c + 16 * h + j + 1)) { x1 = -INFINITY; v1 = 0.f; }
+              }
+              const float p0_ = exp2_fast(x0), p1_ = exp2_fast(x1);
+              sum[0] += p0_;
+              sum[1] += p1_;
+              f[8 * h + j / 2] = pack_f16(p0_ * v0, p1_ * v1);
+            }
+          }
+          tmem_st16(s_at + 16 * c, f);
+        }
+        l += sum[0] + sum[1];
+        opened = true;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) chunk_arrive(&p_full[w]);
+      }
+      // ---- end of the segment -------------------------------------------------------
+      if (any && ok) {
+        ok = chunk_wait(&o_full[w], n_seg++ & 1, &s_stop);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      uint32_t all_ok;
+      asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                   : "=r"(all_ok)
+                   : "r"(static_cast<uint32_t>(ok))
+                   : "memory");
+      if (!all_ok) {
+        ok = false;
+        break;
+      }
+      const long long i0 = u0 + (n - units) - cur.unit, i1 = i0 + cur.t.nt;
+      const bool all = i0 >= u0 && i1 <= u1;
+      XT *dst = static_cast<XT *>(a.out) + (live ? token * a.o_row + head * a.o_head : 0);
+      auto finish = [&](float lsum, float top) {
+        if (live && a.lse) a.lse[token * a.g.H + head] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
+        return lsum == 0.f ? 0.f : __fdividef(1.f, lsum);  // 0: the row saw nothing
+      };
+      float4 *part = reinterpret_cast<float4 *>(a.part + (2 * static_cast<long long>(blockIdx.x) + (i0 >= u0 ? 1 : 0)) * Geo::kPart);
+      const float inv = all ? finish(l, m) : 1.f;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (any) {
+          tmem_ld32(o_at + 32 * c, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          // a row of the tile that saw nothing has weights of 0 only
+          const float4 v = make_float4(o[j] * inv, o[j + 1] * inv, o[j + 2] * inv, o[j + 3] * inv);
+          if (!all) part[(8 * c + j / 4) * kItemRows + r_item] = v;
+          else if (live) store4(dst + 32 * c + j, a.o_vec, v);
+        }
+      }
+      if (!all) {
+        float *ml = reinterpret_cast<float *>(part) + kItemRows * D;
+        ml[r_item] = m;
+        ml[kItemRows + r_item] = l;
+        const int c0 = static_cast<int>(quotient(i0, share)), c1 = static_cast<int>(quotient(i1 - 1, share));
+        __threadfence();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (threadIdx.x == 0) s_last = atomicAdd(a.ticket + c0, 1) == c1 - c0;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (s_last) {
+          __threadfence();
+          auto part_of_block = [&](int c) { return a.part + (2ll * c + (c == c0)) * Geo::kPart; };
+          float top = kNone, lsum = 0.f;
+          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part_of_block(c) + kItemRows * D + r_item));
+          for (int c = c0; c <= c1; ++c) {
+            const float *pm = part_of_block(c) + kItemRows * D + r_item;
+            lsum += __ldcg(pm + kItemRows) * exp2_fast(__ldcg(pm) - top);
+          }
+          const float inv_all = finish(lsum, top);
+#pragma unroll 1
+          for (int d = 0; d < D / 4; d += kMergeParts) {
+            float4 v[kMergeParts];
+#pragma unroll
+            for (int j = 0; j < kMergeParts; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = c0; c <= c1; ++c) {
+              const float *p = part_of_block(c);
+              const float f = exp2_fast(__ldcg(p + kItemRows * D + r_item) - top) * inv_all;
+#pragma unroll
+              for (int j = 0; j < kMergeParts; ++j) {
+                const float4 y = __ldcg(reinterpret_cast<const float4 *>(p) + (d + j) * kItemRows + r_item);
+                v[j].x += y.x * f; v[j].y += y.y * f; v[j].z += y.z * f; v[j].w += y.w * f;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < kMergeParts; ++j)
+              if (live) store4(dst + 4 * (d + j), a.o_vec, v[j]);
+          }
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          if (threadIdx.x == 0) a.ticket[c0] = 0;
+        }
+      }
+      tc_fence_before();
+      for (int i = 0; i < units; ++i) cur.next(a, bt);
+    }
+    if (!ok) give_up();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kIssuer)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <int D>
+int chunk_smem_bytes(int B) {
+  return 1024 + ChunkGeom<D>::kFixed + (B + 1) * static_cast<int>(sizeof(long long)) + 3 * B * static_cast<int>(sizeof(int));
+}
+
+}  // namespace
+
+void kv8_chunk_create(specdec_kv8 *h) {
+  if (h->g.D < 64) return;
+  if (h->g.D == 64)
+    op_cuda(cudaFuncSetAttribute(kv8_chunk_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, chunk_smem_bytes<64>(kChunkMaxBatch)),
+            "cudaFuncSetAttribute");
+  else
+    op_cuda(cudaFuncSetAttribute(kv8_chunk_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, chunk_smem_bytes<128>(kChunkMaxBatch)),
+            "cudaFuncSetAttribute");
+}
+
+size_t kv8_chunk_part_bytes(const specdec_kv8 *h) {
+  if (h->g.D < 64) return 0;
+  return static_cast<size_t>(h->num_sms) * 2 * (kItemRows * (h->g.D + 2)) * sizeof(float);
+}
+
+void kv8_chunk_launch(const specdec_kv8 *h, const AttendArgs &a, cudaStream_t st) {
+  if (h->g.D == 64)
+    op_launch("specdec_kv8_attend", kv8_chunk_kernel<64>, dim3(h->num_sms), kChunkThreads, chunk_smem_bytes<64>(a.b.B), st, 1, a);
+  else
+    op_launch("specdec_kv8_attend", kv8_chunk_kernel<128>, dim3(h->num_sms), kChunkThreads, chunk_smem_bytes<128>(a.b.B), st, 1, a);
+}
+
+}  // namespace specdec

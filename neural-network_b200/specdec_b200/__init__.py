@@ -40,7 +40,8 @@ EXPORTS = ("specdec_create", "specdec_destroy", "specdec_last_error", "specdec_l
            "specdec_prefill", "specdec_prefill_device", "specdec_step", "specdec_step_device",
            "specdec_session_tokens", "specdec_time_attention", "specdec_load_params_device",
            "specdec_kv8_create", "specdec_kv8_destroy", "specdec_kv8_last_error", "specdec_kv8_plan",
-           "specdec_kv8_append", "specdec_kv8_gather", "specdec_kv8_attend", "specdec_sample")
+           "specdec_kv8_append", "specdec_kv8_gather", "specdec_kv8_attend", "specdec_kv8_check",
+           "specdec_sample")
 
 # linear layers of specdec_time_linear
 LIN_QKV, LIN_OPROJ, LIN_FFN_IN, LIN_FFN_OUT, LIN_HEAD = 0, 1, 2, 3, 4
@@ -149,6 +150,7 @@ def load_library(path: str = LIB_PATH):
     lib.specdec_kv8_append.argtypes = [vp, vp, vp, vp, i64, i64, vp, i64, i64, i32, i32, vp]
     lib.specdec_kv8_gather.argtypes = [vp, vp, vp, i32, vp, vp, i32, vp]
     lib.specdec_kv8_attend.argtypes = [vp, vp, vp, vp, i64, i64, i32, i32, vp, i64, i64, vp, i32, C.c_float, i32, vp]
+    lib.specdec_kv8_check.argtypes = [vp, vp]
     lib.specdec_sample.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp]
     _lib = lib
     return lib

@@ -172,6 +172,10 @@ class KV8:
             self.h, self._layer(layer), batch.ptr, qp, qr, qh, _dtype_of(q), q.shape[0], op, orow, oh, lp, max_q,
             1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, stream or None))
 
+    def check(self, stream: int = 0) -> None:
+        """Waits for the stream; raises if a wait inside an attend call on it gave up."""
+        self._check(self._lib.specdec_kv8_check(self.h, stream or None))
+
 
 def sample(logits, u, tokens, probs=None, temperature=None, top_k=None, top_p=None, min_p=None,
            stream: int = 0) -> None:
