@@ -44,7 +44,7 @@ constexpr int kConverterWarps = 4;
 constexpr int kChunkThreads = kSoftmaxThreads + 32 * kConverterWarps + 32;
 constexpr int kScaleSlots = 4;    // the scales of a tile stay until both softmax groups are past it
 constexpr int kWholeChunks = 2;   // items of at most this many units are not split
-constexpr int kMergeParts = 4;
+constexpr int kMergeParts = 8;
 
 template <int D>
 struct ChunkGeom {
@@ -511,29 +511,37 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         const float *slot = scales + (n % kScaleSlots) * (2 * kSlices + 4);
         const uint32_t there4 = *reinterpret_cast<const uint32_t *>(slot + 2 * kSlices);  // two bits a byte
         const bool whole = p0 + kTilePos - 1 <= first_pos && (a.window <= 0 || p0 > last_pos - a.window) && there4 == 0x03030303u;
-        auto slice_there = [&](int s) { return (there4 >> (8 * (s >> 1) + (s & 1))) & 1; };
-        auto hidden = [&](int c) {
-          const int p = p0 + c;
-          return p > lim || (a.window > 0 && p <= lim - a.window) || !slice_there(c >> 4);
+        // bit j: whether this row sees column 32 c + j
+        auto seen = [&](int c) -> uint32_t {
+          const int n = lim - (p0 + 32 * c) + 1;  // columns up to the row's own position
+          uint32_t v = n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+          if (a.window > 0) {
+            const int k = n - a.window;  // columns before the window
+            v = k <= 0 ? v : k >= 32 ? 0u : v & (~0u << k);
+          }
+          const uint32_t two = there4 >> (8 * c);
+          return v & (((two & 1) ? 0xffffu : 0u) | ((two & 2) ? 0xffff0000u : 0u));
         };
         // the largest weight x value scale, by exponent
         float top = kNone;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float s[32];
           tmem_ld32(s_at + 32 * c, s);
           if (!whole) {
+            const uint32_t v = seen(c);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (hidden(32 * c + j)) s[j] = -INFINITY;
+            for (int j = 0; j < 32; ++j) s[j] = (v >> j & 1) ? s[j] : -INFINITY;
           }
+          const float2 ks = *reinterpret_cast<const float2 *>(slot + 2 * c), vs = *reinterpret_cast<const float2 *>(slot + kSlices + 2 * c);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float mx = s[16 * h];
+            float mx[4];
 #pragma unroll
-            for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[16 * h + j]);
-            const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(slot[kSlices + 2 * c + h]) >> 23) - 127, -90));
-            if (mx != -INFINITY) top = fmaxf(top, mx * (cs * slot[2 * c + h]) + ev);
+            for (int j = 0; j < 4; ++j) mx[j] = fmaxf(fmaxf(s[16 * h + j], s[16 * h + 4 + j]), fmaxf(s[16 * h + 8 + j], s[16 * h + 12 + j]));
+            const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(h ? vs.y : vs.x) >> 23) - 127, -90));
+            if (m4 != -INFINITY) top = fmaxf(top, fmaf(m4, cs * (h ? ks.y : ks.x), ev));
           }
         }
         if (__any_sync(0xffffffffu, top > m + kLazy)) {
@@ -557,27 +565,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
           }
         }
         float sum[2] = {0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float s[32];
           uint32_t f[16];
           tmem_ld32(s_at + 32 * c, s);
+          const float2 ks = *reinterpret_cast<const float2 *>(slot + 2 * c), vs = *reinterpret_cast<const float2 *>(slot + kSlices + 2 * c);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float k = cs * slot[2 * c + h], v = slot[kSlices + 2 * c + h];
+          for (int j = 0; j < 32; ++j) s[j] = exp2_fast(fmaf(s[j], cs * (j < 16 ? ks.x : ks.y), -m));
+          if (!whole) {
+            const uint32_t v = seen(c);
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              float x0 = fmaf(s[16 * h + j], k, -m), x1 = fmaf(s[16 * h + j + 1], k, -m);
-              float v0 = v, v1 = v;
-              if (!whole) {  // a scale that a row does not see may be anything
-                if (hidden(32 * c + 16 * h + j)) { x0 = -INFINITY; v0 = 0.f; }
-                if (hidden(32 * c + 16 * h + j + 1)) { x1 = -INFINITY; v1 = 0.f; }
-              }
-              const float p0_ = exp2_fast(x0), p1_ = exp2_fast(x1);
-              sum[0] += p0_;
-              sum[1] += p1_;
-              f[8 * h + j / 2] = pack_f16(p0_ * v0, p1_ * v1);
-            }
+            for (int j = 0; j < 32; ++j) s[j] = (v >> j & 1) ? s[j] : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            sum[0] += s[j];
+            sum[1] += s[j + 1];
+            const float v = j < 16 ? vs.x : vs.y;
+            f[j / 2] = pack_f16(s[j] * v, s[j + 1] * v);
+          }
+          if (!whole) {  // a value scale that a row does not see may be anything
+            const uint32_t v = seen(c);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[j] &= ((v >> (2 * j) & 1) ? 0xffffu : 0u) | ((v >> (2 * j) & 2) ? 0xffff0000u : 0u);
           }
           tmem_st16(s_at + 16 * c, f);
         }
