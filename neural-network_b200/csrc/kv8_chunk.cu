@@ -181,14 +181,24 @@ struct ChunkCursor {
     t = chunk_tile(a, q, len, rt);
   }
   __device__ __forceinline__ int pos() const { return (t.t0 + unit) * kTilePos; }
-  // rows of row tile w, the positions of its first and last row, and whether it sees anything of the tile at p
+  // rows of row tile w, the positions of its first and last row
   __device__ __forceinline__ int rows(int w) const { return max(0, min(kTileRows, t.n - w * kTileRows)); }
   __device__ __forceinline__ int first(const AttendArgs &a, int w) const { return len - q + row_at(a, t.row0 + w * kTileRows).i; }
   __device__ __forceinline__ int last(const AttendArgs &a, int w) const {
     return len - q + row_at(a, t.row0 + w * kTileRows + rows(w) - 1).i;
   }
-  __device__ __forceinline__ bool active(const AttendArgs &a, int w, int p) const {
-    return rows(w) > 0 && p <= last(a, w) && (a.window <= 0 || p + kTilePos - 1 > first(a, w) - a.window);
+  // of the next `units` units, the first of which row tile w sees anything and the one after the last: equal if none
+  __device__ __forceinline__ int2 sees(const AttendArgs &a, int w, int units) const {
+    if (rows(w) == 0) return make_int2(0, 0);
+    const int end = last(a, w), here = t.t0 + unit;
+    const int lo = a.window > 0 ? max(0, max(0, first(a, w) - a.window + 1) / kTilePos - here) : 0;
+    const int hi = min(units, end < 0 ? 0 : end / kTilePos + 1 - here);
+    return hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
+  }
+  // over the next `units` units, which end the item or the block's share
+  __device__ __forceinline__ void skip(const AttendArgs &a, const DecBatch &s, int units) {
+    unit += units - 1;
+    next(a, s);
   }
 };
 
@@ -378,70 +388,65 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
     // ---- products --------------------------------------------------------------
     if (lane == 0 && n_units > 0) {
       bool ok = true;
-      int n_act[2] = {0, 0}, n_seg[2] = {0, 0};  // active units and segments of each row tile so far
-      bool begun[2] = {false, false};            // the segment's first products of a row tile are issued
-      ChunkCursor cur, nxt;
+      uint32_t acts[2] = {0, 0}, segs[2] = {0, 0};  // scores and segments of each row tile so far
+      ChunkCursor cur;
       cur.seek(a, bt, u0);
-      const uint32_t qa = smem_u32(q_smem), ka = smem_u32(k_smem), va = smem_u32(v_smem);
-      auto issue_s = [&](int w, int n, const ChunkCursor &c, bool first) -> bool {
-        if (!chunk_wait(&k_full[n & 1], (n >> 1) & 1, &s_stop)) return false;  // of every unit: phases are told apart by parity
-        if (!c.active(a, w, c.pos())) return true;
-        if (first && !chunk_wait(&q_full[w], n_seg[w]++ & 1, &s_stop)) return false;
-        tc_fence_after();
+      // descriptors hold addresses in 16-byte units in their low bits: offsets are added there
+      const uint64_t q_desc = umma_desc_k128(smem_u32(q_smem)), k_desc = umma_desc_k128(smem_u32(k_smem));
+      const uint64_t v_desc = desc_mn128(smem_u32(v_smem), Geo::kAtom);
+      auto scores = [&](int w, int n) {
+        const uint64_t qd = q_desc + (w * Geo::kTile >> 4), kd = k_desc + ((n & 1) * Geo::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t at = (kk >> 2) * Geo::kAtom + 32 * (kk & 3);
-          tc_mma(tmem + 128 * w, umma_desc_k128(qa + w * Geo::kTile + at), umma_desc_k128(ka + (n & 1) * Geo::kTile + at), kIdescS, kk ? 1u : 0u);
+          const uint32_t at = ((kk >> 2) * Geo::kAtom + 32 * (kk & 3)) >> 4;
+          tc_mma(tmem + 128 * w, qd + at, kd + at, kIdescS, kk ? 1u : 0u);
         }
         tc_commit(&s_full[w]);
-        return true;
       };
-      for (int w = 0; w < 2; ++w) {
-        const bool act = cur.active(a, w, cur.pos());
-        ok = ok && issue_s(w, 0, cur, true);
-        begun[w] = act;
-      }
-      tc_commit(&k_empty[0]);
-      bool opened[2] = {false, false};  // the segment's output has a first product
-      for (int n = 0; n < n_units && ok; ++n) {
-        const bool more = n + 1 < n_units;
-        nxt = cur;
-        if (more) nxt.next(a, bt);
-        const bool ends = !more || nxt.unit == 0;
-        ok = chunk_wait(&v_full[n & 1], (n >> 1) & 1, &s_stop);
+      for (int n = 0; n < n_units && ok;) {
+        const int units = min(cur.t.nt - cur.unit, n_units - n);
+        const int2 see[2] = {cur.sees(a, 0, units), cur.sees(a, 1, units)};
+        // A new segment's scores wait for its queries, which come after both groups have their outputs: not before both
+        // groups' products are issued.  K and V of every unit are waited for: phases are told apart by parity
+        ok = chunk_wait(&k_full[n & 1], (n >> 1) & 1, &s_stop);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if (ok && cur.active(a, w, cur.pos())) {
-            ok = chunk_wait(&p_full[w], n_act[w]++ & 1, &s_stop);
-            if (ok) {
+        for (int w = 0; w < 2; ++w)
+          if (ok && see[w].x == 0 && see[w].y > 0) {
+            ok = chunk_wait(&q_full[w], segs[w]++ & 1, &s_stop);
+            tc_fence_after();
+            if (ok) scores(w, n);
+          }
+        tc_commit(&k_empty[n & 1]);
+        for (int i = 0; i < units && ok; ++i, ++n) {
+          const bool more = i + 1 < units;
+          ok = chunk_wait(&v_full[n & 1], (n >> 1) & 1, &s_stop);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (ok && i >= see[w].x && i < see[w].y) {
+              ok = chunk_wait(&p_full[w], acts[w]++ & 1, &s_stop);
               tc_fence_after();
+              if (ok) {
+                const uint64_t vd = v_desc + ((n & 1) * Geo::kTile >> 4);
 #pragma unroll
-              for (int kk = 0; kk < kTilePos / 16; ++kk)
-                tc_mma_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, desc_mn128(va + (n & 1) * Geo::kTile + 2048 * kk, Geo::kAtom),
-                          idesc_o<D>(), (kk || opened[w]) ? 1u : 0u);
-              opened[w] = true;
+                for (int kk = 0; kk < kTilePos / 16; ++kk)
+                  tc_mma_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, vd + (2048 * kk >> 4), idesc_o<D>(), kk || i > see[w].x ? 1u : 0u);
+              }
+            }
+            if (!more) {
+              if (ok && see[w].y > 0) tc_commit(&o_full[w]);
+            } else if (ok) {
+              if (w == 0) ok = chunk_wait(&k_full[(n + 1) & 1], ((n + 1) >> 1) & 1, &s_stop);
+              if (ok && i + 1 >= see[w].x && i + 1 < see[w].y) {
+                if (i + 1 == see[w].x) ok = chunk_wait(&q_full[w], segs[w]++ & 1, &s_stop);
+                tc_fence_after();
+                if (ok) scores(w, n + 1);
+              }
             }
           }
-          if (ends) {
-            if (ok && opened[w]) tc_commit(&o_full[w]);
-            opened[w] = begun[w] = false;
-          } else if (ok) {
-            const bool act = nxt.active(a, w, nxt.pos());
-            ok = issue_s(w, n + 1, nxt, !begun[w]);
-            begun[w] = begun[w] || act;
-          }
+          tc_commit(&v_empty[n & 1]);
+          if (more) tc_commit(&k_empty[(n + 1) & 1]);
         }
-        // a new segment's scores wait for its queries, which come after both groups have their outputs: not before
-        // both groups' products are issued
-        if (ends && more) {
-          for (int w = 0; w < 2; ++w) {
-            ok = ok && issue_s(w, n + 1, nxt, true);
-            begun[w] = nxt.active(a, w, nxt.pos());
-          }
-        }
-        tc_commit(&v_empty[n & 1]);
-        if (more) tc_commit(&k_empty[(n + 1) & 1]);
-        cur = nxt;
+        cur.skip(a, bt, units);
       }
       if (!ok) give_up();
       tc_commit(&mma_done);  // every product has ended before the block moves on
@@ -460,9 +465,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       // the segment: units of the item within this block's share
       const int units = min(cur.t.nt - cur.unit, n_units - n);
       const int rows = cur.rows(w), first_pos = rows > 0 ? cur.first(a, w) : 0, last_pos = rows > 0 ? cur.last(a, w) : -1;
-      const int p_begin = cur.pos(), p_end = p_begin + units * kTilePos;  // last_pos or the window may leave nothing of it
-      bool any = false;
-      for (int i = 0; i < units && !any; ++i) any = cur.active(a, w, p_begin + i * kTilePos);
+      const int p_begin = cur.pos();
+      const int2 see = cur.sees(a, w, units);
+      const bool any = see.y > 0;
       const RowAt at_row = row_at(a, cur.t.row0 + r_item);
       const bool live = r < rows;
       const int lim = live ? cur.len - cur.q + at_row.i : -1;
@@ -503,7 +508,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       bool opened = false;
       for (int i = 0; i < units; ++i, ++n) {
         const int p0 = p_begin + i * kTilePos;
-        if (!ok || !cur.active(a, w, p0)) continue;
+        if (!ok || i < see.x || i >= see.y) continue;
         ok = chunk_wait(&s_full[w], n_act++ & 1, &s_stop);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) continue;
@@ -682,7 +687,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         }
       }
       tc_fence_before();
-      for (int i = 0; i < units; ++i) cur.next(a, bt);
+      cur.skip(a, bt, units);
     }
     if (!ok) give_up();
   }
