@@ -70,6 +70,13 @@ __device__ __forceinline__ uint64_t desc_mn128(uint32_t saddr, int atom_bytes) {
          (1ull << 46) | (2ull << 61);
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool one_lane() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 // D[tmem] (+)= A[tmem] B
 __device__ __forceinline__ void tc_mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -79,9 +86,8 @@ __device__ __forceinline__ void tc_mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint
       : "memory");
 }
 
-// 32 columns of the warp's 32 lanes.
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of the warp's 32 lanes: asked for (valid after tmem_wait_ld), and waited for.
+__device__ __forceinline__ void tmem_ask32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
@@ -90,7 +96,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ask32(addr, r);
+  tmem_wait_ld();
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -386,7 +396,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
     if (!ok) give_up();
   } else if (warp == kIssuer) {
     // ---- products --------------------------------------------------------------
-    if (lane == 0 && n_units > 0) {
+    // The whole warp walks and waits, so that what describes the products is uniform; one lane issues them.
+    if (n_units > 0) {
+      const bool leader = one_lane();
       bool ok = true;
       uint32_t acts[2] = {0, 0}, segs[2] = {0, 0};  // scores and segments of each row tile so far
       ChunkCursor cur;
@@ -396,60 +408,67 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       const uint64_t v_desc = desc_mn128(smem_u32(v_smem), Geo::kAtom);
       auto scores = [&](int w, int n) {
         const uint64_t qd = q_desc + (w * Geo::kTile >> 4), kd = k_desc + ((n & 1) * Geo::kTile >> 4);
+        if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t at = ((kk >> 2) * Geo::kAtom + 32 * (kk & 3)) >> 4;
-          tc_mma(tmem + 128 * w, qd + at, kd + at, kIdescS, kk ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t at = ((kk >> 2) * Geo::kAtom + 32 * (kk & 3)) >> 4;
+            tc_mma(tmem + 128 * w, qd + at, kd + at, kIdescS, kk ? 1u : 0u);
+          }
+          tc_commit(&s_full[w]);
         }
-        tc_commit(&s_full[w]);
       };
+      auto commit = [&](uint64_t *bar) {
+        if (leader) tc_commit(bar);
+      };
+      auto wait = [&](uint64_t *bar, uint32_t phase) { return __all_sync(0xffffffffu, chunk_wait(bar, phase, &s_stop)) != 0; };
       for (int n = 0; n < n_units && ok;) {
         const int units = min(cur.t.nt - cur.unit, n_units - n);
         const int2 see[2] = {cur.sees(a, 0, units), cur.sees(a, 1, units)};
         // A new segment's scores wait for its queries, which come after both groups have their outputs: not before both
         // groups' products are issued.  K and V of every unit are waited for: phases are told apart by parity
-        ok = chunk_wait(&k_full[n & 1], (n >> 1) & 1, &s_stop);
+        ok = wait(&k_full[n & 1], (n >> 1) & 1);
 #pragma unroll
         for (int w = 0; w < 2; ++w)
           if (ok && see[w].x == 0 && see[w].y > 0) {
-            ok = chunk_wait(&q_full[w], segs[w]++ & 1, &s_stop);
+            ok = wait(&q_full[w], segs[w]++ & 1);
             tc_fence_after();
             if (ok) scores(w, n);
           }
-        tc_commit(&k_empty[n & 1]);
+        commit(&k_empty[n & 1]);
         for (int i = 0; i < units && ok; ++i, ++n) {
           const bool more = i + 1 < units;
-          ok = chunk_wait(&v_full[n & 1], (n >> 1) & 1, &s_stop);
+          ok = wait(&v_full[n & 1], (n >> 1) & 1);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             if (ok && i >= see[w].x && i < see[w].y) {
-              ok = chunk_wait(&p_full[w], acts[w]++ & 1, &s_stop);
+              ok = wait(&p_full[w], acts[w]++ & 1);
               tc_fence_after();
-              if (ok) {
-                const uint64_t vd = v_desc + ((n & 1) * Geo::kTile >> 4);
+              const uint64_t vd = v_desc + ((n & 1) * Geo::kTile >> 4);
+              const uint32_t more_than_one = i > see[w].x;
+              if (ok && leader) {
 #pragma unroll
                 for (int kk = 0; kk < kTilePos / 16; ++kk)
-                  tc_mma_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, vd + (2048 * kk >> 4), idesc_o<D>(), kk || i > see[w].x ? 1u : 0u);
+                  tc_mma_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, vd + (2048 * kk >> 4), idesc_o<D>(), kk ? 1u : more_than_one);
               }
             }
             if (!more) {
-              if (ok && see[w].y > 0) tc_commit(&o_full[w]);
+              if (ok && see[w].y > 0) commit(&o_full[w]);
             } else if (ok) {
-              if (w == 0) ok = chunk_wait(&k_full[(n + 1) & 1], ((n + 1) >> 1) & 1, &s_stop);
+              if (w == 0) ok = wait(&k_full[(n + 1) & 1], ((n + 1) >> 1) & 1);
               if (ok && i + 1 >= see[w].x && i + 1 < see[w].y) {
-                if (i + 1 == see[w].x) ok = chunk_wait(&q_full[w], segs[w]++ & 1, &s_stop);
+                if (i + 1 == see[w].x) ok = wait(&q_full[w], segs[w]++ & 1);
                 tc_fence_after();
                 if (ok) scores(w, n + 1);
               }
             }
           }
-          tc_commit(&v_empty[n & 1]);
-          if (more) tc_commit(&k_empty[(n + 1) & 1]);
+          commit(&v_empty[n & 1]);
+          if (more) commit(&k_empty[(n + 1) & 1]);
         }
         cur.skip(a, bt, units);
       }
       if (!ok) give_up();
-      tc_commit(&mma_done);  // every product has ended before the block moves on
+      commit(&mma_done);  // every product has ended before the block moves on
       if (!chunk_wait(&mma_done, 0, &s_stop) && !mbar_wait(&mma_done, 0)) give_up();
     }
   } else if (warp < (kSoftmaxThreads >> 5)) {
