@@ -44,7 +44,7 @@ constexpr int kConverterWarps = 4;
 constexpr int kChunkThreads = kSoftmaxThreads + 32 * kConverterWarps + 32;
 constexpr int kScaleSlots = 4;    // the scales of a tile stay until both softmax groups are past it
 constexpr int kWholeChunks = 2;   // items of at most this many units are not split
-constexpr int kMergeParts = 8;
+constexpr int kMergeParts = 16;
 
 template <int D>
 struct ChunkGeom {
@@ -97,12 +97,18 @@ __device__ __forceinline__ void tmem_ask32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ask16(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16_nowait(addr, r); }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
   uint32_t r[32];
   tmem_ask32(addr, r);
   tmem_wait_ld();
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -496,29 +502,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       if (any && ok) {
         // the queries: a power of two times f16, and a NaN in cs where the row has a value that is not finite
         const XT *src = static_cast<const XT *>(a.q) + (live ? token * a.q_row + head * a.q_head : 0);
+        Quad<XT> x[D / 4];
+#pragma unroll
+        for (int d = 0; d < D / 4; ++d) x[d].load(src + 4 * d, a.q_vec, live);
         float big = 0.f, bad = 0.f;
-#pragma unroll 8
-        for (int d = 0; d < D; d += 4) {
-          Quad<XT> x;
-          x.load(src + d, a.q_vec, live);
+#pragma unroll
+        for (int d = 0; d < D / 4; ++d)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            big = fmaxf(big, fabsf(x.get(j)));
-            bad = fmaf(x.get(j), 0.f, bad);
+            big = fmaxf(big, fabsf(x[d].get(j)));
+            bad = fmaf(x[d].get(j), 0.f, bad);
           }
-        }
         const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
         const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
         cs = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
         unsigned char *row = q_smem + w * Geo::kTile + r * 128;
-#pragma unroll 4
+#pragma unroll
         for (int d = 0; d < D; d += 8) {
-          Quad<XT> x, y;
-          x.load(src + d, a.q_vec, live);
-          y.load(src + d + 4, a.q_vec, live);
-          const uint4 f = make_uint4(pack_f16(x.get(0) * down, x.get(1) * down), pack_f16(x.get(2) * down, x.get(3) * down),
-                                     pack_f16(y.get(0) * down, y.get(1) * down), pack_f16(y.get(2) * down, y.get(3) * down));
-          *reinterpret_cast<uint4 *>(row + (d >> 6) * Geo::kAtom + ((((d & 63) >> 3) ^ (r & 7)) << 4)) = f;
+          const Quad<XT> &y = x[d / 4], &z = x[d / 4 + 1];
+          *reinterpret_cast<uint4 *>(row + (d >> 6) * Geo::kAtom + ((((d & 63) >> 3) ^ (r & 7)) << 4)) =
+              make_uint4(pack_f16(y.get(0) * down, y.get(1) * down), pack_f16(y.get(2) * down, y.get(3) * down),
+                         pack_f16(z.get(0) * down, z.get(1) * down), pack_f16(z.get(2) * down, z.get(3) * down));
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -535,37 +539,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         const float *slot = scales + (n % kScaleSlots) * (2 * kSlices + 4);
         const uint32_t there4 = *reinterpret_cast<const uint32_t *>(slot + 2 * kSlices);  // two bits a byte
         const bool whole = p0 + kTilePos - 1 <= first_pos && (a.window <= 0 || p0 > last_pos - a.window) && there4 == 0x03030303u;
-        // bit j: whether this row sees column 32 c + j
+        // bit j: whether this row sees column 16 c + j
         auto seen = [&](int c) -> uint32_t {
-          const int n = lim - (p0 + 32 * c) + 1;  // columns up to the row's own position
-          uint32_t v = n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+          const int n = lim - (p0 + 16 * c) + 1;  // columns up to the row's own position
+          uint32_t v = n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1;
           if (a.window > 0) {
             const int k = n - a.window;  // columns before the window
-            v = k <= 0 ? v : k >= 32 ? 0u : v & (~0u << k);
+            v = k <= 0 ? v : k >= 16 ? 0u : v & (~0u << k);
           }
-          const uint32_t two = there4 >> (8 * c);
-          return v & (((two & 1) ? 0xffffu : 0u) | ((two & 2) ? 0xffff0000u : 0u));
+          return (there4 >> (8 * (c >> 1) + (c & 1)) & 1) ? v : 0u;
         };
         // the largest weight x value scale, by exponent
         float top = kNone;
+        auto top_of = [&](const float (&s)[16], int c) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = fmaxf(s[j], s[j + 8]);
+          const float m4 = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+          const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(slot[kSlices + c]) >> 23) - 127, -90));
+          if (m4 != -INFINITY) top = fmaxf(top, fmaf(m4, cs * slot[c], ev));
+        };
+        if (whole) {  // a slice's scores are asked for while the one before is worked on
+          uint32_t x[2][16];
+          tmem_ask16(s_at, x[0]);
+#pragma unroll
+          for (int c = 0; c < kSlices; ++c) {
+            tmem_wait_ld();
+            if (c + 1 < kSlices) tmem_ask16(s_at + 16 * (c + 1), x[(c + 1) & 1]);
+            float s[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(x[c & 1][j]);
+            top_of(s, c);
+          }
+        } else {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float s[32];
-          tmem_ld32(s_at + 32 * c, s);
-          if (!whole) {
+          for (int c = 0; c < kSlices; ++c) {
+            float s[16];
+            tmem_ld16(s_at + 16 * c, s);
             const uint32_t v = seen(c);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s[j] = (v >> j & 1) ? s[j] : -INFINITY;
-          }
-          const float2 ks = *reinterpret_cast<const float2 *>(slot + 2 * c), vs = *reinterpret_cast<const float2 *>(slot + kSlices + 2 * c);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mx[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mx[j] = fmaxf(fmaxf(s[16 * h + j], s[16 * h + 4 + j]), fmaxf(s[16 * h + 8 + j], s[16 * h + 12 + j]));
-            const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(h ? vs.y : vs.x) >> 23) - 127, -90));
-            if (m4 != -INFINITY) top = fmaxf(top, fmaf(m4, cs * (h ? ks.y : ks.x), ev));
+            for (int j = 0; j < 16; ++j) s[j] = (v >> j & 1) ? s[j] : -INFINITY;
+            top_of(s, c);
           }
         }
         if (__any_sync(0xffffffffu, top > m + kLazy)) {
@@ -588,35 +602,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
             }
           }
         }
-        float sum[2] = {0.f, 0.f};
+        // The weights take the place of scores that have been read: 8 columns a slice, the scores 16 columns ahead of them.
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (whole) {
+          uint32_t x[2][16];
+          tmem_ask16(s_at, x[0]);
+#pragma unroll
+          for (int c = 0; c < kSlices; ++c) {
+            tmem_wait_ld();
+            if (c + 1 < kSlices) tmem_ask16(s_at + 16 * (c + 1), x[(c + 1) & 1]);
+            const float k = cs * slot[c], vsc = slot[kSlices + c];
+            uint32_t f[8];
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float p = exp2_fast(fmaf(__uint_as_float(x[c & 1][j]), k, -m));
+              const float q = exp2_fast(fmaf(__uint_as_float(x[c & 1][j + 1]), k, -m));
+              sum[j & 2] += p;
+              sum[(j & 2) + 1] += q;
+              f[j / 2] = pack_f16(p * vsc, q * vsc);
+            }
+            tmem_st8(s_at + 8 * c, f);
+          }
+        } else {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float s[32];
-          uint32_t f[16];
-          tmem_ld32(s_at + 32 * c, s);
-          const float2 ks = *reinterpret_cast<const float2 *>(slot + 2 * c), vs = *reinterpret_cast<const float2 *>(slot + kSlices + 2 * c);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = exp2_fast(fmaf(s[j], cs * (j < 16 ? ks.x : ks.y), -m));
-          if (!whole) {
+          for (int c = 0; c < kSlices; ++c) {
+            float s[16];
+            tmem_ld16(s_at + 16 * c, s);
+            const float k = cs * slot[c], vsc = slot[kSlices + c];
             const uint32_t v = seen(c);
+            uint32_t f[8];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s[j] = (v >> j & 1) ? s[j] : 0.f;
+            for (int j = 0; j < 16; j += 2) {  // a scale that a row does not see may be anything
+              const float p = (v >> j & 1) ? exp2_fast(fmaf(s[j], k, -m)) : 0.f;
+              const float q = (v >> j & 2) ? exp2_fast(fmaf(s[j + 1], k, -m)) : 0.f;
+              sum[0] += p;
+              sum[1] += q;
+              f[j / 2] = pack_f16((v >> j & 1) ? p * vsc : 0.f, (v >> j & 2) ? q * vsc : 0.f);
+            }
+            tmem_st8(s_at + 8 * c, f);
           }
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            sum[0] += s[j];
-            sum[1] += s[j + 1];
-            const float v = j < 16 ? vs.x : vs.y;
-            f[j / 2] = pack_f16(s[j] * v, s[j + 1] * v);
-          }
-          if (!whole) {  // a value scale that a row does not see may be anything
-            const uint32_t v = seen(c);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] &= ((v >> (2 * j) & 1) ? 0xffffu : 0u) | ((v >> (2 * j) & 2) ? 0xffff0000u : 0u);
-          }
-          tmem_st16(s_at + 16 * c, f);
         }
-        l += sum[0] + sum[1];
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         opened = true;
         tmem_wait_st();
         tc_fence_before();
