@@ -875,7 +875,8 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
                        lse,  scale, window, h->part, h->ticket, log2i(h->g.P), log2i(h->g.t),
                        (h->g.G & (h->g.G - 1)) == 0 ? log2i(h->g.G) : -1,
                        rows_aligned(q, q_row_stride, q_head_stride, dtype),
-                       rows_aligned(out, out_row_stride, out_head_stride, dtype), h->err_word};
+                       rows_aligned(out, out_row_stride, out_head_stride, dtype),
+                       aligned16(out) && out_row_stride % 8 == 0 && out_head_stride % 8 == 0, h->err_word};
     const auto st = static_cast<cudaStream_t>(stream);
     // Many rows per kv head: every cached value meets all of them, and the products bound the call, so they go to the
     // 128-row tensor tiles; measured on 4 requests of 32 / 8 heads over 4,096 positions, FIGURES

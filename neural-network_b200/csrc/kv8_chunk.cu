@@ -44,7 +44,7 @@ constexpr int kConverterWarps = 4;
 constexpr int kChunkThreads = kSoftmaxThreads + 32 * kConverterWarps + 32;
 constexpr int kScaleSlots = 4;    // the scales of a tile stay until both softmax groups are past it
 constexpr int kWholeChunks = 2;   // items of at most this many units are not split
-constexpr int kMergeParts = 16;
+constexpr int kMergeParts = 8;
 
 template <int D>
 struct ChunkGeom {
@@ -56,8 +56,10 @@ struct ChunkGeom {
   static constexpr int kPart = kItemRows * (D + 2);     // floats of a partial result
 };
 
-// kind::f16, D fp32, A and B f16, M = 128.  S: A and B K-major, N = 128.  O: A from tensor memory, B (V) MN-major, N = D.
-constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kTilePos >> 3) << 17) | (8u << 24);
+constexpr int kHalfPos = kTilePos / 2;  // positions of a step of the softmax
+
+// kind::f16, D fp32, A and B f16, M = 128.  S: A and B K-major, N = 64.  O: A from tensor memory, B (V) MN-major, N = D.
+constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kHalfPos >> 3) << 17) | (8u << 24);
 template <int D>
 constexpr uint32_t idesc_o() {
   return (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
@@ -233,10 +235,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
   bt.q = bt.q0 + a.b.B;
   bt.len = bt.q + a.b.B;
   __shared__ long long red[kChunkThreads / 32];
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], q_full[2], o_full[2], mma_done;
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2],
+      q_full[2], o_full[2], mma_done;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_stop;
   __shared__ int s_last;
+  __shared__ float row_scale[kItemRows];
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   constexpr int kIssuer = (kSoftmaxThreads >> 5) + kConverterWarps;
 
@@ -250,8 +254,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], kConverterWarps);
       mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s_full[i][h], 1);
+        mbar_init(&p_full[i][h], 4);
+      }
+      mbar_init(&pv_done[i], 1);
       mbar_init(&q_full[i], 4);
       mbar_init(&o_full[i], 1);
     }
@@ -406,21 +413,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
     if (n_units > 0) {
       const bool leader = one_lane();
       bool ok = true;
-      uint32_t acts[2] = {0, 0}, segs[2] = {0, 0};  // scores and segments of each row tile so far
+      uint32_t acts[2] = {0, 0}, segs[2] = {0, 0};  // units and segments of each row tile so far
       ChunkCursor cur;
       cur.seek(a, bt, u0);
       // descriptors hold addresses in 16-byte units in their low bits: offsets are added there
       const uint64_t q_desc = umma_desc_k128(smem_u32(q_smem)), k_desc = umma_desc_k128(smem_u32(k_smem));
       const uint64_t v_desc = desc_mn128(smem_u32(v_smem), Geo::kAtom);
-      auto scores = [&](int w, int n) {
-        const uint64_t qd = q_desc + (w * Geo::kTile >> 4), kd = k_desc + ((n & 1) * Geo::kTile >> 4);
+      auto scores = [&](int w, int h, int n) {  // of half h of unit n
+        const uint64_t qd = q_desc + (w * Geo::kTile >> 4), kd = k_desc + (((n & 1) * Geo::kTile + h * kHalfPos * 128) >> 4);
         if (leader) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t at = ((kk >> 2) * Geo::kAtom + 32 * (kk & 3)) >> 4;
-            tc_mma(tmem + 128 * w, qd + at, kd + at, kIdescS, kk ? 1u : 0u);
+            tc_mma(tmem + 128 * w + kHalfPos * h, qd + at, kd + at, kIdescS, kk ? 1u : 0u);
           }
-          tc_commit(&s_full[w]);
+          tc_commit(&s_full[w][h]);
         }
       };
       auto commit = [&](uint64_t *bar) {
@@ -433,40 +440,49 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         // A new segment's scores wait for its queries, which come after both groups have their outputs: not before both
         // groups' products are issued.  K and V of every unit are waited for: phases are told apart by parity
         ok = wait(&k_full[n & 1], (n >> 1) & 1);
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < 2; ++w)
-          if (ok && see[w].x == 0 && see[w].y > 0) {
-            ok = wait(&q_full[w], segs[w]++ & 1);
+          if (ok && (w ? see[1].x : see[0].x) == 0 && (w ? see[1].y : see[0].y) > 0) {
+            ok = wait(&q_full[w], (w ? segs[1]++ : segs[0]++) & 1);
             tc_fence_after();
-            if (ok) scores(w, n);
+            if (ok) {
+              scores(w, 0, n);
+              scores(w, 1, n);
+            }
           }
         commit(&k_empty[n & 1]);
         for (int i = 0; i < units && ok; ++i, ++n) {
           const bool more = i + 1 < units;
           ok = wait(&v_full[n & 1], (n >> 1) & 1);
+          if (ok && more) ok = wait(&k_full[(n + 1) & 1], ((n + 1) >> 1) & 1);
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+            for (int w = 0; w < 2; ++w) {
+              const bool here = i >= (w ? see[1].x : see[0].x) && i < (w ? see[1].y : see[0].y);
+              const bool then = more && i + 1 >= (w ? see[1].x : see[0].x) && i + 1 < (w ? see[1].y : see[0].y);
+              if (ok && here) {
+                ok = wait(&p_full[w][h], (w ? acts[1] : acts[0]) & 1);
+                tc_fence_after();
+                const uint64_t vd = v_desc + (((n & 1) * Geo::kTile + h * kHalfPos * 128) >> 4);
+                const uint32_t later = h == 1 || i > (w ? see[1].x : see[0].x);
+                if (ok && leader) {
+#pragma unroll
+                  for (int kk = 0; kk < kHalfPos / 16; ++kk)
+                    tc_mma_ta(tmem + 256 + 128 * w, tmem + 128 * w + kHalfPos * h + 8 * kk, vd + (2048 * kk >> 4), idesc_o<D>(), kk ? 1u : later);
+                  tc_commit(&pv_done[w]);
+                }
+              }
+              if (ok && then) {
+                if (h == 0 && !here) ok = wait(&q_full[w], (w ? segs[1]++ : segs[0]++) & 1);
+                tc_fence_after();
+                if (ok) scores(w, h, n + 1);
+              }
+            }
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            if (ok && i >= see[w].x && i < see[w].y) {
-              ok = wait(&p_full[w], acts[w]++ & 1);
-              tc_fence_after();
-              const uint64_t vd = v_desc + ((n & 1) * Geo::kTile >> 4);
-              const uint32_t more_than_one = i > see[w].x;
-              if (ok && leader) {
-#pragma unroll
-                for (int kk = 0; kk < kTilePos / 16; ++kk)
-                  tc_mma_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, vd + (2048 * kk >> 4), idesc_o<D>(), kk ? 1u : more_than_one);
-              }
-            }
-            if (!more) {
-              if (ok && see[w].y > 0) commit(&o_full[w]);
-            } else if (ok) {
-              if (w == 0) ok = wait(&k_full[(n + 1) & 1], ((n + 1) >> 1) & 1);
-              if (ok && i + 1 >= see[w].x && i + 1 < see[w].y) {
-                if (i + 1 == see[w].x) ok = wait(&q_full[w], segs[w]++ & 1);
-                tc_fence_after();
-                if (ok) scores(w, n + 1);
-              }
-            }
+            if (i >= see[w].x && i < see[w].y) ++acts[w];
+            if (!more && ok && see[w].y > 0) commit(&o_full[w]);
           }
           commit(&v_empty[n & 1]);
           if (more) commit(&k_empty[(n + 1) & 1]);
@@ -482,10 +498,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
     const int w = warp >> 2, r = threadIdx.x & 127, r_item = threadIdx.x;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lanes + 128 * w, o_at = tmem + lanes + 256 + 128 * w;
+    constexpr int kRowLanes = D / 8;  // lanes of a row where a warp goes through its 32 rows together
     ChunkCursor cur;
     if (n_units > 0) cur.seek(a, bt, u0);
     bool ok = true;
-    int n_act = 0, n_seg = 0;
+    int n_act = 0, n_seg = 0, n_pv = 0;
     for (int n = 0; n < n_units;) {
       // the segment: units of the item within this block's share
       const int units = min(cur.t.nt - cur.unit, n_units - n);
@@ -500,30 +517,38 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       const int head = cur.h * a.g.G + at_row.h;
       float m = kNone, l = 0.f, cs = 0.f;
       if (any && ok) {
-        // the queries: a power of two times f16, and a NaN in cs where the row has a value that is not finite
-        const XT *src = static_cast<const XT *>(a.q) + (live ? token * a.q_row + head * a.q_head : 0);
-        Quad<XT> x[D / 4];
+        // the warp's 32 query rows, a run of eight dims a lane: a power of two (a NaN where the row has a value that is not
+        // finite) times f16
+#pragma unroll 4
+        for (int it = 0; it < kRowLanes; ++it) {
+          const int rr = 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes, run = lane % kRowLanes;
+          const bool in = rr < rows;
+          const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + rr);
+          const XT *src = static_cast<const XT *>(a.q) + (in ? (cur.q0 + of.i) * a.q_row + (cur.h * a.g.G + of.h) * a.q_head : 0) + 8 * run;
+          Quad<XT> x[2];
+          x[0].load(src, a.q_vec, in);
+          x[1].load(src + 4, a.q_vec, in);
+          float big = 0.f, bad = 0.f;
 #pragma unroll
-        for (int d = 0; d < D / 4; ++d) x[d].load(src + 4 * d, a.q_vec, live);
-        float big = 0.f, bad = 0.f;
-#pragma unroll
-        for (int d = 0; d < D / 4; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            big = fmaxf(big, fabsf(x[d].get(j)));
-            bad = fmaf(x[d].get(j), 0.f, bad);
+          for (int j = 0; j < 8; ++j) {
+            const float f = x[j >> 2].get(j & 3);
+            big = fmaxf(big, fabsf(f));
+            bad = fmaf(f, 0.f, bad);
           }
-        const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
-        const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
-        cs = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
-        unsigned char *row = q_smem + w * Geo::kTile + r * 128;
 #pragma unroll
-        for (int d = 0; d < D; d += 8) {
-          const Quad<XT> &y = x[d / 4], &z = x[d / 4 + 1];
-          *reinterpret_cast<uint4 *>(row + (d >> 6) * Geo::kAtom + ((((d & 63) >> 3) ^ (r & 7)) << 4)) =
-              make_uint4(pack_f16(y.get(0) * down, y.get(1) * down), pack_f16(y.get(2) * down, y.get(3) * down),
-                         pack_f16(z.get(0) * down, z.get(1) * down), pack_f16(z.get(2) * down, z.get(3) * down));
+          for (int o = kRowLanes / 2; o > 0; o >>= 1) {
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            bad += __shfl_xor_sync(0xffffffffu, bad, o);
+          }
+          const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
+          const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+          if (run == 0) row_scale[kTileRows * w + rr] = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
+          *reinterpret_cast<uint4 *>(q_smem + w * Geo::kTile + (run >> 3) * Geo::kAtom + rr * 128 + (((run & 7) ^ (rr & 7)) << 4)) =
+              make_uint4(pack_f16(x[0].get(0) * down, x[0].get(1) * down), pack_f16(x[0].get(2) * down, x[0].get(3) * down),
+                         pack_f16(x[1].get(0) * down, x[1].get(1) * down), pack_f16(x[1].get(2) * down, x[1].get(3) * down));
         }
+        __syncwarp();
+        cs = row_scale[r_item];
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) chunk_arrive(&q_full[w]);
@@ -532,9 +557,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       for (int i = 0; i < units; ++i, ++n) {
         const int p0 = p_begin + i * kTilePos;
         if (!ok || i < see.x || i >= see.y) continue;
-        ok = chunk_wait(&s_full[w], n_act++ & 1, &s_stop);
+#pragma unroll 1
+        for (int half = 0; half < 2 && ok; ++half) {
+        const int c_half = half * (kSlices / 2);                     // the half's first slice
+        const uint32_t h_at = s_at + kHalfPos * half;
+        ok = chunk_wait(&s_full[w][half], n_act & 1, &s_stop);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) continue;
+        if (!ok) break;
         tc_fence_after();
         const float *slot = scales + (n % kScaleSlots) * (2 * kSlices + 4);
         const uint32_t there4 = *reinterpret_cast<const uint32_t *>(slot + 2 * kSlices);  // two bits a byte
@@ -561,25 +590,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         };
         if (whole) {  // a slice's scores are asked for while the one before is worked on
           uint32_t x[2][16];
-          tmem_ask16(s_at, x[0]);
+          tmem_ask16(h_at, x[0]);
 #pragma unroll
-          for (int c = 0; c < kSlices; ++c) {
+          for (int c = 0; c < kSlices / 2; ++c) {
             tmem_wait_ld();
-            if (c + 1 < kSlices) tmem_ask16(s_at + 16 * (c + 1), x[(c + 1) & 1]);
+            if (c + 1 < kSlices / 2) tmem_ask16(h_at + 16 * (c + 1), x[(c + 1) & 1]);
             float s[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(x[c & 1][j]);
-            top_of(s, c);
+            top_of(s, c_half + c);
           }
         } else {
 #pragma unroll 1
-          for (int c = 0; c < kSlices; ++c) {
+          for (int c = 0; c < kSlices / 2; ++c) {
             float s[16];
-            tmem_ld16(s_at + 16 * c, s);
-            const uint32_t v = seen(c);
+            tmem_ld16(h_at + 16 * c, s);
+            const uint32_t v = seen(c_half + c);
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[j] = (v >> j & 1) ? s[j] : -INFINITY;
-            top_of(s, c);
+            top_of(s, c_half + c);
           }
         }
         if (__any_sync(0xffffffffu, top > m + kLazy)) {
@@ -587,7 +616,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
           const float al = exp2_fast(m - nm);
           m = nm;
           l *= al;
-          if (opened) {  // the products so far have ended: this tile's scores were issued after them
+          if (opened) {  // once the last step's product has ended (those before it have: these scores were issued after them)
+            ok = chunk_wait(&pv_done[w], (n_pv - 1) & 1, &s_stop);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               float o[32];
@@ -606,12 +639,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         if (whole) {
           uint32_t x[2][16];
-          tmem_ask16(s_at, x[0]);
+          tmem_ask16(h_at, x[0]);
 #pragma unroll
-          for (int c = 0; c < kSlices; ++c) {
+          for (int c = 0; c < kSlices / 2; ++c) {
             tmem_wait_ld();
-            if (c + 1 < kSlices) tmem_ask16(s_at + 16 * (c + 1), x[(c + 1) & 1]);
-            const float k = cs * slot[c], vsc = slot[kSlices + c];
+            if (c + 1 < kSlices / 2) tmem_ask16(h_at + 16 * (c + 1), x[(c + 1) & 1]);
+            const float k = cs * slot[c_half + c], vsc = slot[kSlices + c_half + c];
             uint32_t f[8];
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
@@ -621,15 +654,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
               sum[(j & 2) + 1] += q;
               f[j / 2] = pack_f16(p * vsc, q * vsc);
             }
-            tmem_st8(s_at + 8 * c, f);
+            tmem_st8(h_at + 8 * c, f);
           }
         } else {
 #pragma unroll 1
-          for (int c = 0; c < kSlices; ++c) {
+          for (int c = 0; c < kSlices / 2; ++c) {
             float s[16];
-            tmem_ld16(s_at + 16 * c, s);
-            const float k = cs * slot[c], vsc = slot[kSlices + c];
-            const uint32_t v = seen(c);
+            tmem_ld16(h_at + 16 * c, s);
+            const float k = cs * slot[c_half + c], vsc = slot[kSlices + c_half + c];
+            const uint32_t v = seen(c_half + c);
             uint32_t f[8];
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {  // a scale that a row does not see may be anything
@@ -639,7 +672,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
               sum[1] += q;
               f[j / 2] = pack_f16((v >> j & 1) ? p * vsc : 0.f, (v >> j & 2) ? q * vsc : 0.f);
             }
-            tmem_st8(s_at + 8 * c, f);
+            tmem_st8(h_at + 8 * c, f);
           }
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -647,7 +680,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) chunk_arrive(&p_full[w]);
+        if (lane == 0) chunk_arrive(&p_full[w][half]);
+        ++n_pv;
+        }
+        ++n_act;
       }
       // ---- end of the segment -------------------------------------------------------
       if (any && ok) {
@@ -666,7 +702,37 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       }
       const long long i0 = u0 + (n - units) - cur.unit, i1 = i0 + cur.t.nt;
       const bool all = i0 >= u0 && i1 <= u1;
-      XT *dst = static_cast<XT *>(a.out) + (live ? token * a.o_row + head * a.o_head : 0);
+      // outputs leave through the query tile of the warp's rows, whose products have ended, so that a row is written by
+      // neighbouring lanes
+      unsigned char *stage = q_smem + w * Geo::kTile;
+      auto put = [&](int run, const float (&v)[8]) {
+        uint32_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          x[j] = *reinterpret_cast<const uint32_t *>(&t);
+        }
+        *reinterpret_cast<uint4 *>(stage + r * (2 * D) + ((run ^ (r & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+      };
+      auto flush = [&]() {
+        __syncwarp();
+#pragma unroll 4
+        for (int it = 0; it < kRowLanes; ++it) {
+          const int rr = 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes, run = lane % kRowLanes;
+          if (rr >= rows) continue;
+          const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + rr);
+          const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * (2 * D) + ((run ^ (rr & 7)) << 4));
+          XT *dst = static_cast<XT *>(a.out) + (cur.q0 + of.i) * a.o_row + (cur.h * a.g.G + of.h) * a.o_head + 8 * run;
+          if (a.o_vec8) {
+            *reinterpret_cast<uint4 *>(dst) = v;
+          } else {
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) reinterpret_cast<unsigned short *>(dst)[j] = static_cast<unsigned short>(x[j >> 1] >> (16 * (j & 1)));
+          }
+        }
+        __syncwarp();
+      };
       auto finish = [&](float lsum, float top) {
         if (live && a.lse) a.lse[token * a.g.H + head] = lsum == 0.f ? -INFINITY : logf(lsum) + top * kLn2;
         return lsum == 0.f ? 0.f : __fdividef(1.f, lsum);  // 0: the row saw nothing
@@ -683,13 +749,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
           for (int j = 0; j < 32; ++j) o[j] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          // a row of the tile that saw nothing has weights of 0 only
-          const float4 v = make_float4(o[j] * inv, o[j + 1] * inv, o[j + 2] * inv, o[j + 3] * inv);
-          if (!all) part[(8 * c + j / 4) * kItemRows + r_item] = v;
-          else if (live) store4(dst + 32 * c + j, a.o_vec, v);
+        for (int j = 0; j < 32; j += 8) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = o[j + k] * inv;
+          if (all) {
+            put(4 * c + j / 8, v);
+          } else {
+            part[(8 * c + j / 4) * kItemRows + r_item] = make_float4(v[0], v[1], v[2], v[3]);
+            part[(8 * c + j / 4 + 1) * kItemRows + r_item] = make_float4(v[4], v[5], v[6], v[7]);
+          }
         }
       }
+      if (all) flush();
       if (!all) {
         float *ml = reinterpret_cast<float *>(part) + kItemRows * D;
         ml[r_item] = m;
@@ -724,9 +796,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
               }
             }
 #pragma unroll
-            for (int j = 0; j < kMergeParts; ++j)
-              if (live) store4(dst + 4 * (d + j), a.o_vec, v[j]);
+            for (int j = 0; j < kMergeParts; j += 2) {
+              const float y[8] = {v[j].x, v[j].y, v[j].z, v[j].w, v[j + 1].x, v[j + 1].y, v[j + 1].z, v[j + 1].w};
+              put((d + j) / 2, y);
+            }
           }
+          flush();
           asm volatile("bar.sync 1, 256;" ::: "memory");
           if (threadIdx.x == 0) a.ticket[c0] = 0;
         }
