@@ -45,7 +45,8 @@ constexpr int kStep = 2;                              // slices a warp takes at 
 constexpr int kUnit = kSlice * kStep * kDecWarps;     // positions of a unit
 constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: registers
 constexpr int kWholeItems = 4;                        // items of at most this many units are not split
-constexpr int kChunkRows = 32;                        // rows of a kv head above which the tensor tiles are faster
+constexpr int kChunkRows = 64;                        // rows of a kv head from which the tensor tiles are faster,
+constexpr int kChunkUnits = 24;                       // given at least this many units of this kernel's for each block
 constexpr int kMergeAhead = 8;                        // partial results read at once
 template <int D, int NT>
 struct DecGeom {
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       bool grow = false;
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
-        fev[i] = static_cast<float>(max(static_cast<int>(__float_as_uint(vsc[i]) >> 23) - 127, -90));
+        fev[i] = static_cast<float>(max(static_cast<int>(__float_as_uint(vsc[i]) >> 23 & 0xff) - 127, -90));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -573,7 +574,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
           for (int j = 0; j < 4; ++j) {
             const float p = exp2_fast(x[i][n][j]);
             l[n][j & 1] += p;
-            w[j] = p * vsc[i];
+            // a scale that is not finite reaches only the rows that see its slice
+            w[j] = whole || x[i][n][j] != -INFINITY ? p * vsc[i] : 0.f;
           }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
@@ -878,9 +880,17 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
                        rows_aligned(out, out_row_stride, out_head_stride, dtype),
                        aligned16(out) && out_row_stride % 8 == 0 && out_head_stride % 8 == 0, h->err_word};
     const auto st = static_cast<cudaStream_t>(stream);
-    // Many rows per kv head: every cached value meets all of them, and the products bound the call, so they go to the
-    // 128-row tensor tiles; measured on 4 requests of 32 / 8 heads over 4,096 positions, FIGURES
-    if (dtype == SPECDEC_BF16 && h->g.D >= 64 && b.B <= kChunkMaxBatch && static_cast<long long>(max_q) * h->g.G > kChunkRows) {
+    // Many rows per kv head: every cached value meets all of them and the products bound the call, so they go to the
+    // 128-row tensor tiles, where there is enough of it to pay for those tiles' longer start and merges.  Measured in us,
+    // this kernel / the tensor tiles (heads of 128, 32 requests over 3,080 positions, then 4 over 4,096):
+    //   32 / 8 heads:  48 rows 150 / 185 and 45 / 63,   64 rows 191 / 186 and 47 / 63,   128 rows 355 / 188 and 73 / 63
+    //   32 / 32 heads: 48 rows 521 / 607 and 104 / 115, 64 rows 686 / 604 and 129 / 116, 128 rows 1344 / 605 and 236 / 116
+    //   16 / 2 heads:  64 rows 63 / 69 and 24 / 57,     96 rows 86 / 71 and 32 / 58,     128 rows 106 / 71 and 34 / 58
+    // The units are those that the tables have room for: 21 a block at 16 / 2 heads and 64 rows, 28 at 32 / 8 and 128.
+    const long long row_tiles = (static_cast<long long>(b.T) * h->g.G + 15) / 16;
+    const long long units = row_tiles * h->g.Hkv * ((static_cast<long long>(b.cols) * h->g.P + kUnit - 1) / kUnit);
+    if (dtype == SPECDEC_BF16 && h->g.D >= 64 && b.B <= kChunkMaxBatch && static_cast<long long>(max_q) * h->g.G >= kChunkRows &&
+        units >= static_cast<long long>(kChunkUnits) * dec_ctas(2) * h->num_sms) {
       kv8_chunk_launch(h, a, st);
       return;
     }

@@ -389,7 +389,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       put(k_smem + buf * Geo::kTile, rk);
       float *slot = scales + (n % kScaleSlots) * (2 * kSlices + 4);
       if (lane < 4) slot[(lane & 1) * kSlices + 2 * w + (lane >> 1)] = sc;
-      if (lane == 0) reinterpret_cast<unsigned char *>(slot + 2 * kSlices)[w] = static_cast<unsigned char>(there);
+      const uint32_t below = __ballot_sync(0xffffffffu, lane < 4 && sc < 0.f);  // of bits 0 and 2: key scales below 0
+      if (lane == 0)
+        reinterpret_cast<unsigned char *>(slot + 2 * kSlices)[w] =
+            static_cast<unsigned char>(there | (below & 1) << 2 | (below & 4) << 1);
       publish(&k_full[buf]);
       uint4 keep[kLoads];
 #pragma unroll
@@ -566,7 +569,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         if (!ok) break;
         tc_fence_after();
         const float *slot = scales + (n % kScaleSlots) * (2 * kSlices + 4);
-        const uint32_t there4 = *reinterpret_cast<const uint32_t *>(slot + 2 * kSlices);  // two bits a byte
+        const uint32_t there4 = *reinterpret_cast<const uint32_t *>(slot + 2 * kSlices);  // a byte for two slices: bits 0, 1 there,
+                                                                                          // bits 2, 3 a key scale below 0
         const bool whole = p0 + kTilePos - 1 <= first_pos && (a.window <= 0 || p0 > last_pos - a.window) && there4 == 0x03030303u;
         // bit j: whether this row sees column 16 c + j
         auto seen = [&](int c) -> uint32_t {
@@ -585,8 +589,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = fmaxf(s[j], s[j + 8]);
           const float m4 = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-          const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(slot[kSlices + c]) >> 23) - 127, -90));
-          if (m4 != -INFINITY) top = fmaxf(top, fmaf(m4, cs * slot[c], ev));
+          const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(slot[kSlices + c]) >> 23 & 0xff) - 127, -90));
+          if (m4 != -INFINITY) top = fmaxf(top, fmaf(m4, cs * fabsf(slot[c]), ev));
         };
         if (whole) {  // a slice's scores are asked for while the one before is worked on
           uint32_t x[2][16];
@@ -606,9 +610,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
             float s[16];
             tmem_ld16(h_at + 16 * c, s);
             const uint32_t v = seen(c_half + c);
+            const int slice = c_half + c;
+            const float sign = there4 >> (8 * (slice >> 1) + 2 + (slice & 1)) & 1 ? -1.f : 1.f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) s[j] = (v >> j & 1) ? s[j] : -INFINITY;
-            top_of(s, c_half + c);
+            for (int j = 0; j < 16; ++j) s[j] = (v >> j & 1) ? s[j] * sign : -INFINITY;
+            top_of(s, slice);
           }
         }
         if (__any_sync(0xffffffffu, top > m + kLazy)) {

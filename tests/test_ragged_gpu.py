@@ -368,6 +368,96 @@ def test_attend_one_handle_many_sizes_and_repeats(gpu_lib):
                 assert np.array_equal(got[0], was[0]) and np.array_equal(got[1], was[1])
 
 
+TILES = [  # heads, kv heads, dim, page, block, q per request, lengths, window
+    (8, 2, 128, 128, 64, [70, 33, 1, 0], [70, 400, 513, 9], 0),
+    (2, 1, 64, 128, 64, [150], [150], 0),
+    (4, 2, 128, 128, 16, [1, 5, 40], [500, 260, 300], 33),
+    (4, 4, 64, 64, 16, [1, 130], [130, 200], 1),
+    (6, 2, 128, 16, 16, [100, 7, 86], [100, 290, 129], 0),
+    (5, 1, 64, 32, 32, [51, 52, 3], [640, 52, 3], 200),
+    (4, 1, 128, 64, 32, [65, 1, 64], [193, 1, 64], 0),
+    (2, 2, 128, 128, 128, [300, 257], [1000, 257], 129),
+    (16, 1, 64, 16, 16, [3, 17], [40, 17], 0),
+]
+WIDE = 8000  # columns of tables with room for far more than there is, as for the longest request that may come
+
+
+@pytest.mark.parametrize("shape", range(len(TILES)))
+def test_attend_many_rows_and_wide_tables(gpu_lib, shape):
+    H, Hkv, D, P, t, q, lens, window = TILES[shape]
+    rng = np.random.default_rng(200 + shape)
+    table, n_pages = make_table(rng, lens, P, spare_cols=WIDE)
+    cache = poison(make_cache(rng, n_pages, Hkv, P, D, t), table, lens, P, t)
+    cuq = np.concatenate([[0], np.cumsum(q)])
+    x = np.asarray(torch.tensor(rng.normal(0, 1, (sum(q), H, D))).bfloat16().float())
+    scale = 1 / math.sqrt(D)
+    want = ref.attend(x, *cache, table, lens, cuq, P, t, scale, window)
+    h = sd.KV8(H, Hkv, D, page_tokens=P, block_tokens=t, max_batch=len(lens))
+    got = run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", scale, window, max_q=500, handle=h)
+    check_attend(*got, *want, "bf16")
+    other = run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", scale, window, max_q=500, q_pad=3, out_pad=5,
+                       stream=torch.cuda.Stream(), handle=h)
+    check_attend(*other, *want, "bf16")
+    again = run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", scale, window, max_q=500, lse=False, handle=h)
+    assert np.array_equal(again[0], got[0])
+    h.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("spare,max_q", [(1, 1), (1, 9), (WIDE, 500)])
+def test_attend_a_bad_block_reaches_only_the_rows_that_see_it(gpu_lib, dtype, spare, max_q):
+    # the last row's own position opens a block: its scales, or its query, are not finite
+    H, Hkv, D, P, t = 8, 2, 128, 128, 16
+    rng = np.random.default_rng(12)
+    lens, q = [17, 145, 641, 33], [2, 5, 1, 1]
+    table, n_pages = make_table(rng, lens, P, spare_cols=spare)
+    k, v, ks, vs = make_cache(rng, n_pages, Hkv, P, D, t)
+    cuq = np.concatenate([[0], np.cumsum(q)])
+    x = np.asarray(torch.tensor(rng.normal(0, 1, (sum(q), H, D))).to(DT[dtype]).float())
+    clean = ref.attend(x, k, v, ks, vs, table, lens, cuq, P, t, 0.0884, 0)
+    sound = np.ones(sum(q), bool)
+    for b, (where, bad) in enumerate([(vs, np.nan), (ks, np.nan), (vs, np.inf)]):
+        where[table[b, (lens[b] - 1) // P], :, (lens[b] - 1) % P // t] = bad
+        sound[cuq[b + 1] - 1] = False
+    x[-1, :, 5] = np.nan
+    sound[-1] = False
+    got, lse = run_attend(x, (k, v, ks, vs), table, lens, cuq, H, Hkv, D, P, t, dtype, 0.0884, 0, max_q=max_q)
+    check_attend(got[sound], lse[sound], *(w[sound] for w in clean), dtype)
+    assert not np.isfinite(got[~sound]).any(axis=2).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("spare,max_q", [(1, 3), (WIDE, 500)])
+def test_attend_negative_scales(gpu_lib, dtype, spare, max_q):
+    H, Hkv, D, P, t = 4, 2, 64, 64, 16
+    rng = np.random.default_rng(13)
+    lens, q = [300, 64], [3, 2]
+    table, n_pages = make_table(rng, lens, P, spare_cols=spare)
+    k, v, ks, vs = make_cache(rng, n_pages, Hkv, P, D, t)
+    ks *= rng.choice([-1, 1], ks.shape).astype(np.float32)
+    vs *= rng.choice([-1, 1], vs.shape).astype(np.float32)
+    cuq = np.concatenate([[0], np.cumsum(q)])
+    x = np.asarray(torch.tensor(rng.normal(0, 1, (sum(q), H, D))).to(DT[dtype]).float())
+    for scale in (0.125, -0.125):
+        want = ref.attend(x, k, v, ks, vs, table, lens, cuq, P, t, scale, 0)
+        got = run_attend(x, (k, v, ks, vs), table, lens, cuq, H, Hkv, D, P, t, dtype, scale, 0, max_q=max_q)
+        check_attend(*got, *want, dtype)
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_attend_over_a_thousand_requests(gpu_lib, max_q):
+    H, Hkv, D, P, t = 4, 2, 64, 16, 16
+    B = 1100
+    rng = np.random.default_rng(14)
+    lens, q = rng.integers(0, 40, B), rng.integers(0, 3, B)
+    table, n_pages = make_table(rng, lens, P, spare_cols=20)
+    cache = make_cache(rng, n_pages, Hkv, P, D, t)
+    cuq = np.concatenate([[0], np.cumsum(q)])
+    x = np.asarray(torch.tensor(rng.normal(0, 1, (int(cuq[-1]), H, D))).bfloat16().float())
+    want = ref.attend(x, *cache, table, lens, cuq, P, t, 0.125, 0)
+    check_attend(*run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", 0.125, 0, max_q=max_q), *want, "bf16")
+
+
 @pytest.mark.parametrize("max_q", [1, 64])
 def test_cache_past_32_bit_offsets(gpu_lib, max_q):
     # a pool of over 2^31 codes; the request lives in its last pages
