@@ -3,7 +3,8 @@
 ``KV8.attend`` and ``sample``.  include/specdec.h has their definitions.
 
 Buffers are CUDA tensors: any object with ``data_ptr()``, ``shape``,
-``stride()``, ``dtype``, ``is_cuda`` and ``is_contiguous()``, as torch's are.
+``stride()``, ``dtype``, ``is_cuda``, ``get_device()`` and ``is_contiguous()``,
+as torch's are, on the device of the cache (``sample``: the current one).
 ``stream`` is a raw cudaStream_t (0: the device's default stream, torch's
 current one unless a caller changed it); tensors must be ready on it.
 Failures raise ``SpecDecError`` (a RuntimeError), wrong arguments before the
@@ -48,6 +49,13 @@ def _optional(t, name: str, dtype: str, shape=None):
     return None if t is None else _buffer(t, name, dtype, shape)
 
 
+def _one_device(tensors) -> int:
+    devices = {t.get_device() for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError("the tensors must be on one device")
+    return devices.pop()
+
+
 class KV8Layer:
     """One layer's cache: codes k, v [pages][kv heads][page tokens][head dim]
     int8 and scales [pages][kv heads][blocks of a page] float32."""
@@ -63,6 +71,7 @@ class KV8Layer:
                                     _buffer(v_scale, "v_scale", "float32", k_scale.shape), k.shape[0])
         self.ptr = C.addressof(self.record)
         self._keep = (k, v, k_scale, v_scale)
+        self.device = _one_device(self._keep)
 
 
 class KV8Batch:
@@ -84,11 +93,14 @@ class KV8Batch:
             _optional(status, "status", "int32", (1,)))
         self.ptr = C.addressof(self.record)
         self._keep = (table, kv_len, cu_q, tok_req, tok_pos, slots, status)
+        self.device = _one_device(self._keep)
 
 
-def _rows(t, heads: int, dim: int, name: str):
+def _rows(t, heads: int, dim: int, name: str, device: int):
     """(address, row stride, head stride) of rows [n][heads][dim] with adjacent dims."""
     sh, st = t.shape, t.stride()
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be a tensor of CUDA device {device}")
     if len(sh) != 3 or sh[1] != heads or sh[2] != dim or st[2] != 1:
         raise ValueError(f"{name} must be rows of {heads} heads x {dim} adjacent values, not {tuple(sh)}")
     return t.data_ptr(), st[0], st[1]
@@ -106,7 +118,7 @@ class KV8:
         rc = lib.specdec_kv8_create(C.byref(cfg), device, C.byref(h))
         if rc:
             raise _sd.SpecDecError(rc, lib.specdec_kv8_last_error(None).decode())
-        self._lib, self.h = lib, h
+        self._lib, self.h, self.device = lib, h, device
         self.n_heads, self.n_kv_heads, self.head_dim = n_heads, n_kv_heads, head_dim
         self.page_tokens, self.block_tokens = page_tokens, block_tokens
 
@@ -126,24 +138,31 @@ class KV8:
         if layer.shape[1:] != (self.n_kv_heads, self.page_tokens, self.head_dim) or \
                 layer.blocks * self.block_tokens != self.page_tokens:
             raise ValueError(f"the layer's codes {layer.shape} and {layer.blocks} blocks a page do not fit this handle")
+        if layer.device != self.device:
+            raise ValueError(f"the layer must be on CUDA device {self.device}")
         return layer.ptr
+
+    def _batch(self, batch: KV8Batch) -> int:
+        if batch.device != self.device:
+            raise ValueError(f"the batch must be on CUDA device {self.device}")
+        return batch.ptr
 
     def plan(self, batch: KV8Batch, held, keep, q_len, ring, ring_state, ring_state_out, stream: int = 0) -> None:
         """Pages, lengths, row and slot maps of a step (specdec_kv8_plan)."""
         n = (batch.n_requests,)
         self._check(self._lib.specdec_kv8_plan(
-            self.h, batch.ptr, _buffer(held, "held", "int32", n), _buffer(keep, "keep", "int32", n),
+            self.h, self._batch(batch), _buffer(held, "held", "int32", n), _buffer(keep, "keep", "int32", n),
             _buffer(q_len, "q_len", "int32", n), _buffer(ring, "ring", "int32"), ring.shape[0],
             _buffer(ring_state, "ring_state", "int32", (2,)), _buffer(ring_state_out, "ring_state_out", "int32", (2,)),
             stream or None))
 
     def append(self, layer: KV8Layer, batch: KV8Batch, k, v, stream: int = 0) -> None:
         """Writes rows k, v [rows][kv heads][head dim] to the requests' last positions."""
-        kp, kr, kh = _rows(k, self.n_kv_heads, self.head_dim, "k")
-        vp, vr, vh = _rows(v, self.n_kv_heads, self.head_dim, "v")
+        kp, kr, kh = _rows(k, self.n_kv_heads, self.head_dim, "k", self.device)
+        vp, vr, vh = _rows(v, self.n_kv_heads, self.head_dim, "v", self.device)
         if v.shape[0] != k.shape[0] or v.dtype != k.dtype:
             raise ValueError("k and v must have the same rows and type")
-        self._check(self._lib.specdec_kv8_append(self.h, self._layer(layer), batch.ptr, kp, kr, kh, vp, vr, vh,
+        self._check(self._lib.specdec_kv8_append(self.h, self._layer(layer), self._batch(batch), kp, kr, kh, vp, vr, vh,
                                                  _dtype_of(k), k.shape[0], stream or None))
 
     def gather(self, layer: KV8Layer, rows, out_k=None, out_v=None, stream: int = 0) -> None:
@@ -153,8 +172,9 @@ class KV8:
         outs = [t for t in (out_k, out_v) if t is not None]
         if not outs:
             return
-        if any(t.shape != shape or not t.is_contiguous() or t.dtype != outs[0].dtype for t in outs):
-            raise ValueError(f"outputs must be contiguous, of one type and shape {shape}")
+        if any(t.shape != shape or not t.is_contiguous() or t.dtype != outs[0].dtype or t.get_device() != self.device
+               for t in outs):
+            raise ValueError(f"outputs must be contiguous, on CUDA device {self.device}, of one type and shape {shape}")
         self._check(self._lib.specdec_kv8_gather(
             self.h, self._layer(layer), _buffer(rows, "rows", "int64"), n, None if out_k is None else out_k.data_ptr(),
             None if out_v is None else out_v.data_ptr(), _dtype_of(outs[0]), stream or None))
@@ -163,14 +183,14 @@ class KV8:
                scale: Optional[float] = None, window: int = 0, stream: int = 0) -> None:
         """Attention of q [rows][heads][head dim] over the cache into out (and lse
         [rows][heads] float32); scale defaults to 1 / sqrt(head dim)."""
-        qp, qr, qh = _rows(q, self.n_heads, self.head_dim, "q")
-        op, orow, oh = _rows(out, self.n_heads, self.head_dim, "out")
+        qp, qr, qh = _rows(q, self.n_heads, self.head_dim, "q", self.device)
+        op, orow, oh = _rows(out, self.n_heads, self.head_dim, "out", self.device)
         if out.shape[0] != q.shape[0] or out.dtype != q.dtype:
             raise ValueError("q and out must have the same rows and type")
         lp = None if lse is None else _buffer(lse, "lse", "float32", q.shape[:2])
         self._check(self._lib.specdec_kv8_attend(
-            self.h, self._layer(layer), batch.ptr, qp, qr, qh, _dtype_of(q), q.shape[0], op, orow, oh, lp, max_q,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, stream or None))
+            self.h, self._layer(layer), self._batch(batch), qp, qr, qh, _dtype_of(q), q.shape[0], op, orow, oh, lp,
+            max_q, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, stream or None))
 
     def check(self, stream: int = 0) -> None:
         """Waits for the stream; raises if a wait inside an attend call on it gave up."""
@@ -182,8 +202,10 @@ def sample(logits, u, tokens, probs=None, temperature=None, top_k=None, top_p=No
     """One token per row of logits [rows][vocab] from the uniforms u (specdec_sample):
     tokens int32, probs float32 [rows]; the parameters are [rows] tensors or None."""
     sh, st = logits.shape, logits.stride()
-    if len(sh) != 2 or (st[1] != 1 and sh[1] > 1):
-        raise ValueError("logits must be rows of adjacent values")
+    if len(sh) != 2 or (st[1] != 1 and sh[1] > 1) or not logits.is_cuda:
+        raise ValueError("logits must be rows of adjacent values on a CUDA device")
+    if u.get_device() != logits.get_device() or tokens.get_device() != logits.get_device():
+        raise ValueError("u and tokens must be on the logits' device")
     n = (sh[0],)
     lib = _sd.load_library()
     rc = lib.specdec_sample(

@@ -625,6 +625,54 @@ def test_sample_frequencies(gpu_lib):
 
 
 # ---------------------------------------------------------------------------
+# a step's operators together
+
+@pytest.mark.parametrize("heads,kv_heads,dim,slots,pages", [(8, 2, 64, 4, 13), (4, 4, 32, 7, None)])
+def test_server(gpu_lib, heads, kv_heads, dim, slots, pages):
+    """Greedy requests that share a pool against each request alone in 64 bits without a cache.
+
+    Codes are off by half a step of a block's largest value (about 4 standard deviations / 127), some times over where
+    the scale grows: 0.02 of a value's deviation for keys and values each.  Two layers and the output rows keep that
+    size, so logits (deviation 1) are off by about 0.06 and two of them by 0.4 at most; the gap of the two largest of
+    1,000 logits is 0.3 on average, so most tokens are the largest's own."""
+    from specdec_b200.ragged_demo import Model, Server
+
+    model = Model(heads=heads, kv_heads=kv_heads, dim=dim, dtype=torch.float32)
+    server = Server(model, slots=slots, max_len=256, pages=pages, page_tokens=32, chunk=20)
+    rng = np.random.default_rng(15)
+    prompts = [rng.integers(0, model.vocab, n).tolist() for n in [1, 70, 20, 21, 33, 64, 5, 100, 1, 40]]
+    out = server.serve(prompts, 12, temperature=0.0)
+    n_pages = server.ring.shape[0]
+    head, free = server.state[server.turn].tolist()
+    assert free == n_pages == server.free and sorted(server.ring.tolist()) == list(range(n_pages))
+    double = Model(heads=heads, kv_heads=kv_heads, dim=dim, dtype=torch.float64)
+    for name in ("embed", "wo", "wqkv"):  # the same weights
+        w = getattr(model, name)
+        setattr(double, name, w.double() if name == "embed" else [x.double() for x in w])
+    own = 0
+    for p, o in zip(prompts, out):
+        assert o[:len(p)] == p and len(o) == len(p) + 12
+
+        def attention(layer, q, k, v):
+            n, g = len(q), heads // kv_heads
+            k, v = (t.repeat_interleave(g, 1) for t in (k, v))
+            s = torch.einsum("ihd,jhd->hij", q, k) / math.sqrt(dim)
+            s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+            return torch.einsum("hij,jhd->ihd", s.softmax(2), v)
+
+        ids = torch.tensor(o, device="cuda")
+        logits = double.forward(ids, torch.arange(len(o), device="cuda"), attention)(slice(len(p) - 1, len(o) - 1))
+        took = logits.gather(1, ids[len(p):, None])[:, 0]
+        best = logits.max(1).values
+        assert bool((took >= best - 0.4).all()), float((best - took).max())
+        own += int((took == best).sum())
+    assert own > 12 * len(prompts) / 2
+    # drawn tokens: the same seed gives the same tokens, whatever ran before
+    a, b = (server.serve(prompts[:6], 9, seed=3) for _ in range(2))
+    assert a == b and all(0 <= t < model.vocab for r in a for t in r)
+
+
+# ---------------------------------------------------------------------------
 # refusals
 
 def test_refusals(gpu_lib):
@@ -679,6 +727,20 @@ def test_refusals(gpu_lib):
         sd.sample(l.T, u, tok)
     with pytest.raises(sd.SpecDecError):
         sd.sample(l[:, :0], u, tok)
+    # buffers of the host are never passed on
+    host = torch.zeros(2, 4, 64)
+    with pytest.raises(ValueError):
+        h.attend(layer, batch, host, q)
+    with pytest.raises(ValueError):
+        h.attend(layer, batch, q, host)
+    with pytest.raises(ValueError):
+        h.append(layer, batch, host[:, :2], host[:, :2])
+    with pytest.raises(ValueError):
+        h.gather(layer, torch.zeros(2, dtype=torch.int64, device="cuda"), host[:, :2].contiguous())
+    with pytest.raises(ValueError):
+        sd.sample(l.cpu(), u, tok)
+    with pytest.raises(ValueError):
+        sd.KV8Batch(torch.zeros(2, 1, dtype=torch.int32), i32([5, 7]), i32([0, 1, 2]))
     # calls of nothing are calls
     none = sd.KV8Batch(torch.zeros(0, 1, dtype=torch.int32, device="cuda"), i32([]), i32([0]))
     h.attend(layer, none, q[:0], q[:0])
