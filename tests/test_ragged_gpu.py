@@ -616,6 +616,39 @@ def test_sample_flat_rows(gpu_lib, dtype):
     check_sample(l, u, one, k, p, zero, *run_sample(l, u, one, k, p, zero, dtype))
 
 
+@pytest.mark.parametrize("V,B", [(320000, 2), (1000000, 1), (320000, 101), (70000, 150)])
+def test_sample_nearly_equal_long_rows(gpu_lib, V, B):
+    # weights just below the largest fill one bin with the whole row
+    rng = np.random.default_rng(V)
+    l = rng.uniform(-1e-3, 0, (B, V)).astype(np.float32)
+    l[:, 7] = 1e-3
+    u = rng.random(B).astype(np.float32).clip(0, 1 - 2.0 ** -24)
+    rows = rng.choice(B, min(B, 3), replace=False)
+    one, none = np.ones(B, np.float32), np.zeros(B, np.int64)
+    for k, p in ((none, one * np.float32(0.5)), (none + V // 3, one), (none + V // 2, one * np.float32(0.9)), (none, one)):
+        tok, prob = run_sample(l, u, one, k, p)
+        check_sample(l[rows], u[rows], one, k, p, 0 * one, tok[rows], prob[rows])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V,B,pad", [(2049, 150, 1), (32000, 160, 0), (32003, 149, 5), (131075, 130, 3)])
+def test_sample_many_rows(gpu_lib, dtype, V, B, pad):
+    # a block a row, and rows that each start at another alignment
+    rng = np.random.default_rng(V + B)
+    l = (rng.standard_normal((B, V), np.float32) * 3).astype(np.float32)
+    l[rng.random((B, V), np.float32) < 0.01] = -np.inf
+    l[:, ::97] = 2.25
+    l = np.asarray(torch.tensor(l).to(DT[dtype]).float())
+    u = rng.random(B).astype(np.float32).clip(0, 1 - 2.0 ** -24)
+    T = rng.choice([0, 0.7, 1, 1.3], B).astype(np.float32)
+    k = rng.choice([0, 1, 50, 300, 5000], B)
+    p = rng.choice([0.3, 0.9, 0.99, 1], B).astype(np.float32)
+    m = rng.choice([0, 0, 0.02], B).astype(np.float32)
+    tok, prob = run_sample(l, u, T, k, p, m, dtype, pad)
+    rows = np.concatenate([[0, B - 1], rng.choice(B, 40, replace=False)])
+    check_sample(l[rows], u[rows], T[rows], k[rows], p[rows], m[rows], tok[rows], prob[rows])
+
+
 def test_sample_frequencies(gpu_lib):
     # 4,096 uniforms on a grid draw each token as often as its weight says, within one draw
     p = np.array([0.5, 0.25, 0.125, 0.0625, 0.0625])
