@@ -15,19 +15,33 @@
 //   O^T [16 dims][8 rows]      += V^T codes [16 dims][16 positions] x P^T   f16
 // The queries enter as whole numbers of three bytes (22 bits of the row's
 // largest value), so the K codes need no conversion and the scores' sums are
-// exact; the weights span too many binades for that and enter as f16.
+// exact; the weights span too many binades for that and enter as f16 (11 bits,
+// two of them for fp32 rows), relative to the largest weight x value scale.
 // A slice of 16 positions lies in one page and has one scale pair.  Every
-// warp owns whole slices and a ring of them in shared memory that it fills
+// warp takes two slices a step from a ring in shared memory that it fills
 // itself with 16-byte asynchronous copies (no barrier between warps until the
 // end of an item), converts V codes to f16 in registers, and keeps its running
-// maximum, sum and output; the block's warps take slices in turn and merge at
-// the end of a (request, kv head, row tile) item.
+// maximum, sum and output; the block's warps take steps in turn and merge at
+// the end of a (request, kv head, row tile) item.  A row's maximum moves only
+// when a weight would pass 2^8: most steps rescale nothing.
 //
-// Work is split evenly whatever the lengths are: all items' 64-position units
+// Work is split evenly whatever the lengths are: all items' 128-position units
 // in a row, an equal share of consecutive units per block.  A block that holds
 // part of an item leaves (maximum, sum, unnormalised output) in the workspace
 // and the last of the item's blocks to arrive merges them in block order, so
 // equal calls give equal bits.
+//
+// Measured (bf16 rows, heads of 128, of the measured 6.55 TB/s):
+//   32 requests of up to 3,080 positions, 5 rows, 32 / 32 heads: 97 us, 5.2 TB/s (0.80)
+//   64 requests of up to 4,096, 1 row, 32 / 8 heads:             72 us, 4.8 TB/s (0.73)
+//   2 requests of 131,071, 1 row, 32 / 8 heads:                 101 us, 5.3 TB/s (0.81)
+//   8 requests of up to 100, 1 fp32 row, 4 heads of 64:         8.2 us: latency
+// The copies alone, without products, run the third in 81 us; conversions,
+// softmax and products take issue slots beside them.  On the way (first case / second / third): codes converted for both products 179 /
+// 121 / 178, scores from bytes 127 / 88 / 134, two slices a step 115 /
+// 82 / 113, queries in shared memory instead of
+// registers and one V buffer 97 / 71 / 101 (three blocks a multiprocessor).
+// Four blocks of 128 registers spill: 118 / 87 / 113.
 #include "kv8_attn.cuh"
 
 #include <cuda_fp16.h>
@@ -44,7 +58,6 @@ constexpr int kSlice = 16;                            // positions of a slice
 constexpr int kStep = 2;                              // slices a warp takes at a time: one page, or two of 16 positions
 constexpr int kUnit = kSlice * kStep * kDecWarps;     // positions of a unit
 constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: registers
-constexpr int kWholeItems = 4;                        // items of at most this many units are not split
 constexpr int kChunkRows = 64;                        // rows of a kv head from which the tensor tiles are faster,
 constexpr int kChunkUnits = 24;                       // given at least this many units of this kernel's for each block
 constexpr int kMergeAhead = 8;                        // partial results read at once
@@ -269,28 +282,15 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = a.g.G, Hkv = a.g.Hkv;
 
-  int longest = 0;
   request_prefix(a.b.B, bt.pre, red, [&](int b) {
     const Kv8Req r = kv8_req(a.b, a.g.P, b);
     DecReq q{b, bt.q0[b] = r.q0, bt.q[b] = r.q, bt.len[b] = r.len, 0, 0, 0};
     dec_shape<ROWS>(a, q);
-    if (q.nr > 0) longest = max(longest, q.nt);
     return static_cast<long long>(q.nr) * q.nt * Hkv;
   });
   const long long total = bt.pre[a.b.B];
   const long long share = quotient(total + gridDim.x - 1, gridDim.x);
-  long long u0 = min(total, share * blockIdx.x), u1 = min(total, u0 + share);
-  // short items stay whole: their few units take less time than merging parts of them would
-  if (!__syncthreads_or(longest > kWholeItems)) {
-    auto item_start = [&](long long u) {  // of the first item that starts at u or later
-      if (u >= total) return total;
-      const int b = request_of(bt.pre, a.b.B, u);
-      const int nt = dec_req<ROWS>(a, bt, b).nt;
-      return bt.pre[b] + quotient(u - bt.pre[b] + nt - 1, nt) * nt;
-    };
-    u0 = item_start(u0);
-    u1 = item_start(u1);
-  }
+  const long long u0 = min(total, share * blockIdx.x), u1 = min(total, u0 + share);
   if (u0 >= u1) return;
   const int n_units = uniform(static_cast<int>(u1 - u0));
 
@@ -894,7 +894,8 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
       kv8_chunk_launch(h, a, st);
       return;
     }
-    // rows of one kv head: one column tile of 8 where they fit, else two
+    // rows of one kv head: one column tile of 8 where they fit, else two (64 requests of up to 4,096, 4 rows a kv head: 69 us
+    // with one tile, 94 with two)
     const bool one = static_cast<long long>(max_q) * h->g.G <= 8;
     if (dtype == SPECDEC_F32)
       one ? dec_launch_dim<float, 1>(h, a, st) : dec_launch_dim<float, 2>(h, a, st);

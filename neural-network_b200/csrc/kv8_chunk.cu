@@ -26,6 +26,20 @@
 // kv8_attn.cu; partial results of an item meet in the workspace.  Every wait
 // is bounded; one that gives up sets the handle's error word and ends the
 // block after the products in flight.
+//
+// Measured (32 / 8 heads of 128): 4 requests of up to 509 rows over up to 4,096
+// positions 140 us back to back (52 GFLOP, 31 us at the measured 1,661
+// TFLOP/s), 512 rows over 8,192 in 123 us, 541 TFLOP/s; 8 x 2,048 rows over
+// themselves with 32 / 32 heads 668 us, 412 TFLOP/s.  The softmax bounds it: of
+// a unit's 7,800 cycles a row's maximum takes 1,400 and its weights 2,900, on
+// two warps a scheduler; the rest waits for the score product that follows the
+// output product of the unit before, in halves of 64 positions so that only
+// half of it shows (whole tiles: 188 us).  A segment's start, its queries'
+// conversion above all, costs 14,000 cycles, a merge up to 35,000.  Slower:
+// 64 columns of scores in registers at once (188 us; its loops outgrow the
+// instruction cache), more registers for the softmax taken from the converters
+// (152 us: 512 threads then share the same file), a maximum over all of a half's
+// scores at once (143 us).
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -43,7 +57,6 @@ constexpr int kSoftmaxThreads = 256;
 constexpr int kConverterWarps = 4;
 constexpr int kChunkThreads = kSoftmaxThreads + 32 * kConverterWarps + 32;
 constexpr int kScaleSlots = 4;    // the scales of a tile stay until both softmax groups are past it
-constexpr int kWholeChunks = 2;   // items of at most this many units are not split
 constexpr int kMergeParts = 8;
 
 template <int D>
@@ -228,7 +241,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
   extern __shared__ unsigned char chunk_smem[];
   unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(chunk_smem) + 1023) & ~uintptr_t(1023));
   unsigned char *q_smem = base, *k_smem = base + 2 * Geo::kTile, *v_smem = base + 4 * Geo::kTile;
-  float *scales = reinterpret_cast<float *>(base + Geo::kTiles);  // per slot: key scales, value scales, slices there
+  float *scales = reinterpret_cast<float *>(base + Geo::kTiles);  // per slot: key scales, value scales, a byte for two slices
   DecBatch bt;
   bt.pre = reinterpret_cast<long long *>(base + Geo::kFixed);
   bt.q0 = reinterpret_cast<int *>(bt.pre + a.b.B + 1);
@@ -266,7 +279,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_stop = 0;
   }
-  int longest = 0;
   request_prefix(a.b.B, bt.pre, red, [&](int b) {
     const Kv8Req r = kv8_req(a.b, a.g.P, b);
     bt.q0[b] = r.q0;
@@ -274,26 +286,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
     bt.len[b] = r.len;
     long long n = 0;
     const int nr = (r.q * a.g.G + kItemRows - 1) / kItemRows;
-    for (int rt = 0; rt < nr; ++rt) {
-      const int nt = chunk_tile(a, r.q, r.len, rt).nt;
-      longest = max(longest, nt);
-      n += nt;
-    }
+    for (int rt = 0; rt < nr; ++rt) n += chunk_tile(a, r.q, r.len, rt).nt;
     return n * a.g.Hkv;
   });
   const long long total = bt.pre[a.b.B];
   const long long share = quotient(total + gridDim.x - 1, gridDim.x);
-  long long u0 = min(total, share * blockIdx.x), u1 = min(total, u0 + share);
-  if (!__syncthreads_or(longest > kWholeChunks)) {  // short items stay whole
-    auto item_start = [&](long long u) {
-      if (u >= total) return total;
-      ChunkCursor c;
-      c.seek(a, bt, u);
-      return c.unit == 0 ? u : u + c.t.nt - c.unit;
-    };
-    u0 = item_start(u0);
-    u1 = item_start(u1);
-  }
+  const long long u0 = min(total, share * blockIdx.x), u1 = min(total, u0 + share);
   const int n_units = uniform(static_cast<int>(u1 - u0));
   tc_fence_before();
   __syncthreads();
@@ -521,34 +519,53 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       float m = kNone, l = 0.f, cs = 0.f;
       if (any && ok) {
         // the warp's 32 query rows, a run of eight dims a lane: a power of two (a NaN where the row has a value that is not
-        // finite) times f16
-#pragma unroll 4
-        for (int it = 0; it < kRowLanes; ++it) {
-          const int rr = 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes, run = lane % kRowLanes;
-          const bool in = rr < rows;
-          const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + rr);
-          const XT *src = static_cast<const XT *>(a.q) + (in ? (cur.q0 + of.i) * a.q_row + (cur.h * a.g.G + of.h) * a.q_head : 0) + 8 * run;
-          Quad<XT> x[2];
-          x[0].load(src, a.q_vec, in);
-          x[1].load(src + 4, a.q_vec, in);
-          float big = 0.f, bad = 0.f;
+        // finite) times f16.  kQueryAhead runs are asked for at once; rows past the last read one that is there
+        constexpr int kQueryAhead = 8;
+#pragma unroll 1
+        for (int it0 = 0; it0 < kRowLanes; it0 += kQueryAhead) {
+          uint4 x[kQueryAhead];
+          auto row_in = [&](int it) { return 32 * (warp & 3) + (it0 + it) * (32 / kRowLanes) + lane / kRowLanes; };
+          const int run = lane % kRowLanes;
+          auto source = [&](int it) {
+            const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + min(row_in(it), rows - 1));
+            return static_cast<const XT *>(a.q) + (cur.q0 + of.i) * a.q_row + (cur.h * a.g.G + of.h) * a.q_head + 8 * run;
+          };
+          if (a.q_vec) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float f = x[j >> 2].get(j & 3);
-            big = fmaxf(big, fabsf(f));
-            bad = fmaf(f, 0.f, bad);
+            for (int it = 0; it < kQueryAhead; ++it) {
+              const uint2 *src = reinterpret_cast<const uint2 *>(source(it));
+              const uint2 lo = __ldg(src), hi = __ldg(src + 1);
+              x[it] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+          } else {
+#pragma unroll
+            for (int it = 0; it < kQueryAhead; ++it) {
+              const unsigned short *u = reinterpret_cast<const unsigned short *>(source(it));
+              x[it] = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+            }
           }
 #pragma unroll
-          for (int o = kRowLanes / 2; o > 0; o >>= 1) {
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-            bad += __shfl_xor_sync(0xffffffffu, bad, o);
+          for (int it = 0; it < kQueryAhead; ++it) {
+            const int rr = row_in(it);
+            if (rr >= rows) x[it] = make_uint4(0, 0, 0, 0);
+            auto mag = [](uint32_t v) {
+              v &= 0x7fff7fffu;
+              return *reinterpret_cast<const __nv_bfloat162 *>(&v);
+            };
+            // bits of the row's largest |x|; those of an infinity or a NaN are the largest there are
+            const __nv_bfloat162 m2 = __hmax2_nan(__hmax2_nan(mag(x[it].x), mag(x[it].y)), __hmax2_nan(mag(x[it].z), mag(x[it].w)));
+            const uint32_t mb = *reinterpret_cast<const uint32_t *>(&m2);
+            uint32_t big = max(mb << 16, mb & 0xffff0000u);
+#pragma unroll
+            for (int o = kRowLanes / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const float bad = big < 0x7f800000u ? 0.f : __uint_as_float(0x7fc00000u);
+            const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 126);
+            const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+            if (run == 0) row_scale[kTileRows * w + rr] = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
+            auto halves = [&](uint32_t v) { return pack_f16(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down); };
+            *reinterpret_cast<uint4 *>(q_smem + w * Geo::kTile + (run >> 3) * Geo::kAtom + rr * 128 + (((run & 7) ^ (rr & 7)) << 4)) =
+                make_uint4(halves(x[it].x), halves(x[it].y), halves(x[it].z), halves(x[it].w));
           }
-          const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
-          const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
-          if (run == 0) row_scale[kTileRows * w + rr] = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
-          *reinterpret_cast<uint4 *>(q_smem + w * Geo::kTile + (run >> 3) * Geo::kAtom + rr * 128 + (((run & 7) ^ (rr & 7)) << 4)) =
-              make_uint4(pack_f16(x[0].get(0) * down, x[0].get(1) * down), pack_f16(x[0].get(2) * down, x[0].get(3) * down),
-                         pack_f16(x[1].get(0) * down, x[1].get(1) * down), pack_f16(x[1].get(2) * down, x[1].get(3) * down));
         }
         __syncwarp();
         cs = row_scale[r_item];
@@ -722,19 +739,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       };
       auto flush = [&]() {
         __syncwarp();
-#pragma unroll 4
-        for (int it = 0; it < kRowLanes; ++it) {
-          const int rr = 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes, run = lane % kRowLanes;
-          if (rr >= rows) continue;
+        const int run = lane % kRowLanes;
+        auto row_in = [&](int it) { return 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes; };
+        auto target = [&](int rr) {
           const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + rr);
-          const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * (2 * D) + ((run ^ (rr & 7)) << 4));
-          XT *dst = static_cast<XT *>(a.out) + (cur.q0 + of.i) * a.o_row + (cur.h * a.g.G + of.h) * a.o_head + 8 * run;
-          if (a.o_vec8) {
-            *reinterpret_cast<uint4 *>(dst) = v;
-          } else {
+          return static_cast<XT *>(a.out) + (cur.q0 + of.i) * a.o_row + (cur.h * a.g.G + of.h) * a.o_head + 8 * run;
+        };
+        auto staged = [&](int rr) { return *reinterpret_cast<const uint4 *>(stage + rr * (2 * D) + ((run ^ (rr & 7)) << 4)); };
+        if (a.o_vec8) {
+#pragma unroll 4
+          for (int it = 0; it < kRowLanes; ++it) {
+            const uint4 v = staged(row_in(it));
+            if (row_in(it) < rows) *reinterpret_cast<uint4 *>(target(row_in(it))) = v;
+          }
+        } else {
+#pragma unroll 1
+          for (int it = 0; it < kRowLanes; ++it) {
+            if (row_in(it) >= rows) continue;
+            const uint4 v = staged(row_in(it));
+            unsigned short *dst = reinterpret_cast<unsigned short *>(target(row_in(it)));
             const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) reinterpret_cast<unsigned short *>(dst)[j] = static_cast<unsigned short>(x[j >> 1] >> (16 * (j & 1)));
+            for (int j = 0; j < 8; ++j) dst[j] = static_cast<unsigned short>(x[j >> 1] >> (16 * (j & 1)));
           }
         }
         __syncwarp();
