@@ -58,8 +58,9 @@ constexpr int kSlice = 16;                            // positions of a slice
 constexpr int kStep = 2;                              // slices a warp takes at a time: one page, or two of 16 positions
 constexpr int kUnit = kSlice * kStep * kDecWarps;     // positions of a unit
 constexpr int dec_ctas(int nt) { return nt == 1 ? 3 : 2; }  // blocks per SM: registers
-constexpr int kChunkRows = 64;                        // rows of a kv head from which the tensor tiles are faster,
-constexpr int kChunkUnits = 24;                       // given at least this many units of this kernel's for each block
+constexpr int kChunkRows = 64;                        // rows of a kv head from which the tensor tiles are faster, given
+constexpr int kChunkUnits = 24;                       // this many of this kernel's units for each of its blocks, or
+constexpr float kChunkItems = 1.5f;                   // this many of its items
 constexpr int kMergeAhead = 8;                        // partial results read at once
 template <int D, int NT>
 struct DecGeom {
@@ -881,16 +882,18 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
                        aligned16(out) && out_row_stride % 8 == 0 && out_head_stride % 8 == 0, h->err_word};
     const auto st = static_cast<cudaStream_t>(stream);
     // Many rows per kv head: every cached value meets all of them and the products bound the call, so they go to the
-    // 128-row tensor tiles, where there is enough of it to pay for those tiles' longer start and merges.  Measured in us,
-    // this kernel / the tensor tiles (heads of 128, 32 requests over 3,080 positions, then 4 over 4,096):
-    //   32 / 8 heads:  48 rows 150 / 185 and 45 / 63,   64 rows 191 / 186 and 47 / 63,   128 rows 355 / 188 and 73 / 63
-    //   32 / 32 heads: 48 rows 521 / 607 and 104 / 115, 64 rows 686 / 604 and 129 / 116, 128 rows 1344 / 605 and 236 / 116
-    //   16 / 2 heads:  64 rows 63 / 69 and 24 / 57,     96 rows 86 / 71 and 32 / 58,     128 rows 106 / 71 and 34 / 58
-    // The units are those that the tables have room for: 21 a block at 16 / 2 heads and 64 rows, 28 at 32 / 8 and 128.
-    const long long row_tiles = (static_cast<long long>(b.T) * h->g.G + 15) / 16;
-    const long long units = row_tiles * h->g.Hkv * ((static_cast<long long>(b.cols) * h->g.P + kUnit - 1) / kUnit);
+    // 128-row tensor tiles, where there is enough of it to pay for those tiles' longer start and merges: units as the
+    // tables have room for, or items (row tiles x kv heads).  Measured in us, this kernel / the tensor tiles (heads of 128):
+    //   units a block  14: 4 x 16 rows over 4,096, 32 / 8 heads 48 / 55       22: 32 x 8 over 3,080, 16 / 2 heads 62 / 61
+    //                  28: 4 x 32 over 4,096, 32 / 8 heads    74 / 57         87: 32 x 16 over 3,080, 32 / 8    192 / 164
+    //   items a block 0.9: 4 x 64 over themselves, 16 / 2     13 / 20        1.7: 4 x 64, 32 / 8 heads           19 / 20
+    //                 1.7: 16 x 16 over 500, 32 / 8 heads     42 / 28        3.5: 4 x 128, 32 / 8 heads          32 / 22
+    //   48 rows of a kv head: 32 x 48 over 3,080, 32 / 32 heads 521 / 536, 32 x 12, 32 / 8 heads 149 / 164
+    const long long items = (static_cast<long long>(b.T) * h->g.G + 15) / 16 * h->g.Hkv;
+    const long long units = items * ((static_cast<long long>(b.cols) * h->g.P + kUnit - 1) / kUnit);
+    const long long blocks = static_cast<long long>(dec_ctas(2)) * h->num_sms;
     if (dtype == SPECDEC_BF16 && h->g.D >= 64 && b.B <= kChunkMaxBatch && static_cast<long long>(max_q) * h->g.G >= kChunkRows &&
-        units >= static_cast<long long>(kChunkUnits) * dec_ctas(2) * h->num_sms) {
+        (units >= kChunkUnits * blocks || items >= kChunkItems * blocks)) {
       kv8_chunk_launch(h, a, st);
       return;
     }
