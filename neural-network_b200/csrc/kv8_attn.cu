@@ -879,6 +879,7 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
                        (h->g.G & (h->g.G - 1)) == 0 ? log2i(h->g.G) : -1,
                        rows_aligned(q, q_row_stride, q_head_stride, dtype),
                        rows_aligned(out, out_row_stride, out_head_stride, dtype),
+                       aligned16(q) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0,
                        aligned16(out) && out_row_stride % 8 == 0 && out_head_stride % 8 == 0, h->err_word};
     const auto st = static_cast<cudaStream_t>(stream);
     // Many rows per kv head: every cached value meets all of them and the products bound the call, so they go to the

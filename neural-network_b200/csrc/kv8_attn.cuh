@@ -24,7 +24,7 @@ struct AttendArgs {
   int p_shift, t_shift;  // log2 of page and block positions
   int g_shift;           // log2 of the query heads of a kv head, -1 where that is no power of two
   int q_vec, o_vec;      // query / output rows start at 4-element boundaries
-  int o_vec8;            // output rows start at 8-element boundaries
+  int q_vec8, o_vec8;    // ... at 8-element boundaries
   int *err;              // set to 1 by a bounded wait that gave up
 };
 

@@ -253,7 +253,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_stop;
   __shared__ int s_last;
-  __shared__ float row_scale[kItemRows];
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   constexpr int kIssuer = (kSoftmaxThreads >> 5) + kConverterWarps;
 
@@ -518,57 +517,50 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       const int head = cur.h * a.g.G + at_row.h;
       float m = kNone, l = 0.f, cs = 0.f;
       if (any && ok) {
-        // the warp's 32 query rows, a run of eight dims a lane: a power of two (a NaN where the row has a value that is not
-        // finite) times f16.  kQueryAhead runs are asked for at once; rows past the last read one that is there
-        constexpr int kQueryAhead = 8;
-#pragma unroll 1
-        for (int it0 = 0; it0 < kRowLanes; it0 += kQueryAhead) {
-          uint4 x[kQueryAhead];
-          auto row_in = [&](int it) { return 32 * (warp & 3) + (it0 + it) * (32 / kRowLanes) + lane / kRowLanes; };
-          const int run = lane % kRowLanes;
-          auto source = [&](int it) {
-            const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + min(row_in(it), rows - 1));
-            return static_cast<const XT *>(a.q) + (cur.q0 + of.i) * a.q_row + (cur.h * a.g.G + of.h) * a.q_head + 8 * run;
-          };
-          if (a.q_vec) {
-#pragma unroll
-            for (int it = 0; it < kQueryAhead; ++it) {
-              const uint2 *src = reinterpret_cast<const uint2 *>(source(it));
-              const uint2 lo = __ldg(src), hi = __ldg(src + 1);
-              x[it] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
+        // the warp's 32 query rows to their places as they are, neighbouring lanes along a row; then each thread brings its
+        // row to a power of two times f16 (NaN where the row has a value that is not finite)
+        unsigned char *tile = q_smem + w * Geo::kTile;
+        auto place = [&](int row, int run) { return tile + (run >> 3) * Geo::kAtom + row * 128 + (((run & 7) ^ (row & 7)) << 4); };
+#pragma unroll 2
+        for (int it = 0; it < kRowLanes; ++it) {
+          const int rr = 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes, run = lane % kRowLanes;
+          const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + min(rr, rows - 1));
+          const XT *src = static_cast<const XT *>(a.q) + (cur.q0 + of.i) * a.q_row + (cur.h * a.g.G + of.h) * a.q_head + 8 * run;
+          if (a.q_vec8) {  // zeros past the last row
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(place(rr, run))), "l"(src), "r"(rr < rows ? 16 : 0)
+                         : "memory");
           } else {
-#pragma unroll
-            for (int it = 0; it < kQueryAhead; ++it) {
-              const unsigned short *u = reinterpret_cast<const unsigned short *>(source(it));
-              x[it] = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
-            }
-          }
-#pragma unroll
-          for (int it = 0; it < kQueryAhead; ++it) {
-            const int rr = row_in(it);
-            if (rr >= rows) x[it] = make_uint4(0, 0, 0, 0);
-            auto mag = [](uint32_t v) {
-              v &= 0x7fff7fffu;
-              return *reinterpret_cast<const __nv_bfloat162 *>(&v);
-            };
-            // bits of the row's largest |x|; those of an infinity or a NaN are the largest there are
-            const __nv_bfloat162 m2 = __hmax2_nan(__hmax2_nan(mag(x[it].x), mag(x[it].y)), __hmax2_nan(mag(x[it].z), mag(x[it].w)));
-            const uint32_t mb = *reinterpret_cast<const uint32_t *>(&m2);
-            uint32_t big = max(mb << 16, mb & 0xffff0000u);
-#pragma unroll
-            for (int o = kRowLanes / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-            const float bad = big < 0x7f800000u ? 0.f : __uint_as_float(0x7fc00000u);
-            const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 126);
-            const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
-            if (run == 0) row_scale[kTileRows * w + rr] = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
-            auto halves = [&](uint32_t v) { return pack_f16(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down); };
-            *reinterpret_cast<uint4 *>(q_smem + w * Geo::kTile + (run >> 3) * Geo::kAtom + rr * 128 + (((run & 7) ^ (rr & 7)) << 4)) =
-                make_uint4(halves(x[it].x), halves(x[it].y), halves(x[it].z), halves(x[it].w));
+            const unsigned short *u = reinterpret_cast<const unsigned short *>(src);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (rr < rows) v = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+            *reinterpret_cast<uint4 *>(place(rr, run)) = v;
           }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
-        cs = row_scale[r_item];
+        // bits of the row's largest |x|; those of an infinity or a NaN are the largest there are
+        uint32_t top2 = 0;
+#pragma unroll 4
+        for (int run = 0; run < kRowLanes; ++run) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(place(r, run));
+          auto mag = [](uint32_t v) {
+            v &= 0x7fff7fffu;
+            return *reinterpret_cast<const __nv_bfloat162 *>(&v);
+          };
+          const __nv_bfloat162 m2 = __hmax2_nan(__hmax2_nan(__hmax2_nan(mag(v.x), mag(v.y)), __hmax2_nan(mag(v.z), mag(v.w))), mag(top2));
+          top2 = *reinterpret_cast<const uint32_t *>(&m2);
+        }
+        const uint32_t big = max(top2 << 16, top2 & 0xffff0000u);
+        const float bad = big < 0x7f800000u ? 0.f : __uint_as_float(0x7fc00000u);
+        const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 126);
+        const float down = __uint_as_float((127 - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+        cs = (__uint_as_float((127 + e) << 23) + bad) * (fabsf(a.scale) * kLog2e);
+#pragma unroll 4
+        for (int run = 0; run < kRowLanes; ++run) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(place(r, run));
+          auto halves = [&](uint32_t v) { return pack_f16(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down); };
+          *reinterpret_cast<uint4 *>(place(r, run)) = make_uint4(halves(v.x), halves(v.y), halves(v.z), halves(v.w));
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) chunk_arrive(&q_full[w]);
