@@ -28,18 +28,20 @@
 // block after the products in flight.
 //
 // Measured (32 / 8 heads of 128): 4 requests of up to 509 rows over up to 4,096
-// positions 140 us back to back (52 GFLOP, 31 us at the measured 1,661
-// TFLOP/s), 512 rows over 8,192 in 123 us, 541 TFLOP/s; 8 x 2,048 rows over
-// themselves with 32 / 32 heads 668 us, 412 TFLOP/s.  The softmax bounds it: of
-// a unit's 7,800 cycles a row's maximum takes 1,400 and its weights 2,900, on
-// two warps a scheduler; the rest waits for the score product that follows the
-// output product of the unit before, in halves of 64 positions so that only
-// half of it shows (whole tiles: 188 us).  A segment's start, its queries'
-// conversion above all, costs 14,000 cycles, a merge up to 35,000.  Slower:
-// 64 columns of scores in registers at once (188 us; its loops outgrow the
-// instruction cache), more registers for the softmax taken from the converters
-// (152 us: 512 threads then share the same file), a maximum over all of a half's
-// scores at once (143 us).
+// positions 119 us (52 GFLOP, 31 us at the measured 1,661 TFLOP/s), 512 rows
+// over 8,192 in 116 us, 572 TFLOP/s; 8 x 2,048 rows over themselves with 32 / 32
+// heads 524 us, 525 TFLOP/s.  The softmax bounds long items: of a unit's cycles
+// a row's maximum takes 1,400 and its weights 2,900, on two warps a scheduler,
+// and part of each wait for the products between them shows, in halves of 64
+// positions (whole tiles: 188 us for the first).  Short items are bound by their
+// start (7,000 cycles: queries in, a first score tile) and end (8,000: outputs
+// out): 64 prompts of 128 rows over themselves 97 us.  There it took loads
+// without a branch around each (166 us before), rows copied as they are and
+// converted by their own thread, addresses without products.  Slower: 64
+// columns of scores in registers at once (its loops outgrow the instruction
+// cache), registers for the softmax taken from the converters (512 threads then
+// share the same file: 152 us for the first where it was 140), a maximum over
+// all of a half's scores at once (143).
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -499,6 +501,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lanes + 128 * w, o_at = tmem + lanes + 256 + 128 * w;
     constexpr int kRowLanes = D / 8;  // lanes of a row where a warp goes through its 32 rows together
+    // the row that a lane has in such a pass: its place in a row array, and on to the next without a product or a division
+    struct RowWalk {
+      const XT *p;
+      long long step, wrap;
+      int h;
+      __device__ __forceinline__ void next(int G) {
+        h += 32 / kRowLanes;
+        p += step;
+        while (h >= G) {
+          h -= G;
+          p += wrap;
+        }
+      }
+    };
+    auto walk = [&](const ChunkCursor &c, int w, const XT *base, long long row, long long head) {
+      const RowAt of = row_at(a, c.t.row0 + kTileRows * w + 32 * (warp & 3) + lane / kRowLanes);
+      return RowWalk{base + (c.q0 + of.i) * row + (c.h * a.g.G + of.h) * head, 32 / kRowLanes * head, row - a.g.G * head, of.h};
+    };
     ChunkCursor cur;
     if (n_units > 0) cur.seek(a, bt, u0);
     bool ok = true;
@@ -521,11 +541,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         // row to a power of two times f16 (NaN where the row has a value that is not finite)
         unsigned char *tile = q_smem + w * Geo::kTile;
         auto place = [&](int row, int run) { return tile + (run >> 3) * Geo::kAtom + row * 128 + (((run & 7) ^ (row & 7)) << 4); };
+        const int run = lane % kRowLanes;
+        RowWalk at = walk(cur, w, static_cast<const XT *>(a.q) + 8 * run, a.q_row, a.q_head);
 #pragma unroll 2
-        for (int it = 0; it < kRowLanes; ++it) {
-          const int rr = 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes, run = lane % kRowLanes;
-          const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + min(rr, rows - 1));
-          const XT *src = static_cast<const XT *>(a.q) + (cur.q0 + of.i) * a.q_row + (cur.h * a.g.G + of.h) * a.q_head + 8 * run;
+        for (int it = 0; it < kRowLanes; ++it, at.next(a.g.G)) {
+          const int rr = 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes;
+          const XT *src = rr < rows ? at.p : static_cast<const XT *>(a.q);
           if (a.q_vec8) {  // zeros past the last row
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(place(rr, run))), "l"(src), "r"(rr < rows ? 16 : 0)
                          : "memory");
@@ -733,23 +754,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
         __syncwarp();
         const int run = lane % kRowLanes;
         auto row_in = [&](int it) { return 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes; };
-        auto target = [&](int rr) {
-          const RowAt of = row_at(a, cur.t.row0 + kTileRows * w + rr);
-          return static_cast<XT *>(a.out) + (cur.q0 + of.i) * a.o_row + (cur.h * a.g.G + of.h) * a.o_head + 8 * run;
-        };
+        RowWalk at = walk(cur, w, static_cast<const XT *>(a.out) + 8 * run, a.o_row, a.o_head);
         auto staged = [&](int rr) { return *reinterpret_cast<const uint4 *>(stage + rr * (2 * D) + ((run ^ (rr & 7)) << 4)); };
         if (a.o_vec8) {
 #pragma unroll 4
-          for (int it = 0; it < kRowLanes; ++it) {
+          for (int it = 0; it < kRowLanes; ++it, at.next(a.g.G)) {
             const uint4 v = staged(row_in(it));
-            if (row_in(it) < rows) *reinterpret_cast<uint4 *>(target(row_in(it))) = v;
+            if (row_in(it) < rows) *reinterpret_cast<uint4 *>(const_cast<XT *>(at.p)) = v;
           }
         } else {
 #pragma unroll 1
-          for (int it = 0; it < kRowLanes; ++it) {
+          for (int it = 0; it < kRowLanes; ++it, at.next(a.g.G)) {
             if (row_in(it) >= rows) continue;
             const uint4 v = staged(row_in(it));
-            unsigned short *dst = reinterpret_cast<unsigned short *>(target(row_in(it)));
+            unsigned short *dst = reinterpret_cast<unsigned short *>(const_cast<XT *>(at.p));
             const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 8; ++j) dst[j] = static_cast<unsigned short>(x[j >> 1] >> (16 * (j & 1)));
