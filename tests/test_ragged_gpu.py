@@ -705,6 +705,64 @@ def test_server(gpu_lib, heads, kv_heads, dim, slots, pages):
     assert a == b and all(0 <= t < model.vocab for r in a for t in r)
 
 
+def test_a_step_in_a_graph(gpu_lib):
+    # the four calls captured once and replayed on new lengths, rows and uniforms give what the calls give
+    H, Hkv, D, P, t, B, cols = 4, 2, 64, 32, 16, 5, 6
+    rng = np.random.default_rng(16)
+    h = sd.KV8(H, Hkv, D, page_tokens=P, block_tokens=t, max_batch=B)
+    z = dict(dtype=torch.int32, device="cuda")
+    T = 16
+
+    def state():
+        s = dict(table=torch.full((B, cols), -1, **z), kv_len=torch.zeros(B, **z), cu_q=torch.zeros(B + 1, **z),
+                 tok_req=torch.zeros(T, **z), tok_pos=torch.zeros(T, **z), slots=torch.zeros(T, dtype=torch.int64, device="cuda"),
+                 status=torch.zeros(1, **z))
+        s["batch"] = sd.KV8Batch(**s)
+        s["layer"] = sd.KV8Layer(*(torch.zeros(B * cols, Hkv, P, D, dtype=torch.int8, device="cuda") for _ in range(2)),
+                                 *(torch.zeros(B * cols, Hkv, P // t, device="cuda") for _ in range(2)))
+        s.update(held=torch.zeros(B, **z), keep=torch.zeros(B, **z), q_len=torch.zeros(B, **z),
+                 ring=torch.arange(B * cols, **z), at=torch.tensor([0, B * cols], **z), at2=torch.zeros(2, **z),
+                 k=torch.zeros(T, Hkv, D, device="cuda"), v=torch.zeros(T, Hkv, D, device="cuda"),
+                 q=torch.zeros(T, H, D, device="cuda"), out=torch.zeros(T, H, D, device="cuda"),
+                 u=torch.zeros(T, device="cuda"), tok=torch.zeros(T, **z))
+        return s
+
+    def run(s):
+        st = torch.cuda.current_stream().cuda_stream
+        h.plan(s["batch"], s["held"], s["keep"], s["q_len"], s["ring"], s["at"], s["at2"], stream=st)
+        h.append(s["layer"], s["batch"], s["k"], s["v"], stream=st)
+        h.attend(s["layer"], s["batch"], s["q"], s["out"], max_q=4, stream=st)
+        sd.sample(s["out"].view(T, H * D)[:, :200], s["u"], s["tok"], stream=st)
+        s["at"].copy_(s["at2"])
+        s["held"].copy_(s["kv_len"])
+
+    a, b = state(), state()
+    run(b)  # nothing yet; kernels are loaded
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(b)
+    held = np.zeros(B, np.int64)
+    for step in range(12):
+        keep = np.maximum(held - rng.integers(0, 3, B), 0)
+        q = rng.integers(0, 4, B)
+        new = dict(keep=keep, q_len=q)
+        rows = {n: rng.normal(0, 1, tuple(a[n].shape)).astype(np.float32) for n in ("k", "v", "q")}
+        rows["u"] = rng.random(T).astype(np.float32).clip(0, 1 - 2.0 ** -24)
+        for s in (a, b):
+            for n, v in new.items():
+                s[n].copy_(i32(v))
+            for n, v in rows.items():
+                s[n].copy_(cu(v))
+        run(a)
+        graph.replay()
+        torch.cuda.synchronize()
+        held = keep + q
+        assert int(a["status"][0]) == 0 and a["kv_len"].tolist() == held.tolist()
+        for n in ("table", "kv_len", "cu_q", "tok_req", "tok_pos", "slots", "ring", "at", "out", "tok"):
+            assert torch.equal(a[n], b[n]), (step, n)
+    h.check()
+
+
 # ---------------------------------------------------------------------------
 # refusals
 
