@@ -10,8 +10,8 @@
 //
 // HBM would let 256 rows of 128,259 bf16 logits (66 MB) take 10 us; latency and
 // issue slots bound it.  Measured, rows with a mix of all filters: that batch
-// 193 us, 160 rows of 32,000 fp32 52 us, a single one 15 us.  Alone in the
-// large batch: arg max 54 us, top-k 50 126, no filter 119, top-p 0.9 249 (438
+// 189 us, 160 rows of 32,000 fp32 51 us, a single one 15 us.  Alone in the
+// large batch: arg max 54 us, top-k 50 121, no filter 119, top-p 0.9 246 (435
 // on flat rows).  A pass over the tokens that takes the exponential costs 60 us
 // there (about 50 instructions a token with the division by the temperature).
 // A block per row that reads it again from L2 in every pass takes 58 us for
@@ -314,6 +314,7 @@ struct alignas(16) Shared {
   int n[kMaxCluster], n_top[kMaxCluster];
   float min_above[kMaxCluster], max_below[kMaxCluster];
   // of this block alone
+  uint4 part[kThreads / 32];
   u64 hist[256], red[32], out[3];
   float redf[32];
   int redi[32], n_local, n_local_top, band[2], at;
@@ -597,14 +598,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
       append4(is, &sh.n_local, [&](int at, int j) { list[at] = make_uint2(__float_as_uint(l[j]), i + j); });
     });
     __syncthreads();
-    above = block_sum_u64(mine, sh.red);
-    min_above = -block_max(-min_above, sh.redf);
-    max_below = block_max(max_below, sh.redf);
-    if (warp == 0) {
-      tell(&sh.above[rank], above);
-      tell(&sh.n[rank], sh.n_local);
-      tell(&sh.min_above[rank], min_above);
-      tell(&sh.max_below[rank], max_below);
+    {  // the block's three results at once: the floats as keys, which integers compare
+      const uint32_t n_warp = __reduce_add_sync(0xffffffffu, mine), low_key = __reduce_min_sync(0xffffffffu, float_key(min_above)),
+                     high_key = __reduce_max_sync(0xffffffffu, float_key(max_below));
+      if (lane == 0) sh.part[warp] = make_uint4(n_warp, low_key, high_key, 0);
+      __syncthreads();
+      if (warp == 0) {
+        const uint4 p = sh.part[lane & (kThreads / 32 - 1)];
+        const uint32_t n_all = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? p.x : 0u);
+        const float lowest = key_float(__reduce_min_sync(0xffffffffu, p.y)), highest = key_float(__reduce_max_sync(0xffffffffu, p.z));
+        tell(&sh.above[rank], static_cast<u64>(n_all));
+        tell(&sh.n[rank], sh.n_local);
+        tell(&sh.min_above[rank], lowest);
+        tell(&sh.max_below[rank], highest);
+      }
     }
     meet();
     above = sum_told(sh.above);
@@ -761,7 +768,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
     }
   }
   auto in_top = [&](float l, int i) { return l > top.hi || (l >= top.lo && keeps(top.key, top.idx, sc, l, i)); };
-  auto e_of = [&](float l, int i) { return has_k && !in_top(l, i) ? 0.f : weight_e(sc.z(l), zmax); };
+  auto e_of = [&](float l, int i) {  // zmax is finite here, so that exp(0) needs no case of its own
+    const float e = expf(__fsub_rn(sc.z(l), zmax));
+    return has_k && !in_top(l, i) ? 0.f : e;
+  };
 
   Cut<uint32_t> nucleus{0, -1, 0, 0};  // top-p's cut, over the bits of e
   if (!slow && has_p) {
