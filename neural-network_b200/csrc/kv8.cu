@@ -318,14 +318,24 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
     int8_t *code = (kv ? a.c.v : a.c.k) + code_at;
     float *sc = (kv ? a.c.vs : a.c.ks) + scale_at;
     const XT *x = static_cast<const XT *>(a.x[kv]) + (r.q0 + p0 - start) * a.row_stride[kv] + h * a.head_stride[kv];
+    // all runs are asked for at once: no branch stands between the loads, those of rows that are not new read one that is
     Run<XT> v[RUNS];
     int row[RUNS];
+    auto load = [&](bool vec) {
 #pragma unroll
-    for (int i = 0; i < RUNS; ++i) {
-      const int e = lane + 32 * WARPS * i;
-      row[i] = e >> per_row_shift;
-      if (row[i] >= n_old && row[i] < n) v[i].load(x + row[i] * a.row_stride[kv] + (e - (row[i] << per_row_shift)) * kRun, a.vec[kv]);
-      else v[i].zero();
+      for (int i = 0; i < RUNS; ++i) {
+        const int e = lane + 32 * WARPS * i;
+        row[i] = e >> per_row_shift;
+        v[i].load(x + min(max(row[i], n_old), n - 1) * a.row_stride[kv] + (e - (row[i] << per_row_shift)) * kRun, vec);
+      }
+    };
+    if (a.vec[kv]) load(true);
+    else load(false);
+    const bool full = n_old == 0 && n == g.t;
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i)
+        if (row[i] < n_old || row[i] >= n) v[i].zero();
     }
     const float old = n_old ? *sc : 0.f;
     uint32_t top = 0;
@@ -368,6 +378,17 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
     else
       __syncwarp();
     if (lane == 0) *sc = s;
+    if (full && finite) {  // the loop below without its cases
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        uint32_t c[kRun];
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) c[j] = rint_bits(__fmul_rn(v[i].get(j), inv));
+        *reinterpret_cast<uint2 *>(code + (lane + 32 * WARPS * i) * kRun) =
+            make_uint2(low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7]));
+      }
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
       uint2 *to = reinterpret_cast<uint2 *>(code + (lane + 32 * WARPS * i) * kRun);
