@@ -179,11 +179,13 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
 // of eight adjacent values a lane (all of them in flight at once), so a block
 // of 16 x 128 takes one warp and no barrier, one of 128 x 128 eight warps.
 // 4 prompts of 2,048 bf16 rows, 32 heads of 128, written and read back (403 MB,
-// 61.5 us at the measured 6.55 TB/s): 103 us, 3.9 TB/s, half of what is moved
-// are stores.  What that took: 738 us with a thread per value, 149 with a warp
-// per block, 128 with rounding by an addition, 110 with K and V together and
-// heads read in one piece, 103 with whole sectors written.  A verify step (160
-// rows; 10 MB) takes 14.3 us for the two launches: latency.
+// 61.5 us at the measured 6.55 TB/s): 81 us, 5.0 TB/s; half of what is moved are
+// stores.  What that took: 738 us with a thread per value, 149 with a warp per
+// block, 128 with rounding by an addition, 110 with K and V together and heads
+// read in one piece, 103 with whole sectors written, 92 without branches between
+// a unit's loads, 84 with the read's places found once, 81 with three blocks a
+// multiprocessor.  A verify step (160 rows; 10 MB) takes 13 us for the two
+// launches: latency.
 constexpr float kInv127 = 1.f / 127.f;
 constexpr int kRun = 8;  // adjacent values that a lane handles together
 
@@ -283,10 +285,16 @@ struct AppendArgs {
 };
 
 constexpr int kAppendThreads = 256;
+// blocks per SM: registers (bf16 rows: 84 us for the case above with two, 81 with three; 4 x 1,024 fp32 rows, blocks of 128:
+// 99 us with one, 85 with two)
+template <typename XT>
+constexpr int append_ctas() {
+  return sizeof(XT) == 2 ? 3 : 2;
+}
 
 // RUNS runs a lane, WARPS warps a unit: RUNS x WARPS x 256 values = block_tokens x head_dim.
 template <typename XT, int RUNS, int WARPS>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, append_ctas<XT>()) kv8_append_kernel(const AppendArgs a) {
   extern __shared__ int append_smem[];
   int *pre = append_smem;  // [B + 1] blocks touched before a request
   __shared__ int red[kAppendThreads / 32];
@@ -494,22 +502,28 @@ __global__ void __launch_bounds__(kGatherThreads, 4) kv8_gather_kernel(const Gat
           s[kv][k] = __ldg((kv ? a.c.vs : a.c.ks) + (at[k] >> scale_shift));
         }
       }
+    const long long step = static_cast<long long>(at_once) * g.Hkv * g.D;  // between two of a lane's rows
+    const int rows_left = static_cast<int>(min(static_cast<long long>(kGatherAhead * at_once), a.n - n0));
+    auto store = [&](bool vec) {
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      if (!a.out[kv]) continue;
+      for (int kv = 0; kv < 2; ++kv) {
+        if (!a.out[kv]) continue;
+        XT *to = static_cast<XT *>(a.out[kv]) + (n0 * g.Hkv + h) * g.D + d;
 #pragma unroll
-      for (int k = 0; k < kGatherAhead; ++k) {
-        const long long n = n0 + k * at_once;
-        if (n >= a.n) break;
-        float f[kRun];
+        for (int k = 0; k < kGatherAhead; ++k, to += step) {
+          if (k * at_once >= rows_left) break;
+          float f[kRun];
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          const uint32_t x = (j < 4 ? w[kv][k].x : w[kv][k].y) ^ 0x80808080u;
-          f[j] = __fmul_rn(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f, s[kv][k]);
+          for (int j = 0; j < kRun; ++j) {
+            const uint32_t x = (j < 4 ? w[kv][k].x : w[kv][k].y) ^ 0x80808080u;
+            f[j] = __fmul_rn(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f, s[kv][k]);
+          }
+          Run<XT>::store(to, f, vec);
         }
-        Run<XT>::store(static_cast<XT *>(a.out[kv]) + (n * g.Hkv + h) * g.D + d, f, a.vec);
       }
-    }
+    };
+    if (a.vec) store(true);
+    else store(false);
   }
 }
 
