@@ -389,8 +389,12 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       const RowAt at_row = row_at(a, r);
       const long long at = live ? (q.q0 + at_row.i) * a.q_row + (cur.h * G + at_row.h) * a.q_head : 0;
       const XT *src = static_cast<const XT *>(a.q) + at + 4 * t;
+      auto load = [&](bool vec) {
 #pragma unroll
-      for (int s = 0; s < KW; ++s) raw[n][s].load(src + 16 * s, a.q_vec, live);
+        for (int s = 0; s < KW; ++s) raw[n][s].load(src + 16 * s, vec, live);
+      };
+      if (a.q_vec) load(true);
+      else load(false);
     }
   };
   // The item's queries, scaled by a power of two to at most 1..2, as whole numbers v = x 2^(21 - e) rounded, where
