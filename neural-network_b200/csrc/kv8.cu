@@ -22,7 +22,7 @@ namespace {
 // whole scan over the requests (12 bytes each, from L2 after the first) so
 // that one launch is enough; the blocks then share tokens, moved pages and
 // requests.  Both scans in one pass of 512 threads, one packed into the other:
-// 6.9 us for 32 requests (an empty launch takes about 3), 8.5 us for 2,048
+// 6.7 us for 32 requests (an empty launch takes about 3), 8.4 us for 2,048
 // requests with 65,000 rows (1.1 MB, 0.2 us of HBM); with two passes of 1,024
 // threads 8.9 and 16.4 us.
 struct PlanArgs {

@@ -32,8 +32,8 @@
 // equal calls give equal bits.
 //
 // Measured (bf16 rows, heads of 128, of the measured 6.55 TB/s):
-//   32 requests of up to 3,080 positions, 5 rows, 32 / 32 heads: 97 us, 5.2 TB/s (0.80)
-//   64 requests of up to 4,096, 1 row, 32 / 8 heads:             72 us, 4.8 TB/s (0.73)
+//   32 requests of up to 3,080 positions, 5 rows, 32 / 32 heads: 100 us, 5.1 TB/s (0.78)
+//   64 requests of up to 4,096, 1 row, 32 / 8 heads:             71 us, 4.8 TB/s (0.74)
 //   2 requests of 131,071, 1 row, 32 / 8 heads:                 101 us, 5.3 TB/s (0.81)
 //   8 requests of up to 100, 1 fp32 row, 4 heads of 64:         8.2 us: latency
 // The copies alone, without products, run the third in 81 us; conversions,
