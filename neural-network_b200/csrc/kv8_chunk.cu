@@ -536,11 +536,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       const long long token = cur.q0 + at_row.i;
       const int head = cur.h * a.g.G + at_row.h;
       float m = kNone, l = 0.f, cs = 0.f;
+      // eight dims of a row in the query tile, for its queries and later for its outputs: a warp's rows are its own, so
+      // that a warp that is through with its outputs may bring in the next segment's queries
+      unsigned char *tile = q_smem + w * Geo::kTile;
+      auto place = [&](int row, int run) { return tile + (run >> 3) * Geo::kAtom + row * 128 + (((run & 7) ^ (row & 7)) << 4); };
       if (any && ok) {
         // the warp's 32 query rows to their places as they are, neighbouring lanes along a row; then each thread brings its
         // row to a power of two times f16 (NaN where the row has a value that is not finite)
-        unsigned char *tile = q_smem + w * Geo::kTile;
-        auto place = [&](int row, int run) { return tile + (run >> 3) * Geo::kAtom + row * 128 + (((run & 7) ^ (row & 7)) << 4); };
         const int run = lane % kRowLanes;
         RowWalk at = walk(cur, w, static_cast<const XT *>(a.q) + 8 * run, a.q_row, a.q_head);
 #pragma unroll 2
@@ -740,7 +742,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       const bool all = i0 >= u0 && i1 <= u1;
       // outputs leave through the query tile of the warp's rows, whose products have ended, so that a row is written by
       // neighbouring lanes
-      unsigned char *stage = q_smem + w * Geo::kTile;
       auto put = [&](int run, const float (&v)[8]) {
         uint32_t x[4];
 #pragma unroll
@@ -748,14 +749,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
           const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
           x[j] = *reinterpret_cast<const uint32_t *>(&t);
         }
-        *reinterpret_cast<uint4 *>(stage + r * (2 * D) + ((run ^ (r & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint4 *>(place(r, run)) = make_uint4(x[0], x[1], x[2], x[3]);
       };
       auto flush = [&]() {
         __syncwarp();
         const int run = lane % kRowLanes;
         auto row_in = [&](int it) { return 32 * (warp & 3) + it * (32 / kRowLanes) + lane / kRowLanes; };
         RowWalk at = walk(cur, w, static_cast<const XT *>(a.out) + 8 * run, a.o_row, a.o_head);
-        auto staged = [&](int rr) { return *reinterpret_cast<const uint4 *>(stage + rr * (2 * D) + ((run ^ (rr & 7)) << 4)); };
+        auto staged = [&](int rr) { return *reinterpret_cast<const uint4 *>(place(rr, run)); };
         if (a.o_vec8) {
 #pragma unroll 4
           for (int it = 0; it < kRowLanes; ++it, at.next(a.g.G)) {

@@ -31,7 +31,8 @@ namespace specdec {
 namespace {
 
 constexpr int kThreads = 512;        // of a block; a cluster of blocks takes a row
-constexpr int kSlice = 16384;        // tokens of a block where the row count gives enough blocks
+constexpr int kSlice = 16384;        // tokens of a block where the row count gives enough blocks: two blocks' fit an SM
+                                     // (160 rows of 32,000: 49 us with 8,192, 51 so, 62 with 32,768; 512 rows: 129, 103)
 constexpr int kMaxSlice = 40960;     // tokens that a block's shared memory holds
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 128;
@@ -978,7 +979,8 @@ template <typename XT>
 void launch(const SampleArgs &args, cudaStream_t st) {
   SampleArgs a = args;
   // a block for every kSlice tokens; more where the rows alone would leave multiprocessors idle (148 of them), down to
-  // 2,048 tokens a block, below which the meetings cost more than the passes
+  // 2,048 tokens a block, below which the meetings cost more than the passes (a row of 32,000: 16.5 us, 18 with 8,192 a block;
+  // 4 rows 23 and 26)
   int c = 1;
   while (c < kMaxCluster && (a.V > c * kSlice || (a.rows * c < 148 && a.V > c * 2048))) c *= 2;
   a.slice = ((a.V + c - 1) / c + 7) / 8 * 8;
