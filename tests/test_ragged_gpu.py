@@ -403,6 +403,26 @@ def test_attend_many_rows_and_wide_tables(gpu_lib, shape):
     h.check()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_many_short_prompts(gpu_lib, D):
+    # several row tiles a block, one after the other through the same shared memory; equal calls give equal bits
+    H, Hkv, P, t = 64, 16, 32, 16
+    rng = np.random.default_rng(17)
+    q = rng.integers(20, 66, 24).tolist()
+    lens = [n + int(rng.integers(0, 3)) * 40 for n in q]
+    table, n_pages = make_table(rng, lens, P)
+    cache = poison(make_cache(rng, n_pages, Hkv, P, D, t), table, lens, P, t)
+    cuq = np.concatenate([[0], np.cumsum(q)])
+    x = np.asarray(torch.tensor(rng.normal(0, 1, (sum(q), H, D))).bfloat16().float())
+    h = sd.KV8(H, Hkv, D, page_tokens=P, block_tokens=t, max_batch=len(lens))
+    got = run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", D ** -0.5, 0, handle=h)
+    check_attend(*got, *ref.attend(x, *cache, table, lens, cuq, P, t, D ** -0.5, 0), "bf16")
+    for _ in range(10):
+        again = run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", D ** -0.5, 0, handle=h)
+        assert np.array_equal(again[0], got[0]) and np.array_equal(again[1], got[1])
+    h.check()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("spare,max_q", [(1, 1), (1, 9), (WIDE, 500)])
 def test_attend_a_bad_block_reaches_only_the_rows_that_see_it(gpu_lib, dtype, spare, max_q):
