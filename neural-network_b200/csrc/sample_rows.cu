@@ -358,6 +358,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   const cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // every block says that it has started, and waits for the others before it first writes to one: the loads lie between
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   extern __shared__ __align__(16) unsigned char sample_smem[];
   Shared &sh = *reinterpret_cast<Shared *>(sample_smem);
   uint32_t *columns = reinterpret_cast<uint32_t *>(sample_smem + sizeof(Shared));  // [kBins][32]; also sorting's spare room
@@ -410,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   }
   const float my_high[2] = {high, second};
   high = block_max(fmaxf(high, second), sh.redf);
+  asm volatile("barrier.cluster.wait;" ::: "memory");
   if (warp == 0) tell(&sh.high[rank], high);
   meet();
   high = -INFINITY;
