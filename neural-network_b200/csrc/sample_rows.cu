@@ -38,7 +38,8 @@ constexpr int kMaxCluster = 8;
 constexpr int kBins = 128;
 constexpr int kCap = 1024;           // tokens that are sorted to settle a cut exactly
 constexpr float kFar = 22.2f;        // nats below the maximum from which the weight is 0: 2^31 exp(-22.2) < 1
-constexpr int kLevels = 4;
+constexpr int kLevels = 4;           // of finer bins for a top-k cut
+constexpr int kNarrow = 8;           // of finer bins for a top-p cut: 2^28 bit patterns at most, down by 64 or so each time
 constexpr int kFewHighs = kThreads / 2;  // k a block up to which the threads' maxima bound the k-th token well
 
 struct SampleArgs {
@@ -873,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
         meet();  // the lists have been read
         break;
       }
-      if (hi - lo == 1) {  // that many equal weights
+      if (hi - lo == 1 || level + 1 == kNarrow) {  // that many equal weights
         slow = true;
         break;
       }
@@ -900,6 +901,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
       slow = b0 >= kBins || b1 >= kBins;
       hi = top_bits + 1 - (static_cast<uint32_t>(b0) << step);
       lo = max(low_bits, top_bits + 1 - (static_cast<uint32_t>(b1 + 1) << step));
+      // A cut at the edge of many equal weights: the shifted sums leave it open whether it lies among them or at the next
+      // lower weight, which may be the lowest of the band, and finer bins tell no more.
+      if (hi == top_bits + 1 && lo == low_bits) slow = true;
     }
   }
   if (slow) {
