@@ -432,7 +432,8 @@ int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int
 /* Attention of the step's query rows [n_tokens][n_heads][head_dim] over the
  * cache: row i of request b stands at position p = kv_len - q + i and sees
  * positions max(0, p - window + 1) .. p (window 0: from 0).  scores = scale x
- * q . k, softmax in 32 bits, out in the rows' type, lse (may be NULL)
+ * q . k, softmax in 32 bits (its weights meet the values with 11 bits for
+ * bf16 rows, 22 for fp32 rows), out in the rows' type, lse (may be NULL)
  * [n_tokens][n_heads] = ln of the sum of exp(scores).  A row that sees
  * nothing gives zeros and -infinity; a position whose page number is outside
  * the pool is not seen; rows past cu_q[n_requests] are left as they are.

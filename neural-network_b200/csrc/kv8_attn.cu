@@ -15,15 +15,16 @@
 //   O^T [16 dims][8 rows]      += V^T codes [16 dims][16 positions] x P^T   f16
 // The queries enter as whole numbers of three bytes (22 bits of the row's
 // largest value), so the K codes need no conversion and the scores' sums are
-// exact; the weights span too many binades for that and enter as f16 (11 bits,
-// two of them for fp32 rows), relative to the largest weight x value scale.
+// exact; the weights span too many binades for that and enter as f16 (11 bits;
+// for fp32 rows a second f16 of what is left, 22 bits), a few binades above 1 at
+// the largest weight x value scale (kRoom, kLowUp).
 // A slice of 16 positions lies in one page and has one scale pair.  Every
 // warp takes two slices a step from a ring in shared memory that it fills
 // itself with 16-byte asynchronous copies (no barrier between warps until the
 // end of an item), converts V codes to f16 in registers, and keeps its running
 // maximum, sum and output; the block's warps take steps in turn and merge at
 // the end of a (request, kv head, row tile) item.  A row's maximum moves only
-// when a weight would pass 2^8: most steps rescale nothing.
+// when a weight would grow by 2^8: most steps rescale nothing.
 //
 // Work is split evenly whatever the lengths are: all items' 128-position units
 // in a row, an equal share of consecutive units per block.  A block that holds
@@ -62,7 +63,16 @@ constexpr int kChunkRows = 64;                        // rows of a kv head from 
 constexpr int kChunkUnits = 24;                       // this many of this kernel's units for each of its blocks, or
 constexpr float kChunkItems = 1.5f;                   // this many of its items
 constexpr int kMergeAhead = 8;                        // partial results read at once
-template <int D, int NT>
+// Steps (of 32 positions) after which a warp's running sums are added to far sums in shared memory and begin anew.  One
+// weight far above a long tail would swallow what follows it, since a lane adds single weights to its sum, and the tensor
+// cores cut an output off at its last bit with every product.  Sixteen steps leave 64 additions and, for fp32 rows, 64
+// products in a run.  64 requests of 100,000 positions, one of them 14 to 22 nats above the others, heads of 128: the
+// log-sum-exp is off by 5e-6 (1.3e-4 in one run and with weights in steps of 2^-24 of the largest), outputs of fp32 rows by
+// 3.3e-6 of the largest value (1.9e-4), with equal weights by 1.7e-7 (7.2e-6); verify rows as below, but fp32, take 115 us
+// (109).  The outputs of bf16 rows stay in one run: up to 2^-24 of them for each 16 positions of a warp's quarter of its
+// block's share, less than half a last bit of theirs below a million positions.
+constexpr int kRunSteps = 16;
+template <typename XT, int D, int NT>
 struct DecGeom {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSliceBytes = kSlice * D;            // K or V codes of a slice
@@ -72,7 +82,10 @@ struct DecGeom {
   static constexpr int kRing = kDecWarps * 3 * kHalf;       // per warp two K buffers and one V buffer
   static constexpr int kTails = kDecWarps * 2 * kTail;
   static constexpr int kQuery = 3 * NT * 32 * (D / 4);      // the rows' three bytes as the products take them
-  static constexpr int kFixed = kRing + kTails + kQuery;
+  static constexpr bool kWide = sizeof(XT) == 4;            // fp32 rows: outputs have far sums too
+  static constexpr int kFarRow = kWide ? 1 + D / 16 : 1;    // per eight rows and thread: (sums, maxima) of two columns, outputs
+  static constexpr int kFar = NT * kFarRow * kDecThreads * 16;
+  static constexpr int kFixed = kRing + kTails + kQuery + kFar;
   static constexpr int kPart = kRows * D + 2 * kRows;       // floats of a partial result
   static_assert(8 * D * 4 == kHalf, "a warp's output of eight rows fits the V buffer that it has just read");
 };
@@ -261,12 +274,12 @@ __device__ __forceinline__ int merge_place(int r, int d4) {
 
 template <typename XT, int D, int NT>
 __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(const __grid_constant__ AttendArgs a) {
-  using Geo = DecGeom<D, NT>;
+  using Geo = DecGeom<XT, D, NT>;
   constexpr int ROWS = Geo::kRows;
   constexpr int KS = D / 16;       // products of 16 dims per score tile, and 16-dim tiles of the output
   constexpr int KW = D / 16;       // words of codes a lane reads of a K row
   constexpr int KM = (KW + 1) / 2; // products of 32 dims per score tile
-  constexpr bool F32 = sizeof(XT) == 4;  // weights as two f16 each: 22 bits
+  constexpr bool F32 = Geo::kWide;  // weights as two f16 each: 22 bits
   constexpr int NP = F32 ? 2 : 1;
   extern __shared__ __align__(128) unsigned char dec_smem[];
   unsigned char *ring = dec_smem;
@@ -299,6 +312,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   const uint32_t my_k = shared_addr(ring) + warp * 3 * Geo::kHalf, my_v = my_k + 2 * Geo::kHalf;
   const uint32_t my_tails = shared_addr(ring) + Geo::kRing + warp * 2 * Geo::kTail;
   const uint32_t queries = shared_addr(ring) + Geo::kRing + Geo::kTails;
+  float4 *far = reinterpret_cast<float4 *>(ring + Geo::kRing + Geo::kTails + Geo::kQuery) + threadIdx.x;
   constexpr int kCopies = (kSlice * D / 16 + 31) / 32;  // 16-byte copies of a lane for a slice's K, and its V
   // copy c of a lane goes 512 c bytes on: 4 rows at D = 128, where the chunk order of every other copy is turned, and
   // 8 rows at D = 64, where it stays
@@ -372,6 +386,42 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   // the item's row tile: its first row and rows; first and last position at which some row is cut off; this warp's
   // next position; positions at which every row sees a whole step
   int row0 = 0, n_rows = 0, min_lim = 0, max_lim = 0, p0 = 0, whole_lo = 0, whole_hi = 0;
+  int run = 0, runs = 0;  // steps of the present run, runs in the far sums
+  // The far sums brought to the present maximum, plus the present run.
+  auto add_far = [&](int n, float4 &sums) {
+    float4 f = far[n * Geo::kFarRow * kDecThreads];
+    const float al[2] = {exp2_fast(f.z - m[n][0]), exp2_fast(f.w - m[n][1])};
+    sums = make_float4(fmaf(f.x, al[0], l[n][0]), fmaf(f.y, al[1], l[n][1]), m[n][0], m[n][1]);
+    if constexpr (F32) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        f = far[(n * Geo::kFarRow + 1 + s) * kDecThreads];
+        o[n][s][0] = fmaf(f.x, al[0], o[n][s][0]);
+        o[n][s][1] = fmaf(f.y, al[1], o[n][s][1]);
+        o[n][s][2] = fmaf(f.z, al[0], o[n][s][2]);
+        o[n][s][3] = fmaf(f.w, al[1], o[n][s][3]);
+      }
+    }
+  };
+  auto end_run = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float4 sums = make_float4(l[n][0], l[n][1], m[n][0], m[n][1]);
+      if (runs > 0) add_far(n, sums);
+      far[n * Geo::kFarRow * kDecThreads] = sums;
+      l[n][0] = l[n][1] = 0.f;
+      if constexpr (F32) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          far[(n * Geo::kFarRow + 1 + s) * kDecThreads] = make_float4(o[n][s][0], o[n][s][1], o[n][s][2], o[n][s][3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][s][j] = 0.f;
+        }
+      }
+    }
+    ++runs;
+    run = 0;
+  };
   Quad<XT> raw[NT][KW];
   auto begin_item = [&]() {  // asks for the item's query rows
     const DecReq &q = cur.q;
@@ -522,7 +572,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       bool grow = false;
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
-        fev[i] = static_cast<float>(max(static_cast<int>(__float_as_uint(vsc[i]) >> 23 & 0xff) - 127, -90));
+        fev[i] = static_cast<float>(max(static_cast<int>(__float_as_uint(vsc[i]) >> 23 & 0xff) - 127, kScaleFloor));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -533,7 +583,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
               if (p > last || (a.window > 0 && p <= last - a.window) || !(here >> i & 1)) x[i][n][j] = -INFINITY;
             }
           }
-          grow |= fmaxf(fmaxf(x[i][n][0], x[i][n][1]), fmaxf(x[i][n][2], x[i][n][3])) > kLazy - fev[i];
+          grow |= fmaxf(fmaxf(x[i][n][0], x[i][n][1]), fmaxf(x[i][n][2], x[i][n][3])) > kLazy + kRoom - fev[i];
         }
       }
       if (__any_sync(0xffffffffu, grow)) {
@@ -551,7 +601,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
             }
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-            const float nm = fmaxf(m[n][j], top);
+            const float nm = fmaxf(m[n][j], top - kRoom);
             const float al = exp2_fast(m[n][j] - nm);
             m[n][j] = nm;
             l[n][j] *= al;
@@ -588,7 +638,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
             pf[0][n][r] = transpose8x8(hi);
             if constexpr (F32) {
               const float2 h = unpack_f16(hi);
-              pf[NP - 1][n][r] = transpose8x8(pack_f16(w[2 * r] - h.x, w[2 * r + 1] - h.y));
+              pf[NP - 1][n][r] = transpose8x8(pack_f16((w[2 * r] - h.x) * kLowUp, (w[2 * r + 1] - h.y) * kLowUp));
             }
           }
         }
@@ -638,9 +688,13 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
               f[2] = f16_codes(__byte_perm(y[0][1], 0x64646464u, sel));
               f[3] = f16_codes(__byte_perm(y[1][1], 0x64646464u, sel));
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
+              for (int n = 0; n < NT; ++n) mma16816(o[n][4 * c + 2 * half + j], f, pf[0][n][0], pf[0][n][1]);
+              if constexpr (F32) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p) mma16816(o[n][4 * c + 2 * half + j], f, pf[p][n][0], pf[p][n][1]);
+                for (int i = 0; i < 4; ++i) f[i] = scale_f16(f[i], 1.f / kLowUp);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816(o[n][4 * c + 2 * half + j], f, pf[NP - 1][n][0], pf[NP - 1][n][1]);
+              }
             }
           }
         }
@@ -654,6 +708,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
     if (!last_of_item) {
       cp_wait<1>();  // a step that no row saw has not waited for its V
       issue_v();
+      if (++run == kRunSteps) end_run();
     }
 
     // ---- end of the item, or of this block's share of it --------------------
@@ -681,6 +736,12 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       __syncwarp();
 #pragma unroll
       for (int n = 0; n < NT; ++n) {  // eight rows at a time
+        if (runs > 0) {
+          float4 sums;
+          add_far(n, sums);
+          l[n][0] = sums.x;
+          l[n][1] = sums.y;
+        }
         float *mine = reinterpret_cast<float *>(ring + (warp * 3 + 2) * Geo::kHalf);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -776,6 +837,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
           if (threadIdx.x == 0) a.ticket[c0] = 0;
         }
       }
+      run = runs = 0;
       if (n_left > 1) put_queries();
       __syncthreads();
       issue_v();
@@ -783,9 +845,9 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
   }
 }
 
-template <int D, int NT>
+template <typename XT, int D, int NT>
 constexpr int dec_smem_bytes(int B) {
-  return DecGeom<D, NT>::kFixed + (B + 1) * static_cast<int>(sizeof(long long)) + 3 * B * static_cast<int>(sizeof(int));
+  return DecGeom<XT, D, NT>::kFixed + (B + 1) * static_cast<int>(sizeof(long long)) + 3 * B * static_cast<int>(sizeof(int));
 }
 
 template <typename XT, int D, int NT>
@@ -793,7 +855,7 @@ void dec_launch(const specdec_kv8 *h, const AttendArgs &a, cudaStream_t st) {
   // at most one item per row and kv head, at least one unit per block
   const long long units = static_cast<long long>(a.b.T) * h->g.Hkv * ((static_cast<long long>(a.b.cols) * h->g.P + kUnit - 1) / kUnit);
   const int grid = static_cast<int>(std::min(units, static_cast<long long>(dec_ctas(NT)) * h->num_sms));
-  op_launch("specdec_kv8_attend", kv8_decode_kernel<XT, D, NT>, dim3(grid), kDecThreads, dec_smem_bytes<D, NT>(a.b.B),
+  op_launch("specdec_kv8_attend", kv8_decode_kernel<XT, D, NT>, dim3(grid), kDecThreads, dec_smem_bytes<XT, D, NT>(a.b.B),
             st, 1, a);
 }
 
@@ -812,10 +874,10 @@ void dec_attrs(int max_batch) {
   auto set = [](auto kernel, int bytes) {
     op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
   };
-  set(kv8_decode_kernel<XT, 16, NT>, dec_smem_bytes<16, NT>(max_batch));
-  set(kv8_decode_kernel<XT, 32, NT>, dec_smem_bytes<32, NT>(max_batch));
-  set(kv8_decode_kernel<XT, 64, NT>, dec_smem_bytes<64, NT>(max_batch));
-  set(kv8_decode_kernel<XT, 128, NT>, dec_smem_bytes<128, NT>(max_batch));
+  set(kv8_decode_kernel<XT, 16, NT>, dec_smem_bytes<XT, 16, NT>(max_batch));
+  set(kv8_decode_kernel<XT, 32, NT>, dec_smem_bytes<XT, 32, NT>(max_batch));
+  set(kv8_decode_kernel<XT, 64, NT>, dec_smem_bytes<XT, 64, NT>(max_batch));
+  set(kv8_decode_kernel<XT, 128, NT>, dec_smem_bytes<XT, 128, NT>(max_batch));
 }
 
 int log2i(int v) {

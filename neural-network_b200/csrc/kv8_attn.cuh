@@ -31,8 +31,17 @@ struct AttendArgs {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNone = -1e30f;                  // the running maximum before anything was seen
-constexpr float kLazy = 8.f;                     // weights may grow to 2^8 before the maximum is moved
-
+constexpr float kLazy = 8.f;                     // weights may grow by 2^8 before the maximum is moved
+// The running maximum is held this many binades below the largest weight x value scale, so that those products are f16
+// values of 2^6 and up to 2^15 (65,504 is the last): f16 has no step below 2^-24, and from 1 upwards all weights under
+// 2^-25 of the largest would be lost, which over a long tail adds up (131,071 positions, one 17 nats above the others, by
+// arithmetic: 4e-4 of the largest value; 9e-6 with the room).
+constexpr float kRoom = 6.f;
+// What fp32 rows add to such an f16 value, w - f16(w), enters 2^12 times larger against codes 2^-12 as large (both exact):
+// 22 bits of every weight down to 2^-25, steps of 2^-36 below (2e-9 of the largest value in the case above).
+constexpr float kLowUp = 4096.f;
+constexpr int kScaleFloor = -84;                 // exponents of value scales count from here: 2^(kLazy + kRoom + 84) stays
+                                                 // far enough below 2^127 for sums of weights
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -47,6 +56,10 @@ __device__ __forceinline__ uint32_t f16_codes(uint32_t biased) {
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t scale_f16(uint32_t pair, float by) {
+  const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&pair), __float2half2_rn(by));
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 // Row r of a kv head's rows of a request: new token r / G, query head r % G.

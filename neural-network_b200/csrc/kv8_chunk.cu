@@ -19,7 +19,7 @@
 //                       memory in the place of the scores
 // The products of one row tile run while the other tile's warps are in their
 // softmax.  Tensor memory: scores 2 x 128 columns, outputs 2 x D.  A row's
-// maximum is moved (and its output rescaled) only when a weight would exceed
+// maximum is moved (and its output rescaled) only when a weight would grow by
 // 2^8.  The queries are scaled by a power of two per row, so that bf16 rows are
 // exact in f16; codes are whole numbers, exact too.
 // Units (tiles of 128 positions) of all items are shared out evenly, as in
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
       const int lim = live ? cur.len - cur.q + at_row.i : -1;
       const long long token = cur.q0 + at_row.i;
       const int head = cur.h * a.g.G + at_row.h;
-      float m = kNone, l = 0.f, cs = 0.f;
+      float m = kNone, l = 0.f, l_err = 0.f, cs = 0.f;  // l_err: what the last additions to l were too much by
       // eight dims of a row in the query tile, for its queries and later for its outputs: a warp's rows are its own, so
       // that a warp that is through with its outputs may bring in the next segment's queries
       unsigned char *tile = q_smem + w * Geo::kTile;
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = fmaxf(s[j], s[j + 8]);
           const float m4 = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-          const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(slot[kSlices + c]) >> 23 & 0xff) - 127, -90));
+          const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(slot[kSlices + c]) >> 23 & 0xff) - 127, kScaleFloor));
           if (m4 != -INFINITY) top = fmaxf(top, fmaf(m4, cs * fabsf(slot[c]), ev));
         };
         if (whole) {  // a slice's scores are asked for while the one before is worked on
@@ -649,11 +649,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
             top_of(s, slice);
           }
         }
-        if (__any_sync(0xffffffffu, top > m + kLazy)) {
-          const float nm = top > m + kLazy ? top : m;
+        if (__any_sync(0xffffffffu, top > m + (kLazy + kRoom))) {
+          const float nm = top > m + (kLazy + kRoom) ? top - kRoom : m;
           const float al = exp2_fast(m - nm);
           m = nm;
           l *= al;
+          l_err *= al;
           if (opened) {  // once the last step's product has ended (those before it have: these scores were issued after them)
             ok = chunk_wait(&pv_done[w], (n_pv - 1) & 1, &s_stop);
             ok = __all_sync(0xffffffffu, ok);
@@ -713,7 +714,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv8_chunk_kernel(const __gri
             tmem_st8(h_at + 8 * c, f);
           }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // compensated: halves of a long tail must not vanish beside one large weight (2,048 halves of 131,072 positions
+        // could lose 6e-5 of the sum)
+        const float add = ((sum[0] + sum[1]) + (sum[2] + sum[3])) - l_err, grown = l + add;
+        l_err = (grown - l) - add;
+        l = grown;
         opened = true;
         tmem_wait_st();
         tc_fence_before();

@@ -4,8 +4,9 @@ test_ragged_gpu.py's."""
 import numpy as np
 import pytest
 
+import ragged_ref as ref
 import specdec_b200 as sd
-from test_ragged_gpu import check_sample, cu, run_sample
+from test_ragged_gpu import WIDE, check_attend, check_sample, cu, make_table, run_attend, run_sample
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -58,3 +59,46 @@ def test_top_p_cut_at_the_edge_of_many_equal_weights(gpu_lib, groups):
     check_sample(rows, u, one, zero.astype(int), p, zero, tok, prob)
     k = np.full(B, int(n.sum()) - 1)  # the same cuts, top-k on as well
     check_sample(rows, u, one, k, p, zero, *run_sample(rows, u, k=k, p=p))
+
+
+# ---------------------------------------------------------------------------
+# attention
+
+@pytest.mark.parametrize("dtype,max_q,spare", [("f32", 1, 1), ("f32", 9, 1), ("bf16", 1, 1), ("bf16", 9, 1), ("bf16", 64, WIDE)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_one_position_far_above_a_long_tail(gpu_lib, dtype, max_q, spare, D):
+    """The first position stands 14 to 22 nats above 100,000 others of equal weight, whose values share a sign: what is
+    lost of their weights adds up.  Requests share their pages and are many, so that a block has a whole request and the
+    first position's warp a quarter of its tail: at 17 nats 7e-5 of the largest value with steps of 2^-24 of the largest
+    weight."""
+    Hkv, G, P, t, L, B = 8, 8 if max_q == 64 else 1, 128, 128, 100_000, 64
+    H = Hkv * G
+    rng = np.random.default_rng(21)
+    table, n_pages = make_table(rng, [L], P, spare_cols=spare)
+    k = np.zeros((n_pages, Hkv, P, D), np.int8)
+    k[table[0, 0], :, 0, 0] = 127
+    v = np.clip(np.rint(rng.normal(20, 30, k.shape)), -127, 127).astype(np.int8)
+    ks = np.full((n_pages, Hkv, 1), 16 / 127, np.float32)
+    vs = np.full((n_pages, Hkv, 1), 0.02, np.float32)
+    x = np.zeros((1, H, D), np.float32)
+    x[0, :, 0] = np.repeat([14, 16, 17, 17.5, 18, 18.5, 20, 22], G) / 16
+    want = ref.attend(x, k, v, ks, vs, table, [L], [0, 1], P, t, 1.0, 0)
+    got = run_attend(np.repeat(x, B, 0), (k, v, ks, vs), np.repeat(table, B, 0), [L] * B, np.arange(B + 1), H, Hkv, D, P, t,
+                     dtype, 1.0, 0, max_q=max_q)
+    check_attend(*got, *(np.repeat(w, B, 0) for w in want), dtype)
+
+
+def test_attend_long_tails_of_uneven_weights(gpu_lib):
+    # keys that spread the tail over 30 nats, some of it above the first position: the maximum moves on the way
+    H, Hkv, D, P, t, L = 4, 1, 64, 64, 16, 60_000
+    rng = np.random.default_rng(22)
+    lens, q = [L, 20_000], [1, 3]
+    table, n_pages = make_table(rng, lens, P)
+    k = np.clip(np.rint(rng.normal(0, 40, (n_pages, Hkv, P, D))), -127, 127).astype(np.int8)
+    k[table[:, 0], :, 0, :] = 50
+    v = np.clip(np.rint(rng.normal(20, 30, k.shape)), -127, 127).astype(np.int8)
+    ks = rng.uniform(0.01, 0.02, (n_pages, Hkv, P // t)).astype(np.float32)
+    vs = rng.choice([0, 1e-3, 0.02, 0.5], (n_pages, Hkv, P // t)).astype(np.float32)
+    x = (rng.normal(0, 1, (4, H, D)) + 0.5).astype(np.float32)
+    want = ref.attend(x, k, v, ks, vs, table, lens, [0, 1, 4], P, t, 0.7, 0)
+    check_attend(*run_attend(x, (k, v, ks, vs), table, lens, [0, 1, 4], H, Hkv, D, P, t, "f32", 0.7, 0), *want, "f32")
