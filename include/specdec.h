@@ -445,8 +445,9 @@ int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer, const spe
                        void *stream);
 
 /* Waits for `stream` and reports what its specdec_kv8_attend calls could not:
- * SPECDEC_ERR_CUDA if a bounded wait inside one gave up (its output is not
- * valid) since the last check. */
+ * SPECDEC_ERR_CUDA if a bounded wait inside one gave up since the last check
+ * (its output and that of later calls is not valid).  The handle may be used
+ * again after it; no other attend call of the handle may be under way. */
 int specdec_kv8_check(specdec_kv8 *h, void *stream);
 
 /* One token per row of logits [rows][vocab] (vocab at most 2^20) from the

@@ -983,7 +983,8 @@ extern "C" int specdec_kv8_check(specdec_kv8 *h, void *stream) {
     op_cuda(cudaMemcpyAsync(&bits, h->err_word, sizeof(int), cudaMemcpyDeviceToHost, st), "specdec_kv8_check");
     op_cuda(cudaStreamSynchronize(st), "specdec_kv8_check");
     if (!bits) return;
-    op_cuda(cudaMemsetAsync(h->err_word, 0, sizeof(int), st), "specdec_kv8_check");
+    // the block that gave up has not arrived at its split items: their tickets go back to 0 with the error word behind them
+    op_cuda(cudaMemsetAsync(h->ticket, 0, (h->err_word - h->ticket + 1) * sizeof(int), st), "specdec_kv8_check");
     op_fail(SPECDEC_ERR_CUDA, "a wait inside specdec_kv8_attend did not end within its limit");
   });
 }

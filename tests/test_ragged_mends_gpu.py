@@ -1,12 +1,14 @@
 """The ragged decode operators on the GPU where they once went wrong.
 Restatements are those of ragged_ref.py or stand here; tolerances are
 test_ragged_gpu.py's."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import ragged_ref as ref
 import specdec_b200 as sd
-from test_ragged_gpu import WIDE, check_attend, check_sample, cu, make_table, run_attend, run_sample
+from test_ragged_gpu import WIDE, check_attend, check_sample, cu, make_cache, make_table, run_attend, run_sample
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -102,3 +104,40 @@ def test_attend_long_tails_of_uneven_weights(gpu_lib):
     x = (rng.normal(0, 1, (4, H, D)) + 0.5).astype(np.float32)
     want = ref.attend(x, k, v, ks, vs, table, lens, [0, 1, 4], P, t, 0.7, 0)
     check_attend(*run_attend(x, (k, v, ks, vs), table, lens, [0, 1, 4], H, Hkv, D, P, t, "f32", 0.7, 0), *want, "f32")
+
+
+class _Words:
+    """Device memory at an address as 32-bit words."""
+
+    def __init__(self, address, n):
+        self.__cuda_array_interface__ = dict(shape=(n,), typestr="<i4", data=(address, False), version=3)
+
+
+@pytest.mark.parametrize("max_q,spare", [(1, 1), (64, WIDE)])
+def test_check_makes_a_handle_whole_again(gpu_lib, max_q, spare):
+    """A block that gives up leaves the arrivals of its split items counted and the error word set; check reports it once
+    and the next calls merge as before."""
+    H, Hkv, D, P, t = 32, 2, 64, 64, 16
+    rng = np.random.default_rng(23)
+    lens, q = [9000, 500], [2, 4]
+    table, n_pages = make_table(rng, lens, P, spare_cols=spare)
+    cache = make_cache(rng, n_pages, Hkv, P, D, t)
+    cuq = np.array([0, 2, 6])
+    x = np.asarray(torch.tensor(rng.normal(0, 1, (6, H, D))).bfloat16().float())
+    want = ref.attend(x, *cache, table, lens, cuq, P, t, 0.125, 0)
+    h = sd.KV8(H, Hkv, D, page_tokens=P, block_tokens=t, max_batch=2)
+    # specdec_kv8: 12 words of geometry, device, multiprocessors, a string of 32 bytes, then part, ticket, err_word
+    sms = C.cast(h.h.value + 52, C.POINTER(C.c_int32))[0]
+    ticket, err = C.cast(h.h.value + 96, C.POINTER(C.c_uint64))[:2]
+    assert sms == torch.cuda.get_device_properties(0).multi_processor_count and err == ticket + 3 * sms * 4
+    words = torch.as_tensor(_Words(ticket, 3 * sms + 1), device="cuda")
+    h.check()
+    assert not words.any()
+    words.fill_(1)
+    with pytest.raises(sd.SpecDecError, match="did not end"):
+        h.check()
+    for _ in range(2):
+        check_attend(*run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", 0.125, 0, max_q=max_q, handle=h), *want,
+                     "bf16")
+    assert not words.any()
+    h.check()
