@@ -908,7 +908,8 @@ void kv8_attn_create(specdec_kv8 *h) {
     op_cuda(e, "cudaMalloc");
   }
   h->err_word = h->ticket + blocks;
-  const cudaError_t z = cudaMemset(h->ticket, 0, (blocks + 1) * sizeof(int));
+  cudaError_t z = cudaMemset(h->ticket, 0, (blocks + 1) * sizeof(int));
+  if (z == cudaSuccess) z = cudaStreamSynchronize(nullptr);  // the first call may be on a stream that does not wait for it
   if (z != cudaSuccess) {
     kv8_attn_destroy(h);
     op_cuda(z, "cudaMemset");

@@ -141,3 +141,16 @@ def test_check_makes_a_handle_whole_again(gpu_lib, max_q, spare):
                      "bf16")
     assert not words.any()
     h.check()
+
+
+def test_a_new_handle_is_ready_for_any_stream(gpu_lib):
+    # its workspace is cleared on the default stream, which other streams need not wait for: create does
+    sd.KV8(4, 4, 64).close()
+    torch.cuda.synchronize()
+    busy = torch.cuda.Event()
+    torch.cuda._sleep(200_000_000)  # a tenth of a second of the default stream
+    busy.record()
+    assert not busy.query()
+    h = sd.KV8(4, 4, 64)
+    assert busy.query()
+    h.close()
