@@ -353,8 +353,8 @@ int specdec_time_attention(specdec_handle *h, int role, int layer, int q_per_req
  * block tables and slot maps, the cache write, the attention, the token.
  *
  * Every buffer is DEVICE memory of the handle's device (specdec_sample: of the
- * current device) and the caller's; `stream` is a cudaStream_t, NULL the
- * device's default stream.  Calls are asynchronous, allocate nothing, read no
+ * logits' device, on which it runs) and the caller's; `stream` is a
+ * cudaStream_t of that device, NULL its default stream.  Calls are asynchronous, allocate nothing, read no
  * device value on the host and may be captured in a graph.  A specdec_kv8
  * owns the attention's workspace: its specdec_kv8_attend calls on different
  * streams must be ordered by the caller.  Values on the device that are out

@@ -1025,6 +1025,10 @@ extern "C" int specdec_sample(const void *logits, int dtype, int rows, int vocab
     if (rows == 0) return;
     op_check(logits && u && tokens, "null sampling buffer");
     op_check(rows <= (1 << 24), "rows must be at most 2^24");
+    cudaPointerAttributes at{};
+    op_cuda(cudaPointerGetAttributes(&at, logits), "specdec_sample");
+    op_check(at.type != cudaMemoryTypeUnregistered, "logits must be device memory");
+    DeviceScope scope(at.device);
     const SampleArgs a{logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, probs, 0};
     const auto st = static_cast<cudaStream_t>(stream);
     dtype == SPECDEC_F32 ? launch<float>(a, st) : launch<__nv_bfloat16>(a, st);

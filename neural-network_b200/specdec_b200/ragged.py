@@ -4,7 +4,7 @@
 
 Buffers are CUDA tensors: any object with ``data_ptr()``, ``shape``,
 ``stride()``, ``dtype``, ``is_cuda``, ``get_device()`` and ``is_contiguous()``,
-as torch's are, on the device of the cache (``sample``: the current one).
+as torch's are, on the device of the cache (``sample``: of the logits).
 ``stream`` is a raw cudaStream_t (0: the device's default stream, torch's
 current one unless a caller changed it); tensors must be ready on it.
 Failures raise ``SpecDecError`` (a RuntimeError), wrong arguments before the
@@ -36,17 +36,19 @@ def _dtype_of(t) -> int:
     return d
 
 
-def _buffer(t, name: str, dtype: str, shape=None):
-    """The address of a contiguous buffer of the given type (and shape)."""
+def _buffer(t, name: str, dtype: str, shape=None, device=None):
+    """The address of a contiguous buffer of the given type (and shape and device)."""
     if (_names.get(t.dtype) or _name_of(t.dtype)) != dtype or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} must be a tensor of CUDA device {device}")
     return t.data_ptr()
 
 
-def _optional(t, name: str, dtype: str, shape=None):
-    return None if t is None else _buffer(t, name, dtype, shape)
+def _optional(t, name: str, dtype: str, shape=None, device=None):
+    return None if t is None else _buffer(t, name, dtype, shape, device)
 
 
 def _one_device(tensors) -> int:
@@ -149,12 +151,12 @@ class KV8:
 
     def plan(self, batch: KV8Batch, held, keep, q_len, ring, ring_state, ring_state_out, stream: int = 0) -> None:
         """Pages, lengths, row and slot maps of a step (specdec_kv8_plan)."""
-        n = (batch.n_requests,)
+        n, d = (batch.n_requests,), self.device
         self._check(self._lib.specdec_kv8_plan(
-            self.h, self._batch(batch), _buffer(held, "held", "int32", n), _buffer(keep, "keep", "int32", n),
-            _buffer(q_len, "q_len", "int32", n), _buffer(ring, "ring", "int32"), ring.shape[0],
-            _buffer(ring_state, "ring_state", "int32", (2,)), _buffer(ring_state_out, "ring_state_out", "int32", (2,)),
-            stream or None))
+            self.h, self._batch(batch), _buffer(held, "held", "int32", n, d), _buffer(keep, "keep", "int32", n, d),
+            _buffer(q_len, "q_len", "int32", n, d), _buffer(ring, "ring", "int32", None, d), ring.shape[0],
+            _buffer(ring_state, "ring_state", "int32", (2,), d),
+            _buffer(ring_state_out, "ring_state_out", "int32", (2,), d), stream or None))
 
     def append(self, layer: KV8Layer, batch: KV8Batch, k, v, stream: int = 0) -> None:
         """Writes rows k, v [rows][kv heads][head dim] to the requests' last positions."""
@@ -176,7 +178,7 @@ class KV8:
                for t in outs):
             raise ValueError(f"outputs must be contiguous, on CUDA device {self.device}, of one type and shape {shape}")
         self._check(self._lib.specdec_kv8_gather(
-            self.h, self._layer(layer), _buffer(rows, "rows", "int64"), n, None if out_k is None else out_k.data_ptr(),
+            self.h, self._layer(layer), _buffer(rows, "rows", "int64", None, self.device), n, None if out_k is None else out_k.data_ptr(),
             None if out_v is None else out_v.data_ptr(), _dtype_of(outs[0]), stream or None))
 
     def attend(self, layer: KV8Layer, batch: KV8Batch, q, out, lse=None, max_q: int = 1,
@@ -187,7 +189,7 @@ class KV8:
         op, orow, oh = _rows(out, self.n_heads, self.head_dim, "out", self.device)
         if out.shape[0] != q.shape[0] or out.dtype != q.dtype:
             raise ValueError("q and out must have the same rows and type")
-        lp = None if lse is None else _buffer(lse, "lse", "float32", q.shape[:2])
+        lp = None if lse is None else _buffer(lse, "lse", "float32", q.shape[:2], self.device)
         self._check(self._lib.specdec_kv8_attend(
             self.h, self._layer(layer), self._batch(batch), qp, qr, qh, _dtype_of(q), q.shape[0], op, orow, oh, lp,
             max_q, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, stream or None))
@@ -204,14 +206,13 @@ def sample(logits, u, tokens, probs=None, temperature=None, top_k=None, top_p=No
     sh, st = logits.shape, logits.stride()
     if len(sh) != 2 or (st[1] != 1 and sh[1] > 1) or not logits.is_cuda:
         raise ValueError("logits must be rows of adjacent values on a CUDA device")
-    if u.get_device() != logits.get_device() or tokens.get_device() != logits.get_device():
-        raise ValueError("u and tokens must be on the logits' device")
-    n = (sh[0],)
+    n, d = (sh[0],), logits.get_device()
     lib = _sd.load_library()
     rc = lib.specdec_sample(
-        logits.data_ptr(), _dtype_of(logits), sh[0], sh[1], st[0], _optional(temperature, "temperature", "float32", n),
-        _optional(top_k, "top_k", "int32", n), _optional(top_p, "top_p", "float32", n),
-        _optional(min_p, "min_p", "float32", n), _buffer(u, "u", "float32", n), _buffer(tokens, "tokens", "int32", n),
-        _optional(probs, "probs", "float32", n), stream or None)
+        logits.data_ptr(), _dtype_of(logits), sh[0], sh[1], st[0],
+        _optional(temperature, "temperature", "float32", n, d), _optional(top_k, "top_k", "int32", n, d),
+        _optional(top_p, "top_p", "float32", n, d), _optional(min_p, "min_p", "float32", n, d),
+        _buffer(u, "u", "float32", n, d), _buffer(tokens, "tokens", "int32", n, d),
+        _optional(probs, "probs", "float32", n, d), stream or None)
     if rc:
         raise _sd.SpecDecError(rc, lib.specdec_last_error(None).decode())

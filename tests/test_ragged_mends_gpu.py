@@ -63,6 +63,13 @@ def test_top_p_cut_at_the_edge_of_many_equal_weights(gpu_lib, groups):
     check_sample(rows, u, one, k, p, zero, *run_sample(rows, u, k=k, p=p))
 
 
+def test_sample_refuses_logits_of_the_host(gpu_lib):
+    # the call runs on the logits' device, which it asks for: memory that has none is refused before any launch
+    l, u, tok = np.zeros((1, 9), np.float32), torch.zeros(1, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    rc = gpu_lib.specdec_sample(l.ctypes.data, sd.F32, 1, 9, 9, None, None, None, None, u.data_ptr(), tok.data_ptr(), None, None)
+    assert rc == 1 and b"device memory" in gpu_lib.specdec_last_error(None)
+
+
 # ---------------------------------------------------------------------------
 # attention
 
