@@ -390,7 +390,8 @@ typedef struct specdec_kv8_batch {
   int32_t *tok_req, *tok_pos; /* [max_tokens] request and position of each row, -1 past the last */
   int64_t *slots;      /* [max_tokens] cache slot of each row, -1 past the last */
   int32_t max_tokens;
-  int32_t *status;     /* [1] 0, or bits: 1 not enough free pages, 2 a bad length (or ring), 4 more rows than max_tokens */
+  int32_t *status;     /* [1] 0, or bits: 1 not enough free pages, 2 a bad length, or a ring whose head or count is
+                        * outside it or that cannot hold the pages that come back, 4 more rows than max_tokens */
 } specdec_kv8_batch;
 
 typedef struct specdec_kv8 specdec_kv8;

@@ -107,9 +107,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
   __syncthreads();
 
   const long long takes = mv[a.B] & 0xffffffffll, gives = mv[a.B] >> 32;
-  const bool ring_ok = head >= 0 && head < a.ring_cap && count >= 0 && count <= a.ring_cap;
-  const int status = ((!ring_ok || takes > count) ? 1 : 0) | (bad ? 2 : 0) | (cu[a.B] > a.T ? 4 : 0) |
-                     ((ring_ok && count - takes + gives > a.ring_cap) ? 2 : 0);
+  // the tail's writes must not reach places that the head's reads come from, whose pages leave only with this step
+  const bool ring_ok = head >= 0 && head < a.ring_cap && count >= 0 && count + gives <= a.ring_cap;
+  const int status = ((ring_ok && takes > count) ? 1 : 0) | (bad || !ring_ok ? 2 : 0) | (cu[a.B] > a.T ? 4 : 0);
   const bool fine = status == 0;
   // ring places wrap at most twice: head, count and the moves are each at most ring_cap
   auto place = [&](long long i) {

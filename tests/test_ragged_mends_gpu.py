@@ -8,10 +8,32 @@ import pytest
 
 import ragged_ref as ref
 import specdec_b200 as sd
-from test_ragged_gpu import WIDE, check_attend, check_sample, cu, make_cache, make_table, run_attend, run_sample
+from test_ragged_gpu import WIDE, check_attend, check_sample, cu, make_cache, make_table, run_attend, run_plan, run_sample
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
+
+
+# ---------------------------------------------------------------------------
+# block tables
+
+@pytest.mark.parametrize("head,count,status", [(-1, 5, 2), (24, 5, 2), (3, -1, 2), (3, 25, 2), (1 << 30, 1 << 30, 2),
+                                               (3, 23, 2), (3, 22, 0), (3, 1, 1)])
+def test_plan_says_what_is_wrong_with_a_ring(gpu_lib, head, count, status):
+    """A head or count outside the ring, or a tail that would come round to pages of this step's head, is a bad ring (2), too
+    few pages are 1: a caller who frees pages and tries again on 1 must not do so on 2."""
+    P, cap = 16, 24
+    held, keep, q = [40, 0, 48], [40, 0, 5], [30, 8, 0]  # takes 2 and 1 pages, gives 2 of 3 back
+    table = np.array([[20, 21, 22, -1, -1], [-1] * 5, [17, 18, 19, -1, -1]], np.int32)
+    ring = np.arange(cap, dtype=np.int32)[::-1].copy()
+    got = run_plan(held, keep, q, table, ring, (head, count), P, 40)
+    assert got[8] == status
+    if status:  # nothing moved
+        want = (table, ring, (head, count), held, [0] * 4, [-1] * 40, [-1] * 40, [-1] * 40, status)
+    else:
+        want = ref.plan(held, keep, q, table, ring, (head, count), P, 40)
+    for g, w in zip(got, want):
+        assert np.array_equal(g, w)
 
 
 # ---------------------------------------------------------------------------
