@@ -417,7 +417,7 @@ int specdec_kv8_plan(specdec_kv8 *h, const specdec_kv8_batch *batch, const int32
 
 /* Writes the step's K and V rows [n_tokens][n_kv_heads][head_dim] to the last
  * q positions of their requests.  Per block of block_tokens positions and kv
- * head: scale' = max(the block's scale if it has older rows, max |x| over its
+ * head: scale' = max(|the block's scale| if it has older rows, max |x| over its
  * new finite values times the 32-bit 1/127), a scale below 2^-126 is 0; older codes become
  * rint(code x (scale / scale')), new codes rint(x x (1 / scale')) within
  * -127 .. 127; a NaN becomes 0, an infinity +-127. */

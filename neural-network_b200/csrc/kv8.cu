@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
 
 // ---------------------------------------------------------------------------
 // Cache write.  One unit = the new rows of one scale block and kv head, K then
-// V: a = max |x| over the finite new values, scale' = max(scale if the block
+// V: a = max |x| over the finite new values, scale' = max(|scale| if the block
 // has older rows, a x (1 / 127)); older rows are brought to scale', new rows
 // become rint(x x (1 / scale')).  A scale below the smallest normal number is
 // 0 (its codes are 0), so 1 / scale' is finite.
@@ -377,10 +377,10 @@ __global__ void __launch_bounds__(kAppendThreads, append_ctas<XT>()) kv8_append_
       }
       m = __uint_as_float(t);
     }
-    float s = fmaxf(old, __fmul_rn(m, kInv127));
+    float s = fmaxf(fabsf(old), __fmul_rn(m, kInv127));  // a block that came with a scale below 0 gets one above
     if (s < 1.17549435e-38f) s = 0.f;
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-    const float factor = s > old ? __fdiv_rn(old, s) : 1.f;
+    const float factor = s > old && s > 0.f ? __fdiv_rn(old, s) : 1.f;  // -1 .. 1
     if constexpr (WARPS > 1)  // every warp of the group has read the scale and the maxima
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WARPS) : "memory");
     else

@@ -8,7 +8,8 @@ import pytest
 
 import ragged_ref as ref
 import specdec_b200 as sd
-from test_ragged_gpu import WIDE, check_attend, check_sample, cu, make_cache, make_table, run_attend, run_plan, run_sample
+from test_ragged_gpu import (WIDE, check_attend, check_sample, cu, make_cache, make_table, run_append, run_attend, run_plan,
+                             run_sample)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -34,6 +35,30 @@ def test_plan_says_what_is_wrong_with_a_ring(gpu_lib, head, count, status):
         want = ref.plan(held, keep, q, table, ring, (head, count), P, 40)
     for g, w in zip(got, want):
         assert np.array_equal(g, w)
+
+
+# ---------------------------------------------------------------------------
+# cache write
+
+@pytest.mark.parametrize("old", [-0.03, -0.002, -1e-39, 0.03, 0.002, 0.0])
+def test_append_over_a_block_of_any_scale(gpu_lib, old):
+    """Older values keep their sign and size, to half a step of the new scale, where their block came with a scale below 0
+    (a cache that another program filled); the new scale is the larger of the two sizes."""
+    P, t, D, H = 32, 16, 16, 2
+    rng = np.random.default_rng(25)
+    cache = make_cache(rng, 1, H, P, D, t)
+    codes = [c.copy() for c in cache[:2]]
+    codes[0][0, 0, 0, :3] = [127, -127, 1]
+    scales = [np.full_like(s, old) for s in cache[2:]]
+    x = rng.normal(0, 0.3, (4, H, D)).astype(np.float32)
+    (k, v, ks, vs), *_ = run_append([x, -2 * x], [*codes, *scales], np.zeros((1, 1), np.int32), [13], [0, 4], P, t, "f32", H, D)
+    for c, s, was, rows in ((k, ks, codes[0], x), (v, vs, codes[1], -2 * x)):
+        new = np.maximum(np.float32(abs(old)), np.abs(rows).max((0, 2)) * (np.float32(1) / np.float32(127)))  # [H]
+        assert np.array_equal(s[0, :, 0], new) and np.array_equal(s[0, :, 1], np.full(H, old, np.float32))
+        value = c[0].astype(np.float64) * new.astype(np.float64)[:, None, None]
+        assert np.all(np.abs(value[:, :9] - was[0, :, :9].astype(np.float64) * np.float32(old)) <= new[:, None, None] * 0.50001)
+        assert np.all(np.abs(value[:, 9:13] - rows.transpose(1, 0, 2)) <= new[:, None, None] * 0.50001)
+        assert np.array_equal(c[0, :, 13:], was[0, :, 13:])
 
 
 # ---------------------------------------------------------------------------
