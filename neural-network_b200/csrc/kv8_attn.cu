@@ -468,8 +468,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, i));
         bad += __shfl_xor_sync(0xffffffffu, bad, i);
       }
-      const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
-      const float down = __uint_as_float((127 + 21 - e) << 23), up = __uint_as_float((127 + e) << 23) + bad;
+      const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 127);
+      const float down = __uint_as_float((127 + 21 - e) << 23), up = __uint_as_float((127 + e - 21) << 23) + bad;
 #pragma unroll
       for (int s = 0; s < KW; ++s) {
         if (s % kDecWarps != warp) continue;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) kv8_decode_kernel(c
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {  // columns 2t + j of this tile: their row's scale sits in lane 4 (2t + j)
-        cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e * (1.f / 2097152.f));
+        cs[n][j] = __shfl_sync(0xffffffffu, up, 4 * (2 * t + j)) * (a.scale * kLog2e);
         const int rr = 8 * n + 2 * t + j;
         lim[n][j] = rr < n_rows ? q.len - q.q + row_at(a, row0 + rr).i : -1;
         m[n][j] = kNone;

@@ -208,3 +208,20 @@ def test_a_new_handle_is_ready_for_any_stream(gpu_lib):
     h = sd.KV8(4, 4, 64)
     assert busy.query()
     h.close()
+
+
+@pytest.mark.parametrize("dtype,max_q,spare", [("f32", 1, 1), ("f32", 9, 1), ("bf16", 1, 1), ("bf16", 9, 1), ("bf16", 64, WIDE)])
+@pytest.mark.parametrize("large", [float(torch.finfo(torch.bfloat16).max), 1.6e38, 1e30])
+def test_attend_queries_at_the_end_of_their_type(gpu_lib, dtype, max_q, spare, large):
+    # values up to the largest bf16, with a scale that leaves scores of ordinary size
+    H, Hkv, D, P, t = 8, 2, 64, 64, 16
+    rng = np.random.default_rng(26)
+    lens, q = [400, 70], [1, 3]
+    table, n_pages = make_table(rng, lens, P, spare_cols=spare)
+    cache = make_cache(rng, n_pages, Hkv, P, D, t)
+    x = np.clip(rng.normal(0, 0.1, (4, H, D)), -1, 1)
+    x[:, :, 3], x[1:, :, 5] = 1, -1
+    x = np.asarray(torch.tensor(x * large).to(torch.float32 if dtype == "f32" else torch.bfloat16).float())
+    scale = float(np.float32(4 / large))
+    want = ref.attend(x, *cache, table, lens, [0, 1, 4], P, t, scale, 0)
+    check_attend(*run_attend(x, cache, table, lens, [0, 1, 4], H, Hkv, D, P, t, dtype, scale, 0, max_q=max_q), *want, dtype)
