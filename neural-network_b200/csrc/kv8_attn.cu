@@ -940,6 +940,8 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
     op_check(std::isfinite(scale), "scale must be finite");
     if (b.B == 0 || b.T == 0) return;
     op_check(q && out, "null row buffer");
+    // a window that no request can be longer than cuts nothing off, and positions less such a window pass 32 bits
+    if (window >= static_cast<long long>(b.cols) * h->g.P) window = 0;
     DeviceScope scope(h->device);
     const AttendArgs a{h->g, c,   b,     q,      q_row_stride, q_head_stride, out, out_row_stride, out_head_stride,
                        lse,  scale, window, h->part, h->ticket, log2i(h->g.P), log2i(h->g.t),

@@ -225,3 +225,20 @@ def test_attend_queries_at_the_end_of_their_type(gpu_lib, dtype, max_q, spare, l
     scale = float(np.float32(4 / large))
     want = ref.attend(x, *cache, table, lens, [0, 1, 4], P, t, scale, 0)
     check_attend(*run_attend(x, cache, table, lens, [0, 1, 4], H, Hkv, D, P, t, dtype, scale, 0, max_q=max_q), *want, dtype)
+
+
+@pytest.mark.parametrize("max_q,spare", [(1, 1), (9, 1), (64, WIDE)])
+def test_attend_windows_that_cut_nothing_off(gpu_lib, max_q, spare):
+    # windows up to the largest integer, beside rows that stand before their request's first position
+    H, Hkv, D, P, t = 8, 2, 64, 16, 16
+    rng = np.random.default_rng(27)
+    lens, q = [3, 40, 0, 100], [6, 2, 3, 70]
+    table, n_pages = make_table(rng, lens, P, spare_cols=spare)
+    cache = make_cache(rng, n_pages, Hkv, P, D, t)
+    cuq = np.concatenate([[0], np.cumsum(q)])
+    x = np.asarray(torch.tensor(rng.normal(0, 1, (sum(q), H, D))).bfloat16().float())
+    want = ref.attend(x, *cache, table, lens, cuq, P, t, 0.125, 0)
+    cap = table.shape[1] * P
+    for window in (100, cap - 1, cap, cap + 1, 2 ** 31 - 5, 2 ** 31 - 1):
+        got = run_attend(x, cache, table, lens, cuq, H, Hkv, D, P, t, "bf16", 0.125, window, max_q=max_q)
+        check_attend(*got, *want, "bf16")
