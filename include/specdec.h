@@ -455,7 +455,7 @@ int specdec_kv8_check(specdec_kv8 *h, void *stream);
  * row's uniform u in [0, 1).  Per row, each array NULL for its default:
  * temperature (<= 0: the arg max; default 1), top_k (<= 0: off), top_p (>= 1:
  * off), min_p (<= 0: off).  z = l / temperature (a NaN logit counts as
- * -infinity), w = floor(2^31 exp(z - max z)); top-k keeps the first k tokens by
+ * -infinity, an infinite one keeps its z at an infinite temperature), w = floor(2^31 exp(z - max z)); top-k keeps the first k tokens by
  * z, ties to the lower index; top-p keeps those of them before which less
  * than max(1, floor(top_p W)) of their mass W lies; min-p keeps those with
  * exp(z - max z) >= min(min_p, 1).  The token is the first in index order at

@@ -2,6 +2,7 @@
 Restatements are those of ragged_ref.py or stand here; tolerances are
 test_ragged_gpu.py's."""
 import ctypes as C
+import math
 
 import numpy as np
 import pytest
@@ -108,6 +109,24 @@ def test_top_p_cut_at_the_edge_of_many_equal_weights(gpu_lib, groups):
     check_sample(rows, u, one, zero.astype(int), p, zero, tok, prob)
     k = np.full(B, int(n.sum()) - 1)  # the same cuts, top-k on as well
     check_sample(rows, u, one, k, p, zero, *run_sample(rows, u, k=k, p=p))
+
+
+@pytest.mark.parametrize("V", [40, 33000, 400003])
+def test_sample_at_an_infinite_temperature(gpu_lib, V):
+    # every finite logit becomes 0 and draws alike; tokens at -infinity stay out whatever the filters
+    l = np.random.default_rng(28).normal(0, 3, (5, V)).astype(np.float32)
+    l[:, ::3] = -np.inf
+    l[0, 4] = np.nan
+    l[4, 7] = np.inf
+    allowed = [np.flatnonzero(np.isfinite(r)) for r in l[:4]]
+    u, T = np.array([0, 0.3, 0.7, 1 - 2.0 ** -24, 0.9], np.float32), [np.inf] * 5
+    for k, p in ((0, 1.0), (9, 1.0), (0, 0.5), (10, 0.5), (V - 1, 1.0)):
+        tok, prob = run_sample(l, u, T=T, k=[k] * 5, p=[p] * 5)
+        for b, a in enumerate(allowed):
+            n = min(k, len(a)) if k else len(a)
+            n = -(-math.floor(p * n * 2 ** 31) // 2 ** 31)
+            assert tok[b] == a[int(np.float64(u[b]) * 2 ** 24) * n >> 24] and abs(prob[b] * n - 1) < 1e-6
+        assert tok[4] == 7 and prob[4] == 1
 
 
 def test_sample_refuses_logits_of_the_host(gpu_lib):
