@@ -438,8 +438,8 @@ int specdec_kv8_gather(specdec_kv8 *h, const specdec_kv8_layer *layer, const int
  * [n_tokens][n_heads] = ln of the sum of exp(scores).  A row that sees
  * nothing gives zeros and -infinity; a position whose page number is outside
  * the pool is not seen; rows past cu_q[n_requests] are left as they are.
- * max_q: the most rows of one request (it selects the kernel; the result does
- * not depend on it). */
+ * max_q: the most rows of one request.  It selects the kernel with the rows and
+ * the table's width; results of different kernels are equal within rounding. */
 int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer, const specdec_kv8_batch *batch, const void *q,
                        int64_t q_row_stride, int64_t q_head_stride, int dtype, int n_tokens, void *out,
                        int64_t out_row_stride, int64_t out_head_stride, float *lse, int max_q, float scale, int window,

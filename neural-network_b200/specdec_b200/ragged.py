@@ -181,15 +181,19 @@ class KV8:
             self.h, self._layer(layer), _buffer(rows, "rows", "int64", None, self.device), n, None if out_k is None else out_k.data_ptr(),
             None if out_v is None else out_v.data_ptr(), _dtype_of(outs[0]), stream or None))
 
-    def attend(self, layer: KV8Layer, batch: KV8Batch, q, out, lse=None, max_q: int = 1,
+    def attend(self, layer: KV8Layer, batch: KV8Batch, q, out, lse=None, max_q: Optional[int] = None,
                scale: Optional[float] = None, window: int = 0, stream: int = 0) -> None:
         """Attention of q [rows][heads][head dim] over the cache into out (and lse
-        [rows][heads] float32); scale defaults to 1 / sqrt(head dim)."""
+        [rows][heads] float32); scale defaults to 1 / sqrt(head dim).  max_q,
+        the most rows of one request, chooses the kernel: by default the mean,
+        right for a batch of equal requests and for one prompt."""
         qp, qr, qh = _rows(q, self.n_heads, self.head_dim, "q", self.device)
         op, orow, oh = _rows(out, self.n_heads, self.head_dim, "out", self.device)
         if out.shape[0] != q.shape[0] or out.dtype != q.dtype:
             raise ValueError("q and out must have the same rows and type")
         lp = None if lse is None else _buffer(lse, "lse", "float32", q.shape[:2], self.device)
+        if max_q is None:
+            max_q = -(-q.shape[0] // max(1, batch.n_requests))
         self._check(self._lib.specdec_kv8_attend(
             self.h, self._layer(layer), self._batch(batch), qp, qr, qh, _dtype_of(q), q.shape[0], op, orow, oh, lp,
             max_q, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, stream or None))

@@ -1,5 +1,6 @@
 """The ragged decode operators' binding where there is no GPU: buffers of
-another device are refused before the library is called."""
+another device are refused before the library is called, and what is left out
+is filled in."""
 import pytest
 
 import specdec_b200 as sd
@@ -85,3 +86,13 @@ def test_a_buffer_of_another_device_is_refused(kv, call, name):
     with pytest.raises(ValueError, match="device"):
         run(*buffers(**{name: 1})[call])
     assert Library.calls == 1
+
+
+@pytest.mark.parametrize("rows,requests,given,passed", [(300, 1, None, 300), (160, 32, None, 5), (64, 64, None, 1), (70, 64, None, 2),
+                                                        (0, 3, None, 0), (300, 1, 1, 1), (5, 2, 9, 9)])
+def test_rows_of_a_request_that_are_not_given(kv, rows, requests, given, passed):
+    # a prompt without max_q must not go the way of single tokens, which reads the cache once for eight rows
+    batch = sd.KV8Batch(Stand("int32", requests, 1), Stand("int32", requests), Stand("int32", requests + 1))
+    q, out = (Stand("float32", rows, 4, 64) for _ in range(2))
+    kv.attend(buffers()["attend"][0], batch, q, out, **({} if given is None else dict(max_q=given)))
+    assert kv._lib.args[12] == passed
