@@ -985,11 +985,14 @@ size_t cluster_smem(int slice) {
 template <typename XT>
 void launch(const SampleArgs &args, cudaStream_t st) {
   SampleArgs a = args;
-  // a block for every kSlice tokens; more where the rows alone would leave multiprocessors idle (148 of them), down to
-  // 2,048 tokens a block, below which the meetings cost more than the passes (a row of 32,000: 16.5 us, 18 with 8,192 a block;
-  // 4 rows 23 and 26)
+  int device = 0, sms = 0;
+  op_cuda(cudaGetDevice(&device), "cudaGetDevice");
+  op_cuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device attributes");
+  // a block for every kSlice tokens; more where the rows alone would leave multiprocessors idle, down to 2,048 tokens a
+  // block, below which the meetings cost more than the passes (a row of 32,000: 16.5 us, 18 with 8,192 a block; 4 rows 23 and
+  // 26)
   int c = 1;
-  while (c < kMaxCluster && (a.V > c * kSlice || (a.rows * c < 148 && a.V > c * 2048))) c *= 2;
+  while (c < kMaxCluster && (a.V > c * kSlice || (static_cast<long long>(a.rows) * c < sms && a.V > c * 2048))) c *= 2;
   a.slice = ((a.V + c - 1) / c + 7) / 8 * 8;
   if (a.slice > kMaxSlice) {
     op_launch("specdec_sample", sample_whole_kernel<XT>, dim3(a.rows), kThreads, 0, st, 1, a);
@@ -997,8 +1000,6 @@ void launch(const SampleArgs &args, cudaStream_t st) {
   }
   const size_t smem = cluster_smem(a.slice);
   static std::atomic<unsigned long long> ready{0};  // devices whose kernel has its shared memory limit
-  int device = 0;
-  op_cuda(cudaGetDevice(&device), "cudaGetDevice");
   const unsigned long long bit = 1ull << (device & 63);
   if (!(ready.load() & bit)) {
     op_cuda(cudaFuncSetAttribute(sample_cluster_kernel<XT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
