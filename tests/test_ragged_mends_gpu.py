@@ -179,6 +179,31 @@ def test_attend_long_tails_of_uneven_weights(gpu_lib):
     check_attend(*run_attend(x, (k, v, ks, vs), table, lens, [0, 1, 4], H, Hkv, D, P, t, "f32", 0.7, 0), *want, "f32")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,P,t,G,q", [(128, 128, 64, 1, 1), (128, 16, 16, 2, 5), (64, 32, 16, 1, 9), (64, 64, 64, 4, 1), (32, 128, 16, 2, 1),
+                                       (16, 16, 16, 1, 3)])
+def test_attend_maxima_that_keep_growing(gpu_lib, dtype, D, P, t, G, q):
+    """Scores that climb by 20 nats along a cache, step after step with some noise, in items that a block does whole and
+    several of: sums of earlier runs meet later maxima, and no item finds another's."""
+    Hkv, B, L = 8, 64, 9_001
+    H = Hkv * G
+    rng = np.random.default_rng(24)
+    table, n_pages = make_table(rng, [L], P)
+    k, v, ks, vs = make_cache(rng, n_pages, Hkv, P, D, t)
+    climb = np.rint(np.linspace(-127, 127, table.shape[1] * P)[:L])
+    for p in range(L):
+        k[table[0, p // P], :, p % P, 0] = climb[p]
+    ks[:] = 0.02
+    x = rng.normal(0, 0.5, (q, H, D)).astype(np.float32)
+    x[:, :, 0] = rng.uniform(2, 6, (q, H))
+    x = np.asarray(torch.tensor(x).to(torch.float32 if dtype == "f32" else torch.bfloat16).float())
+    lens = [L, L - 4000, L - 7500]  # three lengths, one after the other
+    want = [ref.attend(x, k, v, ks, vs, table, [n], [0, q], P, t, 1.0, 0) for n in lens]
+    got = run_attend(np.tile(x, (B, 1, 1)), (k, v, ks, vs), np.repeat(table, B, 0), [lens[b % 3] for b in range(B)],
+                     np.arange(B + 1) * q, H, Hkv, D, P, t, dtype, 1.0, 0, max_q=min(q, 60 // G))
+    check_attend(*got, *(np.concatenate([want[b % 3][i] for b in range(B)]) for i in range(3)), dtype)
+
+
 class _Words:
     """Device memory at an address as 32-bit words."""
 
