@@ -220,7 +220,8 @@ __device__ void sample_whole_row(const SampleArgs &a, int b, u64 *hist, u64 *red
   const int V = a.V;
   auto zat = [&](int i) {
     const float l = no_nan(to_f32(x[i]));
-    return greedy || fabsf(l) == INFINITY ? l : __fdiv_rn(l, T);  // an infinite logit stays one at an infinite T
+    const float z = greedy ? l : __fdiv_rn(l, T);
+    return isnan(z) ? l : z;  // an infinite logit stays one at an infinite T
   };
   __shared__ float redf[32];
   __shared__ int redi[32];
