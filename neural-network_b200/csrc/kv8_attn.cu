@@ -33,10 +33,11 @@
 // equal calls give equal bits.
 //
 // Measured (bf16 rows, heads of 128, of the measured 6.55 TB/s):
-//   32 requests of up to 3,080 positions, 5 rows, 32 / 32 heads: 100 us, 5.1 TB/s (0.78)
-//   64 requests of up to 4,096, 1 row, 32 / 8 heads:             71 us, 4.8 TB/s (0.74)
-//   2 requests of 131,071, 1 row, 32 / 8 heads:                 101 us, 5.3 TB/s (0.81)
-//   8 requests of up to 100, 1 fp32 row, 4 heads of 64:         8.2 us: latency
+//   32 requests of up to 3,080 positions, 5 rows, 32 / 32 heads:  97 us, 5.3 TB/s (0.80); fp32 rows with an empty L2 115, bf16 109
+//   64 requests of up to 4,096, 1 row, 32 / 8 heads:              69 us, 5.0 TB/s (0.76)
+//   2 requests of 131,071, 1 row, 32 / 8 heads:                   97 us, 5.5 TB/s (0.84)
+//   4 requests of up to 509 fp32 rows over up to 4,096, 32 / 8:  440 us (bf16 rows on the tensor tiles 119)
+//   8 requests of up to 100, 1 fp32 row, 4 heads of 64:          8.2 us: latency
 // The copies alone, without products, run the third in 81 us; conversions,
 // softmax and products take issue slots beside them.  On the way (first case / second / third): codes converted for both products 179 /
 // 121 / 178, scores from bytes 127 / 88 / 134, two slices a step 115 /
@@ -959,6 +960,8 @@ extern "C" int specdec_kv8_attend(specdec_kv8 *h, const specdec_kv8_layer *layer
     //   items a block 0.9: 4 x 64 over themselves, 16 / 2     13 / 20        1.7: 4 x 64, 32 / 8 heads           19 / 20
     //                 1.7: 16 x 16 over 500, 32 / 8 heads     42 / 28        3.5: 4 x 128, 32 / 8 heads          32 / 22
     //   48 rows of a kv head: 32 x 48 over 3,080, 32 / 32 heads 521 / 536, 32 x 12, 32 / 8 heads 149 / 164
+    // The host does not know the lengths, so tables that are far wider than the requests are long send small prompts to the
+    // tensor tiles too (4 x 64 rows over themselves, 16 / 2 heads: 20 us instead of 13).
     const long long items = (static_cast<long long>(b.T) * h->g.G + 15) / 16 * h->g.Hkv;
     const long long units = items * ((static_cast<long long>(b.cols) * h->g.P + kUnit - 1) / kUnit);
     const long long blocks = static_cast<long long>(dec_ctas(2)) * h->num_sms;

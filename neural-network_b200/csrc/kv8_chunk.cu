@@ -20,8 +20,9 @@
 // The products of one row tile run while the other tile's warps are in their
 // softmax.  Tensor memory: scores 2 x 128 columns, outputs 2 x D.  A row's
 // maximum is moved (and its output rescaled) only when a weight would grow by
-// 2^8.  The queries are scaled by a power of two per row, so that bf16 rows are
-// exact in f16; codes are whole numbers, exact too.
+// 2^8.  The queries are scaled by a power of two per row: bf16 values down to
+// 2^-17 of the row's largest are exact in f16, smaller ones off by up to 2^-25 of
+// it; codes are whole numbers, exact too.
 // Units (tiles of 128 positions) of all items are shared out evenly, as in
 // kv8_attn.cu; partial results of an item meet in the workspace.  Every wait
 // is bounded; one that gives up sets the handle's error word and ends the

@@ -10,7 +10,9 @@
 //
 // HBM would let 256 rows of 128,259 bf16 logits (66 MB) take 10 us; latency and
 // issue slots bound it.  Measured, rows with a mix of all filters: that batch
-// 180 to 189 us, 160 rows of 32,000 fp32 50 us, a single one 14 us.  Alone in the
+// 175 to 191 us, 160 rows of 32,000 fp32 47 to 52 us, a single one 8 to 27 us.  A
+// cut among more than 1,024 equal weights goes to one block and global memory:
+// rows of 52,000 with 30,000 equal logits take 1.9 to 4.2 ms.  Alone in the
 // large batch: arg max 54 us, top-k 50 121, no filter 119, top-p 0.9 246 (435
 // on flat rows).  A pass over the tokens that takes the exponential costs 60 us
 // there (about 50 instructions a token with the division by the temperature).
